@@ -286,6 +286,73 @@ int q8lin_rope_kv_rows(const float* qkv, int32_t batch, int64_t t, int32_t pos0,
 int q8lin_attention_prefill(const float* q, const float* k_cache, const float* v_cache, int32_t batch, int64_t t,
                             int32_t pos0, int32_t hq, int32_t hkv, int32_t d, int32_t max_t, float* out,
                             q8lin_stream_t stream);
+/*
+ * Attention over the f32 KV caches [batch][hkv][max_t][128] beyond one causal prompt or one
+ * token, and the upkeep of the caches around it.  No counterpart in the reference, whose
+ * attention (crates/voxcpm/src/attention.rs:28-98) is causal over the whole history.
+ *
+ * `pos` [batch] (device int32) is each sequence's number of cache rows before the call, so a
+ * captured graph replays while they grow.  kv head = q head / (hq / hkv), any grouping; d =
+ * 128; scores times the f32 rounding of 1/sqrt(128), softmax statistics and sums in f32.
+ * A row at or past max_t (or of a sequence with pos < 0) is no row: its output is 0, nothing
+ * is written for it and nothing sees it.  Cache rows that no row of the call sees may hold
+ * anything; visible keys and values are finite.  Workspaces need no initialisation, are
+ * 16-byte aligned, and serve one call at a time (a captured graph keeps its own).  All calls
+ * are stream-ordered, allocate nothing, and run on the current device.
+ */
+#define Q8LIN_TREE_MAX 256 /* nodes of a drafted tree */
+size_t q8lin_attention_tree_workspace_size(int32_t batch, int32_t n, int32_t hq, int32_t hkv);
+/* RoPE + KV append + attention of `n` drafted tokens per sequence (1 <= n <= 256).
+ * qkv [batch][n][(hq + 2 hkv) * d]; parents [batch][n]: node i's parent, a node before it, or
+ * -1 for the history (a node with any other parent, and all below it, are no rows).  Node i
+ * takes cache row pos + i and the RoPE position pos + (number of its ancestors), and sees
+ * the history, its ancestors and itself.  cos_t / sin_t: [>= max_t][d/2], 16-byte aligned.
+ * out[batch][n][hq][d]. */
+int q8lin_rope_attention_tree(const float* qkv, const int32_t* parents, const int32_t* pos, const float* cos_t,
+                              const float* sin_t, float* k_cache, float* v_cache, int32_t batch, int32_t n, int32_t hq,
+                              int32_t hkv, int32_t d, int32_t max_t, void* workspace, size_t workspace_bytes,
+                              float* out, q8lin_stream_t stream);
+size_t q8lin_attention_weights_workspace_size(int32_t batch, int32_t t, int32_t hq, int32_t hkv, int32_t max_t);
+/* Causal attention of t rows per sequence at positions pos .. pos + t - 1 (their keys and
+ * values appended before, e.g. by q8lin_rope_kv_rows; q [batch][t][hq][d] rotated), which also
+ * adds to weight[batch][hkv][max_t] every key's softmax weight, summed over the rows and the
+ * heads of the group.  t = 1 is the decode form.  out[batch][t][hq][d]. */
+int q8lin_attention_weights(const float* q, const float* k_cache, const float* v_cache, const int32_t* pos,
+                            int32_t batch, int32_t t, int32_t hq, int32_t hkv, int32_t d, int32_t max_t, float* weight,
+                            void* workspace, size_t workspace_bytes, float* out, q8lin_stream_t stream);
+/* Eviction by accumulated weight: of the length[b] rows of every head, keep min(length[b],
+ * keep): rows [0, sink), rows [length - recent, length) and the heaviest of the others (equal
+ * weights: the lower row; NaN: lowest), sink + recent <= keep <= max_t.  The kept rows of
+ * both caches move together in place, order kept; rows behind them stay as they were.
+ * index[batch][hkv][keep]: the kept rows, ascending, -1 behind the last.  weight_out
+ * [batch][hkv][max_t] (may be weight, or NULL): the kept rows' weights, 0 behind them.
+ * Caches that are NULL are not moved (index and weight_out only). */
+int q8lin_kv_evict(const float* weight, const int32_t* length, int32_t batch, int32_t hkv, int32_t d, int32_t max_t,
+                   int32_t keep, int32_t sink, int32_t recent, float* k_cache, float* v_cache, int32_t* index,
+                   float* weight_out, q8lin_stream_t stream);
+/* Cache row base[b] + i <- row base[b] + index[b][h][i], i < count, in place, for ascending
+ * indices with index[i] >= i (others, and rows past max_t, stay as they are).  index
+ * [batch][index_heads][count], index_heads 1 (all heads alike) or hkv; base NULL: 0.  Moves
+ * the accepted path of a drafted tree together. */
+int q8lin_kv_move_rows(float* k_cache, float* v_cache, const int32_t* index, const int32_t* base, int32_t batch,
+                       int32_t hkv, int32_t index_heads, int32_t d, int32_t max_t, int32_t count,
+                       q8lin_stream_t stream);
+/* keys[batch][hkv][ceil(max_t / block)][d]: the mean key of every block of `block` rows that
+ * rows [pos, pos + t) complete (others stay as they are).  block: 16, 32, 64 or 128. */
+int q8lin_kv_block_keys(const float* k_cache, const int32_t* pos, int32_t batch, int32_t t, int32_t hkv, int32_t d,
+                        int32_t max_t, int32_t block, float* keys, q8lin_stream_t stream);
+size_t q8lin_attention_blocks_workspace_size(int32_t batch, int32_t t, int32_t hq, int32_t hkv);
+/* Attention of t rows per sequence at positions pos .. pos + t - 1 (appended before) over
+ * chosen blocks: the row's own block up to itself, and the topk blocks before its own with
+ * the largest score (sum over the group's heads of q . keys, in f64; equal scores: the
+ * lower block; NaN: lowest).  keys as q8lin_kv_block_keys leaves them; at most 16384
+ * blocks.  index[batch][t][hkv][topk]: the chosen blocks, ascending, -1 behind the last.
+ * out[batch][t][hq][d]. */
+int q8lin_attention_blocks(const float* q, const float* k_cache, const float* v_cache, const float* keys,
+                           const int32_t* pos, int32_t batch, int32_t t, int32_t hq, int32_t hkv, int32_t d,
+                           int32_t max_t, int32_t block, int32_t topk, void* workspace, size_t workspace_bytes,
+                           int32_t* index, float* out, q8lin_stream_t stream);
+
 size_t q8lin_argmax_workspace_size(void);
 /* *token = argmax(logits[0..n)) (lowest index on ties); if pos != NULL, *pos += 1.  The
  * workspace must be zero-filled once before first use. */

@@ -54,6 +54,7 @@ EPILOGUE_NONE, EPILOGUE_SWIGLU = 0, 1
 # Every symbol the header declares, with (restype, argtypes).
 _c_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
+_i32 = ctypes.c_int32
 SIGNATURES = {
     "q8lin_version": (ctypes.c_int, []),
     "q8lin_last_error": (ctypes.c_char_p, []),
@@ -102,6 +103,15 @@ SIGNATURES = {
     "q8lin_attention_prefill": (ctypes.c_int, [_c_p, _c_p, _c_p, ctypes.c_int32, _i64, ctypes.c_int32,
                                                ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _c_p,
                                                _c_p]),
+    "q8lin_attention_tree_workspace_size": (ctypes.c_size_t, [_i32] * 4),
+    "q8lin_rope_attention_tree": (ctypes.c_int, [_c_p] * 7 + [_i32] * 6 + [_c_p, ctypes.c_size_t, _c_p, _c_p]),
+    "q8lin_attention_weights_workspace_size": (ctypes.c_size_t, [_i32] * 5),
+    "q8lin_attention_weights": (ctypes.c_int, [_c_p] * 4 + [_i32] * 6 + [_c_p, _c_p, ctypes.c_size_t, _c_p, _c_p]),
+    "q8lin_kv_evict": (ctypes.c_int, [_c_p] * 2 + [_i32] * 7 + [_c_p] * 5),
+    "q8lin_kv_move_rows": (ctypes.c_int, [_c_p] * 4 + [_i32] * 6 + [_c_p]),
+    "q8lin_kv_block_keys": (ctypes.c_int, [_c_p] * 2 + [_i32] * 6 + [_c_p] * 2),
+    "q8lin_attention_blocks_workspace_size": (ctypes.c_size_t, [_i32] * 4),
+    "q8lin_attention_blocks": (ctypes.c_int, [_c_p] * 5 + [_i32] * 8 + [_c_p, ctypes.c_size_t, _c_p, _c_p, _c_p]),
     "q8lin_peer_alloc": (ctypes.c_int, [ctypes.c_int, ctypes.c_size_t, ctypes.POINTER(_c_p), _c_p]),
     "q8lin_peer_open": (ctypes.c_int, [ctypes.c_int, _c_p, ctypes.POINTER(_c_p)]),
     "q8lin_peer_close": (ctypes.c_int, [ctypes.c_int, _c_p]),

@@ -20,7 +20,8 @@ LIB = os.path.join(PKG, "libq8lin.so")
 OBJDIR = os.path.join(PKG, "_build")
 
 SOURCES = ["abi.cu", "layout.cu", "gemv.cu", "gemm_simt.cu", "gemm_tc.cu", "noalloc.cu", "mlp.cu", "gemm_skinny.cu", "decoder.cu",
-           "step.cu", "gemv_mrow.cu", "gguf.cpp", "tp_mlp.cu", "gemm_mma.cu", "prefill.cu"]
+           "step.cu", "gemv_mrow.cu", "gguf.cpp", "tp_mlp.cu", "gemm_mma.cu", "prefill.cu",
+           "kv_attention.cu", "kv_cache.cu"]
 HEADERS = ["common.cuh", "internal.h"]
 
 NVCC_FLAGS = [

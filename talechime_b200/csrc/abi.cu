@@ -748,6 +748,158 @@ int q8lin_attention_prefill(const float* q, const float* k_cache, const float* v
   return Q8LIN_OK;
 }
 
+namespace {
+// The shape rules of the attention entry points over [batch][hkv][max_t][128] caches; `rows`
+// new rows per sequence.
+int kv_shape_fail(const char* what, int64_t batch, int64_t rows, int64_t hq, int64_t hkv, int64_t d, int64_t max_t) {
+  if (d != 128) return fail(Q8LIN_ERR_SHAPE, std::string(what) + " supports head width 128");
+  if (hq <= 0 || hkv <= 0 || hq % hkv || hq > 65535)
+    return fail(Q8LIN_ERR_SHAPE, std::string(what) + " needs hq a positive multiple of hkv, hq <= 65535");
+  if (batch <= 0 || rows < 0 || max_t <= 0 || batch * hkv > 65535 || rows > (1 << 20) ||
+      batch * rows * hq > (INT64_C(1) << 30) || max_t > (1 << 30))
+    return fail(Q8LIN_ERR_SHAPE, std::string(what) + ": batch, rows or max_t out of range");
+  if (rows > max_t) return fail(Q8LIN_ERR_SHAPE, std::string(what) + ": more rows than the cache holds (context limit)");
+  return Q8LIN_OK;
+}
+int block_shape_fail(int block) {
+  if (block != 16 && block != 32 && block != 64 && block != 128)
+    return fail(Q8LIN_ERR_SHAPE, "blocks have 16, 32, 64 or 128 rows");
+  return Q8LIN_OK;
+}
+int current_device() {
+  int device = 0;
+  cudaGetDevice(&device);
+  return device;
+}
+}  // namespace
+
+size_t q8lin_attention_tree_workspace_size(int32_t batch, int32_t n, int32_t hq, int32_t hkv) {
+  if (batch <= 0 || n <= 0 || n > kKvMaxTree || hq <= 0 || hkv <= 0 || hq % hkv) return 0;
+  return attention_tree_workspace_bytes(batch, n, hq, hkv);
+}
+
+int q8lin_rope_attention_tree(const float* qkv, const int32_t* parents, const int32_t* pos, const float* cos_t,
+                              const float* sin_t, float* k_cache, float* v_cache, int32_t batch, int32_t n, int32_t hq,
+                              int32_t hkv, int32_t d, int32_t max_t, void* workspace, size_t workspace_bytes,
+                              float* out, q8lin_stream_t stream) {
+  if (int st = kv_shape_fail("rope_attention_tree", batch, n, hq, hkv, d, max_t)) return st;
+  if (n < 1 || n > kKvMaxTree) return fail(Q8LIN_ERR_SHAPE, "a tree has 1 to 256 nodes");
+  if (!qkv || !parents || !pos || !cos_t || !sin_t || !k_cache || !v_cache || !workspace || !out)
+    return fail(Q8LIN_ERR_INVALID_ARGUMENT, "rope_attention_tree pointers must be non-null device pointers");
+  if (!aligned16(qkv) || !aligned16(cos_t) || !aligned16(sin_t) || !aligned16(k_cache) || !aligned16(v_cache) ||
+      !aligned16(workspace) || !aligned16(out))
+    return fail(Q8LIN_ERR_ALIGNMENT, "qkv, the tables, the caches, the workspace and out must be 16-byte aligned");
+  if (workspace_bytes < attention_tree_workspace_bytes(batch, n, hq, hkv))
+    return fail(Q8LIN_ERR_WORKSPACE, "workspace too small (see q8lin_attention_tree_workspace_size)");
+  cudaError_t e = launch_rope_attention_tree(qkv, parents, pos, cos_t, sin_t, k_cache, v_cache, batch, n, hq, hkv, max_t,
+                                             workspace, out, current_device(), reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "rope_attention_tree launch");
+  return Q8LIN_OK;
+}
+
+size_t q8lin_attention_weights_workspace_size(int32_t batch, int32_t t, int32_t hq, int32_t hkv, int32_t max_t) {
+  if (batch <= 0 || t <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || max_t <= 0) return 0;
+  return attention_weights_workspace_bytes(batch, t, hq, hkv, max_t);
+}
+
+int q8lin_attention_weights(const float* q, const float* k_cache, const float* v_cache, const int32_t* pos,
+                            int32_t batch, int32_t t, int32_t hq, int32_t hkv, int32_t d, int32_t max_t, float* weight,
+                            void* workspace, size_t workspace_bytes, float* out, q8lin_stream_t stream) {
+  if (int st = kv_shape_fail("attention_weights", batch, t, hq, hkv, d, max_t)) return st;
+  if (t == 0) return Q8LIN_OK;
+  if (!q || !k_cache || !v_cache || !pos || !weight || !workspace || !out)
+    return fail(Q8LIN_ERR_INVALID_ARGUMENT, "attention_weights pointers must be non-null device pointers");
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(workspace) || !aligned16(out))
+    return fail(Q8LIN_ERR_ALIGNMENT, "q, the caches, the workspace and out must be 16-byte aligned");
+  if (workspace_bytes < attention_weights_workspace_bytes(batch, t, hq, hkv, max_t))
+    return fail(Q8LIN_ERR_WORKSPACE, "workspace too small (see q8lin_attention_weights_workspace_size)");
+  cudaError_t e = launch_attention_weights(q, k_cache, v_cache, pos, batch, t, hq, hkv, max_t, weight, workspace, out,
+                                           current_device(), reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "attention_weights launch");
+  return Q8LIN_OK;
+}
+
+int q8lin_kv_evict(const float* weight, const int32_t* length, int32_t batch, int32_t hkv, int32_t d, int32_t max_t,
+                   int32_t keep, int32_t sink, int32_t recent, float* k_cache, float* v_cache, int32_t* index,
+                   float* weight_out, q8lin_stream_t stream) {
+  if (int st = kv_shape_fail("kv_evict", batch, 0, hkv, hkv, d, max_t)) return st;
+  if (keep < 0 || sink < 0 || recent < 0 || keep > max_t || (int64_t)sink + recent > keep)
+    return fail(Q8LIN_ERR_SHAPE, "kv_evict needs 0 <= sink + recent <= keep <= max_t");
+  if (!weight || !length || (keep > 0 && !index) || !k_cache != !v_cache)
+    return fail(Q8LIN_ERR_INVALID_ARGUMENT, "kv_evict needs weight, length and index, and both caches or none");
+  if (k_cache && (!aligned16(k_cache) || !aligned16(v_cache)))
+    return fail(Q8LIN_ERR_ALIGNMENT, "the caches must be 16-byte aligned");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e = launch_kv_evict(weight, length, batch, hkv, max_t, keep, sink, recent, index, weight_out,
+                                  current_device(), s);
+  if (e == cudaSuccess && k_cache && keep > 0)
+    e = launch_kv_move(k_cache, v_cache, index, nullptr, batch, hkv, hkv, max_t, keep, s);
+  if (e != cudaSuccess) return cuda_fail(e, "kv_evict launch");
+  return Q8LIN_OK;
+}
+
+int q8lin_kv_move_rows(float* k_cache, float* v_cache, const int32_t* index, const int32_t* base, int32_t batch,
+                       int32_t hkv, int32_t index_heads, int32_t d, int32_t max_t, int32_t count,
+                       q8lin_stream_t stream) {
+  if (int st = kv_shape_fail("kv_move_rows", batch, count, hkv, hkv, d, max_t)) return st;
+  if (index_heads != 1 && index_heads != hkv)
+    return fail(Q8LIN_ERR_SHAPE, "kv_move_rows takes one index per sequence or one per head");
+  if (count == 0) return Q8LIN_OK;
+  if (!k_cache || !v_cache || !index)
+    return fail(Q8LIN_ERR_INVALID_ARGUMENT, "kv_move_rows pointers must be non-null device pointers");
+  if (!aligned16(k_cache) || !aligned16(v_cache))
+    return fail(Q8LIN_ERR_ALIGNMENT, "the caches must be 16-byte aligned");
+  cudaError_t e = launch_kv_move(k_cache, v_cache, index, base, batch, hkv, index_heads, max_t, count,
+                                 reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "kv_move_rows launch");
+  return Q8LIN_OK;
+}
+
+int q8lin_kv_block_keys(const float* k_cache, const int32_t* pos, int32_t batch, int32_t t, int32_t hkv, int32_t d,
+                        int32_t max_t, int32_t block, float* keys, q8lin_stream_t stream) {
+  if (int st = kv_shape_fail("kv_block_keys", batch, t, hkv, hkv, d, max_t)) return st;
+  if (int st = block_shape_fail(block)) return st;
+  if (t == 0) return Q8LIN_OK;
+  if (!k_cache || !pos || !keys)
+    return fail(Q8LIN_ERR_INVALID_ARGUMENT, "kv_block_keys pointers must be non-null device pointers");
+  cudaError_t e = launch_kv_block_keys(k_cache, pos, batch, t, hkv, max_t, block, keys,
+                                       reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "kv_block_keys launch");
+  return Q8LIN_OK;
+}
+
+size_t q8lin_attention_blocks_workspace_size(int32_t batch, int32_t t, int32_t hq, int32_t hkv) {
+  if (batch <= 0 || t <= 0 || hq <= 0 || hkv <= 0 || hq % hkv) return 0;
+  return attention_blocks_workspace_bytes(batch, t, hq, hkv);
+}
+
+int q8lin_attention_blocks(const float* q, const float* k_cache, const float* v_cache, const float* keys,
+                           const int32_t* pos, int32_t batch, int32_t t, int32_t hq, int32_t hkv, int32_t d,
+                           int32_t max_t, int32_t block, int32_t topk, void* workspace, size_t workspace_bytes,
+                           int32_t* index, float* out, q8lin_stream_t stream) {
+  if (int st = kv_shape_fail("attention_blocks", batch, t, hq, hkv, d, max_t)) return st;
+  if (int st = block_shape_fail(block)) return st;
+  if (((int64_t)max_t + block - 1) / block > kKvMaxBlocks)
+    return fail(Q8LIN_ERR_SHAPE, "attention_blocks takes at most 16384 blocks");
+  if (topk < 1 || topk > kKvMaxBlocks) return fail(Q8LIN_ERR_SHAPE, "attention_blocks needs 1 <= topk <= 16384");
+  if (t == 0) return Q8LIN_OK;
+  if (!q || !k_cache || !v_cache || !keys || !pos || !workspace || !index || !out)
+    return fail(Q8LIN_ERR_INVALID_ARGUMENT, "attention_blocks pointers must be non-null device pointers");
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(keys) || !aligned16(workspace) ||
+      !aligned16(out))
+    return fail(Q8LIN_ERR_ALIGNMENT, "q, the caches, the keys, the workspace and out must be 16-byte aligned");
+  if (workspace_bytes < attention_blocks_workspace_bytes(batch, t, hq, hkv))
+    return fail(Q8LIN_ERR_WORKSPACE, "workspace too small (see q8lin_attention_blocks_workspace_size)");
+  const int device = current_device();
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e = launch_kv_pick(q, keys, pos, batch, t, hq, hkv, max_t, block, topk, index, device, s);
+  if (e == cudaSuccess)
+    e = launch_attention_blocks(q, k_cache, v_cache, pos, index, batch, t, hq, hkv, max_t, block, topk, workspace, out,
+                                device, s);
+  if (e != cudaSuccess) return cuda_fail(e, "attention_blocks launch");
+  return Q8LIN_OK;
+}
+
 int q8lin_add_rmsnorm(float* x, const float* y, const float* weight, int64_t m, int64_t n, float eps, float* h,
                       q8lin_stream_t stream) {
   if (m < 0 || n <= 0 || m > INT32_MAX) return fail(Q8LIN_ERR_SHAPE, "add_rmsnorm needs 0 <= m < 2^31 and n > 0");

@@ -170,6 +170,35 @@ cudaError_t launch_add_rmsnorm(float* x, const float* y, const float* w, float e
 cudaError_t launch_attention_prefill(const float* q, const float* kc, const float* vc, int batch, int t, int pos0,
                                      int hq, int hkv, int max_t, float* out, int device, cudaStream_t s);
 
+// Attention of several rows per kv head over the f32 caches (kv_attention.cu): trees of drafted
+// tokens, rows that accumulate the keys' softmax weights, rows over chosen blocks.  pos is
+// a device array [batch]; arguments checked by the caller.
+constexpr int kKvMaxTree = 256;
+size_t attention_tree_workspace_bytes(int batch, int n, int hq, int hkv);
+cudaError_t launch_rope_attention_tree(const float* qkv, const int* parents, const int* pos, const float* cos_t,
+                                       const float* sin_t, float* kc, float* vc, int batch, int n, int hq, int hkv,
+                                       int max_t, void* ws, float* out, int device, cudaStream_t s);
+size_t attention_weights_workspace_bytes(int batch, int n, int hq, int hkv, int max_t);
+cudaError_t launch_attention_weights(const float* q, const float* kc, const float* vc, const int* pos, int batch, int n,
+                                     int hq, int hkv, int max_t, float* weight, void* ws, float* out, int device,
+                                     cudaStream_t s);
+size_t attention_blocks_workspace_bytes(int batch, int n, int hq, int hkv);
+cudaError_t launch_attention_blocks(const float* q, const float* kc, const float* vc, const int* pos, const int* index,
+                                    int batch, int n, int hq, int hkv, int max_t, int block, int topk, void* ws,
+                                    float* out, int device, cudaStream_t s);
+
+// Cache upkeep (kv_cache.cu): which rows an eviction keeps, moving rows, block keys and the
+// choice of blocks.
+constexpr int kKvMaxBlocks = 16384;  // block scores of a row sit in shared memory
+cudaError_t launch_kv_evict(const float* weight, const int* length, int batch, int hkv, int max_t, int keep, int sink,
+                            int recent, int* index, float* weight_out, int device, cudaStream_t s);
+cudaError_t launch_kv_move(float* kc, float* vc, const int* index, const int* base, int batch, int hkv, int index_heads,
+                           int max_t, int count, cudaStream_t s);
+cudaError_t launch_kv_block_keys(const float* kc, const int* pos, int batch, int t, int hkv, int max_t, int block,
+                                 float* keys, cudaStream_t s);
+cudaError_t launch_kv_pick(const float* q, const float* keys, const int* pos, int batch, int n, int hq, int hkv,
+                           int max_t, int block, int topk, int* index, int device, cudaStream_t s);
+
 // Persistent decode-step kernel (step.cu).
 constexpr int kStepMaxK = 8192;
 enum StepOpKind { kStepOpGemv = 0, kStepOpAttention = 1, kStepOpEmbed = 2, kStepOpArgmax = 3 };

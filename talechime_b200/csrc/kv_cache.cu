@@ -1,0 +1,353 @@
+// Upkeep of the f32 KV cache around the attention kernels: which rows an eviction keeps,
+// moving kept rows together in place, the mean key of every block, and the blocks a query
+// row attends over.
+//
+// Selection: the k largest of n values, equal values by the lower index, without sorting:
+// the value of rank k digit by digit (8 bits at a time from the top, a 256-bin count per
+// digit), then one ordered pass that emits the indices.  Floats compare as unsigned
+// integers after flipping the sign bit (negative: all bits); -0 equals +0; NaN is lowest.
+#include <cmath>
+
+#include "common.cuh"
+#include "internal.h"
+
+namespace q8lin {
+
+namespace {
+
+constexpr int kKvD = 128;
+
+__device__ __forceinline__ uint32_t order_key(float x) {
+  if (x != x) return 0u;
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ unsigned long long order_key(double x) {
+  if (x != x) return 0ull;
+  const unsigned long long u = (unsigned long long)__double_as_longlong(x + 0.0);
+  return u >> 63 ? ~u : u | 0x8000000000000000ull;
+}
+
+struct SelectSmem {
+  unsigned hist[256];
+  unsigned digit, above, bin;
+  unsigned warp[32][2];
+};
+
+// Rank-k threshold of key(0..n): keys with (key & mask) > prefix are chosen, and the first
+// `ties` of those with (key & mask) == prefix.  1 <= k <= n.  Every thread of the CTA calls it.
+template <typename U, typename F>
+__device__ void select_threshold(F key, int n, int k, SelectSmem& sm, U& prefix, U& mask, int& ties) {
+  const int tid = threadIdx.x;
+  prefix = 0;
+  mask = 0;
+  int need = k;
+  for (int shift = (int)sizeof(U) * 8 - 8; shift >= 0; shift -= 8) {
+    for (int i = tid; i < 256; i += blockDim.x) sm.hist[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += blockDim.x) {
+      const U v = key(i);
+      if ((v & mask) == prefix) atomicAdd(&sm.hist[(unsigned)(v >> shift) & 255u], 1u);
+    }
+    __syncthreads();
+    if (tid < 32) {  // lane l: digits 255 - 8l down to 248 - 8l
+      unsigned c[8], sum = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        c[e] = sm.hist[255 - 8 * tid - e];
+        sum += c[e];
+      }
+      unsigned upto = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned v = __shfl_up_sync(kFull, upto, o);
+        if (tid >= o) upto += v;
+      }
+      unsigned at = upto - sum;
+      if (at < (unsigned)need && (unsigned)need <= upto) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (at < (unsigned)need && (unsigned)need <= at + c[e]) {
+            sm.digit = 255 - 8 * tid - e;
+            sm.above = at;
+            sm.bin = c[e];
+          }
+          at += c[e];
+        }
+      }
+    }
+    __syncthreads();
+    prefix |= (U)sm.digit << shift;
+    mask |= (U)255 << shift;
+    need -= (int)sm.above;
+    const bool all = sm.bin == (unsigned)need;  // the whole digit is chosen: no need to go on
+    __syncthreads();
+    if (all) break;
+  }
+  ties = need;
+}
+
+// Calls emit(rank, i) for the chosen of key(0..n) in ascending i.  Every thread calls it.
+template <typename U, typename F, typename E>
+__device__ void select_emit(F key, int n, U prefix, U mask, int ties, SelectSmem& sm, E emit) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  const int per = (n + (int)blockDim.x - 1) / (int)blockDim.x;
+  const int i0 = min(n, tid * per), i1 = min(n, i0 + per);
+  unsigned more = 0, same = 0;
+  for (int i = i0; i < i1; ++i) {
+    const U v = key(i) & mask;
+    more += v > prefix;
+    same += v == prefix;
+  }
+  unsigned um = more, us = same;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned a = __shfl_up_sync(kFull, um, o), b = __shfl_up_sync(kFull, us, o);
+    if (lane >= o) {
+      um += a;
+      us += b;
+    }
+  }
+  if (lane == 31) {
+    sm.warp[warp][0] = um;
+    sm.warp[warp][1] = us;
+  }
+  __syncthreads();
+  unsigned bm = um - more, bs = us - same;  // chosen for certain, and equal ones, before i0
+  for (int w = 0; w < warps; ++w)
+    if (w < warp) {
+      bm += sm.warp[w][0];
+      bs += sm.warp[w][1];
+    }
+  for (int i = i0; i < i1; ++i) {
+    const U v = key(i) & mask;
+    const bool tie = v == prefix;
+    if (v > prefix || (tie && bs < (unsigned)ties)) emit((int)(bm + min(bs, (unsigned)ties)), i);
+    bm += v > prefix;
+    bs += tie;
+  }
+  __syncthreads();
+}
+
+// One CTA per (sequence, kv head): the rows an eviction keeps, ascending, and the weights
+// of the kept rows.  Keys come from shared memory where the row of weights fits.
+constexpr int kEvictThreads = 1024;
+constexpr int kEvictSmemRows = 49152;
+__global__ void __launch_bounds__(kEvictThreads)
+kv_evict_kernel(const float* weight, const int* __restrict__ length, int hkv, int max_t, int keep, int sink,
+                int recent, int staged, int* __restrict__ index, float* weight_out) {
+  extern __shared__ uint32_t ev_keys[];
+  __shared__ SelectSmem sm;
+  const int tid = threadIdx.x;
+  pdl_launch_dependents();
+  pdl_wait();
+  const size_t bh = blockIdx.x;
+  const int len = min(max(length[bh / hkv], 0), max_t);
+  const float* w = weight + bh * (size_t)max_t;
+  int* idx = index + bh * (size_t)keep;
+  const int kept = min(len, keep);
+  if (len <= keep) {
+    for (int i = tid; i < keep; i += kEvictThreads) idx[i] = i < len ? i : -1;
+  } else {
+    const int n = len - sink - recent, k = keep - sink - recent;
+    for (int i = tid; i < sink; i += kEvictThreads) idx[i] = i;
+    for (int i = tid; i < recent; i += kEvictThreads) idx[keep - recent + i] = len - recent + i;
+    if (k > 0) {
+      if (staged)
+        for (int i = tid; i < n; i += kEvictThreads) ev_keys[i] = order_key(w[sink + i]);
+      __syncthreads();
+      auto key = [&](int i) { return staged ? ev_keys[i] : order_key(w[sink + i]); };
+      uint32_t prefix, mask;
+      int ties;
+      select_threshold<uint32_t>(key, n, k, sm, prefix, mask, ties);
+      select_emit<uint32_t>(key, n, prefix, mask, ties, sm, [&](int rank, int i) { idx[sink + rank] = sink + i; });
+    }
+  }
+  if (!weight_out) return;
+  __syncthreads();  // the indices of the CTA are written
+  // weight_out may be weight: a row moves to a lower or the same place, so a group of rows is
+  // read before any of it is written, and nothing behind it is
+  float* wo = weight_out + bh * (size_t)max_t;
+  for (int c = 0; c < kept; c += kEvictThreads) {
+    const int i = c + tid;
+    const float v = i < kept ? w[idx[i]] : 0.0f;
+    __syncthreads();
+    if (i < kept) wo[i] = v;
+  }
+  __syncthreads();
+  for (int i = kept + tid; i < max_t; i += kEvictThreads) wo[i] = 0.0f;
+}
+
+// Row base + i of a cache head <- row base + index[i] for ascending indices, index[i] >= i,
+// in place.  A row moves down, so rows are taken in ascending groups: a group is read whole
+// before any of it is written, and later groups read only rows behind it.  A CTA owns a slice of
+// `lanes` 16-byte pieces of the rows of one head of one cache, so no two CTAs meet.
+constexpr int kMoveThreads = 256;
+constexpr int kMoveDepth = 8;
+__global__ void __launch_bounds__(kMoveThreads)
+kv_move_kernel(float* __restrict__ kc, float* __restrict__ vc, const int* __restrict__ index,
+               const int* __restrict__ base_dev, int hkv, int index_heads, int max_t, int count, int lanes) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int bh = blockIdx.y, b = bh / hkv, h = bh - b * hkv;
+  const int slices = 32 / lanes;
+  const int slice = blockIdx.x % slices;
+  const int base = base_dev ? base_dev[b] : 0;
+  if (base < 0 || base >= max_t) return;
+  float4* cache = reinterpret_cast<float4*>((blockIdx.x / slices ? vc : kc) + (size_t)bh * max_t * kKvD) +
+                  (size_t)base * (kKvD / 4);
+  const int limit = max_t - base;
+  const int* idx = index + ((size_t)b * index_heads + (index_heads == 1 ? 0 : h)) * (size_t)count;
+  const int piece = slice * lanes + threadIdx.x % lanes, r0 = threadIdx.x / lanes, step = kMoveThreads / lanes;
+  for (int c = 0; c < count; c += step * kMoveDepth) {
+    float4 v[kMoveDepth];
+    bool move[kMoveDepth];
+#pragma unroll
+    for (int d = 0; d < kMoveDepth; ++d) {
+      const int i = c + d * step + r0;
+      const int from = i < count ? idx[i] : -1;
+      move[d] = from > i && from < limit;
+      if (move[d]) v[d] = cache[(size_t)from * (kKvD / 4) + piece];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int d = 0; d < kMoveDepth; ++d)
+      if (move[d]) cache[(size_t)(c + d * step + r0) * (kKvD / 4) + piece] = v[d];
+  }
+}
+
+// Mean key of every block that rows [pos, pos + t) complete: f64 sum in row order, rounded
+// once.  grid (blocks that t rows can complete, batch * hkv), one thread per dimension.
+__global__ void __launch_bounds__(kKvD)
+kv_block_keys_kernel(const float* __restrict__ kc, const int* __restrict__ pos_dev, int t, int hkv, int max_t, int block,
+                     int blocks, float* __restrict__ keys) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int bh = blockIdx.y, pos = pos_dev[bh / hkv];
+  if (pos < 0 || pos >= max_t) return;
+  const int end = min((int64_t)pos + t, (int64_t)max_t);
+  const int c = pos / block + blockIdx.x;
+  if ((int64_t)(c + 1) * block > end || c >= blocks) return;
+  const float* k = kc + ((size_t)bh * max_t + (size_t)c * block) * kKvD + threadIdx.x;
+  double s = 0.0;
+#pragma unroll 8
+  for (int r = 0; r < block; ++r) s += (double)k[(size_t)r * kKvD];
+  keys[((size_t)bh * blocks + c) * kKvD + threadIdx.x] = (float)(s / block);
+}
+
+// The blocks a query row attends over besides its own: one CTA per (sequence, token, kv
+// head).  Score of block c: sum over the heads of the group and the dimensions of q times
+// the block's mean key, in f64, so the choice does not hang on the order of the sums.
+constexpr int kPickThreads = 256;
+__global__ void __launch_bounds__(kPickThreads)
+kv_pick_kernel(const float* __restrict__ q, const float* __restrict__ keys, const int* __restrict__ pos_dev, int n, int hq,
+               int hkv, int max_t, int block, int blocks, int topk, int* __restrict__ index) {
+  extern __shared__ unsigned long long pk_keys[];
+  __shared__ SelectSmem sm;
+  __shared__ double qs[kKvD];
+  const int tid = threadIdx.x;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int hk = blockIdx.x % hkv, row = blockIdx.x / hkv, b = row / n, i = row - b * n;
+  const int group = hq / hkv, p = pos_dev[b];
+  int* idx = index + (size_t)blockIdx.x * topk;
+  const int past = p >= 0 && p < max_t - i ? min((p + i) / block, blocks) : 0;
+  if (past <= topk) {
+    for (int e = tid; e < topk; e += kPickThreads) idx[e] = e < past ? e : -1;
+    return;
+  }
+  if (tid < kKvD) {
+    double s = 0.0;
+    for (int h = 0; h < group; ++h) s += (double)q[((size_t)row * hq + hk * group + h) * kKvD + tid];
+    qs[tid] = s;
+  }
+  __syncthreads();
+  const float4* kb = reinterpret_cast<const float4*>(keys + ((size_t)b * hkv + hk) * blocks * kKvD);
+  const int l8 = tid & 7;
+  for (int c0 = 0; c0 < past; c0 += kPickThreads / 8) {
+    const int c = c0 + (tid >> 3);
+    double s = 0.0;
+    if (c < past) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const float4 k4 = kb[(size_t)c * 32 + m * 8 + l8];
+        const double* qd = qs + (m * 8 + l8) * 4;
+        s = fma(qd[0], (double)k4.x, s);
+        s = fma(qd[1], (double)k4.y, s);
+        s = fma(qd[2], (double)k4.z, s);
+        s = fma(qd[3], (double)k4.w, s);
+      }
+    }
+    s += __shfl_xor_sync(kFull, s, 1);
+    s += __shfl_xor_sync(kFull, s, 2);
+    s += __shfl_xor_sync(kFull, s, 4);
+    if (c < past && l8 == 0) pk_keys[c] = order_key(s);
+  }
+  __syncthreads();
+  auto key = [&](int c) { return pk_keys[c]; };
+  unsigned long long prefix, mask;
+  int ties;
+  select_threshold<unsigned long long>(key, past, topk, sm, prefix, mask, ties);
+  select_emit<unsigned long long>(key, past, prefix, mask, ties, sm, [&](int rank, int c) { idx[rank] = c; });
+}
+
+cudaLaunchConfig_t kc_cfg(dim3 grid, dim3 block, size_t smem, cudaStream_t s, cudaLaunchAttribute* attr) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  return cfg;
+}
+
+}  // namespace
+
+cudaError_t launch_kv_evict(const float* weight, const int* length, int batch, int hkv, int max_t, int keep, int sink,
+                            int recent, int* index, float* weight_out, int device, cudaStream_t s) {
+  const bool staged = max_t <= kEvictSmemRows;
+  const size_t smem = staged ? (size_t)max_t * 4 : 0;
+  static int configured[128] = {0};
+  cudaError_t e =
+      ensure_smem((const void*)kv_evict_kernel, configured, device, (size_t)kEvictSmemRows * 4, false);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg = kc_cfg(dim3((unsigned)(batch * hkv)), dim3(kEvictThreads), smem, s, attr);
+  return cudaLaunchKernelEx(&cfg, kv_evict_kernel, weight, length, hkv, max_t, keep, sink, recent, staged ? 1 : 0, index,
+                            weight_out);
+}
+
+cudaError_t launch_kv_move(float* kc, float* vc, const int* index, const int* base, int batch, int hkv, int index_heads,
+                           int max_t, int count, cudaStream_t s) {
+  // slices of 128 bytes, or of 32 (a DRAM sector) where the heads alone leave SMs idle
+  const int lanes = batch * hkv * 2 * 4 >= 296 ? 8 : 2;
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg =
+      kc_cfg(dim3((unsigned)(2 * 32 / lanes), (unsigned)(batch * hkv)), dim3(kMoveThreads), 0, s, attr);
+  return cudaLaunchKernelEx(&cfg, kv_move_kernel, kc, vc, index, base, hkv, index_heads, max_t, count, lanes);
+}
+
+cudaError_t launch_kv_block_keys(const float* kc, const int* pos, int batch, int t, int hkv, int max_t, int block,
+                                 float* keys, cudaStream_t s) {
+  const int blocks = (max_t + block - 1) / block;
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg =
+      kc_cfg(dim3((unsigned)(t / block + 1), (unsigned)(batch * hkv)), dim3(kKvD), 0, s, attr);
+  return cudaLaunchKernelEx(&cfg, kv_block_keys_kernel, kc, pos, t, hkv, max_t, block, blocks, keys);
+}
+
+cudaError_t launch_kv_pick(const float* q, const float* keys, const int* pos, int batch, int n, int hq, int hkv,
+                           int max_t, int block, int topk, int* index, int device, cudaStream_t s) {
+  const int blocks = (max_t + block - 1) / block;
+  static int configured[128] = {0};
+  cudaError_t e = ensure_smem((const void*)kv_pick_kernel, configured, device, (size_t)kKvMaxBlocks * 8, false);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg = kc_cfg(dim3((unsigned)((int64_t)batch * n * hkv)), dim3(kPickThreads), (size_t)blocks * 8, s, attr);
+  return cudaLaunchKernelEx(&cfg, kv_pick_kernel, q, keys, pos, n, hq, hkv, max_t, block, blocks, topk, index);
+}
+
+}  // namespace q8lin
