@@ -756,7 +756,7 @@ int kv_shape_fail(const char* what, int64_t batch, int64_t rows, int64_t hq, int
   if (hq <= 0 || hkv <= 0 || hq % hkv || hq > 65535)
     return fail(Q8LIN_ERR_SHAPE, std::string(what) + " needs hq a positive multiple of hkv, hq <= 65535");
   if (batch <= 0 || rows < 0 || max_t <= 0 || batch * hkv > 65535 || rows > (1 << 20) ||
-      batch * rows * hq > (INT64_C(1) << 30) || max_t > (1 << 30))
+      batch * rows * hq > (INT64_C(1) << 30) || max_t > (1 << 24))
     return fail(Q8LIN_ERR_SHAPE, std::string(what) + ": batch, rows or max_t out of range");
   if (rows > max_t) return fail(Q8LIN_ERR_SHAPE, std::string(what) + ": more rows than the cache holds (context limit)");
   return Q8LIN_OK;

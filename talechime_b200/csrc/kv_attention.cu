@@ -8,7 +8,7 @@
 //
 // Rows: sequence b has n new rows at positions pos[b] + i (pos in device memory).  The
 // `group` query heads of one kv head read the same keys, so the rows of a kv head are
-// numbered r = i * group + head-in-group and taken 16 at a time (a unit).
+// numbered r = i * group + head-in-group and taken 8 or 16 at a time (a unit).
 //
 // Products: f32 operands as tf32 pairs on the tensor cores (mma.sync m16n8k8).  x = hi + lo
 // with hi = x rounded to tf32's 11 significant bits and lo = x - hi (exact) rounded again, and
@@ -24,13 +24,14 @@ namespace q8lin {
 namespace {
 
 constexpr int kKvD = 128;       // head width
-constexpr int kKvRows = 16;     // query rows of a unit
+constexpr int kKvMaxRows = 16;  // query rows of a unit: 8 or 16
 constexpr int kKvChunk = 16;    // keys of a chunk: one warp's step
-constexpr int kKvWarps = 4;
+constexpr int kKvWarps = 8;
 constexpr int kKvThreads = kKvWarps * 32;
-constexpr int kKvStages = 2;    // chunks per warp in flight or in use
+constexpr int kKvSlots = 3;     // half chunks (16 keys or 16 values) of a warp's ring
+constexpr int kKvHalf = kKvChunk * kKvD * 4;
 constexpr int kKvGrid = 148;    // CTAs that share the chunks of all units (one per SM)
-constexpr int kKvSlotFloats = kKvRows * kKvD;
+constexpr int kKvSlotFloats = kKvMaxRows * kKvD;
 
 enum KvMask : int { kMaskCausal = 0, kMaskTree = 1, kMaskBlocks = 2 };
 
@@ -48,7 +49,8 @@ struct KvArgs {
   float* lse;             // causal with weights, else: [batch][hkv][n * group] log2 of the row's sum
   int batch, n, hq, hkv, group, max_t;
   int words, topk, block, score_stride;
-  int rgs;                // row groups of a kv head (tree, causal) or of a row (blocks)
+  int rows;               // rows of a unit: 8 or 16
+  int rgs;                // row groups of a kv head (tree, causal) or of a token (blocks)
   int units;
   int split;              // 1: kKvGrid CTAs share all chunks evenly; 0: one CTA per unit
   float c;                // log2(e) * f32(1/sqrt(128))
@@ -69,14 +71,14 @@ __device__ __forceinline__ KvUnit kv_unit(const KvArgs& a, int u) {
   KvUnit x;
   const int rg = u % a.rgs;
   const int w = u / a.rgs;
-  x.r0 = rg * kKvRows;
+  x.r0 = rg * a.rows;
   x.picked = 0;
   if (MASK == kMaskBlocks) {
     x.hk = w % a.hkv;
     const int row = w / a.hkv;
     x.b = row / a.n;
     x.i0 = row - x.b * a.n;
-    x.nrows = min(kKvRows, a.group - x.r0);
+    x.nrows = min(a.rows, a.group - x.r0);
     x.p = a.pos[x.b];
     const bool ok = x.p >= 0 && x.p < a.max_t - x.i0;
     const int at = x.p + x.i0;
@@ -86,7 +88,7 @@ __device__ __forceinline__ KvUnit kv_unit(const KvArgs& a, int u) {
   } else {
     x.hk = w % a.hkv;
     x.b = w / a.hkv;
-    x.nrows = min(kKvRows, a.n * a.group - x.r0);
+    x.nrows = min(a.rows, a.n * a.group - x.r0);
     x.i0 = x.r0 / a.group;
     x.p = a.pos[x.b];
     const int last = (x.r0 + x.nrows - 1) / a.group;
@@ -143,7 +145,7 @@ __device__ __forceinline__ bool kv_sees(const KvArgs& a, const KvUnit& x, int r,
 
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t a0, const uint32_t a1, const uint32_t a2,
                                          const uint32_t a3, const uint32_t b0, const uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -162,22 +164,24 @@ __device__ __forceinline__ float4 lds_f4(uint32_t addr) {
   return v;
 }
 
+template <int NT>
 struct KvSmem {
-  // the unit's query rows as MMA fragments: [hi, lo][pair of k-steps][rows g, rows g + 8][lane]
-  alignas(16) float4 q[2][8][2][32];
-  alignas(16) float k[kKvWarps][kKvStages][kKvChunk][kKvD];
-  alignas(16) float v[kKvWarps][kKvStages][kKvChunk][kKvD];
-  alignas(16) float o[kKvWarps][kKvRows][kKvD + 4];
-  float m[kKvWarps][kKvRows], l[kKvWarps][kKvRows];
-  int ok[kKvRows];
+  // each warp's ring of half chunks; after a unit's last chunk its output part [row][132]
+  alignas(16) uint8_t ring[kKvWarps][kKvSlots][kKvHalf];
+  // the unit's query rows as MMA fragments: [hi, lo][16 dimensions][8 rows][lane]
+  alignas(16) float4 q[2][8][NT][32];
+  alignas(16) float p[kKvWarps][NT][kKvChunk][8];  // a chunk's probabilities
+  float m[kKvWarps][8 * NT], l[kKvWarps][8 * NT];
+  float f[kKvWarps][8 * NT];
+  float M[8 * NT], L[8 * NT];
   int seg[kKvWarps];
   int unit, off;
 };
 
 // Where CTA `cta` of the shared split starts: fills sm.unit / sm.off and returns the chunk
 // count of one CTA (the whole work when it does not reach this CTA: unit = units).
-template <int MASK>
-__device__ int kv_find(const KvArgs& a, KvSmem& sm, int cta) {
+template <int MASK, int NT>
+__device__ int kv_find(const KvArgs& a, KvSmem<NT>& sm, int cta) {
   const int tid = threadIdx.x;
   const int per = (a.units + kKvThreads - 1) / kKvThreads;
   const int u0 = min(a.units, tid * per), u1 = min(a.units, u0 + per);
@@ -219,10 +223,17 @@ __device__ int kv_find(const KvArgs& a, KvSmem& sm, int cta) {
   return quota;
 }
 
-template <int MASK, bool SCORES>
+// The rows are the N side of the products and the keys, then the dimensions, the M side, so
+// that 8 rows fill a tile: S^T = K Q^T and O^T = V^T P^T.  In an m16n8k8 fragment lane 4g + t
+// holds rows g and g + 8 of A, column g of B, and columns 2t, 2t + 1 of the result.
+//
+// What bounds it: with up to 16 rows a kv head the cache's bytes, read once; the tf32 split of
+// every key and value (4 operations each) and the products run beside the copies.
+template <int MASK, bool SCORES, int NT>
 __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArgs a) {
   extern __shared__ __align__(16) uint8_t kv_smem[];
-  KvSmem& sm = *reinterpret_cast<KvSmem*>(kv_smem);
+  KvSmem<NT>& sm = *reinterpret_cast<KvSmem<NT>*>(kv_smem);
+  constexpr int R = 8 * NT;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
   pdl_wait();
@@ -230,7 +241,7 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArg
 
   int u, off, left;
   if (a.split) {
-    left = kv_find<MASK>(a, sm, blockIdx.x);
+    left = kv_find<MASK, NT>(a, sm, blockIdx.x);
     u = sm.unit;
     off = sm.off;
   } else {
@@ -238,9 +249,7 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArg
     off = 0;
     left = 0x7fffffff;
   }
-  const uint32_t ks = (uint32_t)__cvta_generic_to_shared(&sm.k[warp][0][0][0]);
-  const uint32_t vs = (uint32_t)__cvta_generic_to_shared(&sm.v[warp][0][0][0]);
-  constexpr uint32_t kStage = kKvChunk * kKvD * 4;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(&sm.ring[warp][0][0]);
 
   while (u < a.units && left > 0) {
     const KvUnit x = kv_unit<MASK>(a, u);
@@ -248,33 +257,43 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArg
     const float* kb = a.k + ((size_t)x.b * a.hkv + x.hk) * (size_t)a.max_t * kKvD;
     const float* vb = a.v + ((size_t)x.b * a.hkv + x.hk) * (size_t)a.max_t * kKvD;
 
-    // this warp's chunks: off + warp, off + warp + 4, ...
-    auto load = [&](int c, int stage) {
-      const int j0 = kv_chunk_key<MASK>(a, x, c);
+    // this warp's chunks: off + warp, off + warp + 8, ...  Half h of its stream: the keys
+    // (h even) or values of its chunk h / 2, copied into ring slot h % 3.
+    const int c0 = off + warp;
+    const int halves = c0 < c1 ? 2 * ((c1 - c0 + kKvWarps - 1) / kKvWarps) : 0;
+    auto load = [&](int h, int slot) {
+      if (h < halves) {
+        const int j0 = kv_chunk_key<MASK>(a, x, c0 + (h >> 1) * kKvWarps);
+        const bool val = h & 1;
+        const float* src = (val ? vb : kb) + (size_t)j0 * kKvD + lane * 4;
+        const uint32_t dst = ring + slot * kKvHalf;
+        const bool plain = j0 + kKvChunk <= (MASK == kMaskTree ? x.p : x.keys);
+        if (plain) {
 #pragma unroll
-      for (int r = 0; r < kKvChunk; ++r) {
-        const int j = j0 + r;
-        bool there = j < x.keys;
-        if (MASK == kMaskTree && j >= x.p) {
-          const int e = j - x.p;  // a row no node was written to must not reach the sums
-          there = there && e < a.n && ((a.anc[((size_t)x.b * a.n + e) * a.words + (e >> 5)] >> (e & 31)) & 1u);
+          for (int r = 0; r < kKvChunk; ++r)
+            cp_async16(dst + r * (kKvD * 4) + ((lane ^ (val ? (r & 3) << 1 : (r & 1) << 2)) << 4), src + r * kKvD);
+        } else {
+#pragma unroll 4
+          for (int r = 0; r < kKvChunk; ++r) {
+            const int j = j0 + r;
+            bool there = j < x.keys;
+            if (MASK == kMaskTree && j >= x.p) {
+              const int e = j - x.p;  // a row no node was written to must not reach the sums
+              there = there && e < a.n && ((a.anc[((size_t)x.b * a.n + e) * a.words + (e >> 5)] >> (e & 31)) & 1u);
+            }
+            cp_async16_zfill(dst + r * (kKvD * 4) + ((lane ^ (val ? (r & 3) << 1 : (r & 1) << 2)) << 4),
+                             there ? src + r * kKvD : kb, there);
+          }
         }
-        const size_t o = (size_t)(there ? j : 0) * kKvD + lane * 4;
-        const uint32_t row = stage * kStage + r * (kKvD * 4);
-        cp_async16_zfill(ks + row + ((lane ^ ((r & 1) << 2)) << 4), kb + o, there);
-        cp_async16_zfill(vs + row + ((lane ^ (((r >> 1) & 3) << 1)) << 4), vb + o, there);
       }
-    };
-    int c = off + warp;
-#pragma unroll
-    for (int s = 0; s < kKvStages; ++s) {
-      if (c + s * kKvWarps < c1) load(c + s * kKvWarps, s);
       cp_async_commit();
-    }
+    };
+#pragma unroll
+    for (int h = 0; h < kKvSlots; ++h) load(h, h);
     // query rows -> fragments
-    for (int e = tid; e < 8 * 2 * 32; e += kKvThreads) {
-      const int ln = e & 31, half = (e >> 5) & 1, pair = e >> 6;
-      const int r = (ln >> 2) + 8 * half;
+    for (int e = tid; e < 8 * NT * 32; e += kKvThreads) {
+      const int ln = e & 31, nt = (e >> 5) % NT, pair = (e >> 5) / NT;
+      const int r = (ln >> 2) + 8 * nt;
       float4 qv = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < x.nrows)
         qv = *reinterpret_cast<const float4*>(a.q + kv_row_offset<MASK>(a, x, r) + pair * 16 + (ln & 3) * 4);
@@ -283,112 +302,119 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArg
       split_tf32(qv.y, h.y, w.y);
       split_tf32(qv.z, h.z, w.z);
       split_tf32(qv.w, h.w, w.w);
-      *reinterpret_cast<uint4*>(&sm.q[0][pair][half][ln]) = h;
-      *reinterpret_cast<uint4*>(&sm.q[1][pair][half][ln]) = w;
+      *reinterpret_cast<uint4*>(&sm.q[0][pair][nt][ln]) = h;
+      *reinterpret_cast<uint4*>(&sm.q[1][pair][nt][ln]) = w;
     }
     __syncthreads();
 
     // the first key some row of the unit does not see (chunks below it need no mask)
     const int open = MASK == kMaskTree ? x.p : MASK == kMaskCausal ? x.p + x.i0 + 1 : x.keys;
-    float o[16][4];
+    float o[NT][8][4];
+    float m[NT][2], l[NT][2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.0f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.0f;
+    }
 
-    for (int it = 0; c < c1; c += kKvWarps, ++it) {
-      const int stage = it & (kKvStages - 1);
-      cp_async_wait(kKvStages - 1);
+    int slot = 0;
+    for (int h = 0; h < halves; h += 2) {
+      const int j0 = kv_chunk_key<MASK>(a, x, c0 + (h >> 1) * kKvWarps);
+      cp_async_wait(2);
       __syncwarp();
-      const uint32_t kst = ks + stage * kStage, vst = vs + stage * kStage;
-      const int j0 = kv_chunk_key<MASK>(a, x, c);
-      // scores: a lane takes dimensions 16 pair + 4 t + e of key 8 nt + g.  The tensor cores
-      // cut their f32 sums instead of rounding them, one cut per step: hi.hi runs in chains
-      // of four steps, summed here with rounding; the cross terms are 2^-11 of it and run on.
-      float s[2][4], cross[2][2][4];
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = cross[nt][0][e] = cross[nt][1][e] = 0.0f;
+      // Scores: a lane takes dimensions 16 pair + 4t + e of keys g and g + 8.  The tensor cores
+      // cut their f32 sums instead of rounding them, one cut per step: hi.hi runs in chains of
+      // four steps, summed here with rounding; the cross terms are 2^-11 of it.
+      const uint32_t kst = ring + slot * kKvHalf;
+      float hh[NT][4][4], cross[NT][4][4];
 #pragma unroll
       for (int quad = 0; quad < 4; ++quad) {
-        float h4[2][4];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) h4[nt][e] = 0.0f;
+          for (int e = 0; e < 4; ++e) hh[nt][quad][e] = cross[nt][quad][e] = 0.0f;
 #pragma unroll
         for (int pair = 2 * quad; pair < 2 * quad + 2; ++pair) {
-          const uint4 hg = *reinterpret_cast<const uint4*>(&sm.q[0][pair][0][lane]);
-          const uint4 hh = *reinterpret_cast<const uint4*>(&sm.q[0][pair][1][lane]);
-          const uint4 lg = *reinterpret_cast<const uint4*>(&sm.q[1][pair][0][lane]);
-          const uint4 lh = *reinterpret_cast<const uint4*>(&sm.q[1][pair][1][lane]);
+          const uint32_t at = kst + g * (kKvD * 4) + (((pair * 4 + t) ^ ((g & 1) << 2)) << 4);
+          const float4 ka = lds_f4(at), kb4 = lds_f4(at + 8 * kKvD * 4);
+          uint32_t ah[4], al[4], bh[4], bl[4];
+          split_tf32(ka.x, ah[0], al[0]);
+          split_tf32(ka.y, ah[1], al[1]);
+          split_tf32(ka.z, ah[2], al[2]);
+          split_tf32(ka.w, ah[3], al[3]);
+          split_tf32(kb4.x, bh[0], bl[0]);
+          split_tf32(kb4.y, bh[1], bl[1]);
+          split_tf32(kb4.z, bh[2], bl[2]);
+          split_tf32(kb4.w, bh[3], bl[3]);
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
-            const int r = nt * 8 + g;
-            const float4 kv = lds_f4(kst + r * (kKvD * 4) + (((pair * 4 + t) ^ ((r & 1) << 2)) << 4));
-            uint32_t h0, h1, h2, h3, w0, w1, w2, w3;
-            split_tf32(kv.x, h0, w0);
-            split_tf32(kv.y, h1, w1);
-            split_tf32(kv.z, h2, w2);
-            split_tf32(kv.w, h3, w3);
-            mma_tf32(h4[nt], hg.x, hh.x, hg.y, hh.y, h0, h1);
-            mma_tf32(cross[nt][0], lg.x, lh.x, lg.y, lh.y, h0, h1);
-            mma_tf32(cross[nt][1], hg.x, hh.x, hg.y, hh.y, w0, w1);
-            mma_tf32(h4[nt], hg.z, hh.z, hg.w, hh.w, h2, h3);
-            mma_tf32(cross[nt][0], lg.z, lh.z, lg.w, lh.w, h2, h3);
-            mma_tf32(cross[nt][1], hg.z, hh.z, hg.w, hh.w, w2, w3);
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint4 qh = *reinterpret_cast<const uint4*>(&sm.q[0][pair][nt][lane]);
+            const uint4 ql = *reinterpret_cast<const uint4*>(&sm.q[1][pair][nt][lane]);
+            mma_tf32(hh[nt][quad], ah[0], bh[0], ah[1], bh[1], qh.x, qh.y);
+            mma_tf32(cross[nt][quad], al[0], bl[0], al[1], bl[1], qh.x, qh.y);
+            mma_tf32(hh[nt][quad], ah[2], bh[2], ah[3], bh[3], qh.z, qh.w);
+            mma_tf32(cross[nt][quad], ah[0], bh[0], ah[1], bh[1], ql.x, ql.y);
+            mma_tf32(cross[nt][quad], al[2], bl[2], al[3], bl[3], qh.z, qh.w);
+            mma_tf32(cross[nt][quad], ah[2], bh[2], ah[3], bh[3], ql.z, ql.w);
           }
         }
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][e] += h4[nt][e];
       }
-      float p[2][4];
+      __syncwarp();
+      load(h + 3, slot);  // the keys are in registers: their slot is free
+      slot = slot == kKvSlots - 1 ? 0 : slot + 1;
+
       const bool masked = j0 + kKvChunk > open;
+      float fac[NT][2];
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        float p[4];  // [key g, g + 8][row 2t, 2t + 1] of the n-tile
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          p[nt][e] = __fmul_rn(__fadd_rn(s[nt][e], __fadd_rn(cross[nt][0][e], cross[nt][1][e])), a.c);
+          const float big = __fadd_rn(__fadd_rn(hh[nt][0][e], hh[nt][1][e]), __fadd_rn(hh[nt][2][e], hh[nt][3][e]));
+          const float low =
+              __fadd_rn(__fadd_rn(cross[nt][0][e], cross[nt][1][e]), __fadd_rn(cross[nt][2][e], cross[nt][3][e]));
+          p[e] = __fmul_rn(__fadd_rn(big, low), a.c);
           if (masked) {
-            const int j = j0 + nt * 8 + 2 * t + (e & 1);
-            if (j >= x.keys || !kv_sees<MASK>(a, x, g + (e >> 1) * 8, j)) p[nt][e] = -INFINITY;
+            const int j = j0 + g + (e >> 1) * 8;
+            if (j >= x.keys || !kv_sees<MASK>(a, x, nt * 8 + 2 * t + (e & 1), j)) p[e] = -INFINITY;
           }
         }
-      if (SCORES) {
-        float* sc = a.scores + ((size_t)x.b * a.hkv + x.hk) * x.nrows * (size_t)a.score_stride + j0 + 2 * t;
+        if (SCORES) {
+          float* sc = a.scores + ((size_t)x.b * a.hkv + x.hk) * x.nrows * (size_t)a.score_stride + j0 + g;
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          if (g < x.nrows)
-            *reinterpret_cast<float2*>(sc + (size_t)g * a.score_stride + nt * 8) = make_float2(p[nt][0], p[nt][1]);
-          if (g + 8 < x.nrows)
-            *reinterpret_cast<float2*>(sc + (size_t)(g + 8) * a.score_stride + nt * 8) =
-                make_float2(p[nt][2], p[nt][3]);
+          for (int e = 0; e < 4; ++e) {
+            const int r = nt * 8 + 2 * t + (e & 1);
+            if (r < x.nrows) sc[(size_t)r * a.score_stride + (e >> 1) * 8] = p[e];
+          }
         }
-      }
-      float x0 = fmaxf(fmaxf(p[0][0], p[0][1]), fmaxf(p[1][0], p[1][1]));
-      float x1 = fmaxf(fmaxf(p[0][2], p[0][3]), fmaxf(p[1][2], p[1][3]));
-      x0 = fmaxf(x0, __shfl_xor_sync(kFull, x0, 1));
-      x1 = fmaxf(x1, __shfl_xor_sync(kFull, x1, 1));
-      x0 = fmaxf(x0, __shfl_xor_sync(kFull, x0, 2));
-      x1 = fmaxf(x1, __shfl_xor_sync(kFull, x1, 2));
-      const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-      const float b0 = n0 == -INFINITY ? 0.0f : n0, b1 = n1 == -INFINITY ? 0.0f : n1;
-      const float f0 = exp2f(m0 - b0), f1 = exp2f(m1 - b1);
-      m0 = n0;
-      m1 = n1;
+        float x0 = fmaxf(p[0], p[2]), x1 = fmaxf(p[1], p[3]);
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        p[nt][0] = exp2f(p[nt][0] - b0);
-        p[nt][1] = exp2f(p[nt][1] - b0);
-        p[nt][2] = exp2f(p[nt][2] - b1);
-        p[nt][3] = exp2f(p[nt][3] - b1);
+        for (int s = 4; s < 32; s <<= 1) {
+          x0 = fmaxf(x0, __shfl_xor_sync(kFull, x0, s));
+          x1 = fmaxf(x1, __shfl_xor_sync(kFull, x1, s));
+        }
+        const float n0 = fmaxf(m[nt][0], x0), n1 = fmaxf(m[nt][1], x1);
+        const float b0 = n0 == -INFINITY ? 0.0f : n0, b1 = n1 == -INFINITY ? 0.0f : n1;
+        fac[nt][0] = exp2f(m[nt][0] - b0);
+        fac[nt][1] = exp2f(m[nt][1] - b1);
+        m[nt][0] = n0;
+        m[nt][1] = n1;
+        p[0] = exp2f(p[0] - b0);
+        p[1] = exp2f(p[1] - b1);
+        p[2] = exp2f(p[2] - b0);
+        p[3] = exp2f(p[3] - b1);
+        l[nt][0] = fmaf(l[nt][0], fac[nt][0], p[0] + p[2]);
+        l[nt][1] = fmaf(l[nt][1], fac[nt][1], p[1] + p[3]);
+        *reinterpret_cast<float2*>(&sm.p[warp][nt][g][2 * t]) = make_float2(p[0], p[1]);
+        *reinterpret_cast<float2*>(&sm.p[warp][nt][g + 8][2 * t]) = make_float2(p[2], p[3]);
       }
-      l0 = l0 * f0 + ((p[0][0] + p[0][1]) + (p[1][0] + p[1][1]));
-      l1 = l1 * f1 + ((p[0][2] + p[0][3]) + (p[1][2] + p[1][3]));
+      cp_async_wait(2);
+      __syncwarp();  // the values have landed, the probabilities are written
+      const uint32_t vst = ring + slot * kKvHalf;
       // a value row that is not finite must not reach the rows that do not see it (0 * inf):
       // such a chunk, only where a mask is at work, takes the exact loop below
       bool odd = false;
@@ -401,218 +427,265 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArg
         odd = __any_sync(kFull, odd);
       }
       if (!odd) {
-        // output: a lane takes keys 8 nt + 2t, 2t + 1 and dimensions 32 w + 4 g + e; the chunk's
-        // sum starts from 0 and joins the running one with rounding
-        uint32_t ph[2][4], pl[2][4];
+        // Output: a lane takes keys t, t + 4, t + 8, t + 12 and dimensions 32 w + 4g + e; the
+        // chunk's sum starts from 0 and joins the running one with rounding.
+        uint32_t ph[NT][2][2], pl[NT][2][2];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          split_tf32(p[nt][0], ph[nt][0], pl[nt][0]);
-          split_tf32(p[nt][2], ph[nt][1], pl[nt][1]);
-          split_tf32(p[nt][1], ph[nt][2], pl[nt][2]);
-          split_tf32(p[nt][3], ph[nt][3], pl[nt][3]);
-        }
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) split_tf32(sm.p[warp][nt][ks * 8 + y * 4 + t][g], ph[nt][ks][y], pl[nt][ks][y]);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          float d[4][4];
+          float d[NT][2][4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int y = 0; y < 4; ++y) d[e][y] = 0.0f;
+            for (int z = 0; z < 2; ++z)
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
-            const int r0 = nt * 8 + 2 * t;  // r0 and r0 + 1 have the same swizzle
-            const uint32_t at = vst + r0 * (kKvD * 4) + (((w * 8 + g) ^ (((r0 >> 1) & 3) << 1)) << 4);
-            const float4 va = lds_f4(at), vb4 = lds_f4(at + kKvD * 4);
-            const float av[4] = {va.x, va.y, va.z, va.w}, bv[4] = {vb4.x, vb4.y, vb4.z, vb4.w};
+              for (int y = 0; y < 4; ++y) d[nt][z][y] = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              uint32_t ah, al, bh, bl;
-              split_tf32(av[e], ah, al);
-              split_tf32(bv[e], bh, bl);
-              mma_tf32(d[e], pl[nt][0], pl[nt][1], pl[nt][2], pl[nt][3], ah, bh);
-              mma_tf32(d[e], ph[nt][0], ph[nt][1], ph[nt][2], ph[nt][3], al, bl);
-              mma_tf32(d[e], ph[nt][0], ph[nt][1], ph[nt][2], ph[nt][3], ah, bh);
-            }
+          for (int ks = 0; ks < 2; ++ks) {
+            const uint32_t at = vst + (ks * 8 + t) * (kKvD * 4) + (((w * 8 + g) ^ (t << 1)) << 4);
+            const float4 va = lds_f4(at), vc = lds_f4(at + 4 * kKvD * 4);
+            uint32_t ah[4], al[4], ch[4], cl[4];
+            split_tf32(va.x, ah[0], al[0]);
+            split_tf32(va.y, ah[1], al[1]);
+            split_tf32(va.z, ah[2], al[2]);
+            split_tf32(va.w, ah[3], al[3]);
+            split_tf32(vc.x, ch[0], cl[0]);
+            split_tf32(vc.y, ch[1], cl[1]);
+            split_tf32(vc.z, ch[2], cl[2]);
+            split_tf32(vc.w, ch[3], cl[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int z = 0; z < 2; ++z) {
+                mma_tf32(d[nt][z], al[2 * z], al[2 * z + 1], cl[2 * z], cl[2 * z + 1], ph[nt][ks][0], ph[nt][ks][1]);
+                mma_tf32(d[nt][z], ah[2 * z], ah[2 * z + 1], ch[2 * z], ch[2 * z + 1], pl[nt][ks][0], pl[nt][ks][1]);
+                mma_tf32(d[nt][z], ah[2 * z], ah[2 * z + 1], ch[2 * z], ch[2 * z + 1], ph[nt][ks][0], ph[nt][ks][1]);
+              }
           }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            o[w * 4 + e][0] = fmaf(o[w * 4 + e][0], f0, d[e][0]);
-            o[w * 4 + e][1] = fmaf(o[w * 4 + e][1], f0, d[e][1]);
-            o[w * 4 + e][2] = fmaf(o[w * 4 + e][2], f1, d[e][2]);
-            o[w * 4 + e][3] = fmaf(o[w * 4 + e][3], f1, d[e][3]);
-          }
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int z = 0; z < 2; ++z)
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                o[nt][2 * w + z][y] = fmaf(o[nt][2 * w + z][y], fac[nt][y & 1], d[nt][z][y]);
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          o[i][0] *= f0;
-          o[i][1] *= f0;
-          o[i][2] *= f1;
-          o[i][3] *= f1;
-        }
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int r = 0; r < kKvChunk; ++r) {
-          const int src = (lane & ~3) | ((r & 7) >> 1);
-          const float pa = __shfl_sync(kFull, p[r >> 3][r & 1], src);
-          const float pb = __shfl_sync(kFull, p[r >> 3][2 + (r & 1)], src);
+          for (int i = 0; i < 8; ++i)
 #pragma unroll
-          for (int w = 0; w < 4; ++w)
+            for (int y = 0; y < 4; ++y) o[nt][i][y] *= fac[nt][y & 1];
+          for (int r = 0; r < kKvChunk; ++r) {
+            const float pa = sm.p[warp][nt][r][2 * t], pb = sm.p[warp][nt][r][2 * t + 1];
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {  // accumulator columns 2t + y: dimensions 32 w + 4 (2t + y) + e
-              const float4 q4 = lds_f4(vst + r * (kKvD * 4) + (((w * 8 + 2 * t + y) ^ (((r >> 1) & 3) << 1)) << 4));
+            for (int w = 0; w < 4; ++w) {
+              const float4 q4 = lds_f4(vst + r * (kKvD * 4) + (((w * 8 + g) ^ ((r & 3) << 1)) << 4));
               const float vv[4] = {q4.x, q4.y, q4.z, q4.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                if (pa != 0.0f) o[w * 4 + e][y] = fmaf(pa, vv[e], o[w * 4 + e][y]);
-                if (pb != 0.0f) o[w * 4 + e][2 + y] = fmaf(pb, vv[e], o[w * 4 + e][2 + y]);
+                float* dst = o[nt][2 * w + (e >> 1)] + 2 * (e & 1);
+                if (pa != 0.0f) dst[0] = fmaf(pa, vv[e], dst[0]);
+                if (pb != 0.0f) dst[1] = fmaf(pb, vv[e], dst[1]);
               }
             }
-        }
-      }
-      __syncwarp();  // the stage is free
-      if (c + kKvStages * kKvWarps < c1) load(c + kKvStages * kKvWarps, stage);
-      cp_async_commit();
-    }
-    cp_async_wait(0);
-
-    // the warps' parts, merged in warp order
-    if (tid < x.nrows) sm.ok[tid] = kv_row_valid<MASK>(a, x, tid);
-    l0 += __shfl_xor_sync(kFull, l0, 1);
-    l1 += __shfl_xor_sync(kFull, l1, 1);
-    l0 += __shfl_xor_sync(kFull, l0, 2);
-    l1 += __shfl_xor_sync(kFull, l1, 2);
-    if (t == 0) {
-      sm.m[warp][g] = m0;
-      sm.m[warp][g + 8] = m1;
-      sm.l[warp][g] = l0;
-      sm.l[warp][g + 8] = l1;
-    }
-#pragma unroll
-    for (int w = 0; w < 4; ++w)
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const int d = 32 * w + 4 * (2 * t + y);
-        *reinterpret_cast<float4*>(&sm.o[warp][g][d]) =
-            make_float4(o[w * 4][y], o[w * 4 + 1][y], o[w * 4 + 2][y], o[w * 4 + 3][y]);
-        *reinterpret_cast<float4*>(&sm.o[warp][g + 8][d]) =
-            make_float4(o[w * 4][2 + y], o[w * 4 + 1][2 + y], o[w * 4 + 2][2 + y], o[w * 4 + 3][2 + y]);
-      }
-    __syncthreads();
-    const bool whole = off == 0 && c1 == x.chunks;
-    const size_t slot = a.split ? (size_t)blockIdx.x + u : (size_t)u;
-    for (int r = 0; r < x.nrows; ++r) {
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kKvWarps; ++w) M = fmaxf(M, sm.m[w][r]);
-      if (!sm.ok[r]) M = -INFINITY;
-      float L = 0.0f, A = 0.0f;
-      if (M != -INFINITY) {
-#pragma unroll
-        for (int w = 0; w < kKvWarps; ++w) {
-          const float f = exp2f(sm.m[w][r] - M);
-          if (f != 0.0f) {  // an empty part's sums are 0, and stay out
-            L = fmaf(sm.l[w][r], f, L);
-            A = fmaf(sm.o[w][r][tid], f, A);
           }
         }
       }
-      if (whole)
-        a.out[kv_row_offset<MASK>(a, x, r) + tid] = L > 0.0f ? __fdiv_rn(A, L) : (M == -INFINITY ? 0.0f : A / L);
-      else
-        a.acc[slot * kKvSlotFloats + r * kKvD + tid] = A;
-      if (tid == 0 && a.stat) {
-        a.stat[slot * 32 + r] = M;
-        a.stat[slot * 32 + 16 + r] = L;
+      __syncwarp();
+      load(h + 4, slot);
+      slot = slot == kKvSlots - 1 ? 0 : slot + 1;
+    }
+    cp_async_wait(0);
+    __syncwarp();
+
+    // the warps' parts, merged in warp order
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1) l[nt][y] += __shfl_xor_sync(kFull, l[nt][y], s);
+        if (g == 0) {
+          const int r = nt * 8 + 2 * t + y;
+          sm.m[warp][r] = kv_row_valid<MASK>(a, x, r) ? m[nt][y] : -INFINITY;
+          sm.l[warp][r] = l[nt][y];
+        }
+        float* part = reinterpret_cast<float*>(&sm.ring[warp][0][0]) + (nt * 8 + 2 * t + y) * (kKvD + 4) + 4 * g;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          *reinterpret_cast<float4*>(part + 32 * w) =
+              make_float4(o[nt][2 * w][y], o[nt][2 * w][2 + y], o[nt][2 * w + 1][y], o[nt][2 * w + 1][2 + y]);
       }
-      if (tid == 0 && a.lse && whole)
-        a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + r] = M == -INFINITY ? INFINITY : M + log2f(L);
+    }
+    __syncthreads();
+    const size_t slot_id = a.split ? (size_t)blockIdx.x + u : (size_t)u;
+    const bool whole = off == 0 && c1 == x.chunks;
+    if (tid < x.nrows) {
+      float M = -INFINITY, L = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kKvWarps; ++w) M = fmaxf(M, sm.m[w][tid]);
+#pragma unroll
+      for (int w = 0; w < kKvWarps; ++w) {
+        const float f = M == -INFINITY ? 0.0f : exp2f(sm.m[w][tid] - M);
+        sm.f[w][tid] = f;
+        if (f != 0.0f) L = fmaf(sm.l[w][tid], f, L);  // an empty part's sums stay out
+      }
+      sm.M[tid] = M;
+      sm.L[tid] = L;
+      if (a.stat) {
+        a.stat[slot_id * 2 * kKvMaxRows + tid] = M;
+        a.stat[slot_id * 2 * kKvMaxRows + kKvMaxRows + tid] = L;
+      }
+      if (a.lse && whole)
+        a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + tid] = M == -INFINITY ? INFINITY : M + log2f(L);
+    }
+    __syncthreads();
+    for (int e = tid; e < x.nrows * 32; e += kKvThreads) {
+      const int r = e >> 5, d = (e & 31) * 4;
+      float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kKvWarps; ++w) {
+        const float f = sm.f[w][r];
+        const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(&sm.ring[w][0][0]) +
+                                                          r * (kKvD + 4) + d);
+        if (f != 0.0f) {
+          A.x = fmaf(v.x, f, A.x);
+          A.y = fmaf(v.y, f, A.y);
+          A.z = fmaf(v.z, f, A.z);
+          A.w = fmaf(v.w, f, A.w);
+        }
+      }
+      if (whole) {
+        if (sm.M[r] != -INFINITY) {
+          const float L = sm.L[r];
+          A = make_float4(__fdiv_rn(A.x, L), __fdiv_rn(A.y, L), __fdiv_rn(A.z, L), __fdiv_rn(A.w, L));
+        }
+        *reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, r) + d) = A;
+      } else {
+        *reinterpret_cast<float4*>(a.acc + slot_id * kKvSlotFloats + r * kKvD + d) = A;
+      }
     }
     left -= c1 - off;
     off = 0;
     ++u;
     if (!a.split) break;
-    __syncthreads();  // sm.q, sm.o are free
+    __syncthreads();  // the ring, sm.q and the statistics are free
   }
 }
 
-// Merge of the parts of every unit (one CTA per unit), and the weights of the keys where
-// the scores were stored: weight[j] += sum over the rows of 2^(s_j - log2 sum).
-// grid (units, key ranges): range 0 merges, every range adds its keys' weights.
-constexpr int kKvWeightKeys = 1024;
+// Merge of the parts of every unit, and the weights of the keys where the scores were stored:
+// weight[j] += sum over the rows of 2^(s_j - log2 sum).  grid (units, rows + key ranges): CTA
+// (u, r) merges row r, CTA (u, rows + k) adds the weights of range k.
+constexpr int kKvMergeThreads = 128;
+constexpr int kKvWeightKeys = 512;
 template <int MASK, bool SCORES>
-__global__ void __launch_bounds__(kKvThreads) kv_merge_kernel(const KvArgs a, float* __restrict__ weight) {
-  __shared__ int red[kKvWarps][2];
-  __shared__ float lse[kKvRows];
-  const int tid = threadIdx.x, u = blockIdx.x;
+__global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs a, float* __restrict__ weight) {
+  __shared__ int red[kKvMergeThreads / 32][2];
+  __shared__ float fac[kKvGrid], lse[kKvMaxRows], rm[kKvMergeThreads / 32], rl[kKvMergeThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, u = blockIdx.x;
   pdl_launch_dependents();
   pdl_wait();
   const KvUnit x = kv_unit<MASK>(a, u);
+  const bool merging = (int)blockIdx.y < a.rows;
+  const int row = blockIdx.y;
+  if (merging && (row >= x.nrows || !a.split)) return;
+  if (x.chunks == 0) {  // no CTA came by
+    if (merging) {
+      a.out[kv_row_offset<MASK>(a, x, row) + tid] = 0.0f;
+      if (a.lse && tid == 0) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] = INFINITY;
+    }
+    return;
+  }
+  const int key0 = ((int)blockIdx.y - a.rows) * kKvWeightKeys;
+  if (!merging && key0 >= x.keys) return;
   size_t slot0 = u;
   int parts = 1;
   if (a.split) {
     int before = 0, total = 0;
-    for (int i = tid; i < a.units; i += kKvThreads) {
+    for (int i = tid; i < a.units; i += kKvMergeThreads) {
       const int c = kv_unit<MASK>(a, i).chunks;
       total += c;
       if (i < u) before += c;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      total += __shfl_xor_sync(kFull, total, o);
-      before += __shfl_xor_sync(kFull, before, o);
-    }
-    if ((tid & 31) == 0) {
-      red[tid >> 5][0] = total;
-      red[tid >> 5][1] = before;
+    total = __reduce_add_sync(kFull, total);
+    before = __reduce_add_sync(kFull, before);
+    if (lane == 0) {
+      red[warp][0] = total;
+      red[warp][1] = before;
     }
     __syncthreads();
     total = before = 0;
-    for (int w = 0; w < kKvWarps; ++w) {
+    for (int w = 0; w < kKvMergeThreads / 32; ++w) {
       total += red[w][0];
       before += red[w][1];
     }
     const int quota = max((total + kKvGrid - 1) / kKvGrid, kKvWarps);
-    const int c0 = before / quota, c1 = x.chunks > 0 ? (before + x.chunks - 1) / quota : c0 - 1;
+    const int c0 = before / quota;
     slot0 = (size_t)c0 + u;
-    parts = c1 - c0 + 1;
+    parts = (before + x.chunks - 1) / quota - c0 + 1;
   }
-  if (x.chunks == 0) {  // no CTA came by
-    if (blockIdx.y == 0)
-      for (int r = 0; r < x.nrows; ++r) {
-        a.out[kv_row_offset<MASK>(a, x, r) + tid] = 0.0f;
-        if (a.lse && tid == 0) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + r] = INFINITY;
-      }
+  const float* stat = a.stat + slot0 * 2 * kKvMaxRows;
+  if (merging) {
+    if (parts == 1) return;
+    float M = -INFINITY;
+    for (int s = tid; s < parts; s += kKvMergeThreads) M = fmaxf(M, stat[s * 2 * kKvMaxRows + row]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, o));
+    if (lane == 0) rm[warp] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(rm[0], rm[1]), fmaxf(rm[2], rm[3]));
+    float L = 0.0f;
+    for (int s = tid; s < parts; s += kKvMergeThreads) {
+      const float f = M == -INFINITY ? 0.0f : exp2f(stat[s * 2 * kKvMaxRows + row] - M);
+      fac[s] = f;
+      if (f != 0.0f) L = fmaf(stat[s * 2 * kKvMaxRows + kKvMaxRows + row], f, L);
+    }
+    L = warp_sum(L);
+    if (lane == 0) rl[warp] = L;
+    __syncthreads();
+    L = (rl[0] + rl[1]) + (rl[2] + rl[3]);
+    const float* acc = a.acc + slot0 * kKvSlotFloats + row * kKvD + tid;
+    float A = 0.0f;
+#pragma unroll 8
+    for (int s = 0; s < parts; ++s) {
+      const float f = fac[s], v = acc[(size_t)s * kKvSlotFloats];
+      A = f != 0.0f ? fmaf(v, f, A) : A;
+    }
+    a.out[kv_row_offset<MASK>(a, x, row) + tid] = M == -INFINITY ? 0.0f : __fdiv_rn(A, L);
+    if (a.lse && tid == 0)
+      a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] = M == -INFINITY ? INFINITY : M + log2f(L);
     return;
   }
-  if (!SCORES && parts == 1) return;
-  const bool merge = blockIdx.y == 0 && parts > 1;
-  for (int r = 0; r < x.nrows; ++r) {
-    float M = -INFINITY;
-    for (int s = 0; s < parts; ++s) M = fmaxf(M, a.stat[(slot0 + s) * 32 + r]);
-    float L = 0.0f, A = 0.0f;
-    if (M != -INFINITY)
-      for (int s = 0; s < parts; ++s) {
-        const float f = exp2f(a.stat[(slot0 + s) * 32 + r] - M);
-        if (f != 0.0f) {
-          L = fmaf(a.stat[(slot0 + s) * 32 + 16 + r], f, L);
-          if (merge) A = fmaf(a.acc[(slot0 + s) * kKvSlotFloats + r * kKvD + tid], f, A);
-        }
-      }
-    if (merge) a.out[kv_row_offset<MASK>(a, x, r) + tid] = M == -INFINITY ? 0.0f : __fdiv_rn(A, L);
-    if (tid == 0) {
-      const float z = M == -INFINITY ? INFINITY : M + log2f(L);
-      lse[r] = z;
-      if (a.lse && merge) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + r] = z;
-    }
-  }
   if (SCORES) {
+    for (int r = warp; r < x.nrows; r += kKvMergeThreads / 32) {  // a warp per row
+      float M = -INFINITY, L = 0.0f;
+      for (int s = lane; s < parts; s += 32) M = fmaxf(M, stat[s * 2 * kKvMaxRows + r]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, o));
+      for (int s = lane; s < parts; s += 32) {
+        const float f = M == -INFINITY ? 0.0f : exp2f(stat[s * 2 * kKvMaxRows + r] - M);
+        if (f != 0.0f) L = fmaf(stat[s * 2 * kKvMaxRows + kKvMaxRows + r], f, L);
+      }
+      L = warp_sum(L);
+      if (lane == 0) lse[r] = M == -INFINITY ? INFINITY : M + log2f(L);
+    }
     __syncthreads();
-    const int j1 = min(x.keys, ((int)blockIdx.y + 1) * kKvWeightKeys);
     const size_t bh = (size_t)x.b * a.hkv + x.hk;
-    for (int j = blockIdx.y * kKvWeightKeys + tid; j < j1; j += kKvThreads) {
+    const int j1 = min(x.keys, key0 + kKvWeightKeys);
+    for (int j = key0 + tid; j < j1; j += kKvMergeThreads) {
       float w = 0.0f;
-      for (int r = 0; r < x.nrows; ++r)
-        if (lse[r] != INFINITY) w += exp2f(a.scores[(bh * x.nrows + r) * a.score_stride + j] - lse[r]);
+#pragma unroll 4
+      for (int r = 0; r < x.nrows; ++r) {
+        const float s = a.scores[(bh * x.nrows + r) * a.score_stride + j];
+        if (lse[r] != INFINITY) w += exp2f(s - lse[r]);
+      }
       weight[bh * a.max_t + j] += w;
     }
   }
@@ -621,12 +694,13 @@ __global__ void __launch_bounds__(kKvThreads) kv_merge_kernel(const KvArgs a, fl
 // Column sums of the softmax where the scores were not stored: every score once more, from
 // the rows' log2 sums.  grid (64-key tiles, batch * hkv), a warp holds 16 keys' fragments
 // and goes over the 16-row groups; sums per lane, then over the lanes of a key.
+constexpr int kColWarps = 4, kColThreads = kColWarps * 32, kColRows = 16;
 struct KvColSmem {
-  alignas(16) float k[kKvWarps * kKvChunk][kKvD];
-  alignas(16) float q[2][kKvRows][kKvD];
-  float lse[2][kKvRows];
+  alignas(16) float k[kColWarps * kKvChunk][kKvD];
+  alignas(16) float q[2][kColRows][kKvD];
+  float lse[2][kColRows];
 };
-__global__ void __launch_bounds__(kKvThreads, 1) kv_column_kernel(const KvArgs a, float* __restrict__ weight) {
+__global__ void __launch_bounds__(kColThreads, 1) kv_column_kernel(const KvArgs a, float* __restrict__ weight) {
   extern __shared__ __align__(16) uint8_t kv_smem[];
   KvColSmem& sm = *reinterpret_cast<KvColSmem*>(kv_smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -635,29 +709,29 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_column_kernel(const KvArgs a
   const int b = blockIdx.y / a.hkv, hk = blockIdx.y - b * a.hkv;
   const int p = a.pos[b], rows = a.n * a.group;
   const int keys = (p < 0 || p >= a.max_t) ? 0 : min(p + a.n, a.max_t);
-  const int j0 = blockIdx.x * (kKvWarps * kKvChunk);
+  const int j0 = blockIdx.x * (kColWarps * kKvChunk);
   if (j0 >= keys) return;
   const size_t bh = (size_t)b * a.hkv + hk;
   const float* kb = a.k + bh * (size_t)a.max_t * kKvD;
   const uint32_t ks = (uint32_t)__cvta_generic_to_shared(&sm.k[0][0]);
   const uint32_t qs = (uint32_t)__cvta_generic_to_shared(&sm.q[0][0][0]);
   const int i_first = max(0, j0 - p);  // the first token that sees a key of the tile
-  const int rg0 = (int)(((int64_t)i_first * a.group) / kKvRows);
+  const int rg0 = (int)(((int64_t)i_first * a.group) / kColRows);
   auto load_q = [&](int rg, int buf) {
-    for (int e = tid; e < kKvRows * 32; e += kKvThreads) {
-      const int r = e >> 5, ch = e & 31, row = rg * kKvRows + r;
+    for (int e = tid; e < kColRows * 32; e += kColThreads) {
+      const int r = e >> 5, ch = e & 31, row = rg * kColRows + r;
       const bool there = row < rows;
       const int i = there ? row / a.group : 0, h = hk * a.group + (there ? row - i * a.group : 0);
-      cp_async16_zfill(qs + buf * (kKvRows * kKvD * 4) + r * (kKvD * 4) + ((ch ^ ((r & 1) << 2)) << 4),
+      cp_async16_zfill(qs + buf * (kColRows * kKvD * 4) + r * (kKvD * 4) + ((ch ^ ((r & 1) << 2)) << 4),
                        a.q + (((size_t)b * a.n + i) * a.hq + h) * kKvD + ch * 4, there);
     }
-    if (tid < kKvRows) {
-      const int row = rg * kKvRows + tid;
+    if (tid < kColRows) {
+      const int row = rg * kColRows + tid;
       sm.lse[buf][tid] = row < rows ? a.lse[bh * rows + row] : INFINITY;
     }
     cp_async_commit();
   };
-  for (int e = tid; e < kKvWarps * kKvChunk * 32; e += kKvThreads) {
+  for (int e = tid; e < kColWarps * kKvChunk * 32; e += kColThreads) {
     const int r = e >> 5, ch = e & 31, j = j0 + r;
     cp_async16_zfill(ks + r * (kKvD * 4) + ((ch ^ ((r & 1) << 2)) << 4), kb + (size_t)(j < keys ? j : 0) * kKvD + ch * 4,
                      j < keys);
@@ -678,7 +752,7 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_column_kernel(const KvArgs a
       split_tf32(kv.w, kh[pair][nt][3], kl[pair][nt][3]);
     }
   float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-  const int rgs = (rows + kKvRows - 1) / kKvRows;
+  const int rgs = (rows + kColRows - 1) / kColRows;
   for (int rg = rg0; rg < rgs; ++rg) {
     const int buf = (rg - rg0) & 1;
     if (rg + 1 < rgs) load_q(rg + 1, buf ^ 1);
@@ -691,7 +765,7 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_column_kernel(const KvArgs a
         for (int e = 0; e < 4; ++e) s[nt][z][e] = 0.0f;
 #pragma unroll
     for (int pair = 0; pair < 8; ++pair) {
-      const uint32_t at = qs + buf * (kKvRows * kKvD * 4) + g * (kKvD * 4) + (((pair * 4 + t) ^ ((g & 1) << 2)) << 4);
+      const uint32_t at = qs + buf * (kColRows * kKvD * 4) + g * (kKvD * 4) + (((pair * 4 + t) ^ ((g & 1) << 2)) << 4);
       const float4 qa = lds_f4(at), qb = lds_f4(at + 8 * kKvD * 4);
       uint32_t ah[4], al[4], bh4[4], bl4[4];
       split_tf32(qa.x, ah[0], al[0]);
@@ -713,7 +787,7 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_column_kernel(const KvArgs a
     }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const int r = g + 8 * half, row = rg * kKvRows + r;
+      const int r = g + 8 * half, row = rg * kColRows + r;
       const float z = sm.lse[buf][r];
       const int last = p + row / a.group;  // rows past the cache have an infinite sum
 #pragma unroll
@@ -831,8 +905,9 @@ size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 int tree_words(int n) { return (n + 31) / 32; }
 
-// Rows of `rows` and units, and the parts of the workspace the core needs.
+// How the rows are cut into units and where the core's part of the workspace lies.
 struct KvPlan {
+  int rows = 8;
   int rgs = 1;
   int64_t units = 0;
   bool split = false;
@@ -840,7 +915,8 @@ struct KvPlan {
 };
 KvPlan kv_plan(int64_t lists, int64_t rows_per_list) {
   KvPlan p;
-  p.rgs = (int)((rows_per_list + kKvRows - 1) / kKvRows);
+  p.rows = rows_per_list <= 8 ? 8 : 16;
+  p.rgs = (int)((rows_per_list + p.rows - 1) / p.rows);
   p.units = lists * p.rgs;
   // with two units per SM and more the units themselves fill the GPU
   p.split = p.units < 2 * kKvGrid;
@@ -848,7 +924,7 @@ KvPlan kv_plan(int64_t lists, int64_t rows_per_list) {
   return p;
 }
 size_t core_bytes(const KvPlan& p, bool stat) {
-  return (p.split ? up256(p.slots * kKvSlotFloats * 4) : 0) + (p.split || stat ? up256(p.slots * 32 * 4) : 0);
+  return (p.split ? up256(p.slots * kKvSlotFloats * 4) : 0) + (p.split || stat ? up256(p.slots * 2 * kKvMaxRows * 4) : 0);
 }
 // Sets the core's part of the workspace; returns the bytes it takes.
 size_t core_place(KvArgs& a, const KvPlan& p, bool stat, uint8_t* ws) {
@@ -859,27 +935,34 @@ size_t core_place(KvArgs& a, const KvPlan& p, bool stat, uint8_t* ws) {
   }
   if (p.split || stat) {
     a.stat = reinterpret_cast<float*>(ws + o);
-    o += up256(p.slots * 32 * 4);
+    o += up256(p.slots * 2 * kKvMaxRows * 4);
   }
+  a.rows = p.rows;
   a.rgs = p.rgs;
   a.units = (int)p.units;
   a.split = p.split ? 1 : 0;
   return o;
 }
 
-template <int MASK, bool SCORES>
-cudaError_t launch_core(const KvArgs& a, float* weight, int device, cudaStream_t s) {
+template <int MASK, bool SCORES, int NT>
+cudaError_t launch_core_nt(const KvArgs& a, float* weight, int device, cudaStream_t s) {
   static int configured[128] = {0};
   cudaError_t e =
-      ensure_smem((const void*)kv_attention_kernel<MASK, SCORES>, configured, device, sizeof(KvSmem), false);
+      ensure_smem((const void*)kv_attention_kernel<MASK, SCORES, NT>, configured, device, sizeof(KvSmem<NT>), false);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
-  cudaLaunchConfig_t cfg = kv_cfg(dim3((unsigned)(a.split ? kKvGrid : a.units)), dim3(kKvThreads), sizeof(KvSmem), s, attr);
-  e = cudaLaunchKernelEx(&cfg, kv_attention_kernel<MASK, SCORES>, a);
+  cudaLaunchConfig_t cfg =
+      kv_cfg(dim3((unsigned)(a.split ? kKvGrid : a.units)), dim3(kKvThreads), sizeof(KvSmem<NT>), s, attr);
+  e = cudaLaunchKernelEx(&cfg, kv_attention_kernel<MASK, SCORES, NT>, a);
   if (e != cudaSuccess || (!a.split && !SCORES)) return e;
-  const unsigned ranges = SCORES ? (unsigned)((a.max_t + kKvWeightKeys - 1) / kKvWeightKeys) : 1u;
-  cfg = kv_cfg(dim3((unsigned)a.units, ranges), dim3(kKvThreads), 0, s, attr);
+  const unsigned ranges = SCORES ? (unsigned)((a.max_t + kKvWeightKeys - 1) / kKvWeightKeys) : 0u;
+  cfg = kv_cfg(dim3((unsigned)a.units, (unsigned)a.rows + ranges), dim3(kKvMergeThreads), 0, s, attr);
   return cudaLaunchKernelEx(&cfg, kv_merge_kernel<MASK, SCORES>, a, weight);
+}
+template <int MASK, bool SCORES>
+cudaError_t launch_core(const KvArgs& a, float* weight, int device, cudaStream_t s) {
+  return a.rows == 8 ? launch_core_nt<MASK, SCORES, 1>(a, weight, device, s)
+                     : launch_core_nt<MASK, SCORES, 2>(a, weight, device, s);
 }
 
 KvArgs kv_args(const float* q, const float* kc, const float* vc, const int* pos, int batch, int n, int hq, int hkv,
@@ -901,7 +984,7 @@ KvArgs kv_args(const float* q, const float* kc, const float* vc, const int* pos,
   return a;
 }
 
-bool weights_stored(int n, int group) { return (int64_t)n * group <= kKvRows; }
+bool weights_stored(int n, int group) { return (int64_t)n * group <= kKvMaxRows; }
 int score_stride(int max_t) { return (max_t + kKvChunk - 1) / kKvChunk * kKvChunk; }
 
 }  // namespace
@@ -958,9 +1041,9 @@ cudaError_t launch_attention_weights(const float* q, const float* kc, const floa
   e = ensure_smem((const void*)kv_column_kernel, configured, device, sizeof(KvColSmem), false);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
-  constexpr int tile = kKvWarps * kKvChunk;
+  constexpr int tile = kColWarps * kKvChunk;
   cudaLaunchConfig_t cfg = kv_cfg(dim3((unsigned)((max_t + tile - 1) / tile), (unsigned)(batch * hkv)),
-                                  dim3(kKvThreads), sizeof(KvColSmem), s, attr);
+                                  dim3(kColThreads), sizeof(KvColSmem), s, attr);
   return cudaLaunchKernelEx(&cfg, kv_column_kernel, a, weight);
 }
 
