@@ -180,7 +180,8 @@ uint64_t q8lin_wait_limit_ns(void);
  * Device-side fault word of `device` (bit 0: a tensor-core kernel's bounded wait ran
  * out, bit 1: a streaming GEMV's (M = 1, or the small-batch dp4a kernel), bit 2: the
  * small-batch int8 tensor-core kernel's, bit 3: the fused attention's, bit 4: the
- * persistent decode step's; the kernel returned early and its output is invalid).
+ * persistent decode step's, bit 5: the tensor-core tree / weights attention's; the kernel
+ * returned early and its output is invalid).
  * Reads it with a device synchronisation; `clear` resets it.  No counterpart in the reference (candle's
  * kernels have no bounded waits); this is the library's failure-detection hook.
  */

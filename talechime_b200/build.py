@@ -21,8 +21,8 @@ OBJDIR = os.path.join(PKG, "_build")
 
 SOURCES = ["abi.cu", "layout.cu", "gemv.cu", "gemm_simt.cu", "gemm_tc.cu", "noalloc.cu", "mlp.cu", "gemm_skinny.cu", "decoder.cu",
            "step.cu", "gemv_mrow.cu", "gguf.cpp", "tp_mlp.cu", "gemm_mma.cu", "prefill.cu",
-           "kv_attention.cu", "kv_cache.cu"]
-HEADERS = ["common.cuh", "internal.h"]
+           "kv_attention.cu", "kv_tile.cu", "kv_cache.cu"]
+HEADERS = ["common.cuh", "internal.h", "kv_core.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

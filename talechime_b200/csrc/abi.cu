@@ -478,8 +478,10 @@ int q8lin_fault_status(int device, uint32_t* flags, int clear) {
   unsigned int r = 0;
   if (e == cudaSuccess) e = read_step_fault(&p, clear != 0);
   if (e == cudaSuccess) e = read_mrow_fault(&r, clear != 0);
+  unsigned int t = 0;
+  if (e == cudaSuccess) e = read_kv_tile_fault(&t, clear != 0);
   if (e != cudaSuccess) return cuda_fail(e, "read fault word");
-  *flags = f | g | h | a | p | r;
+  *flags = f | g | h | a | p | r | t;
   return Q8LIN_OK;
 }
 

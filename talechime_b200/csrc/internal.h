@@ -187,6 +187,11 @@ cudaError_t launch_attention_blocks(const float* q, const float* kc, const float
                                     int batch, int n, int hq, int hkv, int max_t, int block, int topk, void* ws,
                                     float* out, int device, cudaStream_t s);
 
+// The tcgen05 form of the core for units of 128 rows (kv_tile.cu); mask: KvMask, not blocks.
+struct KvArgs;
+cudaError_t launch_kv_tile(const KvArgs& a, int mask, int device, cudaStream_t s);
+cudaError_t read_kv_tile_fault(unsigned int* flags, bool clear);  // bit 5
+
 // Cache upkeep (kv_cache.cu): which rows an eviction keeps, moving rows, block keys and the
 // choice of blocks.
 constexpr int kKvMaxBlocks = 16384;  // block scores of a row sit in shared memory

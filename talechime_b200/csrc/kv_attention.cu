@@ -18,130 +18,11 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "kv_core.cuh"
 
 namespace q8lin {
 
 namespace {
-
-constexpr int kKvD = 128;       // head width
-constexpr int kKvMaxRows = 16;  // query rows of a unit: 8 or 16
-constexpr int kKvChunk = 16;    // keys of a chunk: one warp's step
-constexpr int kKvWarps = 8;
-constexpr int kKvThreads = kKvWarps * 32;
-constexpr int kKvSlots = 3;     // half chunks (16 keys or 16 values) of a warp's ring
-constexpr int kKvHalf = kKvChunk * kKvD * 4;
-constexpr int kKvGrid = 148;    // CTAs that share the chunks of all units (one per SM)
-constexpr int kKvSlotFloats = kKvMaxRows * kKvD;
-
-enum KvMask : int { kMaskCausal = 0, kMaskTree = 1, kMaskBlocks = 2 };
-
-struct KvArgs {
-  const float* q;         // [batch][n][hq][128], rotated
-  const float* k;         // [batch][hkv][max_t][128]
-  const float* v;
-  const int* pos;         // [batch]
-  const uint32_t* anc;    // tree: [batch][n][words], bit j: node j is the row's node or above it
-  const int* index;       // blocks: [batch][n][hkv][topk], ascending, -1 behind the last
-  float* out;             // [batch][n][hq][128]
-  float* acc;             // [slot][16][128] unnormalised sums of a unit's part
-  float* stat;            // [slot][2][16] its maxima and sums
-  float* scores;          // causal with weights, n * group <= 16: [batch][hkv][n * group][score_stride]
-  float* lse;             // causal with weights, else: [batch][hkv][n * group] log2 of the row's sum
-  int batch, n, hq, hkv, group, max_t;
-  int words, topk, block, score_stride;
-  int rows;               // rows of a unit: 8 or 16
-  int rgs;                // row groups of a kv head (tree, causal) or of a token (blocks)
-  int units;
-  int split;              // 1: kKvGrid CTAs share all chunks evenly; 0: one CTA per unit
-  float c;                // log2(e) * f32(1/sqrt(128))
-};
-
-// One unit: its rows, its keys.
-struct KvUnit {
-  int b, hk, i0;    // i0: the first row's token
-  int r0, nrows;    // first row of the kv head's numbering (blocks: of the token's heads), rows
-  int p;            // pos[b]
-  int keys;         // causal / tree: keys [0, keys); blocks: last key + 1 of the own block
-  int chunks;
-  int picked;       // blocks: chosen blocks before the own one
-};
-
-template <int MASK>
-__device__ __forceinline__ KvUnit kv_unit(const KvArgs& a, int u) {
-  KvUnit x;
-  const int rg = u % a.rgs;
-  const int w = u / a.rgs;
-  x.r0 = rg * a.rows;
-  x.picked = 0;
-  if (MASK == kMaskBlocks) {
-    x.hk = w % a.hkv;
-    const int row = w / a.hkv;
-    x.b = row / a.n;
-    x.i0 = row - x.b * a.n;
-    x.nrows = min(a.rows, a.group - x.r0);
-    x.p = a.pos[x.b];
-    const bool ok = x.p >= 0 && x.p < a.max_t - x.i0;
-    const int at = x.p + x.i0;
-    x.keys = ok ? at + 1 : 0;
-    x.picked = ok ? min(a.topk, at / a.block) : 0;
-    x.chunks = ok ? x.picked * (a.block / kKvChunk) + (at % a.block) / kKvChunk + 1 : 0;
-  } else {
-    x.hk = w % a.hkv;
-    x.b = w / a.hkv;
-    x.nrows = min(a.rows, a.n * a.group - x.r0);
-    x.i0 = x.r0 / a.group;
-    x.p = a.pos[x.b];
-    const int last = (x.r0 + x.nrows - 1) / a.group;
-    x.keys = (x.p < 0 || x.p >= a.max_t) ? 0 : min(x.p + last + 1, a.max_t);
-    x.chunks = (x.keys + kKvChunk - 1) / kKvChunk;
-  }
-  return x;
-}
-
-// First key of chunk c of the unit.
-template <int MASK>
-__device__ __forceinline__ int kv_chunk_key(const KvArgs& a, const KvUnit& x, int c) {
-  if (MASK != kMaskBlocks) return c * kKvChunk;
-  const int per = a.block / kKvChunk;
-  const int nb = c / per;
-  if (nb < x.picked) {
-    const int blk = a.index[(((size_t)x.b * a.n + x.i0) * a.hkv + x.hk) * a.topk + nb];
-    return blk * a.block + (c - nb * per) * kKvChunk;
-  }
-  return (x.keys - 1) / a.block * a.block + (c - x.picked * per) * kKvChunk;
-}
-
-template <int MASK>
-__device__ __forceinline__ int kv_token(const KvArgs& a, const KvUnit& x, int r) {
-  return MASK == kMaskBlocks ? x.i0 : (x.r0 + r) / a.group;
-}
-// Offset of row r (0 <= r < nrows) of the unit in q and out.
-template <int MASK>
-__device__ __forceinline__ size_t kv_row_offset(const KvArgs& a, const KvUnit& x, int r) {
-  const int i = kv_token<MASK>(a, x, r);
-  const int h = x.hk * a.group + (MASK == kMaskBlocks ? x.r0 + r : (x.r0 + r) % a.group);
-  return (((size_t)x.b * a.n + i) * a.hq + h) * kKvD;
-}
-// Is the row one at all: inside the cache and, in a tree, a node.
-template <int MASK>
-__device__ __forceinline__ bool kv_row_valid(const KvArgs& a, const KvUnit& x, int r) {
-  if (r >= x.nrows || x.p < 0) return false;
-  const int i = kv_token<MASK>(a, x, r);
-  if (x.p >= a.max_t - i) return false;
-  if (MASK == kMaskTree) return (a.anc[((size_t)x.b * a.n + i) * a.words + (i >> 5)] >> (i & 31)) & 1u;
-  return true;
-}
-template <int MASK>
-__device__ __forceinline__ bool kv_sees(const KvArgs& a, const KvUnit& x, int r, int j) {
-  const int i = kv_token<MASK>(a, x, min(r, x.nrows - 1));
-  if (MASK == kMaskTree) {
-    const int e = j - x.p;
-    if (e < 0) return true;
-    if (e >= a.n) return false;
-    return (a.anc[((size_t)x.b * a.n + i) * a.words + (e >> 5)] >> (e & 31)) & 1u;
-  }
-  return j <= x.p + i;
-}
 
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t a0, const uint32_t a1, const uint32_t a2,
                                          const uint32_t a3, const uint32_t b0, const uint32_t b1) {
@@ -174,54 +55,8 @@ struct KvSmem {
   float m[kKvWarps][8 * NT], l[kKvWarps][8 * NT];
   float f[kKvWarps][8 * NT];
   float M[8 * NT], L[8 * NT];
-  int seg[kKvWarps];
-  int unit, off;
+  KvFind find;
 };
-
-// Where CTA `cta` of the shared split starts: fills sm.unit / sm.off and returns the chunk
-// count of one CTA (the whole work when it does not reach this CTA: unit = units).
-template <int MASK, int NT>
-__device__ int kv_find(const KvArgs& a, KvSmem<NT>& sm, int cta) {
-  const int tid = threadIdx.x;
-  const int per = (a.units + kKvThreads - 1) / kKvThreads;
-  const int u0 = min(a.units, tid * per), u1 = min(a.units, u0 + per);
-  int mine = 0;
-  for (int u = u0; u < u1; ++u) mine += kv_unit<MASK>(a, u).chunks;
-  int upto = mine;  // chunks of this thread's units and of those before them
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(kFull, upto, o);
-    if ((tid & 31) >= o) upto += v;
-  }
-  if ((tid & 31) == 31) sm.seg[tid >> 5] = upto;
-  if (tid == 0) {
-    sm.unit = a.units;
-    sm.off = 0;
-  }
-  __syncthreads();
-  int total = 0;
-#pragma unroll
-  for (int w = 0; w < kKvWarps; ++w) {
-    if (w < (tid >> 5)) upto += sm.seg[w];
-    total += sm.seg[w];
-  }
-  const int quota = max((total + kKvGrid - 1) / kKvGrid, kKvWarps);
-  const int start = cta * quota;
-  if (upto - mine <= start && start < upto) {
-    int at = upto - mine;
-    for (int u = u0; u < u1; ++u) {
-      const int c = kv_unit<MASK>(a, u).chunks;
-      if (start < at + c) {
-        sm.unit = u;
-        sm.off = start - at;
-        break;
-      }
-      at += c;
-    }
-  }
-  __syncthreads();
-  return quota;
-}
 
 // The rows are the N side of the products and the keys, then the dimensions, the M side, so
 // that 8 rows fill a tile: S^T = K Q^T and O^T = V^T P^T.  In an m16n8k8 fragment lane 4g + t
@@ -233,7 +68,6 @@ template <int MASK, bool SCORES, int NT>
 __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArgs a) {
   extern __shared__ __align__(16) uint8_t kv_smem[];
   KvSmem<NT>& sm = *reinterpret_cast<KvSmem<NT>*>(kv_smem);
-  constexpr int R = 8 * NT;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
   pdl_wait();
@@ -241,9 +75,9 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArg
 
   int u, off, left;
   if (a.split) {
-    left = kv_find<MASK, NT>(a, sm, blockIdx.x);
-    u = sm.unit;
-    off = sm.off;
+    left = kv_find<MASK, kKvThreads>(a, sm.find, blockIdx.x);
+    u = sm.find.unit;
+    off = sm.find.off;
   } else {
     u = a.units - 1 - (int)blockIdx.x;  // later rows see more keys: longest first
     off = 0;
@@ -540,8 +374,8 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArg
       sm.M[tid] = M;
       sm.L[tid] = L;
       if (a.stat) {
-        a.stat[slot_id * 2 * kKvMaxRows + tid] = M;
-        a.stat[slot_id * 2 * kKvMaxRows + kKvMaxRows + tid] = L;
+        a.stat[slot_id * 2 * a.rows + tid] = M;
+        a.stat[slot_id * 2 * a.rows + a.rows + tid] = L;
       }
       if (a.lse && whole)
         a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + tid] = M == -INFINITY ? INFINITY : M + log2f(L);
@@ -569,7 +403,7 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArg
         }
         *reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, r) + d) = A;
       } else {
-        *reinterpret_cast<float4*>(a.acc + slot_id * kKvSlotFloats + r * kKvD + d) = A;
+        *reinterpret_cast<float4*>(a.acc + (slot_id * a.rows + r) * kKvD + d) = A;
       }
     }
     left -= c1 - off;
@@ -626,16 +460,16 @@ __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs 
       total += red[w][0];
       before += red[w][1];
     }
-    const int quota = max((total + kKvGrid - 1) / kKvGrid, kKvWarps);
+    const int quota = max((total + kKvGrid - 1) / kKvGrid, a.least);
     const int c0 = before / quota;
     slot0 = (size_t)c0 + u;
     parts = (before + x.chunks - 1) / quota - c0 + 1;
   }
-  const float* stat = a.stat + slot0 * 2 * kKvMaxRows;
+  const float* stat = a.stat + slot0 * 2 * a.rows;
   if (merging) {
     if (parts == 1) return;
     float M = -INFINITY;
-    for (int s = tid; s < parts; s += kKvMergeThreads) M = fmaxf(M, stat[s * 2 * kKvMaxRows + row]);
+    for (int s = tid; s < parts; s += kKvMergeThreads) M = fmaxf(M, stat[s * 2 * a.rows + row]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, o));
     if (lane == 0) rm[warp] = M;
@@ -643,19 +477,19 @@ __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs 
     M = fmaxf(fmaxf(rm[0], rm[1]), fmaxf(rm[2], rm[3]));
     float L = 0.0f;
     for (int s = tid; s < parts; s += kKvMergeThreads) {
-      const float f = M == -INFINITY ? 0.0f : exp2f(stat[s * 2 * kKvMaxRows + row] - M);
+      const float f = M == -INFINITY ? 0.0f : exp2f(stat[s * 2 * a.rows + row] - M);
       fac[s] = f;
-      if (f != 0.0f) L = fmaf(stat[s * 2 * kKvMaxRows + kKvMaxRows + row], f, L);
+      if (f != 0.0f) L = fmaf(stat[(s * 2 + 1) * a.rows + row], f, L);
     }
     L = warp_sum(L);
     if (lane == 0) rl[warp] = L;
     __syncthreads();
     L = (rl[0] + rl[1]) + (rl[2] + rl[3]);
-    const float* acc = a.acc + slot0 * kKvSlotFloats + row * kKvD + tid;
+    const float* acc = a.acc + (slot0 * a.rows + row) * kKvD + tid;
     float A = 0.0f;
 #pragma unroll 8
     for (int s = 0; s < parts; ++s) {
-      const float f = fac[s], v = acc[(size_t)s * kKvSlotFloats];
+      const float f = fac[s], v = acc[(size_t)s * a.rows * kKvD];
       A = f != 0.0f ? fmaf(v, f, A) : A;
     }
     a.out[kv_row_offset<MASK>(a, x, row) + tid] = M == -INFINITY ? 0.0f : __fdiv_rn(A, L);
@@ -666,12 +500,12 @@ __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs 
   if (SCORES) {
     for (int r = warp; r < x.nrows; r += kKvMergeThreads / 32) {  // a warp per row
       float M = -INFINITY, L = 0.0f;
-      for (int s = lane; s < parts; s += 32) M = fmaxf(M, stat[s * 2 * kKvMaxRows + r]);
+      for (int s = lane; s < parts; s += 32) M = fmaxf(M, stat[s * 2 * a.rows + r]);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, o));
       for (int s = lane; s < parts; s += 32) {
-        const float f = M == -INFINITY ? 0.0f : exp2f(stat[s * 2 * kKvMaxRows + r] - M);
-        if (f != 0.0f) L = fmaf(stat[s * 2 * kKvMaxRows + kKvMaxRows + r], f, L);
+        const float f = M == -INFINITY ? 0.0f : exp2f(stat[s * 2 * a.rows + r] - M);
+        if (f != 0.0f) L = fmaf(stat[(s * 2 + 1) * a.rows + r], f, L);
       }
       L = warp_sum(L);
       if (lane == 0) lse[r] = M == -INFINITY ? INFINITY : M + log2f(L);
@@ -913,9 +747,11 @@ struct KvPlan {
   bool split = false;
   size_t slots = 0;
 };
-KvPlan kv_plan(int64_t lists, int64_t rows_per_list) {
+// Rows a kv head from which the tcgen05 kernel (128 rows a unit) takes over.
+constexpr int64_t kKvTileMinRows = 17;
+KvPlan kv_plan(int64_t lists, int64_t rows_per_list, bool tile) {
   KvPlan p;
-  p.rows = rows_per_list <= 8 ? 8 : 16;
+  p.rows = tile && rows_per_list >= kKvTileMinRows ? kKvTileRows : rows_per_list <= 8 ? 8 : kKvMaxRows;
   p.rgs = (int)((rows_per_list + p.rows - 1) / p.rows);
   p.units = lists * p.rgs;
   // with two units per SM and more the units themselves fill the GPU
@@ -924,20 +760,22 @@ KvPlan kv_plan(int64_t lists, int64_t rows_per_list) {
   return p;
 }
 size_t core_bytes(const KvPlan& p, bool stat) {
-  return (p.split ? up256(p.slots * kKvSlotFloats * 4) : 0) + (p.split || stat ? up256(p.slots * 2 * kKvMaxRows * 4) : 0);
+  return (p.split ? up256(p.slots * p.rows * kKvD * 4) : 0) + (p.split || stat ? up256(p.slots * 2 * p.rows * 4) : 0);
 }
 // Sets the core's part of the workspace; returns the bytes it takes.
 size_t core_place(KvArgs& a, const KvPlan& p, bool stat, uint8_t* ws) {
   size_t o = 0;
   if (p.split) {
     a.acc = reinterpret_cast<float*>(ws);
-    o += up256(p.slots * kKvSlotFloats * 4);
+    o += up256(p.slots * p.rows * kKvD * 4);
   }
   if (p.split || stat) {
     a.stat = reinterpret_cast<float*>(ws + o);
-    o += up256(p.slots * 2 * kKvMaxRows * 4);
+    o += up256(p.slots * 2 * p.rows * 4);
   }
   a.rows = p.rows;
+  a.chunk = p.rows == kKvTileRows ? kKvTileKeys : kKvChunk;
+  a.least = p.rows == kKvTileRows ? 2 : kKvWarps;
   a.rgs = p.rgs;
   a.units = (int)p.units;
   a.split = p.split ? 1 : 0;
@@ -945,7 +783,7 @@ size_t core_place(KvArgs& a, const KvPlan& p, bool stat, uint8_t* ws) {
 }
 
 template <int MASK, bool SCORES, int NT>
-cudaError_t launch_core_nt(const KvArgs& a, float* weight, int device, cudaStream_t s) {
+cudaError_t launch_core_nt(const KvArgs& a, int device, cudaStream_t s) {
   static int configured[128] = {0};
   cudaError_t e =
       ensure_smem((const void*)kv_attention_kernel<MASK, SCORES, NT>, configured, device, sizeof(KvSmem<NT>), false);
@@ -953,16 +791,20 @@ cudaError_t launch_core_nt(const KvArgs& a, float* weight, int device, cudaStrea
   cudaLaunchAttribute attr[1];
   cudaLaunchConfig_t cfg =
       kv_cfg(dim3((unsigned)(a.split ? kKvGrid : a.units)), dim3(kKvThreads), sizeof(KvSmem<NT>), s, attr);
-  e = cudaLaunchKernelEx(&cfg, kv_attention_kernel<MASK, SCORES, NT>, a);
-  if (e != cudaSuccess || (!a.split && !SCORES)) return e;
-  const unsigned ranges = SCORES ? (unsigned)((a.max_t + kKvWeightKeys - 1) / kKvWeightKeys) : 0u;
-  cfg = kv_cfg(dim3((unsigned)a.units, (unsigned)a.rows + ranges), dim3(kKvMergeThreads), 0, s, attr);
-  return cudaLaunchKernelEx(&cfg, kv_merge_kernel<MASK, SCORES>, a, weight);
+  return cudaLaunchKernelEx(&cfg, kv_attention_kernel<MASK, SCORES, NT>, a);
 }
 template <int MASK, bool SCORES>
 cudaError_t launch_core(const KvArgs& a, float* weight, int device, cudaStream_t s) {
-  return a.rows == 8 ? launch_core_nt<MASK, SCORES, 1>(a, weight, device, s)
-                     : launch_core_nt<MASK, SCORES, 2>(a, weight, device, s);
+  cudaError_t e;
+  if (!SCORES && MASK != kMaskBlocks && a.rows == kKvTileRows)
+    e = launch_kv_tile(a, MASK, device, s);
+  else
+    e = a.rows == 8 ? launch_core_nt<MASK, SCORES, 1>(a, device, s) : launch_core_nt<MASK, SCORES, 2>(a, device, s);
+  if (e != cudaSuccess || (!a.split && !SCORES)) return e;
+  const unsigned ranges = SCORES ? (unsigned)((a.max_t + kKvWeightKeys - 1) / kKvWeightKeys) : 0u;
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg = kv_cfg(dim3((unsigned)a.units, (unsigned)a.rows + ranges), dim3(kKvMergeThreads), 0, s, attr);
+  return cudaLaunchKernelEx(&cfg, kv_merge_kernel<MASK, SCORES>, a, weight);
 }
 
 KvArgs kv_args(const float* q, const float* kc, const float* vc, const int* pos, int batch, int n, int hq, int hkv,
@@ -990,7 +832,7 @@ int score_stride(int max_t) { return (max_t + kKvChunk - 1) / kKvChunk * kKvChun
 }  // namespace
 
 size_t attention_tree_workspace_bytes(int batch, int n, int hq, int hkv) {
-  const KvPlan p = kv_plan((int64_t)batch * hkv, (int64_t)n * (hq / hkv));
+  const KvPlan p = kv_plan((int64_t)batch * hkv, (int64_t)n * (hq / hkv), true);
   return up256((size_t)batch * n * hq * kKvD * 4) + up256((size_t)batch * n * tree_words(n) * 4) + core_bytes(p, false);
 }
 
@@ -1005,7 +847,7 @@ cudaError_t launch_rope_attention_tree(const float* qkv, const int* parents, con
   KvArgs a = kv_args(q, kc, vc, pos, batch, n, hq, hkv, max_t, out);
   a.anc = anc;
   a.words = tree_words(n);
-  core_place(a, kv_plan((int64_t)batch * hkv, (int64_t)n * a.group), false, w);
+  core_place(a, kv_plan((int64_t)batch * hkv, (int64_t)n * a.group, true), false, w);
   cudaLaunchAttribute attr[1];
   cudaLaunchConfig_t cfg = kv_cfg(dim3((unsigned)n, (unsigned)batch), dim3(kKvMaxTree), 0, s, attr);
   cudaError_t e = cudaLaunchKernelEx(&cfg, rope_tree_kernel, qkv, parents, pos, cos_t, sin_t, kc, vc, n, a.words, hq,
@@ -1016,7 +858,7 @@ cudaError_t launch_rope_attention_tree(const float* qkv, const int* parents, con
 
 size_t attention_weights_workspace_bytes(int batch, int n, int hq, int hkv, int max_t) {
   const int group = hq / hkv;
-  const KvPlan p = kv_plan((int64_t)batch * hkv, (int64_t)n * group);
+  const KvPlan p = kv_plan((int64_t)batch * hkv, (int64_t)n * group, true);
   const bool stored = weights_stored(n, group);
   return core_bytes(p, stored) + (stored ? up256((size_t)batch * hq * n * score_stride(max_t) * 4)
                                          : up256((size_t)batch * hq * n * 4));
@@ -1028,7 +870,7 @@ cudaError_t launch_attention_weights(const float* q, const float* kc, const floa
   KvArgs a = kv_args(q, kc, vc, pos, batch, n, hq, hkv, max_t, out);
   const bool stored = weights_stored(n, a.group);
   uint8_t* w = static_cast<uint8_t*>(ws);
-  w += core_place(a, kv_plan((int64_t)batch * hkv, (int64_t)n * a.group), stored, w);
+  w += core_place(a, kv_plan((int64_t)batch * hkv, (int64_t)n * a.group, true), stored, w);
   if (stored) {
     a.scores = reinterpret_cast<float*>(w);
     a.score_stride = score_stride(max_t);
@@ -1048,7 +890,7 @@ cudaError_t launch_attention_weights(const float* q, const float* kc, const floa
 }
 
 size_t attention_blocks_workspace_bytes(int batch, int n, int hq, int hkv) {
-  return up256(core_bytes(kv_plan((int64_t)batch * n * hkv, hq / hkv), false) + 1);  // never 0: it may be allocated
+  return up256(core_bytes(kv_plan((int64_t)batch * n * hkv, hq / hkv, false), false) + 1);  // never 0: it may be allocated
 }
 
 cudaError_t launch_attention_blocks(const float* q, const float* kc, const float* vc, const int* pos, const int* index,
@@ -1058,7 +900,7 @@ cudaError_t launch_attention_blocks(const float* q, const float* kc, const float
   a.index = index;
   a.block = block;
   a.topk = topk;
-  core_place(a, kv_plan((int64_t)batch * n * hkv, a.group), false, static_cast<uint8_t*>(ws));
+  core_place(a, kv_plan((int64_t)batch * n * hkv, a.group, false), false, static_cast<uint8_t*>(ws));
   return launch_core<kMaskBlocks, false>(a, nullptr, device, s);
 }
 

@@ -1,0 +1,183 @@
+// What the attention kernels over the KV cache share (kv_attention.cu, kv_tile.cu): their
+// arguments, the units their work is cut into, and who sees what.
+#pragma once
+
+#include "common.cuh"
+#include "internal.h"
+
+namespace q8lin {
+
+constexpr int kKvD = 128;       // head width
+constexpr int kKvMaxRows = 16;  // query rows of a unit: 8 or 16
+constexpr int kKvChunk = 16;    // keys of a chunk: one warp's step
+constexpr int kKvWarps = 8;
+constexpr int kKvThreads = kKvWarps * 32;
+constexpr int kKvSlots = 3;     // half chunks (16 keys or 16 values) of a warp's ring
+constexpr int kKvHalf = kKvChunk * kKvD * 4;
+constexpr int kKvGrid = 148;    // CTAs that share the chunks of all units (one per SM)
+constexpr int kKvTileRows = 128;  // query rows of a unit of the tcgen05 kernel
+constexpr int kKvTileKeys = 64;   // keys of its tiles
+
+enum KvMask : int { kMaskCausal = 0, kMaskTree = 1, kMaskBlocks = 2 };
+
+struct KvArgs {
+  const float* q;         // [batch][n][hq][128], rotated
+  const float* k;         // [batch][hkv][max_t][128]
+  const float* v;
+  const int* pos;         // [batch]
+  const uint32_t* anc;    // tree: [batch][n][words], bit j: node j is the row's node or above it
+  const int* index;       // blocks: [batch][n][hkv][topk], ascending, -1 behind the last
+  float* out;             // [batch][n][hq][128]
+  float* acc;             // [slot][rows][128] unnormalised sums of a unit's part
+  float* stat;            // [slot][2][rows] its maxima and sums
+  float* scores;          // causal with weights, n * group <= 16: [batch][hkv][n * group][score_stride]
+  float* lse;             // causal with weights, else: [batch][hkv][n * group] log2 of the row's sum
+  int batch, n, hq, hkv, group, max_t;
+  int words, topk, block, score_stride;
+  int rows;               // rows of a unit: 8, 16 or 128
+  int chunk;              // keys of a chunk: 16, or 64 with units of 128 rows
+  int least;              // chunks a CTA takes at least
+  int rgs;                // row groups of a kv head (tree, causal) or of a token (blocks)
+  int units;
+  int split;              // 1: kKvGrid CTAs share all chunks evenly; 0: one CTA per unit
+  float c;                // log2(e) * f32(1/sqrt(128))
+};
+
+// One unit: its rows, its keys.
+struct KvUnit {
+  int b, hk, i0;    // i0: the first row's token
+  int r0, nrows;    // first row of the kv head's numbering (blocks: of the token's heads), rows
+  int p;            // pos[b]
+  int keys;         // causal / tree: keys [0, keys); blocks: last key + 1 of the own block
+  int chunks;
+  int picked;       // blocks: chosen blocks before the own one
+};
+
+template <int MASK>
+__device__ __forceinline__ KvUnit kv_unit(const KvArgs& a, int u) {
+  KvUnit x;
+  const int rg = u % a.rgs;
+  const int w = u / a.rgs;
+  x.r0 = rg * a.rows;
+  x.picked = 0;
+  if (MASK == kMaskBlocks) {
+    x.hk = w % a.hkv;
+    const int row = w / a.hkv;
+    x.b = row / a.n;
+    x.i0 = row - x.b * a.n;
+    x.nrows = min(a.rows, a.group - x.r0);
+    x.p = a.pos[x.b];
+    const bool ok = x.p >= 0 && x.p < a.max_t - x.i0;
+    const int at = x.p + x.i0;
+    x.keys = ok ? at + 1 : 0;
+    x.picked = ok ? min(a.topk, at / a.block) : 0;
+    x.chunks = ok ? x.picked * (a.block / kKvChunk) + (at % a.block) / kKvChunk + 1 : 0;
+  } else {
+    x.hk = w % a.hkv;
+    x.b = w / a.hkv;
+    x.nrows = min(a.rows, a.n * a.group - x.r0);
+    x.i0 = x.r0 / a.group;
+    x.p = a.pos[x.b];
+    const int last = (x.r0 + x.nrows - 1) / a.group;
+    x.keys = (x.p < 0 || x.p >= a.max_t) ? 0 : min(x.p + last + 1, a.max_t);
+    x.chunks = (x.keys + a.chunk - 1) / a.chunk;
+  }
+  return x;
+}
+
+// First key of chunk c of the unit.
+template <int MASK>
+__device__ __forceinline__ int kv_chunk_key(const KvArgs& a, const KvUnit& x, int c) {
+  if (MASK != kMaskBlocks) return c * kKvChunk;
+  const int per = a.block / kKvChunk;
+  const int nb = c / per;
+  if (nb < x.picked) {
+    const int blk = a.index[(((size_t)x.b * a.n + x.i0) * a.hkv + x.hk) * a.topk + nb];
+    return blk * a.block + (c - nb * per) * kKvChunk;
+  }
+  return (x.keys - 1) / a.block * a.block + (c - x.picked * per) * kKvChunk;
+}
+
+template <int MASK>
+__device__ __forceinline__ int kv_token(const KvArgs& a, const KvUnit& x, int r) {
+  return MASK == kMaskBlocks ? x.i0 : (x.r0 + r) / a.group;
+}
+// Offset of row r (0 <= r < nrows) of the unit in q and out.
+template <int MASK>
+__device__ __forceinline__ size_t kv_row_offset(const KvArgs& a, const KvUnit& x, int r) {
+  const int i = kv_token<MASK>(a, x, r);
+  const int h = x.hk * a.group + (MASK == kMaskBlocks ? x.r0 + r : (x.r0 + r) % a.group);
+  return (((size_t)x.b * a.n + i) * a.hq + h) * kKvD;
+}
+// Is the row one at all: inside the cache and, in a tree, a node.
+template <int MASK>
+__device__ __forceinline__ bool kv_row_valid(const KvArgs& a, const KvUnit& x, int r) {
+  if (r >= x.nrows || x.p < 0) return false;
+  const int i = kv_token<MASK>(a, x, r);
+  if (x.p >= a.max_t - i) return false;
+  if (MASK == kMaskTree) return (a.anc[((size_t)x.b * a.n + i) * a.words + (i >> 5)] >> (i & 31)) & 1u;
+  return true;
+}
+template <int MASK>
+__device__ __forceinline__ bool kv_sees(const KvArgs& a, const KvUnit& x, int r, int j) {
+  const int i = kv_token<MASK>(a, x, min(r, x.nrows - 1));
+  if (MASK == kMaskTree) {
+    const int e = j - x.p;
+    if (e < 0) return true;
+    if (e >= a.n) return false;
+    return (a.anc[((size_t)x.b * a.n + i) * a.words + (e >> 5)] >> (e & 31)) & 1u;
+  }
+  return j <= x.p + i;
+}
+
+struct KvFind {
+  int seg[16];  // chunk sums of the warps
+  int unit, off;
+};
+
+// Where CTA `cta` of the shared split starts: fills unit / off and returns the chunk
+// count of one CTA (the whole work when it does not reach this CTA: unit = units).
+template <int MASK, int THREADS>
+__device__ int kv_find(const KvArgs& a, KvFind& sm, int cta) {
+  const int tid = threadIdx.x;
+  const int per = (a.units + THREADS - 1) / THREADS;
+  const int u0 = min(a.units, tid * per), u1 = min(a.units, u0 + per);
+  int mine = 0;
+  for (int u = u0; u < u1; ++u) mine += kv_unit<MASK>(a, u).chunks;
+  int upto = mine;  // chunks of this thread's units and of those before them
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(kFull, upto, o);
+    if ((tid & 31) >= o) upto += v;
+  }
+  if ((tid & 31) == 31) sm.seg[tid >> 5] = upto;
+  if (tid == 0) {
+    sm.unit = a.units;
+    sm.off = 0;
+  }
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < (tid >> 5)) upto += sm.seg[w];
+    total += sm.seg[w];
+  }
+  const int quota = max((total + kKvGrid - 1) / kKvGrid, a.least);
+  const int start = cta * quota;
+  if (upto - mine <= start && start < upto) {
+    int at = upto - mine;
+    for (int u = u0; u < u1; ++u) {
+      const int c = kv_unit<MASK>(a, u).chunks;
+      if (start < at + c) {
+        sm.unit = u;
+        sm.off = start - at;
+        break;
+      }
+      at += c;
+    }
+  }
+  __syncthreads();
+  return quota;
+}
+
+}  // namespace q8lin

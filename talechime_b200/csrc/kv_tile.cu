@@ -1,0 +1,749 @@
+// The attention core over the KV cache on tcgen05: units of 128 query rows against tiles of
+// 64 keys, for kv heads with many rows (wide trees, prompt chunks).
+//
+// Products: f32 operands as pairs of f16 numbers under a power-of-two scale, three
+// tcgen05.mma kind::f16 per product.  x s = hi + lo, s = 2^(13 - exponent of the largest
+// |x|) of the K tile, the V tile or the query row; hi = x s cut to 11 significant bits, lo = x s -
+// hi (exact) rounded to f16; a.b = lo.hi + hi.lo + hi.hi.  lo keeps 2^-25 of scale 2^13, so an
+// element is off by at most 2^-22 of itself or 2^-39 of its tile's largest, and the dropped lo.lo
+// is 2^-20 of a product at most, 2^-22 on average.  Scaling makes f32's exponent range fit.
+//
+// One CTA per SM, nine working warps:
+//   * 4 convert: cache rows to registers one tile ahead, then scaled hi / lo to swizzled shared
+//     memory, K as [64 keys][128 dims], V transposed as [128 dims][64 keys], two stages each;
+//   * 1 issues the MMAs: S = Q K^T (Q in TMEM), O = P V (P in TMEM), S and P double-buffered,
+//     so that QK of a tile runs while the softmax of the one before is at work;
+//   * 4 softmax: a thread owns a row; scores from TMEM, running maximum and sum, P' = 2^14 p
+//     back to TMEM as hi / lo; then the O tile of the tile before is added to 128 registers.
+// The tensor cores cut their f32 sums, so an O tile starts from 0 and joins the running sum with
+// rounding.  TMEM (512 columns): Q 128, S 2 x 64, P 2 x 64, O 128.
+//
+// What bounds it: per 128 rows x 64 keys 24 MMAs of N = 64 and 12 of N = 128, about 1600
+// cycles; conversion, softmax and O need about 1000 issue slots of each scheduler beside them.
+#include <cmath>
+
+#include "common.cuh"
+#include "internal.h"
+#include "kv_core.cuh"
+
+namespace q8lin {
+
+namespace {
+
+constexpr int kKtThreads = 384;   // three warpgroups: softmax, converters, MMA (one of its warps)
+// Registers of a thread: 384 x 168 at launch, then 240 + 208 + 56 = 3 x 168.
+constexpr int kKtRegSoftmax = 240, kKtRegConvert = 208, kKtRegMma = 56;
+constexpr int kKtConvert0 = 128;  // first converter thread
+constexpr int kKtMmaWarp = 8;
+constexpr uint32_t kKtTmemCols = 512;
+constexpr uint32_t kTmQ = 0, kTmS = 128, kTmP = 256, kTmO = 384;
+constexpr int kKtPScale = 14;     // P' = 2^14 p
+
+__device__ unsigned int g_kv_tile_fault;
+__shared__ uint64_t s_kt_wait_ns;
+
+struct KtSmem {
+  alignas(1024) uint8_t k[2][2][2][kKvTileKeys * 128];  // [stage][hi, lo][64 dims][key][128 B]
+  alignas(1024) uint8_t v[2][2][kKvD * 128];            // [stage][hi, lo][dim][64 keys]
+  float ksc[4], vsc[4];                                 // inverse scales of tiles t % 4
+  unsigned long long vbad[4];                           // keys of the tile whose value row is not finite
+  unsigned red[4][4];                                   // the converters' maxima
+  alignas(8) uint64_t kfull[2], kfree[2], vfull[2], vfree[2];
+  uint64_t kinfo[4], vinfo[4];
+  uint64_t sfull[2], pfull[2], qfull, ofull, ofree, done;
+  KvFind find;
+  uint32_t tmem;
+  int abort;
+};
+
+__device__ __forceinline__ uint32_t su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(b)) : "memory");
+}
+// Bounded wait; once one has run out (or another warp's has) every wait of the CTA fails.
+__device__ __forceinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort) {
+  if (mb_wait_ns(bar, parity, s_kt_wait_ns, abort)) return true;
+  if (!*abort) atomicOr(&g_kv_tile_fault, 32u);
+  *abort = 1;
+  return false;
+}
+// By whole warps: the verdict is uniform.
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* abort) {
+  const uint32_t bar = su32(b);
+  return __all_sync(kFull, mb_try(bar, parity) || bar_wait_slow(bar, parity, abort));
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// K-major 128B-swizzled operand: 8-row atoms of 128 bytes, 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_sw128(const void* base) {
+  uint64_t d = (su32(base) >> 4) & 0x3FFFull;
+  d |= (uint64_t)1 << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+// kind::f16, f16 operands, f32 sums, M = 128.
+__host__ __device__ constexpr uint32_t kt_idesc(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
+// D (+)= A (TMEM) B^T (shared memory); called by a converged warp, one lane issues.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(su32(bar))
+      : "memory");
+}
+
+#define KT_R32(a) \
+  a(0), a(1), a(2), a(3), a(4), a(5), a(6), a(7), a(8), a(9), a(10), a(11), a(12), a(13), a(14), a(15), a(16), a(17), \
+      a(18), a(19), a(20), a(21), a(22), a(23), a(24), a(25), a(26), a(27), a(28), a(29), a(30), a(31)
+// 32 columns of the thread's TMEM lane; valid after tm_wait_ld.
+__device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t (&r)[32]) {
+#define KT_OUT(i) "=r"(r[i])
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : KT_R32(KT_OUT)
+      : "r"(addr)
+      : "memory");
+#undef KT_OUT
+}
+__device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t (&r)[32]) {
+#define KT_IN(i) "r"(r[i])
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::KT_R32(KT_IN),
+      "r"(addr)
+      : "memory");
+#undef KT_IN
+}
+__device__ __forceinline__ void tm_ld16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tm_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t tm_ld1(uint32_t addr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(addr) : "memory");
+  return r;
+}
+__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
+        "l"(reinterpret_cast<const uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Two scaled values -> packed hi parts and packed lo parts.
+__device__ __forceinline__ void split_f16(float2 x, uint32_t& hi, uint32_t& lo) {
+  const float2 h = make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffffe000u),
+                               __uint_as_float(__float_as_uint(x.y) & 0xffffe000u));
+  hi = pack_f16(h.x, h.y);
+  const float2 l = fma2(h, make_float2(-1.0f, -1.0f), x);
+  lo = pack_f16(l.x, l.y);
+}
+// Largest magnitude (bits of a float) -> scale 2^(13 - exponent) and its inverse.
+__device__ __forceinline__ void scale_of(unsigned top, float& scale, float& inverse) {
+  const int e = min(253, 267 - (int)(top >> 23));
+  scale = __uint_as_float((unsigned)e << 23);
+  inverse = __uint_as_float((unsigned)(254 - e) << 23);
+}
+__device__ __forceinline__ float mag(float m, float x) { return fmaxf(m, fabsf(x)); }
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// The tiles of this CTA's units, in order.
+template <int MASK>
+struct KtCursor {
+  int u, off, left;  // unit, its first tile here, tiles left of the CTA's share
+  int c, c1;         // current tile, end
+  KvUnit x;
+  bool ok;
+  // Moves to the first unit from u on with work.
+  __device__ void seek(const KvArgs& a) {
+    ok = false;
+    while (u < a.units && left > 0) {
+      x = kv_unit<MASK>(a, u);
+      c = off;
+      c1 = off > x.chunks - left ? x.chunks : off + left;
+      if (c < c1) {
+        ok = true;
+        return;
+      }
+      off = 0;
+      ++u;
+      if (!a.split) return;
+    }
+  }
+  __device__ void next(const KvArgs& a) {
+    if (++c < c1) return;
+    left -= c1 - off;
+    off = 0;
+    ++u;
+    if (a.split)
+      seek(a);
+    else
+      ok = false;
+  }
+};
+
+template <int MASK>
+__device__ __forceinline__ bool kt_row_there(const KvArgs& a, const KvUnit& x, int j) {
+  if (j >= x.keys) return false;
+  if (MASK != kMaskTree || j < x.p) return true;
+  const int e = j - x.p;
+  return e < a.n && ((a.anc[((size_t)x.b * a.n + e) * a.words + (e >> 5)] >> (e & 31)) & 1u);
+}
+
+template <int MASK>
+__global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, uint64_t wait_ns) {
+  extern __shared__ uint8_t kt_raw[];
+  KtSmem& sm = *reinterpret_cast<KtSmem*>((reinterpret_cast<uintptr_t>(kt_raw) + 1023) & ~uintptr_t(1023));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* abort = &sm.abort;
+  if (tid == 0) {
+    s_kt_wait_ns = wait_ns;
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&sm.kfull[i], 4);
+      bar_init(&sm.kfree[i], 1);
+      bar_init(&sm.vfull[i], 4);
+      bar_init(&sm.vfree[i], 1);
+      bar_init(&sm.sfull[i], 1);
+      bar_init(&sm.pfull[i], 4);
+    }
+    for (int i = 0; i < 4; ++i) {
+      bar_init(&sm.kinfo[i], 4);
+      bar_init(&sm.vinfo[i], 4);
+    }
+    bar_init(&sm.qfull, 4);
+    bar_init(&sm.ofull, 1);
+    bar_init(&sm.ofree, 4);
+    bar_init(&sm.done, 1);
+    sm.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kKtMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&sm.tmem)),
+                 "r"(kKtTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  KtCursor<MASK> cur;
+  if (a.split) {
+    cur.left = kv_find<MASK, kKtThreads>(a, sm.find, blockIdx.x);
+    cur.u = sm.find.unit;
+    cur.off = sm.find.off;
+  } else {
+    cur.u = a.units - 1 - (int)blockIdx.x;  // later rows see more keys: longest first
+    cur.off = 0;
+    cur.left = 0x3fffffff;
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = sm.tmem;
+
+  if (warp >= kKtConvert0 / 32 && warp < kKtMmaWarp) {
+    // ---------------- converters ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kKtRegConvert));
+    const int cw = warp - kKtConvert0 / 32, h = lane & 15;
+    float4 kr[16], vr[16];
+    auto load_k = [&](const KtCursor<MASK>& z) {
+      const float* kb = a.k + ((size_t)z.x.b * a.hkv + z.x.hk) * (size_t)a.max_t * kKvD;
+      const int j0 = z.c * kKvTileKeys + cw * 16 + (lane >> 4);
+      const bool plain = z.c * kKvTileKeys + kKvTileKeys <= (MASK == kMaskTree ? z.x.p : z.x.keys);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = j0 + 2 * i;
+        kr[2 * i] = kr[2 * i + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (plain || kt_row_there<MASK>(a, z.x, j)) {
+          const float4* row = reinterpret_cast<const float4*>(kb + (size_t)j * kKvD);
+          kr[2 * i] = row[h];
+          kr[2 * i + 1] = row[16 + h];
+        }
+      }
+    };
+    auto load_v = [&](const KtCursor<MASK>& z) {
+      const float* vb = a.v + ((size_t)z.x.b * a.hkv + z.x.hk) * (size_t)a.max_t * kKvD;
+      const int j0 = z.c * kKvTileKeys + cw * 16;
+      const bool plain = z.c * kKvTileKeys + kKvTileKeys <= (MASK == kMaskTree ? z.x.p : z.x.keys);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        vr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (plain || kt_row_there<MASK>(a, z.x, j0 + i))
+          vr[i] = reinterpret_cast<const float4*>(vb + (size_t)(j0 + i) * kKvD)[lane];
+      }
+    };
+    // The tile's largest magnitude over the four warps; `red` alternates, one barrier each.
+    auto tile_max = [&](unsigned mine, int which) {
+      mine = __reduce_max_sync(kFull, mine);
+      if (lane == 0) sm.red[which][cw] = mine;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      return max(max(sm.red[which][0], sm.red[which][1]), max(sm.red[which][2], sm.red[which][3]));
+    };
+    cur.seek(a);
+    if (cur.ok) {
+      load_k(cur);
+      load_v(cur);
+    }
+    // after a wait that ran out the loop goes on without waiting: the four warps meet at named
+    // barriers, so none may leave
+    bool dead = false;
+    for (int t = 0; cur.ok; ++t) {
+      const int s = t & 1;
+      float scale, inverse;
+      {  // K
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = mag(mag(mag(mag(m, kr[i].x), kr[i].y), kr[i].z), kr[i].w);
+        unsigned top = tile_max(__float_as_uint(m), 2 * s);
+        if (top >= 0x7f800000u) {  // an infinite key: the scale of the others
+          m = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            m = finite(kr[i].x) ? mag(m, kr[i].x) : m;
+            m = finite(kr[i].y) ? mag(m, kr[i].y) : m;
+            m = finite(kr[i].z) ? mag(m, kr[i].z) : m;
+            m = finite(kr[i].w) ? mag(m, kr[i].w) : m;
+          }
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          top = tile_max(__float_as_uint(m), 2 * s);
+        }
+        scale_of(top, scale, inverse);
+        if (t >= 2 && !dead) dead = !bar_wait(&sm.kfree[s], ((t >> 1) - 1) & 1, abort);
+        const float2 sc = make_float2(scale, scale);
+        uint8_t* dst = &sm.k[s][0][h >> 3][0];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = cw * 16 + 2 * i + (lane >> 4);
+          uint4 hi, lo;
+          split_f16(mul2(make_float2(kr[2 * i].x, kr[2 * i].y), sc), hi.x, lo.x);
+          split_f16(mul2(make_float2(kr[2 * i].z, kr[2 * i].w), sc), hi.y, lo.y);
+          split_f16(mul2(make_float2(kr[2 * i + 1].x, kr[2 * i + 1].y), sc), hi.z, lo.z);
+          split_f16(mul2(make_float2(kr[2 * i + 1].z, kr[2 * i + 1].w), sc), hi.w, lo.w);
+          const int at = r * 128 + (((h & 7) ^ (r & 7)) << 4);
+          *reinterpret_cast<uint4*>(dst + at) = hi;
+          *reinterpret_cast<uint4*>(dst + sizeof(sm.k[0][0]) + at) = lo;
+        }
+        if (cw == 0 && lane == 0) sm.ksc[t & 3] = inverse;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          bar_arrive(&sm.kfull[s]);
+          bar_arrive(&sm.kinfo[t & 3]);
+        }
+      }
+      cur.next(a);
+      if (cur.ok) load_k(cur);
+      {  // V
+        float m = 0.0f;
+        float2 z = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          m = mag(mag(mag(mag(m, vr[i].x), vr[i].y), vr[i].z), vr[i].w);
+          z = fma2(make_float2(vr[i].x, vr[i].y), make_float2(0.f, 0.f), z);  // NaN unless all are finite
+          z = fma2(make_float2(vr[i].z, vr[i].w), make_float2(0.f, 0.f), z);
+        }
+        if (cw == 0 && lane == 0) sm.vbad[t & 3] = 0;
+        unsigned top = tile_max(z.x + z.y == 0.0f ? __float_as_uint(m) : 0x7f800000u, 2 * s + 1);
+        if (top >= 0x7f800000u) {
+          // 0 * inf must not reach the rows that do not see the key: its value row leaves the
+          // product (0) and the rows that see it add it one by one
+          m = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const bool bad = __any_sync(kFull, !(finite(vr[i].x) && finite(vr[i].y) && finite(vr[i].z) && finite(vr[i].w)));
+            if (bad) {
+              vr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (lane == 0) atomicOr(&sm.vbad[t & 3], 1ull << (cw * 16 + i));
+            }
+            m = mag(mag(mag(mag(m, vr[i].x), vr[i].y), vr[i].z), vr[i].w);
+          }
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          top = tile_max(__float_as_uint(m), 2 * s + 1);
+        }
+        scale_of(top, scale, inverse);
+        if (t >= 2 && !dead) dead = !bar_wait(&sm.vfree[s], ((t >> 1) - 1) & 1, abort);
+        const float2 sc = make_float2(scale, scale);
+        uint8_t* dst = &sm.v[s][0][0];
+        const float* ve = reinterpret_cast<const float*>(vr);
+#pragma unroll
+        for (int gi = 0; gi < 2; ++gi)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {  // dimension 4 lane + e sits in row 32 e + lane
+            uint4 hi, lo;
+            const float* w = ve + gi * 32 + e;
+            split_f16(mul2(make_float2(w[0], w[4]), sc), hi.x, lo.x);
+            split_f16(mul2(make_float2(w[8], w[12]), sc), hi.y, lo.y);
+            split_f16(mul2(make_float2(w[16], w[20]), sc), hi.z, lo.z);
+            split_f16(mul2(make_float2(w[24], w[28]), sc), hi.w, lo.w);
+            const int at = (32 * e + lane) * 128 + (((cw * 2 + gi) ^ (lane & 7)) << 4);
+            *reinterpret_cast<uint4*>(dst + at) = hi;
+            *reinterpret_cast<uint4*>(dst + sizeof(sm.v[0][0]) + at) = lo;
+          }
+        if (cw == 0 && lane == 0) sm.vsc[t & 3] = inverse;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          bar_arrive(&sm.vfull[s]);
+          bar_arrive(&sm.vinfo[t & 3]);
+        }
+      }
+      if (cur.ok) load_v(cur);
+    }
+  } else if (warp >= kKtMmaWarp) {
+    // ---------------- MMA issue ----------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kKtRegMma));
+    if (warp == kKtMmaWarp) {
+    constexpr uint32_t id_qk = kt_idesc(kKvTileKeys), id_pv = kt_idesc(kKvD);
+    bool ok = true;
+    int t = 0, units = 0;
+    auto pv = [&](int w) {  // O = P V of tile w
+      const int s = w & 1;
+      if (!bar_wait(&sm.vfull[s], (w >> 1) & 1, abort)) return false;
+      if (!bar_wait(&sm.pfull[s], (w >> 1) & 1, abort)) return false;
+      if (w > 0 && !bar_wait(&sm.ofree, (w - 1) & 1, abort)) return false;
+      tc_after();
+      const uint64_t vh = desc_sw128(sm.v[s][0]), vl = desc_sw128(sm.v[s][1]);
+      const uint32_t ph = tmem + kTmP + 64 * s, pl = ph + 32, o = tmem + kTmO;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) mma_ts(o, pl + 8 * kk, vh + 2 * kk, id_pv, kk > 0);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) mma_ts(o, ph + 8 * kk, vl + 2 * kk, id_pv, 1);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) mma_ts(o, ph + 8 * kk, vh + 2 * kk, id_pv, 1);
+      mma_commit(&sm.vfree[s]);
+      mma_commit(&sm.ofull);
+      return true;
+    };
+    cur.seek(a);
+    while (ok && cur.ok) {
+      const int n = cur.c1 - cur.c;
+      ok = bar_wait(&sm.qfull, units & 1, abort);
+      for (int i = 0; ok && i < n; ++i, ++t) {
+        const int s = t & 1;
+        ok = bar_wait(&sm.kfull[s], (t >> 1) & 1, abort);
+        if (!ok) break;
+        tc_after();
+        const uint64_t kh0 = desc_sw128(sm.k[s][0][0]), kh1 = desc_sw128(sm.k[s][0][1]);
+        const uint64_t kl0 = desc_sw128(sm.k[s][1][0]), kl1 = desc_sw128(sm.k[s][1][1]);
+        const uint32_t qh = tmem + kTmQ, ql = qh + 64, d = tmem + kTmS + 64 * s;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) mma_ts(d, ql + 8 * kk, (kk < 4 ? kh0 : kh1) + 2 * (kk & 3), id_qk, kk > 0);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) mma_ts(d, qh + 8 * kk, (kk < 4 ? kl0 : kl1) + 2 * (kk & 3), id_qk, 1);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) mma_ts(d, qh + 8 * kk, (kk < 4 ? kh0 : kh1) + 2 * (kk & 3), id_qk, 1);
+        mma_commit(&sm.kfree[s]);
+        mma_commit(&sm.sfull[s]);
+        if (i > 0) ok = pv(t - 1);
+      }
+      if (ok) ok = pv(t - 1);
+      ++units;
+      cur.c = cur.c1 - 1;
+      cur.next(a);
+    }
+    // nothing of this CTA's may be at work in shared memory or TMEM when it ends
+    mma_commit(&sm.done);
+    mb_wait_ns(su32(&sm.done), 0, kDrainLimitNs, nullptr);
+    }
+  } else {
+    // ---------------- softmax, output ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kKtRegSoftmax));
+    const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
+    const int row = tid;
+    int t = 0;
+    bool ok = true;
+    if (!a.split) {  // a unit without keys has no tiles
+      const KvUnit x = kv_unit<MASK>(a, cur.u);
+      if (x.chunks == 0 && row < x.nrows) {
+        float4* dst = reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, row));
+        for (int i = 0; i < kKvD / 4; ++i) dst[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (a.lse) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] = INFINITY;
+      }
+    }
+    cur.seek(a);
+    while (cur.ok) {
+      const KvUnit x = cur.x;
+      const int c0 = cur.c, n = cur.c1 - cur.c;
+      const bool valid = kv_row_valid<MASK>(a, x, row);
+      const int token = kv_token<MASK>(a, x, min(row, x.nrows - 1));
+      // the query row: scaled hi / lo to TMEM, dimensions in the order of the K tiles
+      float qinv;
+      {
+        const float4* qr = reinterpret_cast<const float4*>(a.q + kv_row_offset<MASK>(a, x, min(row, x.nrows - 1)));
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float4 v = qr[i];
+          m = mag(mag(mag(mag(m, v.x), v.y), v.z), v.w);
+        }
+        float scale;
+        scale_of(min(__float_as_uint(m), 0x7f7fffffu), scale, qinv);
+        const float2 sc = make_float2(scale, scale);
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          uint32_t hi[32], lo[32];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 v = qr[part * 8 + i], w = qr[16 + part * 8 + i];
+            split_f16(mul2(make_float2(v.x, v.y), sc), hi[4 * i], lo[4 * i]);
+            split_f16(mul2(make_float2(v.z, v.w), sc), hi[4 * i + 1], lo[4 * i + 1]);
+            split_f16(mul2(make_float2(w.x, w.y), sc), hi[4 * i + 2], lo[4 * i + 2]);
+            split_f16(mul2(make_float2(w.z, w.w), sc), hi[4 * i + 3], lo[4 * i + 3]);
+          }
+          tm_st32(mine + kTmQ + 32 * part, hi);
+          tm_st32(mine + kTmQ + 64 + 32 * part, lo);
+        }
+        tm_wait_st();
+        tc_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&sm.qfull);
+      }
+      float2 o[64];
+#pragma unroll
+      for (int i = 0; i < 64; ++i) o[i] = make_float2(0.f, 0.f);
+      float m = -INFINITY, l = 0.0f, corr = 0.0f;
+      const int open = MASK == kMaskTree ? x.p : x.p + x.i0 + 1;
+      // o = o * f + the O tile of tile w, whose P stood against the maximum of then
+      auto add_o = [&](int w, int c, float f) {
+        if (!bar_wait(&sm.vinfo[w & 3], (w >> 2) & 1, abort)) return false;
+        const float fv = sm.vsc[w & 3];
+        const unsigned long long bad = sm.vbad[w & 3];
+        if (!bar_wait(&sm.ofull, w & 1, abort)) return false;
+        tc_after();
+        const float2 f2 = make_float2(f, f), v2 = make_float2(fv, fv);
+#pragma unroll
+        for (int part = 0; part < 8; ++part) {
+          uint32_t r[16];
+          tm_ld16(mine + kTmO + 16 * part, r);
+          tm_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            o[part * 8 + i] =
+                fma2(o[part * 8 + i], f2,
+                     mul2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), v2));
+        }
+        if (bad) {
+          const float4* vb = reinterpret_cast<const float4*>(
+              a.v + (((size_t)x.b * a.hkv + x.hk) * (size_t)a.max_t + (size_t)c * kKvTileKeys) * kKvD);
+          for (int key = 0; key < kKvTileKeys; ++key) {
+            if (!((bad >> key) & 1)) continue;
+            const uint32_t hi = tm_ld1(mine + kTmP + 64 * (w & 1) + (key >> 1));
+            const uint32_t lo = tm_ld1(mine + kTmP + 64 * (w & 1) + 32 + (key >> 1));
+            tm_wait_ld();
+            const int sh = (key & 1) * 16;
+            const float p = __half2float(__ushort_as_half((unsigned short)(hi >> sh))) +
+                            __half2float(__ushort_as_half((unsigned short)(lo >> sh)));
+            if (p == 0.0f) continue;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float4 v = vb[(size_t)key * 32 + i];
+              float* e0 = &o[i >> 1].x + (i & 1);
+              float* e1 = &o[16 + (i >> 1)].x + (i & 1);
+              float* e2 = &o[32 + (i >> 1)].x + (i & 1);
+              float* e3 = &o[48 + (i >> 1)].x + (i & 1);
+              *e0 = fmaf(p, v.x, *e0);
+              *e1 = fmaf(p, v.y, *e1);
+              *e2 = fmaf(p, v.z, *e2);
+              *e3 = fmaf(p, v.w, *e3);
+            }
+          }
+          __syncwarp();
+        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&sm.ofree);
+        return true;
+      };
+      for (int i = 0; i < n; ++i, ++t) {
+        const int s = t & 1, j0 = (c0 + i) * kKvTileKeys;
+        ok = bar_wait(&sm.kinfo[t & 3], (t >> 2) & 1, abort);
+        if (!ok) break;
+        const float cc = a.c * qinv * sm.ksc[t & 3];
+        unsigned long long see = ~0ull;  // columns the row sees
+        const bool masked = j0 + kKvTileKeys > open;
+        if (masked) {
+          if (MASK == kMaskTree) {
+            const int e0 = j0 - x.p;  // node number of column 0
+            see = e0 <= -kKvTileKeys ? ~0ull : e0 < 0 ? (1ull << -e0) - 1 : 0ull;
+            const uint32_t* anc = a.anc + ((size_t)x.b * a.n + token) * a.words;
+            for (int w = max(0, e0 >> 5); w < a.words && w * 32 - e0 < kKvTileKeys; ++w) {
+              const int sh = w * 32 - e0;
+              see |= sh >= 0 ? (unsigned long long)anc[w] << sh : (unsigned long long)(anc[w] >> -sh);
+            }
+          } else {
+            const int lim = min(x.p + token + 1, x.keys) - j0;
+            see = lim >= kKvTileKeys ? ~0ull : lim <= 0 ? 0ull : (1ull << lim) - 1;
+          }
+        }
+        ok = bar_wait(&sm.sfull[s], (t >> 1) & 1, abort);
+        if (!ok) break;
+        tc_after();
+        float top = -INFINITY;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          uint32_t r[32];
+          tm_ld32(mine + kTmS + 64 * s + 32 * part, r);
+          tm_wait_ld();
+          const uint32_t bits = (uint32_t)(see >> (32 * part));
+          if (!masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(r[e]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if ((bits >> e) & 1u) top = fmaxf(top, __uint_as_float(r[e]));
+          }
+        }
+        const float n_m = top == -INFINITY ? m : fmaxf(m, top * cc);
+        const float base = n_m == -INFINITY ? 0.0f : n_m;
+        const float next = ex2(m - base);
+        m = n_m;
+        const float2 c2 = make_float2(cc, cc), b2 = make_float2(kKtPScale - base, kKtPScale - base);
+        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int part = 0; part < 4; ++part) {
+          uint32_t r[16], hi[8], lo[8];
+          tm_ld16(mine + kTmS + 64 * s + 16 * part, r);
+          tm_wait_ld();
+          const uint32_t bits = (uint32_t)(see >> (16 * part));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float2 p = fma2(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), c2, b2);
+            p.x = ex2(p.x);
+            p.y = ex2(p.y);
+            if (masked) {
+              if (!((bits >> (2 * e)) & 1u)) p.x = 0.0f;
+              if (!((bits >> (2 * e + 1)) & 1u)) p.y = 0.0f;
+            }
+            sum.x += p.x;
+            sum.y += p.y;
+            split_f16(p, hi[e], lo[e]);
+          }
+          tm_st8(mine + kTmP + 64 * s + 8 * part, hi);
+          tm_st8(mine + kTmP + 64 * s + 32 + 8 * part, lo);
+        }
+        tm_wait_st();
+        tc_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&sm.pfull[s]);
+        l = fmaf(l, next, sum.x + sum.y);
+        if (i > 0) {
+          ok = add_o(t - 1, c0 + i - 1, corr);
+          if (!ok) break;
+        }
+        corr = next;
+      }
+      if (ok) ok = add_o(t - 1, c0 + n - 1, corr);
+      // the row: whole, or this CTA's part of it
+      const bool whole = c0 == 0 && n == x.chunks;
+      const size_t slot = a.split ? (size_t)blockIdx.x + cur.u : (size_t)cur.u;
+      const float nan = __uint_as_float(0x7fffffffu);
+      if (!valid) m = -INFINITY;
+      if (row < x.nrows) {
+        constexpr float kUnscale = 1.0f / (1 << kKtPScale);  // P' = 2^14 p is in both sums
+        float f = kUnscale;
+        if (whole) f = m == -INFINITY ? 0.0f : __fdiv_rn(1.0f, l);
+        if (!ok) f = nan;
+        float4* dst = reinterpret_cast<float4*>(whole ? a.out + kv_row_offset<MASK>(a, x, row)
+                                                      : a.acc + (slot * a.rows + row) * kKvD);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float e0 = i & 1 ? o[i >> 1].y : o[i >> 1].x, e1 = i & 1 ? o[16 + (i >> 1)].y : o[16 + (i >> 1)].x;
+          const float e2 = i & 1 ? o[32 + (i >> 1)].y : o[32 + (i >> 1)].x;
+          const float e3 = i & 1 ? o[48 + (i >> 1)].y : o[48 + (i >> 1)].x;
+          dst[i] = f == 0.0f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(e0 * f, e1 * f, e2 * f, e3 * f);
+        }
+        if (a.stat) {
+          a.stat[slot * 2 * a.rows + row] = m;
+          a.stat[(slot * 2 + 1) * a.rows + row] = ok ? l * kUnscale : nan;
+        }
+        if (a.lse && whole)
+          a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] =
+              m == -INFINITY ? INFINITY : m + log2f(l) - kKtPScale;
+      }
+      if (!ok) break;
+      cur.c = cur.c1 - 1;
+      cur.next(a);
+    }
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  if (warp == kKtMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kKtTmemCols) : "memory");
+}
+
+template <int MASK>
+cudaError_t launch_tile(const KvArgs& a, int device, cudaStream_t s) {
+  static int configured[128] = {0};
+  const size_t smem = sizeof(KtSmem) + 1024;
+  cudaError_t e = ensure_smem((const void*)kv_tile_kernel<MASK>, configured, device, smem, false);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.split ? kKvGrid : a.units));
+  cfg.blockDim = dim3(kKtThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kv_tile_kernel<MASK>, a, wait_limit_ns());
+}
+
+}  // namespace
+
+cudaError_t launch_kv_tile(const KvArgs& a, int mask, int device, cudaStream_t s) {
+  return mask == kMaskTree ? launch_tile<kMaskTree>(a, device, s) : launch_tile<kMaskCausal>(a, device, s);
+}
+
+cudaError_t read_kv_tile_fault(unsigned int* flags, bool clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(flags, g_kv_tile_fault, sizeof(unsigned int));
+  if (e == cudaSuccess && clear) {
+    const unsigned int z = 0;
+    e = cudaMemcpyToSymbol(g_kv_tile_fault, &z, sizeof(z));
+  }
+  return e;
+}
+
+}  // namespace q8lin
