@@ -131,7 +131,7 @@ __device__ __forceinline__ bool kv_sees(const KvArgs& a, const KvUnit& x, int r,
 }
 
 struct KvFind {
-  int seg[16];  // chunk sums of the warps
+  int seg[32];  // chunk sums of the warps
   int unit, off;
 };
 

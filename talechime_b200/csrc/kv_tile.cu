@@ -8,13 +8,14 @@
 // element is off by at most 2^-22 of itself or 2^-39 of its tile's largest, and the dropped lo.lo
 // is 2^-20 of a product at most, 2^-22 on average.  Scaling makes f32's exponent range fit.
 //
-// One CTA per SM, nine working warps:
-//   * 4 convert: cache rows to registers one tile ahead, then scaled hi / lo to swizzled shared
+// One CTA per SM, 17 working warps:
+//   * 8 convert: cache rows to registers one tile ahead, then scaled hi / lo to swizzled shared
 //     memory, K as [64 keys][128 dims], V transposed as [128 dims][64 keys], two stages each;
 //   * 1 issues the MMAs: S = Q K^T (Q in TMEM), O = P V (P in TMEM), S and P double-buffered,
 //     so that QK of a tile runs while the softmax of the one before is at work;
-//   * 4 softmax: a thread owns a row; scores from TMEM, running maximum and sum, P' = 2^14 p
-//     back to TMEM as hi / lo; then the O tile of the tile before is added to 128 registers.
+//   * 8 softmax: two threads a row, one for each half of the keys and then of the dimensions;
+//     scores from TMEM, running maximum and sum, P' = 2^14 p back to TMEM as hi / lo; then the
+//     O tile of the tile before is added to registers.
 // The tensor cores cut their f32 sums, so an O tile starts from 0 and joins the running sum with
 // rounding.  TMEM (512 columns): Q 128, S 2 x 64, P 2 x 64, O 128.
 //
@@ -30,11 +31,10 @@ namespace q8lin {
 
 namespace {
 
-constexpr int kKtThreads = 384;   // three warpgroups: softmax, converters, MMA (one of its warps)
-// Registers of a thread: 384 x 168 at launch, then 240 + 208 + 56 = 3 x 168.
-constexpr int kKtRegSoftmax = 240, kKtRegConvert = 208, kKtRegMma = 56;
-constexpr int kKtConvert0 = 128;  // first converter thread
-constexpr int kKtMmaWarp = 8;
+constexpr int kKtThreads = 640;   // five warpgroups: 2 softmax, 2 converters, MMA (one of its warps)
+constexpr int kKtConvertWarp = 8, kKtMmaWarp = 16;
+// Registers of a thread: 640 x 96 at launch, then 2 x 120 + 2 x 96 + 48 = 5 x 96.
+constexpr int kKtRegSoftmax = 120, kKtRegMma = 48;
 constexpr uint32_t kKtTmemCols = 512;
 constexpr uint32_t kTmQ = 0, kTmS = 128, kTmP = 256, kTmO = 384;
 constexpr int kKtPScale = 14;     // P' = 2^14 p
@@ -47,7 +47,8 @@ struct KtSmem {
   alignas(1024) uint8_t v[2][2][kKvD * 128];            // [stage][hi, lo][dim][64 keys]
   float ksc[4], vsc[4];                                 // inverse scales of tiles t % 4
   unsigned long long vbad[4];                           // keys of the tile whose value row is not finite
-  unsigned red[4][4];                                   // the converters' maxima
+  alignas(16) unsigned red[4][8];                                   // the converters' maxima
+  float top[2][2][kKvTileRows];                         // the rows' maxima over either half of a tile
   alignas(8) uint64_t kfull[2], kfree[2], vfull[2], vfree[2];
   uint64_t kinfo[4], vinfo[4];
   uint64_t sfull[2], pfull[2], qfull, ofull, ofree, done;
@@ -117,15 +118,6 @@ __device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t (&r)[32]) {
       : "r"(addr)
       : "memory");
 #undef KT_OUT
-}
-__device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t (&r)[32]) {
-#define KT_IN(i) "r"(r[i])
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::KT_R32(KT_IN),
-      "r"(addr)
-      : "memory");
-#undef KT_IN
 }
 __device__ __forceinline__ void tm_ld16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
@@ -240,20 +232,20 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
   if (tid == 0) {
     s_kt_wait_ns = wait_ns;
     for (int i = 0; i < 2; ++i) {
-      bar_init(&sm.kfull[i], 4);
+      bar_init(&sm.kfull[i], 8);
       bar_init(&sm.kfree[i], 1);
-      bar_init(&sm.vfull[i], 4);
+      bar_init(&sm.vfull[i], 8);
       bar_init(&sm.vfree[i], 1);
       bar_init(&sm.sfull[i], 1);
-      bar_init(&sm.pfull[i], 4);
+      bar_init(&sm.pfull[i], 8);
     }
     for (int i = 0; i < 4; ++i) {
-      bar_init(&sm.kinfo[i], 4);
-      bar_init(&sm.vinfo[i], 4);
+      bar_init(&sm.kinfo[i], 8);
+      bar_init(&sm.vinfo[i], 8);
     }
-    bar_init(&sm.qfull, 4);
+    bar_init(&sm.qfull, 8);
     bar_init(&sm.ofull, 1);
-    bar_init(&sm.ofree, 4);
+    bar_init(&sm.ofree, 8);
     bar_init(&sm.done, 1);
     sm.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -280,50 +272,57 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
   tc_after();
   const uint32_t tmem = sm.tmem;
 
-  if (warp >= kKtConvert0 / 32 && warp < kKtMmaWarp) {
+  if (warp >= kKtConvertWarp && warp < kKtMmaWarp) {
     // ---------------- converters ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kKtRegConvert));
-    const int cw = warp - kKtConvert0 / 32, h = lane & 15;
-    float4 kr[16], vr[16];
+    const int cw = warp - kKtConvertWarp, h = lane & 15;
+    float4 kr[8], vr[8];  // this warp's 8 keys and values of a tile
     auto load_k = [&](const KtCursor<MASK>& z) {
       const float* kb = a.k + ((size_t)z.x.b * a.hkv + z.x.hk) * (size_t)a.max_t * kKvD;
-      const int j0 = z.c * kKvTileKeys + cw * 16 + (lane >> 4);
-      const bool plain = z.c * kKvTileKeys + kKvTileKeys <= (MASK == kMaskTree ? z.x.p : z.x.keys);
+      const int j0 = z.c * kKvTileKeys + cw * 8 + (lane >> 4);
+      const float4* row = reinterpret_cast<const float4*>(kb + (size_t)j0 * kKvD) + h;
+      if (z.c * kKvTileKeys + kKvTileKeys <= (MASK == kMaskTree ? z.x.p : z.x.keys)) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int j = j0 + 2 * i;
-        kr[2 * i] = kr[2 * i + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (plain || kt_row_there<MASK>(a, z.x, j)) {
-          const float4* row = reinterpret_cast<const float4*>(kb + (size_t)j * kKvD);
-          kr[2 * i] = row[h];
-          kr[2 * i + 1] = row[16 + h];
+        for (int i = 0; i < 4; ++i) {
+          kr[2 * i] = row[i * 64];
+          kr[2 * i + 1] = row[i * 64 + 16];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool there = kt_row_there<MASK>(a, z.x, j0 + 2 * i);
+          kr[2 * i] = there ? row[i * 64] : make_float4(0.f, 0.f, 0.f, 0.f);
+          kr[2 * i + 1] = there ? row[i * 64 + 16] : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
     };
     auto load_v = [&](const KtCursor<MASK>& z) {
       const float* vb = a.v + ((size_t)z.x.b * a.hkv + z.x.hk) * (size_t)a.max_t * kKvD;
-      const int j0 = z.c * kKvTileKeys + cw * 16;
-      const bool plain = z.c * kKvTileKeys + kKvTileKeys <= (MASK == kMaskTree ? z.x.p : z.x.keys);
+      const int j0 = z.c * kKvTileKeys + cw * 8;
+      const float4* row = reinterpret_cast<const float4*>(vb + (size_t)j0 * kKvD) + lane;
+      if (z.c * kKvTileKeys + kKvTileKeys <= (MASK == kMaskTree ? z.x.p : z.x.keys)) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        vr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (plain || kt_row_there<MASK>(a, z.x, j0 + i))
-          vr[i] = reinterpret_cast<const float4*>(vb + (size_t)(j0 + i) * kKvD)[lane];
+        for (int i = 0; i < 8; ++i) vr[i] = row[i * 32];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          vr[i] = kt_row_there<MASK>(a, z.x, j0 + i) ? row[i * 32] : make_float4(0.f, 0.f, 0.f, 0.f);
       }
     };
-    // The tile's largest magnitude over the four warps; `red` alternates, one barrier each.
+    // The tile's largest magnitude over the warps; `red` alternates, one barrier each.
     auto tile_max = [&](unsigned mine, int which) {
       mine = __reduce_max_sync(kFull, mine);
       if (lane == 0) sm.red[which][cw] = mine;
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      return max(max(sm.red[which][0], sm.red[which][1]), max(sm.red[which][2], sm.red[which][3]));
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      const uint4 x = *reinterpret_cast<const uint4*>(&sm.red[which][0]);
+      const uint4 y = *reinterpret_cast<const uint4*>(&sm.red[which][4]);
+      return max(max(max(x.x, x.y), max(x.z, x.w)), max(max(y.x, y.y), max(y.z, y.w)));
     };
     cur.seek(a);
     if (cur.ok) {
       load_k(cur);
       load_v(cur);
     }
-    // after a wait that ran out the loop goes on without waiting: the four warps meet at named
+    // after a wait that ran out the loop goes on without waiting: the warps meet at named
     // barriers, so none may leave
     bool dead = false;
     for (int t = 0; cur.ok; ++t) {
@@ -332,18 +331,18 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       {  // K
         float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) m = mag(mag(mag(mag(m, kr[i].x), kr[i].y), kr[i].z), kr[i].w);
+        for (int i = 0; i < 8; ++i) m = mag(mag(mag(mag(m, kr[i].x), kr[i].y), kr[i].z), kr[i].w);
         unsigned top = tile_max(__float_as_uint(m), 2 * s);
         if (top >= 0x7f800000u) {  // an infinite key: the scale of the others
           m = 0.0f;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < 8; ++i) {
             m = finite(kr[i].x) ? mag(m, kr[i].x) : m;
             m = finite(kr[i].y) ? mag(m, kr[i].y) : m;
             m = finite(kr[i].z) ? mag(m, kr[i].z) : m;
             m = finite(kr[i].w) ? mag(m, kr[i].w) : m;
           }
-          asm volatile("bar.sync 1, 128;" ::: "memory");
+          asm volatile("bar.sync 1, 256;" ::: "memory");
           top = tile_max(__float_as_uint(m), 2 * s);
         }
         scale_of(top, scale, inverse);
@@ -351,8 +350,8 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         const float2 sc = make_float2(scale, scale);
         uint8_t* dst = &sm.k[s][0][h >> 3][0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = cw * 16 + 2 * i + (lane >> 4);
+        for (int i = 0; i < 4; ++i) {
+          const int r = cw * 8 + 2 * i + (lane >> 4);
           uint4 hi, lo;
           split_f16(mul2(make_float2(kr[2 * i].x, kr[2 * i].y), sc), hi.x, lo.x);
           split_f16(mul2(make_float2(kr[2 * i].z, kr[2 * i].w), sc), hi.y, lo.y);
@@ -376,7 +375,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         float m = 0.0f;
         float2 z = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < 8; ++i) {
           m = mag(mag(mag(mag(m, vr[i].x), vr[i].y), vr[i].z), vr[i].w);
           z = fma2(make_float2(vr[i].x, vr[i].y), make_float2(0.f, 0.f), z);  // NaN unless all are finite
           z = fma2(make_float2(vr[i].z, vr[i].w), make_float2(0.f, 0.f), z);
@@ -388,36 +387,35 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
           // product (0) and the rows that see it add it one by one
           m = 0.0f;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < 8; ++i) {
             const bool bad = __any_sync(kFull, !(finite(vr[i].x) && finite(vr[i].y) && finite(vr[i].z) && finite(vr[i].w)));
             if (bad) {
               vr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (lane == 0) atomicOr(&sm.vbad[t & 3], 1ull << (cw * 16 + i));
+              if (lane == 0) atomicOr(&sm.vbad[t & 3], 1ull << (cw * 8 + i));
             }
             m = mag(mag(mag(mag(m, vr[i].x), vr[i].y), vr[i].z), vr[i].w);
           }
-          asm volatile("bar.sync 1, 128;" ::: "memory");
+          asm volatile("bar.sync 1, 256;" ::: "memory");
           top = tile_max(__float_as_uint(m), 2 * s + 1);
         }
         scale_of(top, scale, inverse);
         if (t >= 2 && !dead) dead = !bar_wait(&sm.vfree[s], ((t >> 1) - 1) & 1, abort);
         const float2 sc = make_float2(scale, scale);
         uint8_t* dst = &sm.v[s][0][0];
-        const float* ve = reinterpret_cast<const float*>(vr);
-#pragma unroll
-        for (int gi = 0; gi < 2; ++gi)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {  // dimension 4 lane + e sits in row 32 e + lane
-            uint4 hi, lo;
-            const float* w = ve + gi * 32 + e;
-            split_f16(mul2(make_float2(w[0], w[4]), sc), hi.x, lo.x);
-            split_f16(mul2(make_float2(w[8], w[12]), sc), hi.y, lo.y);
-            split_f16(mul2(make_float2(w[16], w[20]), sc), hi.z, lo.z);
-            split_f16(mul2(make_float2(w[24], w[28]), sc), hi.w, lo.w);
-            const int at = (32 * e + lane) * 128 + (((cw * 2 + gi) ^ (lane & 7)) << 4);
-            *reinterpret_cast<uint4*>(dst + at) = hi;
-            *reinterpret_cast<uint4*>(dst + sizeof(sm.v[0][0]) + at) = lo;
-          }
+        auto put = [&](int e, const float (&w)[8]) {  // dimension 4 lane + e sits in row 32 e + lane
+          uint4 hi, lo;
+          split_f16(mul2(make_float2(w[0], w[1]), sc), hi.x, lo.x);
+          split_f16(mul2(make_float2(w[2], w[3]), sc), hi.y, lo.y);
+          split_f16(mul2(make_float2(w[4], w[5]), sc), hi.z, lo.z);
+          split_f16(mul2(make_float2(w[6], w[7]), sc), hi.w, lo.w);
+          const int at = (32 * e + lane) * 128 + ((cw ^ (lane & 7)) << 4);
+          *reinterpret_cast<uint4*>(dst + at) = hi;
+          *reinterpret_cast<uint4*>(dst + sizeof(sm.v[0][0]) + at) = lo;
+        };
+        put(0, {vr[0].x, vr[1].x, vr[2].x, vr[3].x, vr[4].x, vr[5].x, vr[6].x, vr[7].x});
+        put(1, {vr[0].y, vr[1].y, vr[2].y, vr[3].y, vr[4].y, vr[5].y, vr[6].y, vr[7].y});
+        put(2, {vr[0].z, vr[1].z, vr[2].z, vr[3].z, vr[4].z, vr[5].z, vr[6].z, vr[7].z});
+        put(3, {vr[0].w, vr[1].w, vr[2].w, vr[3].w, vr[4].w, vr[5].w, vr[6].w, vr[7].w});
         if (cw == 0 && lane == 0) sm.vsc[t & 3] = inverse;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -487,13 +485,21 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
   } else {
     // ---------------- softmax, output ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kKtRegSoftmax));
-    const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
-    const int row = tid;
+    // thread (row, half): keys 32 half .. + 32 of a tile, output columns 64 half .. + 64, which are
+    // dimensions 4 i + 2 half and 4 i + 2 half + 1 (i < 32)
+    const int row = tid & 127, half = tid >> 7;
+    const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     int t = 0;
+    // after a wait that ran out the loops go on without waiting (the two warps of a row meet at
+    // named barriers) and the rows get NaN
     bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (ok) ok = bar_wait(bar, parity, abort);
+    };
+    auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory"); };
     if (!a.split) {  // a unit without keys has no tiles
       const KvUnit x = kv_unit<MASK>(a, cur.u);
-      if (x.chunks == 0 && row < x.nrows) {
+      if (x.chunks == 0 && row < x.nrows && half == 0) {
         float4* dst = reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, row));
         for (int i = 0; i < kKvD / 4; ++i) dst[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (a.lse) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] = INFINITY;
@@ -503,14 +509,13 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
     while (cur.ok) {
       const KvUnit x = cur.x;
       const int c0 = cur.c, n = cur.c1 - cur.c;
-      const bool valid = kv_row_valid<MASK>(a, x, row);
       const int token = kv_token<MASK>(a, x, min(row, x.nrows - 1));
-      // the query row: scaled hi / lo to TMEM, dimensions in the order of the K tiles
+      // half of the query row: scaled hi / lo to TMEM, dimensions in the order of the K tiles
       float qinv;
       {
         const float4* qr = reinterpret_cast<const float4*>(a.q + kv_row_offset<MASK>(a, x, min(row, x.nrows - 1)));
         float m = 0.0f;
-#pragma unroll
+#pragma unroll 8
         for (int i = 0; i < 32; ++i) {
           const float4 v = qr[i];
           m = mag(mag(mag(mag(m, v.x), v.y), v.z), v.w);
@@ -519,50 +524,50 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         scale_of(min(__float_as_uint(m), 0x7f7fffffu), scale, qinv);
         const float2 sc = make_float2(scale, scale);
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          uint32_t hi[32], lo[32];
+        for (int part = 0; part < 4; ++part) {
+          uint32_t hi[8], lo[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 v = qr[part * 8 + i], w = qr[16 + part * 8 + i];
+          for (int i = 0; i < 2; ++i) {
+            const float4 v = qr[half * 8 + part * 2 + i], w = qr[16 + half * 8 + part * 2 + i];
             split_f16(mul2(make_float2(v.x, v.y), sc), hi[4 * i], lo[4 * i]);
             split_f16(mul2(make_float2(v.z, v.w), sc), hi[4 * i + 1], lo[4 * i + 1]);
             split_f16(mul2(make_float2(w.x, w.y), sc), hi[4 * i + 2], lo[4 * i + 2]);
             split_f16(mul2(make_float2(w.z, w.w), sc), hi[4 * i + 3], lo[4 * i + 3]);
           }
-          tm_st32(mine + kTmQ + 32 * part, hi);
-          tm_st32(mine + kTmQ + 64 + 32 * part, lo);
+          tm_st8(mine + kTmQ + 32 * half + 8 * part, hi);
+          tm_st8(mine + kTmQ + 64 + 32 * half + 8 * part, lo);
         }
         tm_wait_st();
         tc_before();
         __syncwarp();
         if (lane == 0) bar_arrive(&sm.qfull);
       }
-      float2 o[64];
+      float2 o[32];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) o[i] = make_float2(0.f, 0.f);
+      for (int i = 0; i < 32; ++i) o[i] = make_float2(0.f, 0.f);
       float m = -INFINITY, l = 0.0f, corr = 0.0f;
       const int open = MASK == kMaskTree ? x.p : x.p + x.i0 + 1;
-      // o = o * f + the O tile of tile w, whose P stood against the maximum of then
+      // o = o * f + the O tile of tile w (cache tile c), whose P stood against the maximum of then
       auto add_o = [&](int w, int c, float f) {
-        if (!bar_wait(&sm.vinfo[w & 3], (w >> 2) & 1, abort)) return false;
+        wait(&sm.vinfo[w & 3], (w >> 2) & 1);
         const float fv = sm.vsc[w & 3];
         const unsigned long long bad = sm.vbad[w & 3];
-        if (!bar_wait(&sm.ofull, w & 1, abort)) return false;
+        wait(&sm.ofull, w & 1);
         tc_after();
         const float2 f2 = make_float2(f, f), v2 = make_float2(fv, fv);
 #pragma unroll
-        for (int part = 0; part < 8; ++part) {
-          uint32_t r[16];
-          tm_ld16(mine + kTmO + 16 * part, r);
+        for (int part = 0; part < 2; ++part) {
+          uint32_t r[32];
+          tm_ld32(mine + kTmO + 64 * half + 32 * part, r);
           tm_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            o[part * 8 + i] =
-                fma2(o[part * 8 + i], f2,
+          for (int i = 0; i < 16; ++i)
+            o[part * 16 + i] =
+                fma2(o[part * 16 + i], f2,
                      mul2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), v2));
         }
         if (bad) {
-          const float4* vb = reinterpret_cast<const float4*>(
+          const float2* vb = reinterpret_cast<const float2*>(
               a.v + (((size_t)x.b * a.hkv + x.hk) * (size_t)a.max_t + (size_t)c * kKvTileKeys) * kKvD);
           for (int key = 0; key < kKvTileKeys; ++key) {
             if (!((bad >> key) & 1)) continue;
@@ -572,67 +577,63 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
             const int sh = (key & 1) * 16;
             const float p = __half2float(__ushort_as_half((unsigned short)(hi >> sh))) +
                             __half2float(__ushort_as_half((unsigned short)(lo >> sh)));
-            if (p == 0.0f) continue;
+            if (p != 0.0f) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float4 v = vb[(size_t)key * 32 + i];
-              float* e0 = &o[i >> 1].x + (i & 1);
-              float* e1 = &o[16 + (i >> 1)].x + (i & 1);
-              float* e2 = &o[32 + (i >> 1)].x + (i & 1);
-              float* e3 = &o[48 + (i >> 1)].x + (i & 1);
-              *e0 = fmaf(p, v.x, *e0);
-              *e1 = fmaf(p, v.y, *e1);
-              *e2 = fmaf(p, v.z, *e2);
-              *e3 = fmaf(p, v.w, *e3);
+              for (int i = 0; i < 16; ++i) {
+                const float2 v = vb[(size_t)key * 64 + 4 * i + half], w2 = vb[(size_t)key * 64 + 4 * i + 2 + half];
+                o[i].x = fmaf(p, v.x, o[i].x);
+                o[i].y = fmaf(p, w2.x, o[i].y);
+                o[16 + i].x = fmaf(p, v.y, o[16 + i].x);
+                o[16 + i].y = fmaf(p, w2.y, o[16 + i].y);
+              }
             }
+            __syncwarp();
           }
-          __syncwarp();
         }
         tc_before();
         __syncwarp();
         if (lane == 0) bar_arrive(&sm.ofree);
-        return true;
       };
       for (int i = 0; i < n; ++i, ++t) {
         const int s = t & 1, j0 = (c0 + i) * kKvTileKeys;
-        ok = bar_wait(&sm.kinfo[t & 3], (t >> 2) & 1, abort);
-        if (!ok) break;
+        wait(&sm.kinfo[t & 3], (t >> 2) & 1);
         const float cc = a.c * qinv * sm.ksc[t & 3];
-        unsigned long long see = ~0ull;  // columns the row sees
+        uint32_t see = ~0u;  // which of the thread's 32 keys the row sees
         const bool masked = j0 + kKvTileKeys > open;
         if (masked) {
+          const int j = j0 + 32 * half;
           if (MASK == kMaskTree) {
-            const int e0 = j0 - x.p;  // node number of column 0
-            see = e0 <= -kKvTileKeys ? ~0ull : e0 < 0 ? (1ull << -e0) - 1 : 0ull;
+            const int e0 = j - x.p;  // node number of the first
+            see = e0 <= -32 ? ~0u : e0 < 0 ? (1u << -e0) - 1 : 0u;
             const uint32_t* anc = a.anc + ((size_t)x.b * a.n + token) * a.words;
-            for (int w = max(0, e0 >> 5); w < a.words && w * 32 - e0 < kKvTileKeys; ++w) {
+            for (int w = max(0, e0 >> 5); w < a.words && w * 32 - e0 < 32; ++w) {
               const int sh = w * 32 - e0;
-              see |= sh >= 0 ? (unsigned long long)anc[w] << sh : (unsigned long long)(anc[w] >> -sh);
+              see |= sh >= 0 ? anc[w] << sh : anc[w] >> -sh;
             }
           } else {
-            const int lim = min(x.p + token + 1, x.keys) - j0;
-            see = lim >= kKvTileKeys ? ~0ull : lim <= 0 ? 0ull : (1ull << lim) - 1;
+            const int lim = min(x.p + token + 1, x.keys) - j;
+            see = lim >= 32 ? ~0u : lim <= 0 ? 0u : (1u << lim) - 1;
           }
         }
-        ok = bar_wait(&sm.sfull[s], (t >> 1) & 1, abort);
-        if (!ok) break;
+        wait(&sm.sfull[s], (t >> 1) & 1);
         tc_after();
         float top = -INFINITY;
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
+        {
           uint32_t r[32];
-          tm_ld32(mine + kTmS + 64 * s + 32 * part, r);
+          tm_ld32(mine + kTmS + 64 * s + 32 * half, r);
           tm_wait_ld();
-          const uint32_t bits = (uint32_t)(see >> (32 * part));
           if (!masked) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(r[e]));
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if ((bits >> e) & 1u) top = fmaxf(top, __uint_as_float(r[e]));
+              if ((see >> e) & 1u) top = fmaxf(top, __uint_as_float(r[e]));
           }
         }
+        sm.top[s][half][row] = top;
+        meet();
+        top = fmaxf(top, sm.top[s][half ^ 1][row]);
         const float n_m = top == -INFINITY ? m : fmaxf(m, top * cc);
         const float base = n_m == -INFINITY ? 0.0f : n_m;
         const float next = ex2(m - base);
@@ -640,67 +641,69 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         const float2 c2 = make_float2(cc, cc), b2 = make_float2(kKtPScale - base, kKtPScale - base);
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int part = 0; part < 4; ++part) {
+        for (int part = 0; part < 2; ++part) {
           uint32_t r[16], hi[8], lo[8];
-          tm_ld16(mine + kTmS + 64 * s + 16 * part, r);
+          tm_ld16(mine + kTmS + 64 * s + 32 * half + 16 * part, r);
           tm_wait_ld();
-          const uint32_t bits = (uint32_t)(see >> (16 * part));
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             float2 p = fma2(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), c2, b2);
             p.x = ex2(p.x);
             p.y = ex2(p.y);
             if (masked) {
-              if (!((bits >> (2 * e)) & 1u)) p.x = 0.0f;
-              if (!((bits >> (2 * e + 1)) & 1u)) p.y = 0.0f;
+              if (!((see >> (16 * part + 2 * e)) & 1u)) p.x = 0.0f;
+              if (!((see >> (16 * part + 2 * e + 1)) & 1u)) p.y = 0.0f;
             }
             sum.x += p.x;
             sum.y += p.y;
             split_f16(p, hi[e], lo[e]);
           }
-          tm_st8(mine + kTmP + 64 * s + 8 * part, hi);
-          tm_st8(mine + kTmP + 64 * s + 32 + 8 * part, lo);
+          tm_st8(mine + kTmP + 64 * s + 16 * half + 8 * part, hi);
+          tm_st8(mine + kTmP + 64 * s + 32 + 16 * half + 8 * part, lo);
         }
         tm_wait_st();
         tc_before();
         __syncwarp();
         if (lane == 0) bar_arrive(&sm.pfull[s]);
         l = fmaf(l, next, sum.x + sum.y);
-        if (i > 0) {
-          ok = add_o(t - 1, c0 + i - 1, corr);
-          if (!ok) break;
-        }
+        if (i > 0) add_o(t - 1, c0 + i - 1, corr);
         corr = next;
       }
-      if (ok) ok = add_o(t - 1, c0 + n - 1, corr);
+      add_o(t - 1, c0 + n - 1, corr);
+      // the row's sum over both halves (the maxima's place is free: the last tile's was read
+      // before its P was given away, and t moves on)
+      meet();
+      sm.top[0][half][row] = l;
+      meet();
+      l = sm.top[0][0][row] + sm.top[0][1][row];
+      meet();
       // the row: whole, or this CTA's part of it
       const bool whole = c0 == 0 && n == x.chunks;
       const size_t slot = a.split ? (size_t)blockIdx.x + cur.u : (size_t)cur.u;
       const float nan = __uint_as_float(0x7fffffffu);
-      if (!valid) m = -INFINITY;
+      if (!kv_row_valid<MASK>(a, x, row)) m = -INFINITY;
       if (row < x.nrows) {
         constexpr float kUnscale = 1.0f / (1 << kKtPScale);  // P' = 2^14 p is in both sums
         float f = kUnscale;
         if (whole) f = m == -INFINITY ? 0.0f : __fdiv_rn(1.0f, l);
         if (!ok) f = nan;
-        float4* dst = reinterpret_cast<float4*>(whole ? a.out + kv_row_offset<MASK>(a, x, row)
-                                                      : a.acc + (slot * a.rows + row) * kKvD);
+        float2* dst = reinterpret_cast<float2*>(whole ? a.out + kv_row_offset<MASK>(a, x, row)
+                                                      : a.acc + (slot * a.rows + row) * kKvD) + half;
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           const float e0 = i & 1 ? o[i >> 1].y : o[i >> 1].x, e1 = i & 1 ? o[16 + (i >> 1)].y : o[16 + (i >> 1)].x;
-          const float e2 = i & 1 ? o[32 + (i >> 1)].y : o[32 + (i >> 1)].x;
-          const float e3 = i & 1 ? o[48 + (i >> 1)].y : o[48 + (i >> 1)].x;
-          dst[i] = f == 0.0f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(e0 * f, e1 * f, e2 * f, e3 * f);
+          dst[2 * i] = f == 0.0f ? make_float2(0.f, 0.f) : make_float2(e0 * f, e1 * f);
         }
-        if (a.stat) {
-          a.stat[slot * 2 * a.rows + row] = m;
-          a.stat[(slot * 2 + 1) * a.rows + row] = ok ? l * kUnscale : nan;
+        if (half == 0) {
+          if (a.stat) {
+            a.stat[slot * 2 * a.rows + row] = m;
+            a.stat[(slot * 2 + 1) * a.rows + row] = ok ? l * kUnscale : nan;
+          }
+          if (a.lse && whole)
+            a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] =
+                m == -INFINITY ? INFINITY : m + log2f(l) - kKtPScale;
         }
-        if (a.lse && whole)
-          a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] =
-              m == -INFINITY ? INFINITY : m + log2f(l) - kKtPScale;
       }
-      if (!ok) break;
       cur.c = cur.c1 - 1;
       cur.next(a);
     }
