@@ -2,11 +2,14 @@
 // 64 keys, for kv heads with many rows (wide trees, prompt chunks).
 //
 // Products: f32 operands as pairs of f16 numbers under a power-of-two scale, three
-// tcgen05.mma kind::f16 per product.  x s = hi + lo, s = 2^(13 - exponent of the largest
-// |x|) of the K tile, the V tile or the query row; hi = x s cut to 11 significant bits, lo = x s -
-// hi (exact) rounded to f16; a.b = lo.hi + hi.lo + hi.hi.  lo keeps 2^-25 of scale 2^13, so an
-// element is off by at most 2^-22 of itself or 2^-39 of its tile's largest, and the dropped lo.lo
-// is 2^-20 of a product at most, 2^-22 on average.  Scaling makes f32's exponent range fit.
+// tcgen05.mma kind::f16 per product.  x s = hi + lo with a power of two s for each query row and
+// each group of 8 keys or values, which brings the largest |x s| of them into [2^10, 2^14); hi =
+// x s cut to 11 significant bits, lo = x s - hi (exact) rounded to f16; a.b = lo.hi + hi.lo +
+// hi.hi.  An element is off by at most 2^-22 of itself or 2^-35 of its group's largest, and the
+// dropped lo.lo is 2^-20 of a product at most, 2^-22 on average.  So f32's exponent range fits.
+// The keys' scales leave with the scores' factor.  The values' scales differ inside a sum: the
+// probabilities of a group are lowered by its scale over the tile's smallest, which leaves one
+// factor for the tile.
 //
 // One CTA per SM, 17 working warps:
 //   * 8 convert: cache rows to registers one tile ahead, then scaled hi / lo to swizzled shared
@@ -45,9 +48,8 @@ __shared__ uint64_t s_kt_wait_ns;
 struct KtSmem {
   alignas(1024) uint8_t k[2][2][2][kKvTileKeys * 128];  // [stage][hi, lo][64 dims][key][128 B]
   alignas(1024) uint8_t v[2][2][kKvD * 128];            // [stage][hi, lo][dim][64 keys]
-  float ksc[4], vsc[4];                                 // inverse scales of tiles t % 4
-  unsigned long long vbad[4];                           // keys of the tile whose value row is not finite
-  alignas(16) unsigned red[4][8];                                   // the converters' maxima
+  alignas(16) float ksc[4][8], vsc[4][8];               // inverse scales of the groups of tiles t % 4
+  alignas(8) uint8_t vbad[4][8];                        // keys of the tile whose value row is not finite
   float top[2][2][kKvTileRows];                         // the rows' maxima over either half of a tile
   alignas(8) uint64_t kfull[2], kfree[2], vfull[2], vfree[2];
   uint64_t kinfo[4], vinfo[4];
@@ -119,6 +121,15 @@ __device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t (&r)[32]) {
       : "memory");
 #undef KT_OUT
 }
+__device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t (&r)[32]) {
+#define KT_IN(i) "r"(r[i])
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::KT_R32(KT_IN),
+      "r"(addr)
+      : "memory");
+#undef KT_IN
+}
 __device__ __forceinline__ void tm_ld16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -137,6 +148,9 @@ __device__ __forceinline__ uint32_t tm_ld1(uint32_t addr) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(addr) : "memory");
   return r;
 }
+__device__ __forceinline__ void tm_st1(uint32_t addr, uint32_t r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%1], {%0};" ::"r"(r), "r"(addr) : "memory");
+}
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -153,6 +167,12 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
       : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
   return d;
 }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -163,55 +183,53 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+__device__ __forceinline__ float2 lo2(const float4& v) { return make_float2(v.x, v.y); }
+__device__ __forceinline__ float2 hi2(const float4& v) { return make_float2(v.z, v.w); }
+// Cut to 11 significant bits.
+__device__ __forceinline__ float2 cut2(float2 x) {
+  return make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffffe000u),
+                     __uint_as_float(__float_as_uint(x.y) & 0xffffe000u));
+}
 // Two scaled values -> packed hi parts and packed lo parts.
 __device__ __forceinline__ void split_f16(float2 x, uint32_t& hi, uint32_t& lo) {
-  const float2 h = make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffffe000u),
-                               __uint_as_float(__float_as_uint(x.y) & 0xffffe000u));
+  const float2 h = cut2(x);
   hi = pack_f16(h.x, h.y);
   const float2 l = fma2(h, make_float2(-1.0f, -1.0f), x);
   lo = pack_f16(l.x, l.y);
 }
-// Largest magnitude (bits of a float) -> scale 2^(13 - exponent) and its inverse.
+// Largest magnitude (bits of a float) -> the scale that brings it into [2^10, 2^14) and its
+// inverse.  Exponents in steps of 4: neighbouring groups mostly agree.
 __device__ __forceinline__ void scale_of(unsigned top, float& scale, float& inverse) {
-  const int e = min(253, 267 - (int)(top >> 23));
+  const int e = min(251, 267 - (int)(top >> 23 | 3u));
   scale = __uint_as_float((unsigned)e << 23);
   inverse = __uint_as_float((unsigned)(254 - e) << 23);
 }
 __device__ __forceinline__ float mag(float m, float x) { return fmaxf(m, fabsf(x)); }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
-// The tiles of this CTA's units, in order.
+// The units of this CTA and their tiles, in order.
 template <int MASK>
 struct KtCursor {
   int u, off, left;  // unit, its first tile here, tiles left of the CTA's share
-  int c, c1;         // current tile, end
+  int n;             // tiles of the unit here
   KvUnit x;
-  bool ok;
-  // Moves to the first unit from u on with work.
-  __device__ void seek(const KvArgs& a) {
-    ok = false;
+  // Moves to the first unit from u on with work; false when there is none.
+  __device__ bool seek(const KvArgs& a) {
     while (u < a.units && left > 0) {
       x = kv_unit<MASK>(a, u);
-      c = off;
-      c1 = off > x.chunks - left ? x.chunks : off + left;
-      if (c < c1) {
-        ok = true;
-        return;
-      }
+      n = min(x.chunks - off, left);
+      if (n > 0) return true;
       off = 0;
       ++u;
-      if (!a.split) return;
+      if (!a.split) break;
     }
+    return false;
   }
-  __device__ void next(const KvArgs& a) {
-    if (++c < c1) return;
-    left -= c1 - off;
+  __device__ bool next(const KvArgs& a) {
+    left -= n;
     off = 0;
     ++u;
-    if (a.split)
-      seek(a);
-    else
-      ok = false;
+    return a.split && seek(a);
   }
 };
 
@@ -274,157 +292,162 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
 
   if (warp >= kKtConvertWarp && warp < kKtMmaWarp) {
     // ---------------- converters ----------------
+    // warp cw: keys and values 8 cw .. + 8 of every tile, on its own (no barrier between warps)
     const int cw = warp - kKtConvertWarp, h = lane & 15;
-    float4 kr[8], vr[8];  // this warp's 8 keys and values of a tile
-    auto load_k = [&](const KtCursor<MASK>& z) {
-      const float* kb = a.k + ((size_t)z.x.b * a.hkv + z.x.hk) * (size_t)a.max_t * kKvD;
-      const int j0 = z.c * kKvTileKeys + cw * 8 + (lane >> 4);
-      const float4* row = reinterpret_cast<const float4*>(kb + (size_t)j0 * kKvD) + h;
-      if (z.c * kKvTileKeys + kKvTileKeys <= (MASK == kMaskTree ? z.x.p : z.x.keys)) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          kr[2 * i] = row[i * 64];
-          kr[2 * i + 1] = row[i * 64 + 16];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool there = kt_row_there<MASK>(a, z.x, j0 + 2 * i);
-          kr[2 * i] = there ? row[i * 64] : make_float4(0.f, 0.f, 0.f, 0.f);
-          kr[2 * i + 1] = there ? row[i * 64 + 16] : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-      }
-    };
-    auto load_v = [&](const KtCursor<MASK>& z) {
-      const float* vb = a.v + ((size_t)z.x.b * a.hkv + z.x.hk) * (size_t)a.max_t * kKvD;
-      const int j0 = z.c * kKvTileKeys + cw * 8;
-      const float4* row = reinterpret_cast<const float4*>(vb + (size_t)j0 * kKvD) + lane;
-      if (z.c * kKvTileKeys + kKvTileKeys <= (MASK == kMaskTree ? z.x.p : z.x.keys)) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) vr[i] = row[i * 32];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          vr[i] = kt_row_there<MASK>(a, z.x, j0 + i) ? row[i * 32] : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-    };
-    // The tile's largest magnitude over the warps; `red` alternates, one barrier each.
-    auto tile_max = [&](unsigned mine, int which) {
-      mine = __reduce_max_sync(kFull, mine);
-      if (lane == 0) sm.red[which][cw] = mine;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      const uint4 x = *reinterpret_cast<const uint4*>(&sm.red[which][0]);
-      const uint4 y = *reinterpret_cast<const uint4*>(&sm.red[which][4]);
-      return max(max(max(x.x, x.y), max(x.z, x.w)), max(max(y.x, y.y), max(y.z, y.w)));
-    };
-    cur.seek(a);
-    if (cur.ok) {
-      load_k(cur);
-      load_v(cur);
-    }
-    // after a wait that ran out the loop goes on without waiting: the warps meet at named
-    // barriers, so none may leave
+    // where the lane's pieces go: K row 2 i + lane / 16, dimensions in 16-byte pieces of 4 h .. and
+    // 64 + 4 h ..; V row (dimension) 32 e + lane, the piece of its 8 keys
+    const int kat = (cw * 8 + (lane >> 4)) * 128, kx = h & 7, ky = lane >> 4;
+    const int vat = lane * 128 + ((cw ^ (lane & 7)) << 4);
     bool dead = false;
-    for (int t = 0; cur.ok; ++t) {
-      const int s = t & 1;
-      float scale, inverse;
-      {  // K
-        float m = 0.0f;
+    int t = 0;
+    for (bool more = cur.seek(a); more; more = cur.next(a)) {
+      const KvUnit& x = cur.x;
+      const size_t head = ((size_t)x.b * a.hkv + x.hk) * (size_t)a.max_t;
+      const float4* kp = reinterpret_cast<const float4*>(a.k + (head + cur.off * kKvTileKeys + cw * 8 + ky) * kKvD) + h;
+      const float4* vp = reinterpret_cast<const float4*>(a.v + (head + cur.off * kKvTileKeys + cw * 8) * kKvD) + lane;
+      const int plain = MASK == kMaskTree ? x.p : x.keys;  // rows below need no look
+      float4 kr[8], vr[8];
+      auto load_k = [&](int c) {
+        if ((c + 1) * kKvTileKeys <= plain) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = mag(mag(mag(mag(m, kr[i].x), kr[i].y), kr[i].z), kr[i].w);
-        unsigned top = tile_max(__float_as_uint(m), 2 * s);
-        if (top >= 0x7f800000u) {  // an infinite key: the scale of the others
-          m = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            m = finite(kr[i].x) ? mag(m, kr[i].x) : m;
-            m = finite(kr[i].y) ? mag(m, kr[i].y) : m;
-            m = finite(kr[i].z) ? mag(m, kr[i].z) : m;
-            m = finite(kr[i].w) ? mag(m, kr[i].w) : m;
+          for (int i = 0; i < 4; ++i) {
+            kr[2 * i] = kp[i * 64];
+            kr[2 * i + 1] = kp[i * 64 + 16];
           }
-          asm volatile("bar.sync 1, 256;" ::: "memory");
-          top = tile_max(__float_as_uint(m), 2 * s);
-        }
-        scale_of(top, scale, inverse);
-        if (t >= 2 && !dead) dead = !bar_wait(&sm.kfree[s], ((t >> 1) - 1) & 1, abort);
-        const float2 sc = make_float2(scale, scale);
-        uint8_t* dst = &sm.k[s][0][h >> 3][0];
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = cw * 8 + 2 * i + (lane >> 4);
-          uint4 hi, lo;
-          split_f16(mul2(make_float2(kr[2 * i].x, kr[2 * i].y), sc), hi.x, lo.x);
-          split_f16(mul2(make_float2(kr[2 * i].z, kr[2 * i].w), sc), hi.y, lo.y);
-          split_f16(mul2(make_float2(kr[2 * i + 1].x, kr[2 * i + 1].y), sc), hi.z, lo.z);
-          split_f16(mul2(make_float2(kr[2 * i + 1].z, kr[2 * i + 1].w), sc), hi.w, lo.w);
-          const int at = r * 128 + (((h & 7) ^ (r & 7)) << 4);
-          *reinterpret_cast<uint4*>(dst + at) = hi;
-          *reinterpret_cast<uint4*>(dst + sizeof(sm.k[0][0]) + at) = lo;
+          for (int i = 0; i < 4; ++i) {
+            const bool there = kt_row_there<MASK>(a, x, c * kKvTileKeys + cw * 8 + ky + 2 * i);
+            kr[2 * i] = there ? kp[i * 64] : make_float4(0.f, 0.f, 0.f, 0.f);
+            kr[2 * i + 1] = there ? kp[i * 64 + 16] : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
         }
-        if (cw == 0 && lane == 0) sm.ksc[t & 3] = inverse;
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
-          bar_arrive(&sm.kfull[s]);
-          bar_arrive(&sm.kinfo[t & 3]);
-        }
-      }
-      cur.next(a);
-      if (cur.ok) load_k(cur);
-      {  // V
-        float m = 0.0f;
-        float2 z = make_float2(0.f, 0.f);
+        kp += kKvTileKeys * (kKvD / 4);
+      };
+      auto load_v = [&](int c) {
+        if ((c + 1) * kKvTileKeys <= plain) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          m = mag(mag(mag(mag(m, vr[i].x), vr[i].y), vr[i].z), vr[i].w);
-          z = fma2(make_float2(vr[i].x, vr[i].y), make_float2(0.f, 0.f), z);  // NaN unless all are finite
-          z = fma2(make_float2(vr[i].z, vr[i].w), make_float2(0.f, 0.f), z);
-        }
-        if (cw == 0 && lane == 0) sm.vbad[t & 3] = 0;
-        unsigned top = tile_max(z.x + z.y == 0.0f ? __float_as_uint(m) : 0x7f800000u, 2 * s + 1);
-        if (top >= 0x7f800000u) {
-          // 0 * inf must not reach the rows that do not see the key: its value row leaves the
-          // product (0) and the rows that see it add it one by one
-          m = 0.0f;
+          for (int i = 0; i < 8; ++i) vr[i] = vp[i * 32];
+        } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const bool bad = __any_sync(kFull, !(finite(vr[i].x) && finite(vr[i].y) && finite(vr[i].z) && finite(vr[i].w)));
-            if (bad) {
-              vr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (lane == 0) atomicOr(&sm.vbad[t & 3], 1ull << (cw * 8 + i));
+          for (int i = 0; i < 8; ++i)
+            vr[i] = kt_row_there<MASK>(a, x, c * kKvTileKeys + cw * 8 + i) ? vp[i * 32] : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        vp += kKvTileKeys * (kKvD / 4);
+      };
+      load_k(cur.off);
+      load_v(cur.off);
+      const int end = cur.off + cur.n;
+      for (int c = cur.off; c < end; ++c, ++t) {
+        const int s = t & 1;
+        float scale, inverse;
+        {  // K
+          float m = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) m = mag(mag(mag(mag(m, kr[i].x), kr[i].y), kr[i].z), kr[i].w);
+          unsigned top = __reduce_max_sync(kFull, __float_as_uint(m));
+          if (top >= 0x7f800000u) {  // an infinite key: the scale of the others
+            m = 0.0f;
+            for (int i = 0; i < 8; ++i) {
+              m = finite(kr[i].x) ? mag(m, kr[i].x) : m;
+              m = finite(kr[i].y) ? mag(m, kr[i].y) : m;
+              m = finite(kr[i].z) ? mag(m, kr[i].z) : m;
+              m = finite(kr[i].w) ? mag(m, kr[i].w) : m;
             }
-            m = mag(mag(mag(mag(m, vr[i].x), vr[i].y), vr[i].z), vr[i].w);
+            top = __reduce_max_sync(kFull, __float_as_uint(m));
           }
-          asm volatile("bar.sync 1, 256;" ::: "memory");
-          top = tile_max(__float_as_uint(m), 2 * s + 1);
+          scale_of(top, scale, inverse);
+          if (t >= 2 && !dead) dead = !bar_wait(&sm.kfree[s], ((t >> 1) - 1) & 1, abort);
+          const float2 sc = make_float2(scale, scale);
+          uint8_t* dst = &sm.k[s][0][h >> 3][kat];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint4 hi, lo;
+            split_f16(mul2(make_float2(kr[2 * i].x, kr[2 * i].y), sc), hi.x, lo.x);
+            split_f16(mul2(make_float2(kr[2 * i].z, kr[2 * i].w), sc), hi.y, lo.y);
+            split_f16(mul2(make_float2(kr[2 * i + 1].x, kr[2 * i + 1].y), sc), hi.z, lo.z);
+            split_f16(mul2(make_float2(kr[2 * i + 1].z, kr[2 * i + 1].w), sc), hi.w, lo.w);
+            const int at = i * 256 + ((kx ^ (2 * i + ky)) << 4);
+            *reinterpret_cast<uint4*>(dst + at) = hi;
+            *reinterpret_cast<uint4*>(dst + sizeof(sm.k[0][0]) + at) = lo;
+          }
+          if (lane == 0) sm.ksc[t & 3][cw] = inverse;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            bar_arrive(&sm.kfull[s]);
+            bar_arrive(&sm.kinfo[t & 3]);
+          }
         }
-        scale_of(top, scale, inverse);
-        if (t >= 2 && !dead) dead = !bar_wait(&sm.vfree[s], ((t >> 1) - 1) & 1, abort);
-        const float2 sc = make_float2(scale, scale);
-        uint8_t* dst = &sm.v[s][0][0];
-        auto put = [&](int e, const float (&w)[8]) {  // dimension 4 lane + e sits in row 32 e + lane
-          uint4 hi, lo;
-          split_f16(mul2(make_float2(w[0], w[1]), sc), hi.x, lo.x);
-          split_f16(mul2(make_float2(w[2], w[3]), sc), hi.y, lo.y);
-          split_f16(mul2(make_float2(w[4], w[5]), sc), hi.z, lo.z);
-          split_f16(mul2(make_float2(w[6], w[7]), sc), hi.w, lo.w);
-          const int at = (32 * e + lane) * 128 + ((cw ^ (lane & 7)) << 4);
-          *reinterpret_cast<uint4*>(dst + at) = hi;
-          *reinterpret_cast<uint4*>(dst + sizeof(sm.v[0][0]) + at) = lo;
-        };
-        put(0, {vr[0].x, vr[1].x, vr[2].x, vr[3].x, vr[4].x, vr[5].x, vr[6].x, vr[7].x});
-        put(1, {vr[0].y, vr[1].y, vr[2].y, vr[3].y, vr[4].y, vr[5].y, vr[6].y, vr[7].y});
-        put(2, {vr[0].z, vr[1].z, vr[2].z, vr[3].z, vr[4].z, vr[5].z, vr[6].z, vr[7].z});
-        put(3, {vr[0].w, vr[1].w, vr[2].w, vr[3].w, vr[4].w, vr[5].w, vr[6].w, vr[7].w});
-        if (cw == 0 && lane == 0) sm.vsc[t & 3] = inverse;
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
-          bar_arrive(&sm.vfull[s]);
-          bar_arrive(&sm.vinfo[t & 3]);
+        if (c + 1 < end) load_k(c + 1);
+        {  // V
+          float m = 0.0f;
+          float2 z = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            m = mag(mag(mag(mag(m, vr[i].x), vr[i].y), vr[i].z), vr[i].w);
+            z = fma2(make_float2(vr[i].x, vr[i].y), make_float2(0.f, 0.f), z);  // NaN unless all are finite
+            z = fma2(make_float2(vr[i].z, vr[i].w), make_float2(0.f, 0.f), z);
+          }
+          unsigned top = __reduce_max_sync(kFull, z.x + z.y == 0.0f ? __float_as_uint(m) : 0x7f800000u);
+          unsigned bad = 0;
+          if (top >= 0x7f800000u) {
+            // 0 * inf must not reach the rows that do not see the key: its value row leaves the
+            // product (0) and the rows that see it add it one by one
+            m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (__any_sync(kFull, !(finite(vr[i].x) && finite(vr[i].y) && finite(vr[i].z) && finite(vr[i].w)))) {
+                vr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                bad |= 1u << i;
+              }
+              m = mag(mag(mag(mag(m, vr[i].x), vr[i].y), vr[i].z), vr[i].w);
+            }
+            top = __reduce_max_sync(kFull, __float_as_uint(m));
+          }
+          scale_of(top, scale, inverse);
+          if (t >= 2 && !dead) dead = !bar_wait(&sm.vfree[s], ((t >> 1) - 1) & 1, abort);
+          const float2 sc = make_float2(scale, scale);
+          uint8_t* dst = &sm.v[s][0][vat];
+          // dimensions 4 lane + e and 4 lane + e + 1 of all 8 keys at a time
+          auto put = [&](int e, float2 w0, float2 w1, float2 w2, float2 w3, float2 w4, float2 w5, float2 w6, float2 w7) {
+            float2 w[8] = {mul2(w0, sc), mul2(w1, sc), mul2(w2, sc), mul2(w3, sc),
+                           mul2(w4, sc), mul2(w5, sc), mul2(w6, sc), mul2(w7, sc)};
+            uint4 h0, h1, l0, l1;
+            uint32_t* ph0 = &h0.x;
+            uint32_t* ph1 = &h1.x;
+            uint32_t* pl0 = &l0.x;
+            uint32_t* pl1 = &l1.x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 b0 = cut2(w[2 * i]), b1 = cut2(w[2 * i + 1]);
+              ph0[i] = pack_f16(b0.x, b1.x);
+              ph1[i] = pack_f16(b0.y, b1.y);
+              const float2 r0 = fma2(b0, make_float2(-1.0f, -1.0f), w[2 * i]);
+              const float2 r1 = fma2(b1, make_float2(-1.0f, -1.0f), w[2 * i + 1]);
+              pl0[i] = pack_f16(r0.x, r1.x);
+              pl1[i] = pack_f16(r0.y, r1.y);
+            }
+            *reinterpret_cast<uint4*>(dst + e * 4096) = h0;
+            *reinterpret_cast<uint4*>(dst + e * 4096 + 4096) = h1;
+            *reinterpret_cast<uint4*>(dst + sizeof(sm.v[0][0]) + e * 4096) = l0;
+            *reinterpret_cast<uint4*>(dst + sizeof(sm.v[0][0]) + e * 4096 + 4096) = l1;
+          };
+          put(0, lo2(vr[0]), lo2(vr[1]), lo2(vr[2]), lo2(vr[3]), lo2(vr[4]), lo2(vr[5]), lo2(vr[6]), lo2(vr[7]));
+          put(2, hi2(vr[0]), hi2(vr[1]), hi2(vr[2]), hi2(vr[3]), hi2(vr[4]), hi2(vr[5]), hi2(vr[6]), hi2(vr[7]));
+          if (lane == 0) {
+            sm.vsc[t & 3][cw] = inverse;
+            sm.vbad[t & 3][cw] = (uint8_t)bad;
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            bar_arrive(&sm.vfull[s]);
+            bar_arrive(&sm.vinfo[t & 3]);
+          }
         }
+        if (c + 1 < end) load_v(c + 1);
       }
-      if (cur.ok) load_v(cur);
     }
   } else if (warp >= kKtMmaWarp) {
     // ---------------- MMA issue ----------------
@@ -451,9 +474,8 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       mma_commit(&sm.ofull);
       return true;
     };
-    cur.seek(a);
-    while (ok && cur.ok) {
-      const int n = cur.c1 - cur.c;
+    for (bool more = cur.seek(a); ok && more; more = cur.next(a)) {
+      const int n = cur.n;
       ok = bar_wait(&sm.qfull, units & 1, abort);
       for (int i = 0; ok && i < n; ++i, ++t) {
         const int s = t & 1;
@@ -475,8 +497,6 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       }
       if (ok) ok = pv(t - 1);
       ++units;
-      cur.c = cur.c1 - 1;
-      cur.next(a);
     }
     // nothing of this CTA's may be at work in shared memory or TMEM when it ends
     mma_commit(&sm.done);
@@ -505,10 +525,9 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         if (a.lse) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] = INFINITY;
       }
     }
-    cur.seek(a);
-    while (cur.ok) {
-      const KvUnit x = cur.x;
-      const int c0 = cur.c, n = cur.c1 - cur.c;
+    for (bool more = cur.seek(a); more; more = cur.next(a)) {
+      const KvUnit& x = cur.x;
+      const int c0 = cur.off, n = cur.n;
       const int token = kv_token<MASK>(a, x, min(row, x.nrows - 1));
       // half of the query row: scaled hi / lo to TMEM, dimensions in the order of the K tiles
       float qinv;
@@ -548,10 +567,9 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       float m = -INFINITY, l = 0.0f, corr = 0.0f;
       const int open = MASK == kMaskTree ? x.p : x.p + x.i0 + 1;
       // o = o * f + the O tile of tile w (cache tile c), whose P stood against the maximum of then
-      auto add_o = [&](int w, int c, float f) {
-        wait(&sm.vinfo[w & 3], (w >> 2) & 1);
-        const float fv = sm.vsc[w & 3];
-        const unsigned long long bad = sm.vbad[w & 3];
+      float vtop = 0.0f;  // the tile's factor of the values, one tile back when it is used
+      unsigned long long bad = 0;
+      auto add_o = [&](int w, int c, float f, float fv, unsigned long long bad) {
         wait(&sm.ofull, w & 1);
         tc_after();
         const float2 f2 = make_float2(f, f), v2 = make_float2(fv, fv);
@@ -597,79 +615,116 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       for (int i = 0; i < n; ++i, ++t) {
         const int s = t & 1, j0 = (c0 + i) * kKvTileKeys;
         wait(&sm.kinfo[t & 3], (t >> 2) & 1);
-        const float cc = a.c * qinv * sm.ksc[t & 3];
-        uint32_t see = ~0u;  // which of the thread's 32 keys the row sees
-        const bool masked = j0 + kKvTileKeys > open;
-        if (masked) {
-          const int j = j0 + 32 * half;
-          if (MASK == kMaskTree) {
-            const int e0 = j - x.p;  // node number of the first
-            see = e0 <= -32 ? ~0u : e0 < 0 ? (1u << -e0) - 1 : 0u;
-            const uint32_t* anc = a.anc + ((size_t)x.b * a.n + token) * a.words;
-            for (int w = max(0, e0 >> 5); w < a.words && w * 32 - e0 < 32; ++w) {
-              const int sh = w * 32 - e0;
-              see |= sh >= 0 ? anc[w] << sh : anc[w] >> -sh;
-            }
-          } else {
-            const int lim = min(x.p + token + 1, x.keys) - j;
-            see = lim >= 32 ? ~0u : lim <= 0 ? 0u : (1u << lim) - 1;
-          }
+        float cc[4];  // the factors of the thread's four groups of 8 keys
+        {
+          const float4 k4 = *reinterpret_cast<const float4*>(&sm.ksc[t & 3][4 * half]);
+          const float cq = a.c * qinv;
+          cc[0] = fmaxf(cq * k4.x, 1.17549435e-38f);  // a factor of 0 would make NaN of -inf
+          cc[1] = fmaxf(cq * k4.y, 1.17549435e-38f);
+          cc[2] = fmaxf(cq * k4.z, 1.17549435e-38f);
+          cc[3] = fmaxf(cq * k4.w, 1.17549435e-38f);
         }
+        const uint32_t sat = mine + kTmS + 64 * s + 32 * half;
         wait(&sm.sfull[s], (t >> 1) & 1);
         tc_after();
         float top = -INFINITY;
         {
           uint32_t r[32];
-          tm_ld32(mine + kTmS + 64 * s + 32 * half, r);
+          tm_ld32(sat, r);
           tm_wait_ld();
-          if (!masked) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(r[e]));
-          } else {
+          if (j0 + kKvTileKeys > open) {  // some row of the unit does not see some key
+            uint32_t see;
+            const int j = j0 + 32 * half;
+            if (MASK == kMaskTree) {
+              const int e0 = j - x.p;  // node number of the first
+              see = e0 <= -32 ? ~0u : e0 < 0 ? (1u << -e0) - 1 : 0u;
+              const uint32_t* anc = a.anc + ((size_t)x.b * a.n + token) * a.words;
+              for (int w = max(0, e0 >> 5); w < a.words && w * 32 - e0 < 32; ++w) {
+                const int sh = w * 32 - e0;
+                see |= sh >= 0 ? anc[w] << sh : anc[w] >> -sh;
+              }
+            } else {
+              const int lim = min(x.p + token + 1, x.keys) - j;
+              see = lim >= 32 ? ~0u : lim <= 0 ? 0u : (1u << lim) - 1;
+            }
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if ((see >> e) & 1u) top = fmaxf(top, __uint_as_float(r[e]));
+              if (!((see >> e) & 1u)) r[e] = 0xff800000u;  // -inf, back in TMEM for the second pass
+            tm_st32(sat, r);
+            tm_wait_st();
+          }
+#pragma unroll
+          for (int gi = 0; gi < 4; ++gi) {
+            float y = __uint_as_float(r[8 * gi]);
+#pragma unroll
+            for (int e = 1; e < 8; ++e) y = fmaxf(y, __uint_as_float(r[8 * gi + e]));
+            top = fmaxf(top, y * cc[gi]);
           }
         }
         sm.top[s][half][row] = top;
         meet();
-        top = fmaxf(top, sm.top[s][half ^ 1][row]);
-        const float n_m = top == -INFINITY ? m : fmaxf(m, top * cc);
+        const float n_m = fmaxf(m, fmaxf(top, sm.top[s][half ^ 1][row]));
         const float base = n_m == -INFINITY ? 0.0f : n_m;
         const float next = ex2(m - base);
         m = n_m;
-        const float2 c2 = make_float2(cc, cc), b2 = make_float2(kKtPScale - base, kKtPScale - base);
+        // the values' scales: the largest inverse is the tile's factor, each group's share of it
+        // (1 but for groups of another magnitude) goes to its probabilities
+        wait(&sm.vinfo[t & 3], (t >> 2) & 1);
+        const float4 va = *reinterpret_cast<const float4*>(&sm.vsc[t & 3][4 * half]);
+        const float4 vb = *reinterpret_cast<const float4*>(&sm.vsc[t & 3][4 * (half ^ 1)]);
+        const unsigned long long bad_t = *reinterpret_cast<const unsigned long long*>(&sm.vbad[t & 3][0]);
+        const float vt = fmaxf(fmaxf(fmaxf(va.x, va.y), fmaxf(va.z, va.w)), fmaxf(fmaxf(vb.x, vb.y), fmaxf(vb.z, vb.w)));
+        const float vi = __uint_as_float((254u << 23) - __float_as_uint(vt));  // 1 / vt, a power of two
+        const float share[4] = {va.x * vi, va.y * vi, va.z * vi, va.w * vi};
+        const float b14 = kKtPScale - base;
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
           uint32_t r[16], hi[8], lo[8];
-          tm_ld16(mine + kTmS + 64 * s + 32 * half + 16 * part, r);
+          tm_ld16(sat + 16 * part, r);
           tm_wait_ld();
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            float2 p = fma2(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), c2, b2);
+            const float c1 = cc[2 * part + (e >> 2)], sh = share[2 * part + (e >> 2)];
+            float2 p = fma2(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), make_float2(c1, c1),
+                            make_float2(b14, b14));
             p.x = ex2(p.x);
             p.y = ex2(p.y);
-            if (masked) {
-              if (!((see >> (16 * part + 2 * e)) & 1u)) p.x = 0.0f;
-              if (!((see >> (16 * part + 2 * e + 1)) & 1u)) p.y = 0.0f;
-            }
-            sum.x += p.x;
-            sum.y += p.y;
-            split_f16(p, hi[e], lo[e]);
+            sum = add2(sum, p);
+            split_f16(mul2(p, make_float2(sh, sh)), hi[e], lo[e]);
           }
           tm_st8(mine + kTmP + 64 * s + 16 * half + 8 * part, hi);
           tm_st8(mine + kTmP + 64 * s + 32 + 16 * half + 8 * part, lo);
+        }
+        if (bad_t) {
+          // a key whose value row is left out keeps its probability as it is, for add_o
+          tm_wait_st();
+          for (int e = 0; e < 32; ++e) {
+            if (!((bad_t >> (32 * half + e)) & 1)) continue;
+            const uint32_t at = mine + kTmP + 64 * s + 16 * half + (e >> 1);
+            const uint32_t sv = tm_ld1(sat + e), ph = tm_ld1(at), pl = tm_ld1(at + 32);
+            tm_wait_ld();
+            const float p = ex2(fmaf(__uint_as_float(sv), fmaxf(a.c * qinv * sm.ksc[t & 3][4 * half + (e >> 3)],
+                                                                1.17549435e-38f), b14));
+            uint32_t hi, lo;
+            split_f16(make_float2(p, p), hi, lo);
+            const uint32_t mask = e & 1 ? 0xffff0000u : 0xffffu;
+            tm_st1(at, (ph & ~mask) | (hi & mask));
+            tm_st1(at + 32, (pl & ~mask) | (lo & mask));
+            tm_wait_st();
+          }
         }
         tm_wait_st();
         tc_before();
         __syncwarp();
         if (lane == 0) bar_arrive(&sm.pfull[s]);
         l = fmaf(l, next, sum.x + sum.y);
-        if (i > 0) add_o(t - 1, c0 + i - 1, corr);
+        if (i > 0) add_o(t - 1, c0 + i - 1, corr, vtop, bad);
         corr = next;
+        vtop = vt;
+        bad = bad_t;
       }
-      add_o(t - 1, c0 + n - 1, corr);
+      add_o(t - 1, c0 + n - 1, corr, vtop, bad);
       // the row's sum over both halves (the maxima's place is free: the last tile's was read
       // before its P was given away, and t moves on)
       meet();
@@ -704,8 +759,6 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
                 m == -INFINITY ? INFINITY : m + log2f(l) - kKtPScale;
         }
       }
-      cur.c = cur.c1 - 1;
-      cur.next(a);
     }
   }
   tc_before();

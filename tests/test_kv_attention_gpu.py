@@ -320,6 +320,51 @@ def test_weights_large_and_small_numbers(cuda_device):
         assert float((w.double() - wref).norm() / wref.norm()) <= tol
 
 
+@pytest.mark.parametrize("t", [1, 40])
+def test_weights_values_of_very_different_sizes(cuda_device, t):
+    """Keys and values whose sizes differ by 2^40 from one stretch of the cache to the next: each
+    output against float64 within the error its largest value allows, which rows that see only
+    the small values show at their own size."""
+    dev, hq, hkv, max_t, p0 = cuda_device, 16, 2, 400, 200
+    g = _gen(12, dev)
+    k, v = _caches(g, 1, hkv, max_t, dev)
+    size = torch.ones(max_t, device=dev)
+    size[:64], size[64:72], size[100:130], size[215:] = 2.0 ** -20, 2.0 ** 20, 2.0 ** -10, 2.0 ** 25
+    v *= size[:, None]
+    k *= size.clamp(max=1.0)[:, None]
+    q = torch.randn((1, t, hq, D), generator=g, device=dev)
+    k[0, :, 64:72] = -100 * q[0, 0].view(hkv, 8, D).sum(1, keepdim=True)  # unseen in effect by token 0
+    ref, wref = _weights_ref(q, k, v, [p0], torch.zeros((1, hkv, max_t), device=dev))
+    w = torch.zeros((1, hkv, max_t), device=dev)
+    out = attention.attention_weights(q, k, v, _i32([p0], dev), w)
+    for i in range(t):
+        err, top = float((out[0, i].double() - ref[0, i]).norm()), float(ref[0, i].norm())
+        assert err <= 10 * REL_L2 * top, (i, err / top)  # scores up to 100 * |q|^2: their f32 rounding
+    assert float((w.double() - wref).norm() / wref.norm()) <= 10 * REL_L2
+
+
+@pytest.mark.parametrize("n,hq,hkv", [(12, 4, 2), (40, 16, 2)])
+def test_tree_finite_part_of_a_value_row_counts(cuda_device, n, hq, hkv):
+    """A history value with one infinite dimension spoils that dimension of the rows that see it
+    and counts as it is in the others."""
+    dev, max_t, p0 = cuda_device, 200, 100
+    g = _gen(14, dev)
+    k, v = _caches(g, 1, hkv, max_t, dev)
+    v[0, :, 97, 9] = math.inf  # in the last tile, before the tree
+    v[0, :, 97, 10:] *= 50.0
+    v[0, :, 20, 9] = -math.inf  # in a tile without a mask
+    qkv = torch.randn((1, n, (hq + 2 * hkv) * D), generator=g, device=dev)
+    parents = _i32([[-1] + [i // 2 for i in range(n - 1)]], dev)
+    cos, sin = _tables(max_t, dev)
+    clean = v.clone()
+    clean[0, :, 97, 9] = clean[0, :, 20, 9] = 0.0
+    ref, _, _ = _tree_ref(qkv, parents, [p0], cos, sin, k, clean, hq)
+    out = attention.rope_attention_tree(qkv, parents, _i32([p0], dev), cos, sin, k, v)
+    assert not torch.isfinite(out[..., 9]).any()
+    rest = [d for d in range(D) if d != 9]
+    _close(out[..., rest], ref[..., rest])
+
+
 # ---- eviction ------------------------------------------------------------------------------
 
 def _evict_ref(w, length, keep, sink, recent):
