@@ -525,130 +525,6 @@ __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs 
   }
 }
 
-// Column sums of the softmax where the scores were not stored: every score once more, from
-// the rows' log2 sums.  grid (64-key tiles, batch * hkv), a warp holds 16 keys' fragments
-// and goes over the 16-row groups; sums per lane, then over the lanes of a key.
-constexpr int kColWarps = 4, kColThreads = kColWarps * 32, kColRows = 16;
-struct KvColSmem {
-  alignas(16) float k[kColWarps * kKvChunk][kKvD];
-  alignas(16) float q[2][kColRows][kKvD];
-  float lse[2][kColRows];
-};
-__global__ void __launch_bounds__(kColThreads, 1) kv_column_kernel(const KvArgs a, float* __restrict__ weight) {
-  extern __shared__ __align__(16) uint8_t kv_smem[];
-  KvColSmem& sm = *reinterpret_cast<KvColSmem*>(kv_smem);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  pdl_launch_dependents();
-  pdl_wait();
-  const int b = blockIdx.y / a.hkv, hk = blockIdx.y - b * a.hkv;
-  const int p = a.pos[b], rows = a.n * a.group;
-  const int keys = (p < 0 || p >= a.max_t) ? 0 : min(p + a.n, a.max_t);
-  const int j0 = blockIdx.x * (kColWarps * kKvChunk);
-  if (j0 >= keys) return;
-  const size_t bh = (size_t)b * a.hkv + hk;
-  const float* kb = a.k + bh * (size_t)a.max_t * kKvD;
-  const uint32_t ks = (uint32_t)__cvta_generic_to_shared(&sm.k[0][0]);
-  const uint32_t qs = (uint32_t)__cvta_generic_to_shared(&sm.q[0][0][0]);
-  const int i_first = max(0, j0 - p);  // the first token that sees a key of the tile
-  const int rg0 = (int)(((int64_t)i_first * a.group) / kColRows);
-  auto load_q = [&](int rg, int buf) {
-    for (int e = tid; e < kColRows * 32; e += kColThreads) {
-      const int r = e >> 5, ch = e & 31, row = rg * kColRows + r;
-      const bool there = row < rows;
-      const int i = there ? row / a.group : 0, h = hk * a.group + (there ? row - i * a.group : 0);
-      cp_async16_zfill(qs + buf * (kColRows * kKvD * 4) + r * (kKvD * 4) + ((ch ^ ((r & 1) << 2)) << 4),
-                       a.q + (((size_t)b * a.n + i) * a.hq + h) * kKvD + ch * 4, there);
-    }
-    if (tid < kColRows) {
-      const int row = rg * kColRows + tid;
-      sm.lse[buf][tid] = row < rows ? a.lse[bh * rows + row] : INFINITY;
-    }
-    cp_async_commit();
-  };
-  for (int e = tid; e < kColWarps * kKvChunk * 32; e += kColThreads) {
-    const int r = e >> 5, ch = e & 31, j = j0 + r;
-    cp_async16_zfill(ks + r * (kKvD * 4) + ((ch ^ ((r & 1) << 2)) << 4), kb + (size_t)(j < keys ? j : 0) * kKvD + ch * 4,
-                     j < keys);
-  }
-  load_q(rg0, 0);
-  cp_async_wait(0);
-  __syncthreads();
-  uint32_t kh[8][2][4], kl[8][2][4];
-#pragma unroll
-  for (int pair = 0; pair < 8; ++pair)
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      const int r = warp * kKvChunk + nt * 8 + g;
-      const float4 kv = lds_f4(ks + r * (kKvD * 4) + (((pair * 4 + t) ^ ((r & 1) << 2)) << 4));
-      split_tf32(kv.x, kh[pair][nt][0], kl[pair][nt][0]);
-      split_tf32(kv.y, kh[pair][nt][1], kl[pair][nt][1]);
-      split_tf32(kv.z, kh[pair][nt][2], kl[pair][nt][2]);
-      split_tf32(kv.w, kh[pair][nt][3], kl[pair][nt][3]);
-    }
-  float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-  const int rgs = (rows + kColRows - 1) / kColRows;
-  for (int rg = rg0; rg < rgs; ++rg) {
-    const int buf = (rg - rg0) & 1;
-    if (rg + 1 < rgs) load_q(rg + 1, buf ^ 1);
-    float s[2][3][4];
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-      for (int z = 0; z < 3; ++z)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][z][e] = 0.0f;
-#pragma unroll
-    for (int pair = 0; pair < 8; ++pair) {
-      const uint32_t at = qs + buf * (kColRows * kKvD * 4) + g * (kKvD * 4) + (((pair * 4 + t) ^ ((g & 1) << 2)) << 4);
-      const float4 qa = lds_f4(at), qb = lds_f4(at + 8 * kKvD * 4);
-      uint32_t ah[4], al[4], bh4[4], bl4[4];
-      split_tf32(qa.x, ah[0], al[0]);
-      split_tf32(qa.y, ah[1], al[1]);
-      split_tf32(qa.z, ah[2], al[2]);
-      split_tf32(qa.w, ah[3], al[3]);
-      split_tf32(qb.x, bh4[0], bl4[0]);
-      split_tf32(qb.y, bh4[1], bl4[1]);
-      split_tf32(qb.z, bh4[2], bl4[2]);
-      split_tf32(qb.w, bh4[3], bl4[3]);
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int h = 0; h < 4; h += 2) {
-          mma_tf32(s[nt][0], ah[h], bh4[h], ah[h + 1], bh4[h + 1], kh[pair][nt][h], kh[pair][nt][h + 1]);
-          mma_tf32(s[nt][1], al[h], bl4[h], al[h + 1], bl4[h + 1], kh[pair][nt][h], kh[pair][nt][h + 1]);
-          mma_tf32(s[nt][2], ah[h], bh4[h], ah[h + 1], bh4[h + 1], kl[pair][nt][h], kl[pair][nt][h + 1]);
-        }
-    }
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int r = g + 8 * half, row = rg * kColRows + r;
-      const float z = sm.lse[buf][r];
-      const int last = p + row / a.group;  // rows past the cache have an infinite sum
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int j = j0 + warp * kKvChunk + nt * 8 + 2 * t + e;
-          const float v = s[nt][0][half * 2 + e] + (s[nt][1][half * 2 + e] + s[nt][2][half * 2 + e]);
-          if (j <= last && z != INFINITY) sum[nt][e] += exp2f(__fmul_rn(v, a.c) - z);
-        }
-    }
-    cp_async_wait(0);
-    __syncthreads();
-  }
-#pragma unroll
-  for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float v = sum[nt][e];
-      v += __shfl_xor_sync(kFull, v, 4);
-      v += __shfl_xor_sync(kFull, v, 8);
-      v += __shfl_xor_sync(kFull, v, 16);
-      const int j = j0 + warp * kKvChunk + nt * 8 + 2 * t + e;
-      if (g == 0 && j < keys) weight[bh * a.max_t + j] += v;
-    }
-}
-
 // RoPE and append of a tree: one CTA per (sequence, node).  The node's path to the context is
 // found by pointer doubling over the parents of its sequence (all nodes at once, log2(depth)
 // rounds): jump[i] the ancestor 2^k above, path[i] the bits of the nodes from i up to it.
@@ -861,7 +737,8 @@ size_t attention_weights_workspace_bytes(int batch, int n, int hq, int hkv, int 
   const KvPlan p = kv_plan((int64_t)batch * hkv, (int64_t)n * group, true);
   const bool stored = weights_stored(n, group);
   return core_bytes(p, stored) + (stored ? up256((size_t)batch * hq * n * score_stride(max_t) * 4)
-                                         : up256((size_t)batch * hq * n * 4));
+                                         : up256((size_t)batch * hq * n * 4) +
+                                               up256(kv_column_tile_bytes(batch, n, hq, hkv, max_t)));
 }
 
 cudaError_t launch_attention_weights(const float* q, const float* kc, const float* vc, const int* pos, int batch, int n,
@@ -879,14 +756,8 @@ cudaError_t launch_attention_weights(const float* q, const float* kc, const floa
   a.lse = reinterpret_cast<float*>(w);
   cudaError_t e = launch_core<kMaskCausal, false>(a, weight, device, s);
   if (e != cudaSuccess) return e;
-  static int configured[128] = {0};
-  e = ensure_smem((const void*)kv_column_kernel, configured, device, sizeof(KvColSmem), false);
-  if (e != cudaSuccess) return e;
-  cudaLaunchAttribute attr[1];
-  constexpr int tile = kColWarps * kKvChunk;
-  cudaLaunchConfig_t cfg = kv_cfg(dim3((unsigned)((max_t + tile - 1) / tile), (unsigned)(batch * hkv)),
-                                  dim3(kColThreads), sizeof(KvColSmem), s, attr);
-  return cudaLaunchKernelEx(&cfg, kv_column_kernel, a, weight);
+  w += up256((size_t)batch * hq * n * 4);
+  return launch_kv_column_tile(a, weight, reinterpret_cast<float*>(w), device, s);
 }
 
 size_t attention_blocks_workspace_bytes(int batch, int n, int hq, int hkv) {

@@ -11,14 +11,14 @@
 // probabilities of a group are lowered by its scale over the tile's smallest, which leaves one
 // factor for the tile.
 //
-// One CTA per SM, 17 working warps:
+// One CTA per SM, 16 warps of 128 registers:
 //   * 8 convert: cache rows to registers one tile ahead, then scaled hi / lo to swizzled shared
 //     memory, K as [64 keys][128 dims], V transposed as [128 dims][64 keys], two stages each;
-//   * 1 issues the MMAs: S = Q K^T (Q in TMEM), O = P V (P in TMEM), S and P double-buffered,
-//     so that QK of a tile runs while the softmax of the one before is at work;
 //   * 8 softmax: two threads a row, one for each half of the keys and then of the dimensions;
 //     scores from TMEM, running maximum and sum, P' = 2^14 p back to TMEM as hi / lo; then the
-//     O tile of the tile before is added to registers.
+//     O tile of the tile before is added to registers.  The first of them also issues the MMAs,
+//     O = P V of its tile and S = Q K^T two tiles ahead (Q and P in TMEM, S and P double-
+//     buffered), which run while the warps are at the next tile.
 // The tensor cores cut their f32 sums, so an O tile starts from 0 and joins the running sum with
 // rounding.  TMEM (512 columns): Q 128, S 2 x 64, P 2 x 64, O 128.
 //
@@ -34,10 +34,8 @@ namespace q8lin {
 
 namespace {
 
-constexpr int kKtThreads = 640;   // five warpgroups: 2 softmax, 2 converters, MMA (one of its warps)
-constexpr int kKtConvertWarp = 8, kKtMmaWarp = 16;
-// Registers of a thread: 640 x 96 at launch, then 2 x 120 + 2 x 96 + 48 = 5 x 96.
-constexpr int kKtRegSoftmax = 120, kKtRegMma = 48;
+constexpr int kKtThreads = 512;
+constexpr int kKtConvertWarp = 8;
 constexpr uint32_t kKtTmemCols = 512;
 constexpr uint32_t kTmQ = 0, kTmS = 128, kTmP = 256, kTmO = 384;
 constexpr int kKtPScale = 14;     // P' = 2^14 p
@@ -66,17 +64,30 @@ __device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
 __device__ __forceinline__ void bar_arrive(uint64_t* b) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(b)) : "memory");
 }
-// Bounded wait; once one has run out (or another warp's has) every wait of the CTA fails.
+// Bounded wait; once one has run out (or another warp's has) every wait of the CTA fails.  A try
+// sleeps up to kKtSleepNs in the barrier unit instead of polling.
+constexpr uint32_t kKtSleepNs = 20000;
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
+               : "=r"(ok) : "r"(bar), "r"(parity), "r"(kKtSleepNs) : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort) {
-  if (mb_wait_ns(bar, parity, s_kt_wait_ns, abort)) return true;
-  if (!*abort) atomicOr(&g_kv_tile_fault, 32u);
-  *abort = 1;
+  const uint64_t t0 = global_ns();
+  while (!*abort) {
+    if (bar_try(bar, parity)) return true;
+    if (global_ns() - t0 > s_kt_wait_ns) {
+      atomicOr(&g_kv_tile_fault, 32u);
+      *abort = 1;
+    }
+  }
   return false;
 }
 // By whole warps: the verdict is uniform.
 __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* abort) {
   const uint32_t bar = su32(b);
-  return __all_sync(kFull, mb_try(bar, parity) || bar_wait_slow(bar, parity, abort));
+  return __all_sync(kFull, bar_try(bar, parity) || bar_wait_slow(bar, parity, abort));
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -244,7 +255,8 @@ __device__ __forceinline__ bool kt_row_there(const KvArgs& a, const KvUnit& x, i
 template <int MASK>
 __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, uint64_t wait_ns) {
   extern __shared__ uint8_t kt_raw[];
-  KtSmem& sm = *reinterpret_cast<KtSmem*>((reinterpret_cast<uintptr_t>(kt_raw) + 1023) & ~uintptr_t(1023));
+  // aligned by an offset, not by a cast, so that the compiler keeps seeing shared memory
+  KtSmem& sm = *reinterpret_cast<KtSmem*>(kt_raw + ((1024 - (su32(kt_raw) & 1023)) & 1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort = &sm.abort;
   if (tid == 0) {
@@ -268,7 +280,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
     sm.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kKtMmaWarp) {
+  if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&sm.tmem)),
                  "r"(kKtTmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -290,7 +302,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
   tc_after();
   const uint32_t tmem = sm.tmem;
 
-  if (warp >= kKtConvertWarp && warp < kKtMmaWarp) {
+  if (warp >= kKtConvertWarp) {
     // ---------------- converters ----------------
     // warp cw: keys and values 8 cw .. + 8 of every tile, on its own (no barrier between warps)
     const int cw = warp - kKtConvertWarp, h = lane & 15;
@@ -449,62 +461,8 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         if (c + 1 < end) load_v(c + 1);
       }
     }
-  } else if (warp >= kKtMmaWarp) {
-    // ---------------- MMA issue ----------------
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kKtRegMma));
-    if (warp == kKtMmaWarp) {
-    constexpr uint32_t id_qk = kt_idesc(kKvTileKeys), id_pv = kt_idesc(kKvD);
-    bool ok = true;
-    int t = 0, units = 0;
-    auto pv = [&](int w) {  // O = P V of tile w
-      const int s = w & 1;
-      if (!bar_wait(&sm.vfull[s], (w >> 1) & 1, abort)) return false;
-      if (!bar_wait(&sm.pfull[s], (w >> 1) & 1, abort)) return false;
-      if (w > 0 && !bar_wait(&sm.ofree, (w - 1) & 1, abort)) return false;
-      tc_after();
-      const uint64_t vh = desc_sw128(sm.v[s][0]), vl = desc_sw128(sm.v[s][1]);
-      const uint32_t ph = tmem + kTmP + 64 * s, pl = ph + 32, o = tmem + kTmO;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) mma_ts(o, pl + 8 * kk, vh + 2 * kk, id_pv, kk > 0);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) mma_ts(o, ph + 8 * kk, vl + 2 * kk, id_pv, 1);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) mma_ts(o, ph + 8 * kk, vh + 2 * kk, id_pv, 1);
-      mma_commit(&sm.vfree[s]);
-      mma_commit(&sm.ofull);
-      return true;
-    };
-    for (bool more = cur.seek(a); ok && more; more = cur.next(a)) {
-      const int n = cur.n;
-      ok = bar_wait(&sm.qfull, units & 1, abort);
-      for (int i = 0; ok && i < n; ++i, ++t) {
-        const int s = t & 1;
-        ok = bar_wait(&sm.kfull[s], (t >> 1) & 1, abort);
-        if (!ok) break;
-        tc_after();
-        const uint64_t kh0 = desc_sw128(sm.k[s][0][0]), kh1 = desc_sw128(sm.k[s][0][1]);
-        const uint64_t kl0 = desc_sw128(sm.k[s][1][0]), kl1 = desc_sw128(sm.k[s][1][1]);
-        const uint32_t qh = tmem + kTmQ, ql = qh + 64, d = tmem + kTmS + 64 * s;
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) mma_ts(d, ql + 8 * kk, (kk < 4 ? kh0 : kh1) + 2 * (kk & 3), id_qk, kk > 0);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) mma_ts(d, qh + 8 * kk, (kk < 4 ? kl0 : kl1) + 2 * (kk & 3), id_qk, 1);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) mma_ts(d, qh + 8 * kk, (kk < 4 ? kh0 : kh1) + 2 * (kk & 3), id_qk, 1);
-        mma_commit(&sm.kfree[s]);
-        mma_commit(&sm.sfull[s]);
-        if (i > 0) ok = pv(t - 1);
-      }
-      if (ok) ok = pv(t - 1);
-      ++units;
-    }
-    // nothing of this CTA's may be at work in shared memory or TMEM when it ends
-    mma_commit(&sm.done);
-    mb_wait_ns(su32(&sm.done), 0, kDrainLimitNs, nullptr);
-    }
   } else {
     // ---------------- softmax, output ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kKtRegSoftmax));
     // thread (row, half): keys 32 half .. + 32 of a tile, output columns 64 half .. + 64, which are
     // dimensions 4 i + 2 half and 4 i + 2 half + 1 (i < 32)
     const int row = tid & 127, half = tid >> 7;
@@ -525,7 +483,45 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         if (a.lse) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] = INFINITY;
       }
     }
-    for (bool more = cur.seek(a); more; more = cur.next(a)) {
+    // MMA issue, by warp 0
+    constexpr uint32_t id_qk = kt_idesc(kKvTileKeys), id_pv = kt_idesc(kKvD);
+    auto issue_qk = [&](int w) {  // S = Q K^T of tile w
+      const int s = w & 1;
+      wait(&sm.kfull[s], (w >> 1) & 1);
+      if (!ok) return;
+      tc_after();
+      const uint64_t kh0 = desc_sw128(sm.k[s][0][0]), kh1 = desc_sw128(sm.k[s][0][1]);
+      const uint64_t kl0 = desc_sw128(sm.k[s][1][0]), kl1 = desc_sw128(sm.k[s][1][1]);
+      const uint32_t qh = tmem + kTmQ, ql = qh + 64, d = tmem + kTmS + 64 * s;
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) mma_ts(d, ql + 8 * kk, (kk < 4 ? kh0 : kh1) + 2 * (kk & 3), id_qk, kk > 0);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) mma_ts(d, qh + 8 * kk, (kk < 4 ? kl0 : kl1) + 2 * (kk & 3), id_qk, 1);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) mma_ts(d, qh + 8 * kk, (kk < 4 ? kh0 : kh1) + 2 * (kk & 3), id_qk, 1);
+      mma_commit(&sm.kfree[s]);
+      mma_commit(&sm.sfull[s]);
+    };
+    auto issue_pv = [&](int w) {  // O = P V of tile w, once every warp wrote its P and has the O before
+      const int s = w & 1;
+      wait(&sm.vfull[s], (w >> 1) & 1);
+      wait(&sm.pfull[s], (w >> 1) & 1);
+      if (w > 0) wait(&sm.ofree, (w - 1) & 1);
+      if (!ok) return;
+      tc_after();
+      const uint64_t vh = desc_sw128(sm.v[s][0]), vl = desc_sw128(sm.v[s][1]);
+      const uint32_t ph = tmem + kTmP + 64 * s, pl = ph + 32, d = tmem + kTmO;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) mma_ts(d, pl + 8 * kk, vh + 2 * kk, id_pv, kk > 0);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) mma_ts(d, ph + 8 * kk, vl + 2 * kk, id_pv, 1);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) mma_ts(d, ph + 8 * kk, vh + 2 * kk, id_pv, 1);
+      mma_commit(&sm.vfree[s]);
+      mma_commit(&sm.ofull);
+    };
+    int units = 0;
+    for (bool more = cur.seek(a); more; more = cur.next(a), ++units) {
       const KvUnit& x = cur.x;
       const int c0 = cur.off, n = cur.n;
       const int token = kv_token<MASK>(a, x, min(row, x.nrows - 1));
@@ -560,6 +556,11 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         tc_before();
         __syncwarp();
         if (lane == 0) bar_arrive(&sm.qfull);
+      }
+      if (warp == 0) {
+        wait(&sm.qfull, units & 1);
+        issue_qk(t);
+        if (n > 1) issue_qk(t + 1);
       }
       float2 o[32];
 #pragma unroll
@@ -720,6 +721,10 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         if (lane == 0) bar_arrive(&sm.pfull[s]);
         l = fmaf(l, next, sum.x + sum.y);
         if (i > 0) add_o(t - 1, c0 + i - 1, corr, vtop, bad);
+        if (warp == 0) {
+          issue_pv(t);
+          if (i + 2 < n) issue_qk(t + 2);
+        }
         corr = next;
         vtop = vt;
         bad = bad_t;
@@ -760,12 +765,269 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         }
       }
     }
+    if (warp == 0) {
+      // nothing of this CTA's may be at work in shared memory or TMEM when it ends
+      mma_commit(&sm.done);
+      mb_wait_ns(su32(&sm.done), 0, kDrainLimitNs, nullptr);
+    }
   }
   tc_before();
   __syncthreads();
   tc_after();
-  if (warp == kKtMmaWarp)
+  if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kKtTmemCols) : "memory");
+}
+
+// ---------------------------------------------------------------------------------
+// Column sums of the softmax of causal rows: weight[j] += sum over the rows that see key j of
+// 2^(s_rj - z_r), z_r the rows' log2 sums, from every score once more.  Keys are the M side
+// (128 a CTA, hi / lo in TMEM, a thread owns a key), tiles of 64 rows the N side, so a key's sum
+// stays in one register.  grid (key tiles, batch * hkv, splits): split z takes row tiles z, z +
+// splits, ... and leaves its sums in part[z]; kv_column_add_kernel adds them in split order.
+// Two CTAs per SM: 4 warps exponentials, 8 converters, 1 MMA; 24 MMAs of N = 64 a tile, about
+// 820 cycles, beside 512 cycles of exponentials.
+constexpr int kKcThreads = 416, kKcConvertWarp = 4, kKcMmaWarp = 12;
+constexpr uint32_t kKcTmemCols = 256;
+constexpr int kKcKeys = 128, kKcRows = 64;
+
+struct KcSmem {
+  alignas(1024) uint8_t q[2][2][2][kKcRows * 128];  // [stage][hi, lo][64 dims][row][128 B]
+  alignas(16) float qsc[4][8];                      // inverse scales of the groups of 8 rows
+  alignas(16) float lse[4][kKcRows];
+  alignas(16) int last[4][kKcRows];                 // the last key a row sees
+  alignas(8) uint64_t qfull[2], qfree[2], info[4], sfull[2], sfree[2], kfull, done;
+  uint32_t tmem;
+  int abort;
+};
+
+__global__ void __launch_bounds__(kKcThreads, 2)
+kv_column_tile_kernel(const KvArgs a, float* weight, float* __restrict__ part, uint64_t wait_ns) {
+  extern __shared__ uint8_t kt_raw[];
+  KcSmem& sm = *reinterpret_cast<KcSmem*>(kt_raw + ((1024 - (su32(kt_raw) & 1023)) & 1023));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* abort = &sm.abort;
+  if (tid == 0) {
+    s_kt_wait_ns = wait_ns;
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&sm.qfull[i], 8);
+      bar_init(&sm.qfree[i], 1);
+      bar_init(&sm.sfull[i], 1);
+      bar_init(&sm.sfree[i], 4);
+    }
+    for (int i = 0; i < 4; ++i) bar_init(&sm.info[i], 8);
+    bar_init(&sm.kfull, 4);
+    bar_init(&sm.done, 1);
+    sm.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kKcMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&sm.tmem)),
+                 "r"(kKcTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  const int b = blockIdx.y / a.hkv, hk = blockIdx.y - b * a.hkv;
+  const int p = a.pos[b], rows = a.n * a.group;
+  const int keys = (p < 0 || p >= a.max_t) ? 0 : min(p + a.n, a.max_t);
+  const int j0 = blockIdx.x * kKcKeys;
+  // row tiles first, first + splits, ...: from the one that holds the first row to see a key
+  const int splits = gridDim.z;
+  const int seen = j0 < keys ? (int)(((int64_t)max(0, j0 - p) * a.group) / kKcRows) : 0;
+  const int first = seen + blockIdx.z;
+  const int tiles = j0 < keys ? (rows + kKcRows - 1) / kKcRows : 0;
+  const int n = first < tiles ? (tiles - 1 - first) / splits + 1 : 0;
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = sm.tmem;
+  const size_t bh = blockIdx.y;
+
+  if (warp >= kKcConvertWarp && warp < kKcMmaWarp) {
+    // ---------------- converters: query rows 8 cw .. + 8 of every tile ----------------
+    const int cw = warp - kKcConvertWarp, h = lane & 15, ky = lane >> 4;
+    const float4* qb = reinterpret_cast<const float4*>(a.q + ((size_t)b * a.n * a.hq + hk * a.group) * kKvD) + h;
+    const int there = keys - p <= 0 ? 0 : min(rows, (keys - p) * a.group);  // rows inside the cache
+    float4 qr[8];
+    auto load = [&](int rt) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = rt * kKcRows + cw * 8 + ky + 2 * i;
+        qr[2 * i] = qr[2 * i + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < there) {
+          const int tok = r / a.group;
+          const float4* row = qb + ((size_t)tok * a.hq + (r - tok * a.group)) * (kKvD / 4);
+          qr[2 * i] = row[0];
+          qr[2 * i + 1] = row[16];
+        }
+      }
+    };
+    bool dead = false;
+    if (n > 0) load(first);
+    for (int t = 0; t < n; ++t) {
+      const int s = t & 1, rt = first + t * splits;
+      float m = 0.0f, scale, inverse;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = mag(mag(mag(mag(m, qr[i].x), qr[i].y), qr[i].z), qr[i].w);
+      scale_of(min(__reduce_max_sync(kFull, __float_as_uint(m)), 0x7f7fffffu), scale, inverse);
+      if (t >= 2 && !dead) dead = !bar_wait(&sm.qfree[s], ((t >> 1) - 1) & 1, abort);
+      const float2 sc = make_float2(scale, scale);
+      uint8_t* dst = &sm.q[s][0][h >> 3][(cw * 8 + ky) * 128];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint4 hi, lo;
+        split_f16(mul2(lo2(qr[2 * i]), sc), hi.x, lo.x);
+        split_f16(mul2(hi2(qr[2 * i]), sc), hi.y, lo.y);
+        split_f16(mul2(lo2(qr[2 * i + 1]), sc), hi.z, lo.z);
+        split_f16(mul2(hi2(qr[2 * i + 1]), sc), hi.w, lo.w);
+        const int at = i * 256 + (((h & 7) ^ (2 * i + ky)) << 4);
+        *reinterpret_cast<uint4*>(dst + at) = hi;
+        *reinterpret_cast<uint4*>(dst + sizeof(sm.q[0][0]) + at) = lo;
+      }
+      if (lane == 0) sm.qsc[t & 3][cw] = inverse;
+      if (lane < 8) {
+        const int r = rt * kKcRows + cw * 8 + lane;
+        sm.lse[t & 3][cw * 8 + lane] = r < there ? a.lse[bh * rows + r] : INFINITY;
+        sm.last[t & 3][cw * 8 + lane] = p + r / a.group;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        bar_arrive(&sm.qfull[s]);
+        bar_arrive(&sm.info[t & 3]);
+      }
+      if (t + 1 < n) load(rt + splits);
+    }
+  } else if (warp == kKcMmaWarp) {
+    constexpr uint32_t id = kt_idesc(kKcRows);
+    bool ok = n == 0 || bar_wait(&sm.kfull, 0, abort);
+    for (int t = 0; ok && t < n; ++t) {
+      const int s = t & 1;
+      ok = bar_wait(&sm.qfull[s], (t >> 1) & 1, abort);
+      if (ok && t >= 2) ok = bar_wait(&sm.sfree[s], ((t >> 1) - 1) & 1, abort);
+      if (!ok) break;
+      tc_after();
+      const uint64_t qh0 = desc_sw128(sm.q[s][0][0]), qh1 = desc_sw128(sm.q[s][0][1]);
+      const uint64_t ql0 = desc_sw128(sm.q[s][1][0]), ql1 = desc_sw128(sm.q[s][1][1]);
+      const uint32_t kh = tmem, kl = tmem + 64, d = tmem + 128 + 64 * s;
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) mma_ts(d, kl + 8 * kk, (kk < 4 ? qh0 : qh1) + 2 * (kk & 3), id, kk > 0);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) mma_ts(d, kh + 8 * kk, (kk < 4 ? ql0 : ql1) + 2 * (kk & 3), id, 1);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) mma_ts(d, kh + 8 * kk, (kk < 4 ? qh0 : qh1) + 2 * (kk & 3), id, 1);
+      mma_commit(&sm.qfree[s]);
+      mma_commit(&sm.sfull[s]);
+    }
+    mma_commit(&sm.done);
+    mb_wait_ns(su32(&sm.done), 0, kDrainLimitNs, nullptr);
+  } else if (warp < kKcConvertWarp) {
+    // ---------------- a key per thread ----------------
+    const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
+    const int j = j0 + tid;
+    float kinv = 0.0f;
+    if (n > 0) {
+      const float4* kr = reinterpret_cast<const float4*>(a.k + (bh * a.max_t + min(j, keys - 1)) * kKvD);
+      float m = 0.0f;
+#pragma unroll 8
+      for (int i = 0; i < 32; ++i) {
+        const float4 v = kr[i];
+        m = mag(mag(mag(mag(m, v.x), v.y), v.z), v.w);
+      }
+      float scale;
+      scale_of(min(__float_as_uint(m), 0x7f7fffffu), scale, kinv);
+      const float2 sc = make_float2(scale, scale);
+#pragma unroll
+      for (int part = 0; part < 8; ++part) {
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float4 v = kr[part * 2 + i], w = kr[16 + part * 2 + i];
+          split_f16(mul2(lo2(v), sc), hi[4 * i], lo[4 * i]);
+          split_f16(mul2(hi2(v), sc), hi[4 * i + 1], lo[4 * i + 1]);
+          split_f16(mul2(lo2(w), sc), hi[4 * i + 2], lo[4 * i + 2]);
+          split_f16(mul2(hi2(w), sc), hi[4 * i + 3], lo[4 * i + 3]);
+        }
+        tm_st8(mine + 8 * part, hi);
+        tm_st8(mine + 64 + 8 * part, lo);
+      }
+      tm_wait_st();
+      tc_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&sm.kfull);
+    }
+    bool ok = true;
+    const float ck = a.c * kinv;
+    float2 sum = make_float2(0.f, 0.f);
+    for (int t = 0; ok && t < n; ++t) {
+      const int s = t & 1;
+      ok = bar_wait(&sm.info[t & 3], (t >> 2) & 1, abort) && bar_wait(&sm.sfull[s], (t >> 1) & 1, abort);
+      if (!ok) break;
+      tc_after();
+      // rows from this one on see the whole key tile
+      const bool masked = p + (first + t * splits) * kKcRows / a.group < j0 + kKcKeys - 1;
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        uint32_t r[32];
+        tm_ld32(mine + 128 + 64 * s + 32 * part, r);
+        tm_wait_ld();
+        const float4 q4 = *reinterpret_cast<const float4*>(&sm.qsc[t & 3][4 * part]);
+        const float cc[4] = {ck * q4.x, ck * q4.y, ck * q4.z, ck * q4.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float4 z = *reinterpret_cast<const float4*>(&sm.lse[t & 3][32 * part + 4 * e]);
+          const float c1 = cc[e >> 1];
+          float2 x = fma2(make_float2(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1])), make_float2(c1, c1),
+                          make_float2(-z.x, -z.y));
+          float2 y = fma2(make_float2(__uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3])), make_float2(c1, c1),
+                          make_float2(-z.z, -z.w));
+          x = make_float2(ex2(x.x), ex2(x.y));
+          y = make_float2(ex2(y.x), ex2(y.y));
+          if (masked) {
+            const int4 la = *reinterpret_cast<const int4*>(&sm.last[t & 3][32 * part + 4 * e]);
+            x.x = j <= la.x ? x.x : 0.0f;
+            x.y = j <= la.y ? x.y : 0.0f;
+            y.x = j <= la.z ? y.x : 0.0f;
+            y.y = j <= la.w ? y.y : 0.0f;
+          }
+          sum = add2(sum, add2(x, y));
+        }
+      }
+      tc_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&sm.sfree[s]);  // after the last look at the tile's constants too
+    }
+    if (j < keys) {
+      const float w = ok ? sum.x + sum.y : __uint_as_float(0x7fffffffu);
+      if (part)
+        part[((size_t)blockIdx.z * gridDim.y + bh) * a.max_t + j] = w;
+      else
+        weight[bh * a.max_t + j] += w;
+    }
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  if (warp == kKcMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kKcTmemCols) : "memory");
+}
+
+__global__ void __launch_bounds__(256)
+kv_column_add_kernel(const float* __restrict__ part, const int* __restrict__ pos, int n, int hkv, int max_t, int splits,
+                     float* __restrict__ weight) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int bh = blockIdx.y, p = pos[bh / hkv], j = blockIdx.x * 256 + threadIdx.x;
+  if (p < 0 || p >= max_t || j >= min(p + n, max_t)) return;
+  float s = 0.0f;
+  for (int z = 0; z < splits; ++z) s += part[((size_t)z * gridDim.y + bh) * max_t + j];
+  weight[(size_t)bh * max_t + j] += s;
+}
+
+int column_splits(int n, int group) {
+  // about 8 row tiles a CTA: its start, a key tile to TMEM, costs as much as two
+  const int64_t tiles = ((int64_t)n * group + kKcRows - 1) / kKcRows;
+  return (int)(tiles < 16 ? 1 : tiles / 8 > 16 ? 16 : tiles / 8);
 }
 
 template <int MASK>
@@ -791,6 +1053,35 @@ cudaError_t launch_tile(const KvArgs& a, int device, cudaStream_t s) {
 
 cudaError_t launch_kv_tile(const KvArgs& a, int mask, int device, cudaStream_t s) {
   return mask == kMaskTree ? launch_tile<kMaskTree>(a, device, s) : launch_tile<kMaskCausal>(a, device, s);
+}
+
+size_t kv_column_tile_bytes(int batch, int n, int hq, int hkv, int max_t) {
+  const int splits = column_splits(n, hq / hkv);
+  return splits > 1 ? (size_t)splits * batch * hkv * max_t * 4 : 0;
+}
+
+cudaError_t launch_kv_column_tile(const KvArgs& a, float* weight, float* part, int device, cudaStream_t s) {
+  static int configured[128] = {0};
+  const size_t smem = sizeof(KcSmem) + 1024;
+  cudaError_t e = ensure_smem((const void*)kv_column_tile_kernel, configured, device, smem, true);
+  if (e != cudaSuccess) return e;
+  const int splits = column_splits(a.n, a.group);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((a.max_t + kKcKeys - 1) / kKcKeys), (unsigned)(a.batch * a.hkv), (unsigned)splits);
+  cfg.blockDim = dim3(kKcThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, kv_column_tile_kernel, a, weight, splits > 1 ? part : nullptr, wait_limit_ns());
+  if (e != cudaSuccess || splits == 1) return e;
+  cfg.gridDim = dim3((unsigned)((a.max_t + 255) / 256), (unsigned)(a.batch * a.hkv));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, kv_column_add_kernel, (const float*)part, a.pos, a.n, a.hkv, a.max_t, splits, weight);
 }
 
 cudaError_t read_kv_tile_fault(unsigned int* flags, bool clear) {
