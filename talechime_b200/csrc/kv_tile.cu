@@ -12,8 +12,10 @@
 // factor for the tile.
 //
 // One CTA per SM, 16 warps of 128 registers:
-//   * 8 convert: cache rows to registers one tile ahead, then scaled hi / lo to swizzled shared
-//     memory, K as [64 keys][128 dims], V transposed as [128 dims][64 keys], two stages each;
+//   * 8 convert: cache rows to registers, then scaled hi / lo to swizzled shared memory, K as
+//     [64 keys][128 dims] in two stages, V transposed as [128 dims][64 keys] in three.  K runs two
+//     tiles ahead of V: a V stage is free only after the PV at the end of a softmax, and K behind
+//     it in the same warps would hold up the next QK;
 //   * 8 softmax: two threads a row, one for each half of the keys and then of the dimensions;
 //     scores from TMEM, running maximum and sum, P' = 2^14 p back to TMEM as hi / lo; then the
 //     O tile of the tile before is added to registers.  The first of them also issues the MMAs,
@@ -45,13 +47,14 @@ __shared__ uint64_t s_kt_wait_ns;
 
 struct KtSmem {
   alignas(1024) uint8_t k[2][2][2][kKvTileKeys * 128];  // [stage][hi, lo][64 dims][key][128 B]
-  alignas(1024) uint8_t v[2][2][kKvD * 128];            // [stage][hi, lo][dim][64 keys]
+  alignas(1024) uint8_t v[3][2][kKvD * 128];            // [stage][hi, lo][dim][64 keys]
   alignas(16) float ksc[4][8], vsc[4][8];               // inverse scales of the groups of tiles t % 4
   alignas(8) uint8_t vbad[4][8];                        // keys of the tile whose value row is not finite
   float top[2][2][kKvTileRows];                         // the rows' maxima over either half of a tile
-  alignas(8) uint64_t kfull[2], kfree[2], vfull[2], vfree[2];
+  alignas(8) uint64_t kfull[2], kfree[2], vfull[3], vfree[3];
   uint64_t kinfo[4], vinfo[4];
   uint64_t sfull[2], pfull[2], qfull, ofull, ofree, done;
+  alignas(16) float turn[2][4][32][36];  // rows of four warps: coalesced memory <-> a thread per row
   KvFind find;
   uint32_t tmem;
   int abort;
@@ -218,6 +221,13 @@ __device__ __forceinline__ void scale_of(unsigned top, float& scale, float& inve
 __device__ __forceinline__ float mag(float m, float x) { return fmaxf(m, fabsf(x)); }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
+// Cache rows pass the SM once: past L1, whose small rest beside 200 KB of shared memory holds
+// the tree's masks and what registers cannot (a reload from L2 is 600 cycles of a warp's time).
+__device__ __forceinline__ float4 ld_row(const float4* p) {
+  const int4 v = ld_stream_v4(p);
+  return make_float4(__int_as_float(v.x), __int_as_float(v.y), __int_as_float(v.z), __int_as_float(v.w));
+}
+
 // The units of this CTA and their tiles, in order.
 template <int MASK>
 struct KtCursor {
@@ -264,10 +274,12 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
     for (int i = 0; i < 2; ++i) {
       bar_init(&sm.kfull[i], 8);
       bar_init(&sm.kfree[i], 1);
-      bar_init(&sm.vfull[i], 8);
-      bar_init(&sm.vfree[i], 1);
       bar_init(&sm.sfull[i], 1);
       bar_init(&sm.pfull[i], 8);
+    }
+    for (int i = 0; i < 3; ++i) {
+      bar_init(&sm.vfull[i], 8);
+      bar_init(&sm.vfree[i], 1);
     }
     for (int i = 0; i < 4; ++i) {
       bar_init(&sm.kinfo[i], 8);
@@ -323,15 +335,15 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         if ((c + 1) * kKvTileKeys <= plain) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            kr[2 * i] = kp[i * 64];
-            kr[2 * i + 1] = kp[i * 64 + 16];
+            kr[2 * i] = ld_row(kp + i * 64);
+            kr[2 * i + 1] = ld_row(kp + i * 64 + 16);
           }
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const bool there = kt_row_there<MASK>(a, x, c * kKvTileKeys + cw * 8 + ky + 2 * i);
-            kr[2 * i] = there ? kp[i * 64] : make_float4(0.f, 0.f, 0.f, 0.f);
-            kr[2 * i + 1] = there ? kp[i * 64 + 16] : make_float4(0.f, 0.f, 0.f, 0.f);
+            kr[2 * i] = there ? ld_row(kp + i * 64) : make_float4(0.f, 0.f, 0.f, 0.f);
+            kr[2 * i + 1] = there ? ld_row(kp + i * 64 + 16) : make_float4(0.f, 0.f, 0.f, 0.f);
           }
         }
         kp += kKvTileKeys * (kKvD / 4);
@@ -339,21 +351,18 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       auto load_v = [&](int c) {
         if ((c + 1) * kKvTileKeys <= plain) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) vr[i] = vp[i * 32];
+          for (int i = 0; i < 8; ++i) vr[i] = ld_row(vp + i * 32);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            vr[i] = kt_row_there<MASK>(a, x, c * kKvTileKeys + cw * 8 + i) ? vp[i * 32] : make_float4(0.f, 0.f, 0.f, 0.f);
+            vr[i] = kt_row_there<MASK>(a, x, c * kKvTileKeys + cw * 8 + i) ? ld_row(vp + i * 32)
+                                                                            : make_float4(0.f, 0.f, 0.f, 0.f);
         }
         vp += kKvTileKeys * (kKvD / 4);
       };
-      load_k(cur.off);
-      load_v(cur.off);
-      const int end = cur.off + cur.n;
-      for (int c = cur.off; c < end; ++c, ++t) {
+      auto convert_k = [&](int t) {
         const int s = t & 1;
         float scale, inverse;
-        {  // K
           float m = 0.0f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) m = mag(mag(mag(mag(m, kr[i].x), kr[i].y), kr[i].z), kr[i].w);
@@ -390,9 +399,10 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
             bar_arrive(&sm.kfull[s]);
             bar_arrive(&sm.kinfo[t & 3]);
           }
-        }
-        if (c + 1 < end) load_k(c + 1);
-        {  // V
+      };
+      auto convert_v = [&](int t) {
+        const int s = t % 3;
+        float scale, inverse;
           float m = 0.0f;
           float2 z = make_float2(0.f, 0.f);
 #pragma unroll
@@ -418,7 +428,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
             top = __reduce_max_sync(kFull, __float_as_uint(m));
           }
           scale_of(top, scale, inverse);
-          if (t >= 2 && !dead) dead = !bar_wait(&sm.vfree[s], ((t >> 1) - 1) & 1, abort);
+          if (t >= 3 && !dead) dead = !bar_wait(&sm.vfree[s], (t / 3 - 1) & 1, abort);
           const float2 sc = make_float2(scale, scale);
           uint8_t* dst = &sm.v[s][0][vat];
           // dimensions 4 lane + e and 4 lane + e + 1 of all 8 keys at a time
@@ -457,8 +467,23 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
             bar_arrive(&sm.vfull[s]);
             bar_arrive(&sm.vinfo[t & 3]);
           }
+      };
+      const int c0 = cur.off, n = cur.n;
+      load_k(c0);
+      load_v(c0);
+      convert_k(t);
+      if (n > 1) load_k(c0 + 1);
+      for (int i = 0; i < n; ++i, ++t) {
+        if (i + 1 < n && i == 0) {
+          convert_k(t + 1);
+          if (n > 2) load_k(c0 + 2);
         }
-        if (c + 1 < end) load_v(c + 1);
+        convert_v(t);
+        if (i + 1 < n) load_v(c0 + i + 1);
+        if (i + 2 < n) {
+          convert_k(t + 2);
+          if (i + 3 < n) load_k(c0 + i + 3);
+        }
       }
     }
   } else {
@@ -503,13 +528,13 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       mma_commit(&sm.sfull[s]);
     };
     auto issue_pv = [&](int w) {  // O = P V of tile w, once every warp wrote its P and has the O before
-      const int s = w & 1;
-      wait(&sm.vfull[s], (w >> 1) & 1);
+      const int s = w & 1, vs = w % 3;
+      wait(&sm.vfull[vs], (w / 3) & 1);
       wait(&sm.pfull[s], (w >> 1) & 1);
       if (w > 0) wait(&sm.ofree, (w - 1) & 1);
       if (!ok) return;
       tc_after();
-      const uint64_t vh = desc_sw128(sm.v[s][0]), vl = desc_sw128(sm.v[s][1]);
+      const uint64_t vh = desc_sw128(sm.v[vs][0]), vl = desc_sw128(sm.v[vs][1]);
       const uint32_t ph = tmem + kTmP + 64 * s, pl = ph + 32, d = tmem + kTmO;
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) mma_ts(d, pl + 8 * kk, vh + 2 * kk, id_pv, kk > 0);
@@ -517,7 +542,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       for (int kk = 0; kk < 4; ++kk) mma_ts(d, ph + 8 * kk, vl + 2 * kk, id_pv, 1);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) mma_ts(d, ph + 8 * kk, vh + 2 * kk, id_pv, 1);
-      mma_commit(&sm.vfree[s]);
+      mma_commit(&sm.vfree[vs]);
       mma_commit(&sm.ofull);
     };
     int units = 0;
@@ -525,16 +550,37 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       const KvUnit& x = cur.x;
       const int c0 = cur.off, n = cur.n;
       const int token = kv_token<MASK>(a, x, min(row, x.nrows - 1));
-      // half of the query row: scaled hi / lo to TMEM, dimensions in the order of the K tiles
+      // half of the query row: scaled hi / lo to TMEM, dimensions in the order of the K tiles (32
+      // half .. + 32 and 64 + 32 half .. + 32).  A thread that reads its own row takes 32 memory
+      // transactions an access (that cost 10 us a unit), so the warp reads rows and turns them.
       float qinv;
       {
-        const float4* qr = reinterpret_cast<const float4*>(a.q + kv_row_offset<MASK>(a, x, min(row, x.nrows - 1)));
-        float m = 0.0f;
-#pragma unroll 8
-        for (int i = 0; i < 32; ++i) {
-          const float4 v = qr[i];
-          m = mag(mag(mag(mag(m, v.x), v.y), v.z), v.w);
+        float4 mine4[16];
+        float4* turn = reinterpret_cast<float4*>(&sm.turn[half][warp & 3][0][0]);
+        const int row0 = (warp & 3) * 32;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {  // the two stretches of 32 dimensions
+          float4 v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = row0 + 4 * i + (lane >> 3);
+            v[i] = reinterpret_cast<const float4*>(a.q + kv_row_offset<MASK>(a, x, min(r, x.nrows - 1)))
+                [part * 16 + half * 8 + (lane & 7)];
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) turn[(4 * i + (lane >> 3)) * 9 + (lane & 7)] = v[i];
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) mine4[part * 8 + i] = turn[lane * 9 + i];
+          __syncwarp();
         }
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = mag(mag(mag(mag(m, mine4[i].x), mine4[i].y), mine4[i].z), mine4[i].w);
+        sm.top[0][half][row] = m;
+        meet();
+        m = fmaxf(m, sm.top[0][half ^ 1][row]);
+        meet();
         float scale;
         scale_of(min(__float_as_uint(m), 0x7f7fffffu), scale, qinv);
         const float2 sc = make_float2(scale, scale);
@@ -543,11 +589,11 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
           uint32_t hi[8], lo[8];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float4 v = qr[half * 8 + part * 2 + i], w = qr[16 + half * 8 + part * 2 + i];
-            split_f16(mul2(make_float2(v.x, v.y), sc), hi[4 * i], lo[4 * i]);
-            split_f16(mul2(make_float2(v.z, v.w), sc), hi[4 * i + 1], lo[4 * i + 1]);
-            split_f16(mul2(make_float2(w.x, w.y), sc), hi[4 * i + 2], lo[4 * i + 2]);
-            split_f16(mul2(make_float2(w.z, w.w), sc), hi[4 * i + 3], lo[4 * i + 3]);
+            const float4 v = mine4[part * 2 + i], w = mine4[8 + part * 2 + i];
+            split_f16(mul2(lo2(v), sc), hi[4 * i], lo[4 * i]);
+            split_f16(mul2(hi2(v), sc), hi[4 * i + 1], lo[4 * i + 1]);
+            split_f16(mul2(lo2(w), sc), hi[4 * i + 2], lo[4 * i + 2]);
+            split_f16(mul2(hi2(w), sc), hi[4 * i + 3], lo[4 * i + 3]);
           }
           tm_st8(mine + kTmQ + 32 * half + 8 * part, hi);
           tm_st8(mine + kTmQ + 64 + 32 * half + 8 * part, lo);
@@ -742,18 +788,40 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       const size_t slot = a.split ? (size_t)blockIdx.x + cur.u : (size_t)cur.u;
       const float nan = __uint_as_float(0x7fffffffu);
       if (!kv_row_valid<MASK>(a, x, row)) m = -INFINITY;
-      if (row < x.nrows) {
-        constexpr float kUnscale = 1.0f / (1 << kKtPScale);  // P' = 2^14 p is in both sums
-        float f = kUnscale;
-        if (whole) f = m == -INFINITY ? 0.0f : __fdiv_rn(1.0f, l);
-        if (!ok) f = nan;
-        float2* dst = reinterpret_cast<float2*>(whole ? a.out + kv_row_offset<MASK>(a, x, row)
-                                                      : a.acc + (slot * a.rows + row) * kKvD) + half;
+      constexpr float kUnscale = 1.0f / (1 << kKtPScale);  // P' = 2^14 p is in both sums
+      float f = kUnscale;
+      if (whole) f = m == -INFINITY ? 0.0f : __fdiv_rn(1.0f, l);
+      if (!ok) f = nan;
+      {
+        // 32 dimensions of the pair's 32 rows at a time, turned back and written by rows
+        float* turn = &sm.turn[0][warp & 3][0][0];
+        const int r0 = (warp & 3) * 32 + 16 * half + (lane >> 3);
+        float4* dst[4];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float e0 = i & 1 ? o[i >> 1].y : o[i >> 1].x, e1 = i & 1 ? o[16 + (i >> 1)].y : o[16 + (i >> 1)].x;
-          dst[2 * i] = f == 0.0f ? make_float2(0.f, 0.f) : make_float2(e0 * f, e1 * f);
+        for (int i = 0; i < 4; ++i) {
+          const int r = min(r0 + 4 * i, x.nrows - 1);
+          dst[i] = reinterpret_cast<float4*>(whole ? a.out + kv_row_offset<MASK>(a, x, r)
+                                                   : a.acc + (slot * a.rows + r) * kKvD) + (lane & 7);
         }
+#pragma unroll
+        for (int part = 0; part < 4; ++part) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int k = part * 8 + i;
+            const float e0 = k & 1 ? o[k >> 1].y : o[k >> 1].x, e1 = k & 1 ? o[16 + (k >> 1)].y : o[16 + (k >> 1)].x;
+            *reinterpret_cast<float2*>(turn + lane * 36 + 4 * i + 2 * half) =
+                f == 0.0f ? make_float2(0.f, 0.f) : make_float2(e0 * f, e1 * f);
+          }
+          meet();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 v = *reinterpret_cast<const float4*>(turn + (16 * half + 4 * i + (lane >> 3)) * 36 + 4 * (lane & 7));
+            if (r0 + 4 * i < x.nrows) dst[i][part * 8] = v;
+          }
+          meet();
+        }
+      }
+      if (row < x.nrows) {
         if (half == 0) {
           if (a.stat) {
             a.stat[slot * 2 * a.rows + row] = m;
