@@ -12,15 +12,16 @@
 // factor for the tile.
 //
 // One CTA per SM, 16 warps of 128 registers:
-//   * 8 convert: cache rows to registers, then scaled hi / lo to swizzled shared memory, K as
-//     [64 keys][128 dims] in two stages, V transposed as [128 dims][64 keys] in three.  K runs two
-//     tiles ahead of V: a V stage is free only after the PV at the end of a softmax, and K behind
-//     it in the same warps would hold up the next QK;
+//   * 7 convert, in turn, groups of 8 keys or values: cache rows to registers one group ahead, then
+//     scaled hi / lo to swizzled shared memory, K as [64 keys][128 dims] in two stages, V transposed
+//     as [128 dims][64 keys] in three.  K runs two tiles ahead of V: a V stage is free only after
+//     the PV that follows a softmax, and K behind it would hold up the next QK;
+//   * 1 issues the MMAs, S = Q K^T and O = P V (Q and P in TMEM, S and P double-buffered), so that
+//     QK of a tile runs while the softmax of the one before is at work.  Issuing waits for the
+//     tensor cores' queue, 1600 cycles a tile: a warp with other work cannot do it beside;
 //   * 8 softmax: two threads a row, one for each half of the keys and then of the dimensions;
 //     scores from TMEM, running maximum and sum, P' = 2^14 p back to TMEM as hi / lo; then the
-//     O tile of the tile before is added to registers.  The first of them also issues the MMAs,
-//     O = P V of its tile and S = Q K^T two tiles ahead (Q and P in TMEM, S and P double-
-//     buffered), which run while the warps are at the next tile.
+//     O tile of the tile before is added to registers.
 // The tensor cores cut their f32 sums, so an O tile starts from 0 and joins the running sum with
 // rounding.  TMEM (512 columns): Q 128, S 2 x 64, P 2 x 64, O 128.
 //
@@ -37,13 +38,40 @@ namespace q8lin {
 namespace {
 
 constexpr int kKtThreads = 512;
-constexpr int kKtConvertWarp = 8;
+constexpr int kKtConvertWarp = 8, kKtConverters = 7, kKtMmaWarp = 15;
 constexpr uint32_t kKtTmemCols = 512;
 constexpr uint32_t kTmQ = 0, kTmS = 128, kTmP = 256, kTmO = 384;
 constexpr int kKtPScale = 14;     // P' = 2^14 p
 
 __device__ unsigned int g_kv_tile_fault;
 __shared__ uint64_t s_kt_wait_ns;
+
+// The units of this CTA and their tiles, in order.
+struct KtCursor {
+  int u, off, left;  // unit, its first tile here, tiles left of the CTA's share
+  int n;             // tiles of the unit here
+  KvUnit x;
+  // Moves to the first unit from u on with work; false when there is none.
+  template <int MASK>
+  __device__ bool seek(const KvArgs& a) {
+    while (u < a.units && left > 0) {
+      x = kv_unit<MASK>(a, u);
+      n = min(x.chunks - off, left);
+      if (n > 0) return true;
+      off = 0;
+      ++u;
+      if (!a.split) break;
+    }
+    return false;
+  }
+  template <int MASK>
+  __device__ bool next(const KvArgs& a) {
+    left -= n;
+    off = 0;
+    ++u;
+    return a.split && seek<MASK>(a);
+  }
+};
 
 struct KtSmem {
   alignas(1024) uint8_t k[2][2][2][kKvTileKeys * 128];  // [stage][hi, lo][64 dims][key][128 B]
@@ -52,8 +80,9 @@ struct KtSmem {
   alignas(8) uint8_t vbad[4][8];                        // keys of the tile whose value row is not finite
   float top[2][2][kKvTileRows];                         // the rows' maxima over either half of a tile
   alignas(8) uint64_t kfull[2], kfree[2], vfull[3], vfree[3];
-  uint64_t kinfo[4], vinfo[4];
+  uint64_t vinfo[4];
   uint64_t sfull[2], pfull[2], qfull, ofull, ofree, done;
+  KtCursor cursor[8];                  // the softmax warps' (registers are short there)
   alignas(16) float turn[2][4][32][36];  // rows of four warps: coalesced memory <-> a thread per row
   KvFind find;
   uint32_t tmem;
@@ -67,19 +96,11 @@ __device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
 __device__ __forceinline__ void bar_arrive(uint64_t* b) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(b)) : "memory");
 }
-// Bounded wait; once one has run out (or another warp's has) every wait of the CTA fails.  A try
-// sleeps up to kKtSleepNs in the barrier unit instead of polling.
-constexpr uint32_t kKtSleepNs = 20000;
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
-               : "=r"(ok) : "r"(bar), "r"(parity), "r"(kKtSleepNs) : "memory");
-  return ok != 0;
-}
+// Bounded wait; once one has run out (or another warp's has) every wait of the CTA fails.
 __device__ __forceinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort) {
   const uint64_t t0 = global_ns();
   while (!*abort) {
-    if (bar_try(bar, parity)) return true;
+    if (mb_try(bar, parity)) return true;
     if (global_ns() - t0 > s_kt_wait_ns) {
       atomicOr(&g_kv_tile_fault, 32u);
       *abort = 1;
@@ -90,7 +111,7 @@ __device__ __forceinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, vol
 // By whole warps: the verdict is uniform.
 __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* abort) {
   const uint32_t bar = su32(b);
-  return __all_sync(kFull, bar_try(bar, parity) || bar_wait_slow(bar, parity, abort));
+  return __all_sync(kFull, mb_try(bar, parity) || bar_wait_slow(bar, parity, abort));
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -228,32 +249,6 @@ __device__ __forceinline__ float4 ld_row(const float4* p) {
   return make_float4(__int_as_float(v.x), __int_as_float(v.y), __int_as_float(v.z), __int_as_float(v.w));
 }
 
-// The units of this CTA and their tiles, in order.
-template <int MASK>
-struct KtCursor {
-  int u, off, left;  // unit, its first tile here, tiles left of the CTA's share
-  int n;             // tiles of the unit here
-  KvUnit x;
-  // Moves to the first unit from u on with work; false when there is none.
-  __device__ bool seek(const KvArgs& a) {
-    while (u < a.units && left > 0) {
-      x = kv_unit<MASK>(a, u);
-      n = min(x.chunks - off, left);
-      if (n > 0) return true;
-      off = 0;
-      ++u;
-      if (!a.split) break;
-    }
-    return false;
-  }
-  __device__ bool next(const KvArgs& a) {
-    left -= n;
-    off = 0;
-    ++u;
-    return a.split && seek(a);
-  }
-};
-
 template <int MASK>
 __device__ __forceinline__ bool kt_row_there(const KvArgs& a, const KvUnit& x, int j) {
   if (j >= x.keys) return false;
@@ -274,17 +269,14 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
     for (int i = 0; i < 2; ++i) {
       bar_init(&sm.kfull[i], 8);
       bar_init(&sm.kfree[i], 1);
-      bar_init(&sm.sfull[i], 1);
+      bar_init(&sm.sfull[i], 2);
       bar_init(&sm.pfull[i], 8);
     }
     for (int i = 0; i < 3; ++i) {
       bar_init(&sm.vfull[i], 8);
       bar_init(&sm.vfree[i], 1);
     }
-    for (int i = 0; i < 4; ++i) {
-      bar_init(&sm.kinfo[i], 8);
-      bar_init(&sm.vinfo[i], 8);
-    }
+    for (int i = 0; i < 4; ++i) bar_init(&sm.vinfo[i], 8);
     bar_init(&sm.qfull, 8);
     bar_init(&sm.ofull, 1);
     bar_init(&sm.ofree, 8);
@@ -292,124 +284,138 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
     sm.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 0) {
+  if (warp == kKtMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&sm.tmem)),
                  "r"(kKtTmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait();
   pdl_launch_dependents();
-  KtCursor<MASK> cur;
+  KtCursor start;
   if (a.split) {
-    cur.left = kv_find<MASK, kKtThreads>(a, sm.find, blockIdx.x);
-    cur.u = sm.find.unit;
-    cur.off = sm.find.off;
+    start.left = kv_find<MASK, kKtThreads>(a, sm.find, blockIdx.x);
+    start.u = sm.find.unit;
+    start.off = sm.find.off;
   } else {
-    cur.u = a.units - 1 - (int)blockIdx.x;  // later rows see more keys: longest first
-    cur.off = 0;
-    cur.left = 0x3fffffff;
+    start.u = a.units - 1 - (int)blockIdx.x;  // later rows see more keys: longest first
+    start.off = 0;
+    start.left = 0x3fffffff;
   }
   tc_before();
   __syncthreads();
   tc_after();
   const uint32_t tmem = sm.tmem;
 
-  if (warp >= kKtConvertWarp) {
+  if (warp >= kKtConvertWarp && warp < kKtMmaWarp) {
     // ---------------- converters ----------------
-    // warp cw: keys and values 8 cw .. + 8 of every tile, on its own (no barrier between warps)
-    const int cw = warp - kKtConvertWarp, h = lane & 15;
-    // where the lane's pieces go: K row 2 i + lane / 16, dimensions in 16-byte pieces of 4 h .. and
-    // 64 + 4 h ..; V row (dimension) 32 e + lane, the piece of its 8 keys
-    const int kat = (cw * 8 + (lane >> 4)) * 128, kx = h & 7, ky = lane >> 4;
-    const int vat = lane * 128 + ((cw ^ (lane & 7)) << 4);
+    // The unit's groups in order: K of tile 0, K of tile 1, then V of tile i and K of tile i + 2 in
+    // turn, 8 groups each; warp w takes groups w, w + 7, ..., with no barrier between warps.
+    const int h = lane & 15, ky = lane >> 4;
+    KtCursor cur = start;
     bool dead = false;
-    int t = 0;
-    for (bool more = cur.seek(a); more; more = cur.next(a)) {
+    int t0 = 0;  // the unit's first tile in the CTA's count
+    for (bool more = cur.seek<MASK>(a); more; t0 += cur.n, more = cur.next<MASK>(a)) {
       const KvUnit& x = cur.x;
       const size_t head = ((size_t)x.b * a.hkv + x.hk) * (size_t)a.max_t;
-      const float4* kp = reinterpret_cast<const float4*>(a.k + (head + cur.off * kKvTileKeys + cw * 8 + ky) * kKvD) + h;
-      const float4* vp = reinterpret_cast<const float4*>(a.v + (head + cur.off * kKvTileKeys + cw * 8) * kKvD) + lane;
+      // lane's pieces of a row: K dimensions 4 h .. and 64 + 4 h .. of row 2 i + lane / 16, V
+      // dimensions 4 lane .. of row i
+      const float4* kp = reinterpret_cast<const float4*>(a.k + (head + ky) * kKvD) + h;
+      const float4* vp = reinterpret_cast<const float4*>(a.v + head * kKvD) + lane;
+      const int c0 = cur.off, n = cur.n, items = (2 * n + 1) * 8;
       const int plain = MASK == kMaskTree ? x.p : x.keys;  // rows below need no look
-      float4 kr[8], vr[8];
-      auto load_k = [&](int c) {
-        if ((c + 1) * kKvTileKeys <= plain) {
+      // item -> tile of the unit, or -1 where there is none
+      auto tile_of = [&](int item) {
+        const int s = item >> 3;
+        const int c = s == 0 ? 0 : s & 1 ? (s + 1) >> 1 : (s - 2) >> 1;
+        return c < n ? c : -1;
+      };
+      auto is_v = [](int item) { return item >= 16 && !((item >> 3) & 1); };
+      float4 nx[8];
+      auto load = [&](int item) {
+        const int c = tile_of(item);
+        if (c < 0) return;
+        const int j0 = (c0 + c) * kKvTileKeys + (item & 7) * 8;
+        if (is_v(item)) {
+          const float4* row = vp + (size_t)j0 * (kKvD / 4);
+          if (j0 + 8 <= plain) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            kr[2 * i] = ld_row(kp + i * 64);
-            kr[2 * i + 1] = ld_row(kp + i * 64 + 16);
+            for (int i = 0; i < 8; ++i) nx[i] = ld_row(row + i * 32);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              nx[i] = kt_row_there<MASK>(a, x, j0 + i) ? ld_row(row + i * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
           }
         } else {
+          const float4* row = kp + (size_t)j0 * (kKvD / 4);
+          if (j0 + 8 <= plain) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool there = kt_row_there<MASK>(a, x, c * kKvTileKeys + cw * 8 + ky + 2 * i);
-            kr[2 * i] = there ? ld_row(kp + i * 64) : make_float4(0.f, 0.f, 0.f, 0.f);
-            kr[2 * i + 1] = there ? ld_row(kp + i * 64 + 16) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < 4; ++i) {
+              nx[2 * i] = ld_row(row + i * 64);
+              nx[2 * i + 1] = ld_row(row + i * 64 + 16);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool there = kt_row_there<MASK>(a, x, j0 + ky + 2 * i);
+              nx[2 * i] = there ? ld_row(row + i * 64) : make_float4(0.f, 0.f, 0.f, 0.f);
+              nx[2 * i + 1] = there ? ld_row(row + i * 64 + 16) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
           }
         }
-        kp += kKvTileKeys * (kKvD / 4);
       };
-      auto load_v = [&](int c) {
-        if ((c + 1) * kKvTileKeys <= plain) {
+      int item = warp - kKtConvertWarp;
+      load(item);
+      for (; item < items; item += kKtConverters) {
+        float4 r[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) vr[i] = ld_row(vp + i * 32);
-        } else {
+        for (int i = 0; i < 8; ++i) r[i] = nx[i];
+        if (item + kKtConverters < items) load(item + kKtConverters);
+        const int c = tile_of(item), g = item & 7;
+        if (c < 0) continue;
+        const int t = t0 + c;
+        float m = 0.0f, scale, inverse;
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            vr[i] = kt_row_there<MASK>(a, x, c * kKvTileKeys + cw * 8 + i) ? ld_row(vp + i * 32)
-                                                                            : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-        vp += kKvTileKeys * (kKvD / 4);
-      };
-      auto convert_k = [&](int t) {
-        const int s = t & 1;
-        float scale, inverse;
-          float m = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) m = mag(mag(mag(mag(m, kr[i].x), kr[i].y), kr[i].z), kr[i].w);
+        for (int i = 0; i < 8; ++i) m = mag(mag(mag(mag(m, r[i].x), r[i].y), r[i].z), r[i].w);
+        if (!is_v(item)) {
+          const int s = t & 1;
           unsigned top = __reduce_max_sync(kFull, __float_as_uint(m));
           if (top >= 0x7f800000u) {  // an infinite key: the scale of the others
             m = 0.0f;
+#pragma unroll
             for (int i = 0; i < 8; ++i) {
-              m = finite(kr[i].x) ? mag(m, kr[i].x) : m;
-              m = finite(kr[i].y) ? mag(m, kr[i].y) : m;
-              m = finite(kr[i].z) ? mag(m, kr[i].z) : m;
-              m = finite(kr[i].w) ? mag(m, kr[i].w) : m;
+              m = finite(r[i].x) ? mag(m, r[i].x) : m;
+              m = finite(r[i].y) ? mag(m, r[i].y) : m;
+              m = finite(r[i].z) ? mag(m, r[i].z) : m;
+              m = finite(r[i].w) ? mag(m, r[i].w) : m;
             }
             top = __reduce_max_sync(kFull, __float_as_uint(m));
           }
           scale_of(top, scale, inverse);
           if (t >= 2 && !dead) dead = !bar_wait(&sm.kfree[s], ((t >> 1) - 1) & 1, abort);
           const float2 sc = make_float2(scale, scale);
-          uint8_t* dst = &sm.k[s][0][h >> 3][kat];
+          uint8_t* dst = &sm.k[s][0][h >> 3][(g * 8 + ky) * 128];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint4 hi, lo;
-            split_f16(mul2(make_float2(kr[2 * i].x, kr[2 * i].y), sc), hi.x, lo.x);
-            split_f16(mul2(make_float2(kr[2 * i].z, kr[2 * i].w), sc), hi.y, lo.y);
-            split_f16(mul2(make_float2(kr[2 * i + 1].x, kr[2 * i + 1].y), sc), hi.z, lo.z);
-            split_f16(mul2(make_float2(kr[2 * i + 1].z, kr[2 * i + 1].w), sc), hi.w, lo.w);
-            const int at = i * 256 + ((kx ^ (2 * i + ky)) << 4);
+            split_f16(mul2(lo2(r[2 * i]), sc), hi.x, lo.x);
+            split_f16(mul2(hi2(r[2 * i]), sc), hi.y, lo.y);
+            split_f16(mul2(lo2(r[2 * i + 1]), sc), hi.z, lo.z);
+            split_f16(mul2(hi2(r[2 * i + 1]), sc), hi.w, lo.w);
+            const int at = i * 256 + (((h & 7) ^ (2 * i + ky)) << 4);
             *reinterpret_cast<uint4*>(dst + at) = hi;
             *reinterpret_cast<uint4*>(dst + sizeof(sm.k[0][0]) + at) = lo;
           }
-          if (lane == 0) sm.ksc[t & 3][cw] = inverse;
+          if (lane == 0) sm.ksc[t & 3][g] = inverse;
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0) {
-            bar_arrive(&sm.kfull[s]);
-            bar_arrive(&sm.kinfo[t & 3]);
-          }
-      };
-      auto convert_v = [&](int t) {
-        const int s = t % 3;
-        float scale, inverse;
-          float m = 0.0f;
-          float2 z = make_float2(0.f, 0.f);
+          if (lane == 0) bar_arrive(&sm.kfull[s]);
+        } else {
+          const int s = t % 3;
+          float2 z = make_float2(0.f, 0.f);  // NaN unless all are finite
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            m = mag(mag(mag(mag(m, vr[i].x), vr[i].y), vr[i].z), vr[i].w);
-            z = fma2(make_float2(vr[i].x, vr[i].y), make_float2(0.f, 0.f), z);  // NaN unless all are finite
-            z = fma2(make_float2(vr[i].z, vr[i].w), make_float2(0.f, 0.f), z);
+            z = fma2(lo2(r[i]), make_float2(0.f, 0.f), z);
+            z = fma2(hi2(r[i]), make_float2(0.f, 0.f), z);
           }
           unsigned top = __reduce_max_sync(kFull, z.x + z.y == 0.0f ? __float_as_uint(m) : 0x7f800000u);
           unsigned bad = 0;
@@ -419,47 +425,44 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
             m = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              if (__any_sync(kFull, !(finite(vr[i].x) && finite(vr[i].y) && finite(vr[i].z) && finite(vr[i].w)))) {
-                vr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (__any_sync(kFull, !(finite(r[i].x) && finite(r[i].y) && finite(r[i].z) && finite(r[i].w)))) {
+                r[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                 bad |= 1u << i;
               }
-              m = mag(mag(mag(mag(m, vr[i].x), vr[i].y), vr[i].z), vr[i].w);
+              m = mag(mag(mag(mag(m, r[i].x), r[i].y), r[i].z), r[i].w);
             }
             top = __reduce_max_sync(kFull, __float_as_uint(m));
           }
           scale_of(top, scale, inverse);
           if (t >= 3 && !dead) dead = !bar_wait(&sm.vfree[s], (t / 3 - 1) & 1, abort);
           const float2 sc = make_float2(scale, scale);
-          uint8_t* dst = &sm.v[s][0][vat];
-          // dimensions 4 lane + e and 4 lane + e + 1 of all 8 keys at a time
+          // dimension 4 lane + e sits in row 32 e + lane, the group's 8 keys in one piece of it
+          uint8_t* dst = &sm.v[s][0][lane * 128 + ((g ^ (lane & 7)) << 4)];
           auto put = [&](int e, float2 w0, float2 w1, float2 w2, float2 w3, float2 w4, float2 w5, float2 w6, float2 w7) {
-            float2 w[8] = {mul2(w0, sc), mul2(w1, sc), mul2(w2, sc), mul2(w3, sc),
-                           mul2(w4, sc), mul2(w5, sc), mul2(w6, sc), mul2(w7, sc)};
-            uint4 h0, h1, l0, l1;
-            uint32_t* ph0 = &h0.x;
-            uint32_t* ph1 = &h1.x;
-            uint32_t* pl0 = &l0.x;
-            uint32_t* pl1 = &l1.x;
+            const float2 w[8] = {mul2(w0, sc), mul2(w1, sc), mul2(w2, sc), mul2(w3, sc),
+                                 mul2(w4, sc), mul2(w5, sc), mul2(w6, sc), mul2(w7, sc)};
+            uint32_t h0[4], h1[4], l0[4], l1[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const float2 b0 = cut2(w[2 * i]), b1 = cut2(w[2 * i + 1]);
-              ph0[i] = pack_f16(b0.x, b1.x);
-              ph1[i] = pack_f16(b0.y, b1.y);
+              h0[i] = pack_f16(b0.x, b1.x);
+              h1[i] = pack_f16(b0.y, b1.y);
               const float2 r0 = fma2(b0, make_float2(-1.0f, -1.0f), w[2 * i]);
               const float2 r1 = fma2(b1, make_float2(-1.0f, -1.0f), w[2 * i + 1]);
-              pl0[i] = pack_f16(r0.x, r1.x);
-              pl1[i] = pack_f16(r0.y, r1.y);
+              l0[i] = pack_f16(r0.x, r1.x);
+              l1[i] = pack_f16(r0.y, r1.y);
             }
-            *reinterpret_cast<uint4*>(dst + e * 4096) = h0;
-            *reinterpret_cast<uint4*>(dst + e * 4096 + 4096) = h1;
-            *reinterpret_cast<uint4*>(dst + sizeof(sm.v[0][0]) + e * 4096) = l0;
-            *reinterpret_cast<uint4*>(dst + sizeof(sm.v[0][0]) + e * 4096 + 4096) = l1;
+            constexpr int low = sizeof(sm.v[0][0]);
+            *reinterpret_cast<uint4*>(dst + e * 4096) = make_uint4(h0[0], h0[1], h0[2], h0[3]);
+            *reinterpret_cast<uint4*>(dst + e * 4096 + 4096) = make_uint4(h1[0], h1[1], h1[2], h1[3]);
+            *reinterpret_cast<uint4*>(dst + low + e * 4096) = make_uint4(l0[0], l0[1], l0[2], l0[3]);
+            *reinterpret_cast<uint4*>(dst + low + e * 4096 + 4096) = make_uint4(l1[0], l1[1], l1[2], l1[3]);
           };
-          put(0, lo2(vr[0]), lo2(vr[1]), lo2(vr[2]), lo2(vr[3]), lo2(vr[4]), lo2(vr[5]), lo2(vr[6]), lo2(vr[7]));
-          put(2, hi2(vr[0]), hi2(vr[1]), hi2(vr[2]), hi2(vr[3]), hi2(vr[4]), hi2(vr[5]), hi2(vr[6]), hi2(vr[7]));
+          put(0, lo2(r[0]), lo2(r[1]), lo2(r[2]), lo2(r[3]), lo2(r[4]), lo2(r[5]), lo2(r[6]), lo2(r[7]));
+          put(2, hi2(r[0]), hi2(r[1]), hi2(r[2]), hi2(r[3]), hi2(r[4]), hi2(r[5]), hi2(r[6]), hi2(r[7]));
           if (lane == 0) {
-            sm.vsc[t & 3][cw] = inverse;
-            sm.vbad[t & 3][cw] = (uint8_t)bad;
+            sm.vsc[t & 3][g] = inverse;
+            sm.vbad[t & 3][g] = (uint8_t)bad;
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
@@ -467,25 +470,61 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
             bar_arrive(&sm.vfull[s]);
             bar_arrive(&sm.vinfo[t & 3]);
           }
-      };
-      const int c0 = cur.off, n = cur.n;
-      load_k(c0);
-      load_v(c0);
-      convert_k(t);
-      if (n > 1) load_k(c0 + 1);
-      for (int i = 0; i < n; ++i, ++t) {
-        if (i + 1 < n && i == 0) {
-          convert_k(t + 1);
-          if (n > 2) load_k(c0 + 2);
-        }
-        convert_v(t);
-        if (i + 1 < n) load_v(c0 + i + 1);
-        if (i + 2 < n) {
-          convert_k(t + 2);
-          if (i + 3 < n) load_k(c0 + i + 3);
         }
       }
     }
+  } else if (warp == kKtMmaWarp) {
+    // ---------------- MMA issue ----------------
+    constexpr uint32_t id_qk = kt_idesc(kKvTileKeys), id_pv = kt_idesc(kKvD);
+    bool ok = true;
+    int t = 0, units = 0;
+    auto issue_pv = [&](int w) {  // O = P V of tile w, once every warp wrote its P and has the O before
+      const int s = w & 1, vs = w % 3;
+      ok = ok && bar_wait(&sm.vfull[vs], (w / 3) & 1, abort);
+      ok = ok && bar_wait(&sm.pfull[s], (w >> 1) & 1, abort);
+      if (w > 0) ok = ok && bar_wait(&sm.ofree, (w - 1) & 1, abort);
+      if (!ok) return;
+      tc_after();
+      const uint64_t vh = desc_sw128(sm.v[vs][0]), vl = desc_sw128(sm.v[vs][1]);
+      const uint32_t ph = tmem + kTmP + 64 * s, pl = ph + 32, d = tmem + kTmO;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) mma_ts(d, pl + 8 * kk, vh + 2 * kk, id_pv, kk > 0);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) mma_ts(d, ph + 8 * kk, vl + 2 * kk, id_pv, 1);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) mma_ts(d, ph + 8 * kk, vh + 2 * kk, id_pv, 1);
+      mma_commit(&sm.vfree[vs]);
+      mma_commit(&sm.ofull);
+    };
+    KtCursor cur = start;
+    for (bool more = cur.seek<MASK>(a); ok && more; more = cur.next<MASK>(a), ++units) {
+      ok = bar_wait(&sm.qfull, units & 1, abort);
+      for (int i = 0; ok && i < cur.n; ++i, ++t) {
+        // S = Q K^T; its buffer is free: P of tile t - 2 was waited for
+        const int s = t & 1;
+        ok = bar_wait(&sm.kfull[s], (t >> 1) & 1, abort);
+        if (!ok) break;
+        if (lane == 0) bar_arrive(&sm.sfull[s]);  // passes on what the converters wrote beside the tile
+        tc_after();
+        const uint64_t kh0 = desc_sw128(sm.k[s][0][0]), kh1 = desc_sw128(sm.k[s][0][1]);
+        const uint64_t kl0 = desc_sw128(sm.k[s][1][0]), kl1 = desc_sw128(sm.k[s][1][1]);
+        const uint32_t qh = tmem + kTmQ, ql = qh + 64, d = tmem + kTmS + 64 * s;
+        __syncwarp();
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) mma_ts(d, ql + 8 * kk, (kk < 4 ? kh0 : kh1) + 2 * (kk & 3), id_qk, kk > 0);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) mma_ts(d, qh + 8 * kk, (kk < 4 ? kl0 : kl1) + 2 * (kk & 3), id_qk, 1);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) mma_ts(d, qh + 8 * kk, (kk < 4 ? kh0 : kh1) + 2 * (kk & 3), id_qk, 1);
+        mma_commit(&sm.kfree[s]);
+        mma_commit(&sm.sfull[s]);
+        if (i > 0) issue_pv(t - 1);
+      }
+      issue_pv(t - 1);
+    }
+    // nothing of this CTA's may be at work in shared memory or TMEM when it ends
+    mma_commit(&sm.done);
+    mb_wait_ns(su32(&sm.done), 0, kDrainLimitNs, nullptr);
   } else {
     // ---------------- softmax, output ----------------
     // thread (row, half): keys 32 half .. + 32 of a tile, output columns 64 half .. + 64, which are
@@ -501,52 +540,16 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
     };
     auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory"); };
     if (!a.split) {  // a unit without keys has no tiles
-      const KvUnit x = kv_unit<MASK>(a, cur.u);
+      const KvUnit x = kv_unit<MASK>(a, start.u);
       if (x.chunks == 0 && row < x.nrows && half == 0) {
         float4* dst = reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, row));
         for (int i = 0; i < kKvD / 4; ++i) dst[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (a.lse) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] = INFINITY;
       }
     }
-    // MMA issue, by warp 0
-    constexpr uint32_t id_qk = kt_idesc(kKvTileKeys), id_pv = kt_idesc(kKvD);
-    auto issue_qk = [&](int w) {  // S = Q K^T of tile w
-      const int s = w & 1;
-      wait(&sm.kfull[s], (w >> 1) & 1);
-      if (!ok) return;
-      tc_after();
-      const uint64_t kh0 = desc_sw128(sm.k[s][0][0]), kh1 = desc_sw128(sm.k[s][0][1]);
-      const uint64_t kl0 = desc_sw128(sm.k[s][1][0]), kl1 = desc_sw128(sm.k[s][1][1]);
-      const uint32_t qh = tmem + kTmQ, ql = qh + 64, d = tmem + kTmS + 64 * s;
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk) mma_ts(d, ql + 8 * kk, (kk < 4 ? kh0 : kh1) + 2 * (kk & 3), id_qk, kk > 0);
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk) mma_ts(d, qh + 8 * kk, (kk < 4 ? kl0 : kl1) + 2 * (kk & 3), id_qk, 1);
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk) mma_ts(d, qh + 8 * kk, (kk < 4 ? kh0 : kh1) + 2 * (kk & 3), id_qk, 1);
-      mma_commit(&sm.kfree[s]);
-      mma_commit(&sm.sfull[s]);
-    };
-    auto issue_pv = [&](int w) {  // O = P V of tile w, once every warp wrote its P and has the O before
-      const int s = w & 1, vs = w % 3;
-      wait(&sm.vfull[vs], (w / 3) & 1);
-      wait(&sm.pfull[s], (w >> 1) & 1);
-      if (w > 0) wait(&sm.ofree, (w - 1) & 1);
-      if (!ok) return;
-      tc_after();
-      const uint64_t vh = desc_sw128(sm.v[vs][0]), vl = desc_sw128(sm.v[vs][1]);
-      const uint32_t ph = tmem + kTmP + 64 * s, pl = ph + 32, d = tmem + kTmO;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) mma_ts(d, pl + 8 * kk, vh + 2 * kk, id_pv, kk > 0);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) mma_ts(d, ph + 8 * kk, vl + 2 * kk, id_pv, 1);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) mma_ts(d, ph + 8 * kk, vh + 2 * kk, id_pv, 1);
-      mma_commit(&sm.vfree[vs]);
-      mma_commit(&sm.ofull);
-    };
-    int units = 0;
-    for (bool more = cur.seek(a); more; more = cur.next(a), ++units) {
+    KtCursor& cur = sm.cursor[warp];
+    cur = start;
+    for (bool more = cur.seek<MASK>(a); more; more = cur.next<MASK>(a)) {
       const KvUnit& x = cur.x;
       const int c0 = cur.off, n = cur.n;
       const int token = kv_token<MASK>(a, x, min(row, x.nrows - 1));
@@ -603,11 +606,6 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         __syncwarp();
         if (lane == 0) bar_arrive(&sm.qfull);
       }
-      if (warp == 0) {
-        wait(&sm.qfull, units & 1);
-        issue_qk(t);
-        if (n > 1) issue_qk(t + 1);
-      }
       float2 o[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) o[i] = make_float2(0.f, 0.f);
@@ -661,7 +659,9 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       };
       for (int i = 0; i < n; ++i, ++t) {
         const int s = t & 1, j0 = (c0 + i) * kKvTileKeys;
-        wait(&sm.kinfo[t & 3], (t >> 2) & 1);
+        const uint32_t sat = mine + kTmS + 64 * s + 32 * half;
+        wait(&sm.sfull[s], (t >> 1) & 1);
+        tc_after();
         float cc[4];  // the factors of the thread's four groups of 8 keys
         {
           const float4 k4 = *reinterpret_cast<const float4*>(&sm.ksc[t & 3][4 * half]);
@@ -671,9 +671,6 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
           cc[2] = fmaxf(cq * k4.z, 1.17549435e-38f);
           cc[3] = fmaxf(cq * k4.w, 1.17549435e-38f);
         }
-        const uint32_t sat = mine + kTmS + 64 * s + 32 * half;
-        wait(&sm.sfull[s], (t >> 1) & 1);
-        tc_after();
         float top = -INFINITY;
         {
           uint32_t r[32];
@@ -767,10 +764,6 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         if (lane == 0) bar_arrive(&sm.pfull[s]);
         l = fmaf(l, next, sum.x + sum.y);
         if (i > 0) add_o(t - 1, c0 + i - 1, corr, vtop, bad);
-        if (warp == 0) {
-          issue_pv(t);
-          if (i + 2 < n) issue_qk(t + 2);
-        }
         corr = next;
         vtop = vt;
         bad = bad_t;
@@ -833,16 +826,11 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         }
       }
     }
-    if (warp == 0) {
-      // nothing of this CTA's may be at work in shared memory or TMEM when it ends
-      mma_commit(&sm.done);
-      mb_wait_ns(su32(&sm.done), 0, kDrainLimitNs, nullptr);
-    }
   }
   tc_before();
   __syncthreads();
   tc_after();
-  if (warp == 0)
+  if (warp == kKtMmaWarp)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kKtTmemCols) : "memory");
 }
 
