@@ -232,6 +232,11 @@ __device__ __forceinline__ void split_f16(float2 x, uint32_t& hi, uint32_t& lo) 
   const float2 l = fma2(h, make_float2(-1.0f, -1.0f), x);
   lo = pack_f16(l.x, l.y);
 }
+// The largest of a tile's inverse scales.
+__device__ __forceinline__ float tile_factor(const float* inv) {
+  const float4 a = *reinterpret_cast<const float4*>(inv), b = *reinterpret_cast<const float4*>(inv + 4);
+  return fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w)));
+}
 // Largest magnitude (bits of a float) -> the scale that brings it into [2^10, 2^14) and its
 // inverse.  Exponents in steps of 4: neighbouring groups mostly agree.
 __device__ __forceinline__ void scale_of(unsigned top, float& scale, float& inverse) {
@@ -612,11 +617,11 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       float m = -INFINITY, l = 0.0f, corr = 0.0f;
       const int open = MASK == kMaskTree ? x.p : x.p + x.i0 + 1;
       // o = o * f + the O tile of tile w (cache tile c), whose P stood against the maximum of then
-      float vtop = 0.0f;  // the tile's factor of the values, one tile back when it is used
-      unsigned long long bad = 0;
-      auto add_o = [&](int w, int c, float f, float fv, unsigned long long bad) {
+      // (the tile's scales are still in place: their next writer waits for the PV after this)
+      auto add_o = [&](int w, int c, float f) {
         wait(&sm.ofull, w & 1);
         tc_after();
+        const float fv = tile_factor(sm.vsc[w & 3]);
         const float2 f2 = make_float2(f, f), v2 = make_float2(fv, fv);
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
@@ -629,7 +634,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
                 fma2(o[part * 16 + i], f2,
                      mul2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), v2));
         }
-        if (bad) {
+        if (const unsigned long long bad = *reinterpret_cast<const unsigned long long*>(&sm.vbad[w & 3][0])) {
           const float2* vb = reinterpret_cast<const float2*>(
               a.v + (((size_t)x.b * a.hkv + x.hk) * (size_t)a.max_t + (size_t)c * kKvTileKeys) * kKvD);
           for (int key = 0; key < kKvTileKeys; ++key) {
@@ -715,10 +720,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         // (1 but for groups of another magnitude) goes to its probabilities
         wait(&sm.vinfo[t & 3], (t >> 2) & 1);
         const float4 va = *reinterpret_cast<const float4*>(&sm.vsc[t & 3][4 * half]);
-        const float4 vb = *reinterpret_cast<const float4*>(&sm.vsc[t & 3][4 * (half ^ 1)]);
-        const unsigned long long bad_t = *reinterpret_cast<const unsigned long long*>(&sm.vbad[t & 3][0]);
-        const float vt = fmaxf(fmaxf(fmaxf(va.x, va.y), fmaxf(va.z, va.w)), fmaxf(fmaxf(vb.x, vb.y), fmaxf(vb.z, vb.w)));
-        const float vi = __uint_as_float((254u << 23) - __float_as_uint(vt));  // 1 / vt, a power of two
+        const float vi = __uint_as_float((254u << 23) - __float_as_uint(tile_factor(sm.vsc[t & 3])));  // 1 / a power of 2
         const float share[4] = {va.x * vi, va.y * vi, va.z * vi, va.w * vi};
         const float b14 = kKtPScale - base;
         float2 sum = make_float2(0.f, 0.f);
@@ -740,7 +742,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
           tm_st8(mine + kTmP + 64 * s + 16 * half + 8 * part, hi);
           tm_st8(mine + kTmP + 64 * s + 32 + 16 * half + 8 * part, lo);
         }
-        if (bad_t) {
+        if (const unsigned long long bad_t = *reinterpret_cast<const unsigned long long*>(&sm.vbad[t & 3][0])) {
           // a key whose value row is left out keeps its probability as it is, for add_o
           tm_wait_st();
           for (int e = 0; e < 32; ++e) {
@@ -763,12 +765,10 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         __syncwarp();
         if (lane == 0) bar_arrive(&sm.pfull[s]);
         l = fmaf(l, next, sum.x + sum.y);
-        if (i > 0) add_o(t - 1, c0 + i - 1, corr, vtop, bad);
+        if (i > 0) add_o(t - 1, c0 + i - 1, corr);
         corr = next;
-        vtop = vt;
-        bad = bad_t;
       }
-      add_o(t - 1, c0 + n - 1, corr, vtop, bad);
+      add_o(t - 1, c0 + n - 1, corr);
       // the row's sum over both halves (the maxima's place is free: the last tile's was read
       // before its P was given away, and t moves on)
       meet();
