@@ -50,6 +50,7 @@ __shared__ uint64_t s_kt_wait_ns;
 struct KtCursor {
   int u, off, left;  // unit, its first tile here, tiles left of the CTA's share
   int n;             // tiles of the unit here
+  int t0 = 0;        // tiles of the CTA before it
   KvUnit x;
   // Moves to the first unit from u on with work; false when there is none.
   template <int MASK>
@@ -67,6 +68,7 @@ struct KtCursor {
   template <int MASK>
   __device__ bool next(const KvArgs& a) {
     left -= n;
+    t0 += n;
     off = 0;
     ++u;
     return a.split && seek<MASK>(a);
@@ -318,8 +320,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
     const int h = lane & 15, ky = lane >> 4;
     KtCursor cur = start;
     bool dead = false;
-    int t0 = 0;  // the unit's first tile in the CTA's count
-    for (bool more = cur.seek<MASK>(a); more; t0 += cur.n, more = cur.next<MASK>(a)) {
+    for (bool more = cur.seek<MASK>(a); more; more = cur.next<MASK>(a)) {
       const KvUnit& x = cur.x;
       const size_t head = ((size_t)x.b * a.hkv + x.hk) * (size_t)a.max_t;
       // lane's pieces of a row: K dimensions 4 h .. and 64 + 4 h .. of row 2 i + lane / 16, V
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         if (item + kKtConverters < items) load(item + kKtConverters);
         const int c = tile_of(item), g = item & 7;
         if (c < 0) continue;
-        const int t = t0 + c;
+        const int t = cur.t0 + c;
         float m = 0.0f, scale, inverse;
 #pragma unroll
         for (int i = 0; i < 8; ++i) m = mag(mag(mag(mag(m, r[i].x), r[i].y), r[i].z), r[i].w);
@@ -556,8 +557,6 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
     cur = start;
     for (bool more = cur.seek<MASK>(a); more; more = cur.next<MASK>(a)) {
       const KvUnit& x = cur.x;
-      const int c0 = cur.off, n = cur.n;
-      const int token = kv_token<MASK>(a, x, min(row, x.nrows - 1));
       // half of the query row: scaled hi / lo to TMEM, dimensions in the order of the K tiles (32
       // half .. + 32 and 64 + 32 half .. + 32).  A thread that reads its own row takes 32 memory
       // transactions an access (that cost 10 us a unit), so the warp reads rows and turns them.
@@ -615,10 +614,11 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
 #pragma unroll
       for (int i = 0; i < 32; ++i) o[i] = make_float2(0.f, 0.f);
       float m = -INFINITY, l = 0.0f, corr = 0.0f;
-      const int open = MASK == kMaskTree ? x.p : x.p + x.i0 + 1;
-      // o = o * f + the O tile of tile w (cache tile c), whose P stood against the maximum of then
+      // tiles from this one on hold a key that some row of the unit does not see
+      const int tend = cur.t0 + cur.n, tmask = cur.t0 - cur.off + (MASK == kMaskTree ? x.p : x.p + x.i0 + 1) / kKvTileKeys;
+      // o = o * f + the O tile of tile w, whose P stood against the maximum of then
       // (the tile's scales are still in place: their next writer waits for the PV after this)
-      auto add_o = [&](int w, int c, float f) {
+      auto add_o = [&](int w, float f) {
         wait(&sm.ofull, w & 1);
         tc_after();
         const float fv = tile_factor(sm.vsc[w & 3]);
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         }
         if (const unsigned long long bad = *reinterpret_cast<const unsigned long long*>(&sm.vbad[w & 3][0])) {
           const float2* vb = reinterpret_cast<const float2*>(
-              a.v + (((size_t)x.b * a.hkv + x.hk) * (size_t)a.max_t + (size_t)c * kKvTileKeys) * kKvD);
+              a.v + (((size_t)x.b * a.hkv + x.hk) * (size_t)a.max_t + (size_t)(cur.off + w - cur.t0) * kKvTileKeys) * kKvD);
           for (int key = 0; key < kKvTileKeys; ++key) {
             if (!((bad >> key) & 1)) continue;
             const uint32_t hi = tm_ld1(mine + kTmP + 64 * (w & 1) + (key >> 1));
@@ -662,8 +662,8 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         __syncwarp();
         if (lane == 0) bar_arrive(&sm.ofree);
       };
-      for (int i = 0; i < n; ++i, ++t) {
-        const int s = t & 1, j0 = (c0 + i) * kKvTileKeys;
+      for (; t < tend; ++t) {
+        const int s = t & 1;
         const uint32_t sat = mine + kTmS + 64 * s + 32 * half;
         wait(&sm.sfull[s], (t >> 1) & 1);
         tc_after();
@@ -681,9 +681,10 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
           uint32_t r[32];
           tm_ld32(sat, r);
           tm_wait_ld();
-          if (j0 + kKvTileKeys > open) {  // some row of the unit does not see some key
+          if (t >= tmask) {
             uint32_t see;
-            const int j = j0 + 32 * half;
+            const int j = (cur.off + t - cur.t0) * kKvTileKeys + 32 * half;
+            const int token = kv_token<MASK>(a, x, min(row, x.nrows - 1));
             if (MASK == kMaskTree) {
               const int e0 = j - x.p;  // node number of the first
               see = e0 <= -32 ? ~0u : e0 < 0 ? (1u << -e0) - 1 : 0u;
@@ -765,10 +766,10 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         __syncwarp();
         if (lane == 0) bar_arrive(&sm.pfull[s]);
         l = fmaf(l, next, sum.x + sum.y);
-        if (i > 0) add_o(t - 1, c0 + i - 1, corr);
+        if (t > cur.t0) add_o(t - 1, corr);
         corr = next;
       }
-      add_o(t - 1, c0 + n - 1, corr);
+      add_o(t - 1, corr);
       // the row's sum over both halves (the maxima's place is free: the last tile's was read
       // before its P was given away, and t moves on)
       meet();
@@ -777,7 +778,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       l = sm.top[0][0][row] + sm.top[0][1][row];
       meet();
       // the row: whole, or this CTA's part of it
-      const bool whole = c0 == 0 && n == x.chunks;
+      const bool whole = cur.off == 0 && cur.n == x.chunks;
       const size_t slot = a.split ? (size_t)blockIdx.x + cur.u : (size_t)cur.u;
       const float nan = __uint_as_float(0x7fffffffu);
       if (!kv_row_valid<MASK>(a, x, row)) m = -INFINITY;
