@@ -4,9 +4,9 @@
 // Products: f32 operands as pairs of f16 numbers under a power-of-two scale, three
 // tcgen05.mma kind::f16 per product.  x s = hi + lo with a power of two s for each query row and
 // each group of 8 keys or values, which brings the largest |x s| of them into [2^10, 2^14); hi =
-// x s cut to 11 significant bits, lo = x s - hi (exact) rounded to f16; a.b = lo.hi + hi.lo +
-// hi.hi.  An element is off by at most 2^-22 of itself or 2^-35 of its group's largest, and the
-// dropped lo.lo is 2^-20 of a product at most, 2^-22 on average.  So f32's exponent range fits.
+// x s rounded to f16, lo = x s - hi (exact) rounded to f16; a.b = lo.hi + hi.lo + hi.hi.  An
+// element is off by at most 2^-23 of itself or 2^-35 of its group's largest, and the dropped
+// lo.lo is at most 2^-22 of a product.  So f32's exponent range fits.
 // The keys' scales leave with the scores' factor.  The values' scales differ inside a sum: the
 // probabilities of a group are lowered by its scale over the tile's smallest, which leaves one
 // factor for the tile.
@@ -222,16 +222,14 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 __device__ __forceinline__ float2 lo2(const float4& v) { return make_float2(v.x, v.y); }
 __device__ __forceinline__ float2 hi2(const float4& v) { return make_float2(v.z, v.w); }
-// Cut to 11 significant bits.
-__device__ __forceinline__ float2 cut2(float2 x) {
-  return make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffffe000u),
-                     __uint_as_float(__float_as_uint(x.y) & 0xffffe000u));
+__device__ __forceinline__ float2 unpack_f16(uint32_t h) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
-// Two scaled values -> packed hi parts and packed lo parts.
+// Two scaled values -> packed hi parts and packed lo parts.  (hi is read back from f16: cutting it
+// with integer operations and then packing it loads the narrower integer pipe instead.)
 __device__ __forceinline__ void split_f16(float2 x, uint32_t& hi, uint32_t& lo) {
-  const float2 h = cut2(x);
-  hi = pack_f16(h.x, h.y);
-  const float2 l = fma2(h, make_float2(-1.0f, -1.0f), x);
+  hi = pack_f16(x.x, x.y);
+  const float2 l = fma2(unpack_f16(hi), make_float2(-1.0f, -1.0f), x);
   lo = pack_f16(l.x, l.y);
 }
 // The largest of a tile's inverse scales.
@@ -450,13 +448,9 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
             uint32_t h0[4], h1[4], l0[4], l1[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float2 b0 = cut2(w[2 * i]), b1 = cut2(w[2 * i + 1]);
-              h0[i] = pack_f16(b0.x, b1.x);
-              h1[i] = pack_f16(b0.y, b1.y);
-              const float2 r0 = fma2(b0, make_float2(-1.0f, -1.0f), w[2 * i]);
-              const float2 r1 = fma2(b1, make_float2(-1.0f, -1.0f), w[2 * i + 1]);
-              l0[i] = pack_f16(r0.x, r1.x);
-              l1[i] = pack_f16(r0.y, r1.y);
+              const float2 u = w[2 * i], v = w[2 * i + 1];
+              split_f16(make_float2(u.x, v.x), h0[i], l0[i]);
+              split_f16(make_float2(u.y, v.y), h1[i], l1[i]);
             }
             constexpr int low = sizeof(sm.v[0][0]);
             *reinterpret_cast<uint4*>(dst + e * 4096) = make_uint4(h0[0], h0[1], h0[2], h0[3]);
