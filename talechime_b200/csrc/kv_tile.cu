@@ -846,6 +846,7 @@ struct KcSmem {
   alignas(16) float qsc[4][8];                      // inverse scales of the groups of 8 rows
   alignas(16) float lse[4][kKcRows];
   alignas(16) int last[4][kKcRows];                 // the last key a row sees
+  alignas(16) float turn[4][32 * 20];               // rows of a warp's keys: memory <-> a thread per key
   alignas(8) uint64_t qfull[2], qfree[2], info[4], sfull[2], sfree[2], kfull, done;
   uint32_t tmem;
   int abort;
@@ -978,22 +979,32 @@ kv_column_tile_kernel(const KvArgs a, float* weight, float* __restrict__ part, u
     const int j = j0 + tid;
     float kinv = 0.0f;
     if (n > 0) {
-      const float4* kr = reinterpret_cast<const float4*>(a.k + (bh * a.max_t + min(j, keys - 1)) * kKvD);
-      float m = 0.0f;
+      // the warp reads its 32 rows and turns them (see the tile kernel's query rows)
+      const float4* kr = reinterpret_cast<const float4*>(a.k + bh * a.max_t * kKvD);
+      const int row0 = j0 + warp * 32;
+      unsigned m = 0;
 #pragma unroll 8
       for (int i = 0; i < 32; ++i) {
-        const float4 v = kr[i];
-        m = mag(mag(mag(mag(m, v.x), v.y), v.z), v.w);
+        const float4 v = kr[(size_t)min(row0 + i, keys - 1) * 32 + lane];
+        const unsigned top = __reduce_max_sync(kFull, __float_as_uint(mag(mag(mag(mag(0.0f, v.x), v.y), v.z), v.w)));
+        if (i == lane) m = top;
       }
       float scale;
-      scale_of(min(__float_as_uint(m), 0x7f7fffffu), scale, kinv);
+      scale_of(min(m, 0x7f7fffffu), scale, kinv);
       const float2 sc = make_float2(scale, scale);
+      float4* turn = reinterpret_cast<float4*>(&sm.turn[warp][0]);
 #pragma unroll
-      for (int part = 0; part < 8; ++part) {
+      for (int part = 0; part < 8; ++part) {  // dimensions 8 part .. + 8 and 64 + 8 part .. + 8
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 8 * i + (lane >> 2), c = lane & 3;
+          turn[r * 5 + c] = kr[(size_t)min(row0 + r, keys - 1) * 32 + (c >> 1) * 16 + part * 2 + (c & 1)];
+        }
+        __syncwarp();
         uint32_t hi[8], lo[8];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float4 v = kr[part * 2 + i], w = kr[16 + part * 2 + i];
+          const float4 v = turn[lane * 5 + i], w = turn[lane * 5 + 2 + i];
           split_f16(mul2(lo2(v), sc), hi[4 * i], lo[4 * i]);
           split_f16(mul2(hi2(v), sc), hi[4 * i + 1], lo[4 * i + 1]);
           split_f16(mul2(lo2(w), sc), hi[4 * i + 2], lo[4 * i + 2]);
@@ -1001,6 +1012,7 @@ kv_column_tile_kernel(const KvArgs a, float* weight, float* __restrict__ part, u
         }
         tm_st8(mine + 8 * part, hi);
         tm_st8(mine + 64 + 8 * part, lo);
+        __syncwarp();
       }
       tm_wait_st();
       tc_before();
@@ -1075,10 +1087,14 @@ kv_column_add_kernel(const float* __restrict__ part, const int* __restrict__ pos
   weight[(size_t)bh * max_t + j] += s;
 }
 
-int column_splits(int n, int group) {
-  // about 8 row tiles a CTA: its start, a key tile to TMEM, costs as much as two
+// Row splits of the column sums: about 444 CTAs (three for each of two places on an SM) over the
+// keys of the new rows alone, 8 row tiles a CTA at least (its start costs as much as some tiles).
+int column_splits(int batch, int n, int hkv, int group) {
   const int64_t tiles = ((int64_t)n * group + kKcRows - 1) / kKcRows;
-  return (int)(tiles < 16 ? 1 : tiles / 8 > 16 ? 16 : tiles / 8);
+  const int64_t places = (int64_t)batch * hkv * ((n + kKcKeys - 1) / kKcKeys);
+  const int64_t want = (444 + places - 1) / places;
+  const int64_t most = tiles / 8 > 64 ? 64 : tiles / 8;
+  return (int)(want < most ? want : most < 1 ? 1 : most);
 }
 
 template <int MASK>
@@ -1107,7 +1123,7 @@ cudaError_t launch_kv_tile(const KvArgs& a, int mask, int device, cudaStream_t s
 }
 
 size_t kv_column_tile_bytes(int batch, int n, int hq, int hkv, int max_t) {
-  const int splits = column_splits(n, hq / hkv);
+  const int splits = column_splits(batch, n, hkv, hq / hkv);
   return splits > 1 ? (size_t)splits * batch * hkv * max_t * 4 : 0;
 }
 
@@ -1116,7 +1132,7 @@ cudaError_t launch_kv_column_tile(const KvArgs& a, float* weight, float* part, i
   const size_t smem = sizeof(KcSmem) + 1024;
   cudaError_t e = ensure_smem((const void*)kv_column_tile_kernel, configured, device, smem, true);
   if (e != cudaSuccess) return e;
-  const int splits = column_splits(a.n, a.group);
+  const int splits = column_splits(a.batch, a.n, a.hkv, a.group);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((a.max_t + kKcKeys - 1) / kKcKeys), (unsigned)(a.batch * a.hkv), (unsigned)splits);
   cfg.blockDim = dim3(kKcThreads);
