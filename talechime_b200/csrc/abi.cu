@@ -760,6 +760,8 @@ int kv_shape_fail(const char* what, int64_t batch, int64_t rows, int64_t hq, int
   if (batch <= 0 || rows < 0 || max_t <= 0 || batch * hkv > 65535 || rows > (1 << 20) ||
       batch * rows * hq > (INT64_C(1) << 30) || max_t > (1 << 24))
     return fail(Q8LIN_ERR_SHAPE, std::string(what) + ": batch, rows or max_t out of range");
+  if (batch * hkv * ((rows * (hq / hkv) + 127) / 128) * ((max_t + 63) / 64) > (INT64_C(1) << 30))
+    return fail(Q8LIN_ERR_SHAPE, std::string(what) + ": too much work for one call");
   if (rows > max_t) return fail(Q8LIN_ERR_SHAPE, std::string(what) + ": more rows than the cache holds (context limit)");
   return Q8LIN_OK;
 }

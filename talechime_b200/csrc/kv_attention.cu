@@ -632,7 +632,7 @@ KvPlan kv_plan(int64_t lists, int64_t rows_per_list, bool tile) {
   p.units = lists * p.rgs;
   // with two units per SM and more the units themselves fill the GPU
   p.split = p.units < 2 * kKvGrid;
-  p.slots = p.split ? (size_t)(kKvGrid + p.units) : (size_t)p.units;
+  p.slots = !p.split ? (size_t)p.units : p.rows == kKvTileRows ? (size_t)(2 * kKvGrid) : (size_t)(kKvGrid + p.units);
   return p;
 }
 size_t core_bytes(const KvPlan& p, bool stat) {
@@ -673,7 +673,7 @@ template <int MASK, bool SCORES>
 cudaError_t launch_core(const KvArgs& a, float* weight, int device, cudaStream_t s) {
   cudaError_t e;
   if (!SCORES && MASK != kMaskBlocks && a.rows == kKvTileRows)
-    e = launch_kv_tile(a, MASK, device, s);
+    return launch_kv_tile(a, MASK, device, s);
   else
     e = a.rows == 8 ? launch_core_nt<MASK, SCORES, 1>(a, device, s) : launch_core_nt<MASK, SCORES, 2>(a, device, s);
   if (e != cudaSuccess || (!a.split && !SCORES)) return e;

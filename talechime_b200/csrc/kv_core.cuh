@@ -39,7 +39,7 @@ struct KvArgs {
   int least;              // chunks a CTA takes at least
   int rgs;                // row groups of a kv head (tree, causal) or of a token (blocks)
   int units;
-  int split;              // 1: kKvGrid CTAs share all chunks evenly; 0: one CTA per unit
+  int split;              // 1: kKvGrid CTAs share all chunks evenly; 0: whole units
   float c;                // log2(e) * f32(1/sqrt(128))
 };
 

@@ -46,32 +46,38 @@ constexpr int kKtPScale = 14;     // P' = 2^14 p
 __device__ unsigned int g_kv_tile_fault;
 __shared__ uint64_t s_kt_wait_ns;
 
-// The units of this CTA and their tiles, in order.
+// The units of this CTA and their tiles, in order.  With few units all CTAs share all tiles evenly
+// (split); with many, CTA c takes whole units c, c + 148, ..., the ones with the latest rows, which
+// see most, first.
 struct KtCursor {
-  int u, off, left;  // unit, its first tile here, tiles left of the CTA's share
+  int u, off, left;  // split: unit, its first tile here, tiles left of the CTA's share; else: u-th in the order
   int n;             // tiles of the unit here
   int t0 = 0;        // tiles of the CTA before it
   KvUnit x;
+  template <int MASK>
+  __device__ static KvUnit in_order(const KvArgs& a, int k) {
+    const int lists = a.units / a.rgs;
+    return kv_unit<MASK>(a, k % lists * a.rgs + a.rgs - 1 - k / lists);
+  }
   // Moves to the first unit from u on with work; false when there is none.
   template <int MASK>
   __device__ bool seek(const KvArgs& a) {
     while (u < a.units && left > 0) {
-      x = kv_unit<MASK>(a, u);
+      x = a.split ? kv_unit<MASK>(a, u) : in_order<MASK>(a, u);
       n = min(x.chunks - off, left);
       if (n > 0) return true;
       off = 0;
-      ++u;
-      if (!a.split) break;
+      u += a.split ? 1 : kKvGrid;
     }
     return false;
   }
   template <int MASK>
   __device__ bool next(const KvArgs& a) {
-    left -= n;
+    if (a.split) left -= n;
     t0 += n;
     off = 0;
-    ++u;
-    return a.split && seek<MASK>(a);
+    u += a.split ? 1 : kKvGrid;
+    return seek<MASK>(a);
   }
 };
 
@@ -302,9 +308,9 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
     start.u = sm.find.unit;
     start.off = sm.find.off;
   } else {
-    start.u = a.units - 1 - (int)blockIdx.x;  // later rows see more keys: longest first
+    start.left = 0x7fffffff;
+    start.u = blockIdx.x;
     start.off = 0;
-    start.left = 0x3fffffff;
   }
   tc_before();
   __syncthreads();
@@ -539,14 +545,14 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       if (ok) ok = bar_wait(bar, parity, abort);
     };
     auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory"); };
-    if (!a.split) {  // a unit without keys has no tiles
-      const KvUnit x = kv_unit<MASK>(a, start.u);
-      if (x.chunks == 0 && row < x.nrows && half == 0) {
+    if (!a.split)  // units without keys have no tiles
+      for (int u = blockIdx.x; u < a.units; u += kKvGrid) {
+        const KvUnit x = KtCursor::in_order<MASK>(a, u);
+        if (x.chunks > 0 || row >= x.nrows || half > 0) continue;
         float4* dst = reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, row));
         for (int i = 0; i < kKvD / 4; ++i) dst[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (a.lse) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] = INFINITY;
       }
-    }
     KtCursor& cur = sm.cursor[warp];
     cur = start;
     for (bool more = cur.seek<MASK>(a); more; more = cur.next<MASK>(a)) {
@@ -773,7 +779,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       meet();
       // the row: whole, or this CTA's part of it
       const bool whole = cur.off == 0 && cur.n == x.chunks;
-      const size_t slot = a.split ? (size_t)blockIdx.x + cur.u : (size_t)cur.u;
+      const size_t slot = 2 * (size_t)blockIdx.x + (cur.off > 0 ? 0 : 1);
       const float nan = __uint_as_float(0x7fffffffu);
       if (!kv_row_valid<MASK>(a, x, row)) m = -INFINITY;
       constexpr float kUnscale = 1.0f / (1 << kKtPScale);  // P' = 2^14 p is in both sums
@@ -811,7 +817,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       }
       if (row < x.nrows) {
         if (half == 0) {
-          if (a.stat) {
+          if (!whole) {
             a.stat[slot * 2 * a.rows + row] = m;
             a.stat[(slot * 2 + 1) * a.rows + row] = ok ? l * kUnscale : nan;
           }
@@ -827,6 +833,52 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
   tc_after();
   if (warp == kKtMmaWarp)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kKtTmemCols) : "memory");
+}
+
+// After a split: the parts of the units that more than one CTA worked on, in the order of the CTAs, and
+// zeros for units without keys.  A CTA has at most two parts: the rest of a unit that began before it (slot
+// 2 cta) and the beginning of one that ends after it (slot 2 cta + 1).  Block (c, y) merges rows 8 y
+// .. + 8 of the unit that CTA c began and did not end.
+constexpr int kKtMergeRows = 8;
+template <int MASK>
+__global__ void __launch_bounds__(kKtMergeRows * 32) kv_tile_merge_kernel(const KvArgs a) {
+  __shared__ KvFind find;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y * kKtMergeRows + warp;
+  pdl_launch_dependents();
+  pdl_wait();
+  for (int u = blockIdx.x; u < a.units; u += kKvGrid) {
+    const KvUnit x = kv_unit<MASK>(a, u);
+    if (x.chunks > 0 || r >= x.nrows) continue;
+    reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, r))[lane] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (a.lse && lane == 0) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + r] = INFINITY;
+  }
+  const int quota = kv_find<MASK, kKtMergeRows * 32>(a, find, blockIdx.x + 1);
+  const int u = find.unit, off = find.off;
+  if (u >= a.units || off == 0 || off > quota) return;  // nothing of CTA c's goes on in the next
+  const KvUnit x = kv_unit<MASK>(a, u);
+  if (r >= x.nrows) return;
+  const int parts = 1 + (x.chunks - off + quota - 1) / quota;
+  auto slot = [&](int s) { return 2 * ((size_t)blockIdx.x + s) + (s == 0 ? 1 : 0); };
+  float M = -INFINITY, L = 0.0f;
+  for (int s = lane; s < parts; s += 32) M = fmaxf(M, a.stat[slot(s) * 2 * a.rows + r]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, o));
+  float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (M != -INFINITY) {
+#pragma unroll 4
+    for (int s = 0; s < parts; ++s) {
+      const float f = exp2f(a.stat[slot(s) * 2 * a.rows + r] - M), l = a.stat[(slot(s) * 2 + 1) * a.rows + r];
+      const float4 v = reinterpret_cast<const float4*>(a.acc + (slot(s) * a.rows + r) * kKvD)[lane];
+      if (f != 0.0f) {  // an empty part's sums are 0, and stay out
+        L = fmaf(l, f, L);
+        A = make_float4(fmaf(v.x, f, A.x), fmaf(v.y, f, A.y), fmaf(v.z, f, A.z), fmaf(v.w, f, A.w));
+      }
+    }
+    A = make_float4(__fdiv_rn(A.x, L), __fdiv_rn(A.y, L), __fdiv_rn(A.z, L), __fdiv_rn(A.w, L));
+  }
+  reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, r))[lane] = A;
+  if (a.lse && lane == 0)
+    a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + r] = M == -INFINITY ? INFINITY : M + log2f(L);
 }
 
 // ---------------------------------------------------------------------------------
@@ -1104,7 +1156,7 @@ cudaError_t launch_tile(const KvArgs& a, int device, cudaStream_t s) {
   cudaError_t e = ensure_smem((const void*)kv_tile_kernel<MASK>, configured, device, smem, false);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.split ? kKvGrid : a.units));
+  cfg.gridDim = dim3(kKvGrid);
   cfg.blockDim = dim3(kKtThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -1113,7 +1165,13 @@ cudaError_t launch_tile(const KvArgs& a, int device, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kv_tile_kernel<MASK>, a, wait_limit_ns());
+  e = cudaLaunchKernelEx(&cfg, kv_tile_kernel<MASK>, a, wait_limit_ns());
+  if (e != cudaSuccess || !a.split) return e;
+  const int rows = a.units > a.batch * a.hkv ? kKvTileRows : a.n * a.group;  // of the largest unit
+  cfg.gridDim = dim3(kKvGrid, (unsigned)((rows + kKtMergeRows - 1) / kKtMergeRows));
+  cfg.blockDim = dim3(kKtMergeRows * 32);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, kv_tile_merge_kernel<MASK>, a);
 }
 
 }  // namespace
