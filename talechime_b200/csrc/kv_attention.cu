@@ -11,9 +11,9 @@
 // numbered r = i * group + head-in-group and taken 8 or 16 at a time (a unit).
 //
 // Products: f32 operands as tf32 pairs on the tensor cores (mma.sync m16n8k8).  x = hi + lo
-// with hi = x rounded to tf32's 11 significant bits and lo = x - hi (exact) rounded again, and
-// a.b = hi.hi + lo.hi + hi.lo: what is dropped (lo.lo and lo's rounding) is below 3 * 2^-24 of
-// each product, about f32's own rounding; f32's exponent range stays.
+// with hi = x rounded to tf32's 11 significant bits and lo = x - hi (exact) cut to them, and
+// a.b = hi.hi + lo.hi + hi.lo: what is dropped (lo.lo and lo's cut) is below 9 * 2^-24 of each
+// product, on average f32's own rounding; f32's exponent range stays.
 #include <cmath>
 
 #include "common.cuh"
@@ -31,9 +31,12 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t a0, const
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The tensor cores read the upper 19 bits of a tf32 operand: lo goes in as it is and is cut there.
+// (Integer rounding of hi, one operation each: cvt.rna.tf32 took the 16-row kernel from 70 to 79 us
+// at 16 K rows x 16 heads, cutting lo here too cost 8 % of it.)
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
   hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
-  lo = (__float_as_uint(__fsub_rn(x, __uint_as_float(hi))) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(__fsub_rn(x, __uint_as_float(hi)));
 }
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool there) {
   const uint32_t n = there ? 16u : 0u;
@@ -418,7 +421,7 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArg
 // weight[j] += sum over the rows of 2^(s_j - log2 sum).  grid (units, rows + key ranges): CTA
 // (u, r) merges row r, CTA (u, rows + k) adds the weights of range k.
 constexpr int kKvMergeThreads = 128;
-constexpr int kKvWeightKeys = 512;
+constexpr int kKvWeightKeys = kKvMergeThreads;  // one key a thread
 template <int MASK, bool SCORES>
 __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs a, float* __restrict__ weight) {
   __shared__ int red[kKvMergeThreads / 32][2];
@@ -498,6 +501,16 @@ __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs 
     return;
   }
   if (SCORES) {
+    // the key's scores are on their way while the rows' sums are put together
+    const size_t bh = (size_t)x.b * a.hkv + x.hk;
+    const int key = key0 + tid;
+    float sc[kKvMaxRows], old = 0.0f;
+    if (key < x.keys) {
+      old = weight[bh * a.max_t + key];
+#pragma unroll
+      for (int r = 0; r < kKvMaxRows; ++r)
+        if (r < x.nrows) sc[r] = a.scores[(bh * x.nrows + r) * a.score_stride + key];
+    }
     for (int r = warp; r < x.nrows; r += kKvMergeThreads / 32) {  // a warp per row
       float M = -INFINITY, L = 0.0f;
       for (int s = lane; s < parts; s += 32) M = fmaxf(M, stat[s * 2 * a.rows + r]);
@@ -511,17 +524,12 @@ __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs 
       if (lane == 0) lse[r] = M == -INFINITY ? INFINITY : M + log2f(L);
     }
     __syncthreads();
-    const size_t bh = (size_t)x.b * a.hkv + x.hk;
-    const int j1 = min(x.keys, key0 + kKvWeightKeys);
-    for (int j = key0 + tid; j < j1; j += kKvMergeThreads) {
-      float w = 0.0f;
-#pragma unroll 4
-      for (int r = 0; r < x.nrows; ++r) {
-        const float s = a.scores[(bh * x.nrows + r) * a.score_stride + j];
-        if (lse[r] != INFINITY) w += exp2f(s - lse[r]);
-      }
-      weight[bh * a.max_t + j] += w;
-    }
+    if (key >= x.keys) return;
+    float w = 0.0f;
+#pragma unroll
+    for (int r = 0; r < kKvMaxRows; ++r)
+      if (r < x.nrows && lse[r] != INFINITY) w += exp2f(sc[r] - lse[r]);
+    weight[bh * a.max_t + key] = old + w;
   }
 }
 
