@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArg
 // weight[j] += sum over the rows of 2^(s_j - log2 sum).  grid (units, rows + key ranges): CTA
 // (u, r) merges row r, CTA (u, rows + k) adds the weights of range k.
 constexpr int kKvMergeThreads = 128;
-constexpr int kKvWeightKeys = kKvMergeThreads;  // one key a thread
+constexpr int kKvWeightKeys = kKvMergeThreads;  // one key a thread at a time
 template <int MASK, bool SCORES>
 __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs a, float* __restrict__ weight) {
   __shared__ int red[kKvMergeThreads / 32][2];
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs 
     }
     return;
   }
-  const int key0 = ((int)blockIdx.y - a.rows) * kKvWeightKeys;
+  const int key0 = ((int)blockIdx.y - a.rows) * kKvWeightKeys * a.weight_reps;
   if (!merging && key0 >= x.keys) return;
   size_t slot0 = u;
   int parts = 1;
@@ -501,16 +501,17 @@ __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs 
     return;
   }
   if (SCORES) {
-    // the key's scores are on their way while the rows' sums are put together
+    // the first keys' scores are on their way while the rows' sums are put together
     const size_t bh = (size_t)x.b * a.hkv + x.hk;
-    const int key = key0 + tid;
     float sc[kKvMaxRows], old = 0.0f;
-    if (key < x.keys) {
+    auto load = [&](int key) {
+      if (key >= x.keys) return;
       old = weight[bh * a.max_t + key];
 #pragma unroll
       for (int r = 0; r < kKvMaxRows; ++r)
         if (r < x.nrows) sc[r] = a.scores[(bh * x.nrows + r) * a.score_stride + key];
-    }
+    };
+    load(key0 + tid);
     for (int r = warp; r < x.nrows; r += kKvMergeThreads / 32) {  // a warp per row
       float M = -INFINITY, L = 0.0f;
       for (int s = lane; s < parts; s += 32) M = fmaxf(M, stat[s * 2 * a.rows + r]);
@@ -524,12 +525,16 @@ __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs 
       if (lane == 0) lse[r] = M == -INFINITY ? INFINITY : M + log2f(L);
     }
     __syncthreads();
-    if (key >= x.keys) return;
-    float w = 0.0f;
+    for (int rep = 0; rep < a.weight_reps; ++rep) {
+      const int key = key0 + rep * kKvWeightKeys + tid;
+      if (key >= x.keys) return;
+      if (rep > 0) load(key);
+      float w = 0.0f;
 #pragma unroll
-    for (int r = 0; r < kKvMaxRows; ++r)
-      if (r < x.nrows && lse[r] != INFINITY) w += exp2f(sc[r] - lse[r]);
-    weight[bh * a.max_t + key] = old + w;
+      for (int r = 0; r < kKvMaxRows; ++r)
+        if (r < x.nrows && lse[r] != INFINITY) w += exp2f(sc[r] - lse[r]);
+      weight[bh * a.max_t + key] = old + w;
+    }
   }
 }
 
@@ -685,7 +690,8 @@ cudaError_t launch_core(const KvArgs& a, float* weight, int device, cudaStream_t
   else
     e = a.rows == 8 ? launch_core_nt<MASK, SCORES, 1>(a, device, s) : launch_core_nt<MASK, SCORES, 2>(a, device, s);
   if (e != cudaSuccess || (!a.split && !SCORES)) return e;
-  const unsigned ranges = SCORES ? (unsigned)((a.max_t + kKvWeightKeys - 1) / kKvWeightKeys) : 0u;
+  const unsigned ranges =
+      SCORES ? (unsigned)((a.max_t + kKvWeightKeys * a.weight_reps - 1) / (kKvWeightKeys * a.weight_reps)) : 0u;
   cudaLaunchAttribute attr[1];
   cudaLaunchConfig_t cfg = kv_cfg(dim3((unsigned)a.units, (unsigned)a.rows + ranges), dim3(kKvMergeThreads), 0, s, attr);
   return cudaLaunchKernelEx(&cfg, kv_merge_kernel<MASK, SCORES>, a, weight);
@@ -759,6 +765,9 @@ cudaError_t launch_attention_weights(const float* q, const float* kc, const floa
   if (stored) {
     a.scores = reinterpret_cast<float*>(w);
     a.score_stride = score_stride(max_t);
+    // about eight CTAs an SM: each starts with a look at all units
+    const int64_t groups = (int64_t)a.units * ((max_t + kKvWeightKeys - 1) / kKvWeightKeys);
+    a.weight_reps = (int)(groups / 1184 < 1 ? 1 : groups / 1184 > 16 ? 16 : groups / 1184);
     return launch_core<kMaskCausal, true>(a, weight, device, s);
   }
   a.lse = reinterpret_cast<float*>(w);

@@ -28,8 +28,12 @@ __device__ __forceinline__ unsigned long long order_key(double x) {
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
 
+// Counts are kept eightfold, by lane: exponents crowd into few bins, and lanes of a warp that meet
+// in one take turns.
+constexpr int kHistCopies = 8, kHistStride = 257;
 struct SelectSmem {
-  unsigned hist[256];
+  unsigned hist[kHistCopies * kHistStride];
+  unsigned count[256];
   unsigned digit, above, bin;
   unsigned warp[32][2];
 };
@@ -43,18 +47,26 @@ __device__ void select_threshold(F key, int n, int k, SelectSmem& sm, U& prefix,
   mask = 0;
   int need = k;
   for (int shift = (int)sizeof(U) * 8 - 8; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += blockDim.x) sm.hist[i] = 0;
+    for (int i = tid; i < kHistCopies * kHistStride; i += blockDim.x) sm.hist[i] = 0;
     __syncthreads();
+    unsigned* mine = sm.hist + (tid & (kHistCopies - 1)) * kHistStride;
     for (int i = tid; i < n; i += blockDim.x) {
       const U v = key(i);
-      if ((v & mask) == prefix) atomicAdd(&sm.hist[(unsigned)(v >> shift) & 255u], 1u);
+      if ((v & mask) == prefix) atomicAdd(&mine[(unsigned)(v >> shift) & 255u], 1u);
+    }
+    __syncthreads();
+    if (tid < 256) {
+      unsigned c = 0;
+#pragma unroll
+      for (int h = 0; h < kHistCopies; ++h) c += sm.hist[h * kHistStride + tid];
+      sm.count[tid] = c;
     }
     __syncthreads();
     if (tid < 32) {  // lane l: digits 255 - 8l down to 248 - 8l
       unsigned c[8], sum = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        c[e] = sm.hist[255 - 8 * tid - e];
+        c[e] = sm.count[255 - 8 * tid - e];
         sum += c[e];
       }
       unsigned upto = sum;
@@ -184,7 +196,7 @@ kv_evict_kernel(const float* weight, const int* __restrict__ length, int hkv, in
 // `lanes` 16-byte pieces of the rows of one head of one cache, so no two CTAs meet.
 constexpr int kMoveThreads = 256;
 constexpr int kMoveDepth = 8;
-__global__ void __launch_bounds__(kMoveThreads)
+__global__ void __launch_bounds__(kMoveThreads, 4)
 kv_move_kernel(float* __restrict__ kc, float* __restrict__ vc, const int* __restrict__ index,
                const int* __restrict__ base_dev, int hkv, int index_heads, int max_t, int count, int lanes) {
   pdl_launch_dependents();
@@ -235,60 +247,169 @@ kv_block_keys_kernel(const float* __restrict__ kc, const int* __restrict__ pos_d
   keys[((size_t)bh * blocks + c) * kKvD + threadIdx.x] = (float)(s / block);
 }
 
-// The blocks a query row attends over besides its own: one CTA per (sequence, token, kv
-// head).  Score of block c: sum over the heads of the group and the dimensions of q times
-// the block's mean key, in f64, so the choice does not hang on the order of the sums.
+// The blocks a query row attends over besides its own.  Score of block c: sum over the heads of
+// the group and the dimensions of q times the block's mean key, in f64, so the choice does not
+// hang on the order of the sums.
+//
+// A block of 8 lanes takes 16 dimensions each of a block's key for the ROWS tokens of the CTA at
+// once (the keys are what is read most), two keys in flight.  ROWS = 1 splits a row's blocks over a
+// cluster of CTAs where rows alone leave SMs idle: each writes its order keys into the first
+// CTA's shared memory, which chooses.
 constexpr int kPickThreads = 256;
+constexpr int kPickRows = 8;
+template <int ROWS>
 __global__ void __launch_bounds__(kPickThreads)
 kv_pick_kernel(const float* __restrict__ q, const float* __restrict__ keys, const int* __restrict__ pos_dev, int n, int hq,
                int hkv, int max_t, int block, int blocks, int topk, int* __restrict__ index) {
-  extern __shared__ unsigned long long pk_keys[];
+  extern __shared__ unsigned long long pk_keys[];  // [ROWS][blocks]
   __shared__ SelectSmem sm;
-  __shared__ double qs[kKvD];
+  __shared__ alignas(16) double qs[ROWS][kKvD];
   const int tid = threadIdx.x;
   pdl_launch_dependents();
+  uint32_t rank = 0, ranks = 1;
+  if (ROWS == 1) {
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+    // every CTA of the cluster runs before another writes into its shared memory
+    if (ranks > 1)
+      asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
   pdl_wait();
-  const int hk = blockIdx.x % hkv, row = blockIdx.x / hkv, b = row / n, i = row - b * n;
+  // a list: ROWS tokens of one sequence and kv head
+  const int groups = (n + ROWS - 1) / ROWS;
+  const int list = blockIdx.x / ranks, hk = list % hkv, bg = list / hkv, b = bg / groups, i0 = (bg - b * groups) * ROWS;
   const int group = hq / hkv, p = pos_dev[b];
-  int* idx = index + (size_t)blockIdx.x * topk;
-  const int past = p >= 0 && p < max_t - i ? min((p + i) / block, blocks) : 0;
-  if (past <= topk) {
-    for (int e = tid; e < topk; e += kPickThreads) idx[e] = e < past ? e : -1;
-    return;
-  }
-  if (tid < kKvD) {
-    double s = 0.0;
-    for (int h = 0; h < group; ++h) s += (double)q[((size_t)row * hq + hk * group + h) * kKvD + tid];
-    qs[tid] = s;
-  }
-  __syncthreads();
-  const float4* kb = reinterpret_cast<const float4*>(keys + ((size_t)b * hkv + hk) * blocks * kKvD);
-  const int l8 = tid & 7;
-  for (int c0 = 0; c0 < past; c0 += kPickThreads / 8) {
-    const int c = c0 + (tid >> 3);
-    double s = 0.0;
-    if (c < past) {
+  auto row_past = [&](int i) { return i < n && p >= 0 && p < max_t - i ? min((p + i) / block, blocks) : 0; };
+  auto row_index = [&](int i) { return index + (((size_t)b * n + i) * hkv + hk) * topk; };
+  int past = 0;  // blocks some row of the list has before its own: the last row's
+  for (int r = 0; r < ROWS; ++r) past = max(past, row_past(i0 + r));
+  if (past > topk) {
+    for (int e = tid; e < ROWS * kKvD; e += kPickThreads) {
+      const int r = e / kKvD, d = e % kKvD;
+      double s = 0.0;
+      if (i0 + r < n) {
+        const float* row = q + (((size_t)b * n + i0 + r) * hq + hk * group) * kKvD + d;
+#pragma unroll 8
+        for (int h = 0; h < group; ++h) s += (double)row[(size_t)h * kKvD];
+      }
+      qs[r][d] = s;
+    }
+    __syncthreads();
+    const float4* kb = reinterpret_cast<const float4*>(keys + ((size_t)b * hkv + hk) * blocks * kKvD);
+    const int l8 = tid & 7;
+    uint32_t first = (uint32_t)__cvta_generic_to_shared(pk_keys);
+    if (ROWS == 1 && ranks > 1) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(first) : "r"(first));
+    constexpr int kStep = kPickThreads / 8;
+    for (int c0 = (int)rank * kStep + (tid >> 3); c0 - (tid >> 3) < past; c0 += 2 * kStep * (int)ranks) {
+      float4 k4[2][4];
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const float4 k4 = kb[(size_t)c * 32 + m * 8 + l8];
-        const double* qd = qs + (m * 8 + l8) * 4;
-        s = fma(qd[0], (double)k4.x, s);
-        s = fma(qd[1], (double)k4.y, s);
-        s = fma(qd[2], (double)k4.z, s);
-        s = fma(qd[3], (double)k4.w, s);
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const int c = c0 + u * kStep * (int)ranks;
+          k4[u][m] = c < past ? kb[(size_t)c * 32 + m * 8 + l8] : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      double s[2][ROWS];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        s[0][r] = s[1][r] = 0.0;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const double2* qd = reinterpret_cast<const double2*>(&qs[r][(m * 8 + l8) * 4]);
+          const double2 qa = qd[0], qb = qd[1];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            s[u][r] = fma(qa.x, (double)k4[u][m].x, s[u][r]);
+            s[u][r] = fma(qa.y, (double)k4[u][m].y, s[u][r]);
+            s[u][r] = fma(qb.x, (double)k4[u][m].z, s[u][r]);
+            s[u][r] = fma(qb.y, (double)k4[u][m].w, s[u][r]);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int c = c0 + u * kStep * (int)ranks;
+        if (ROWS == 1) {
+          double v = s[u][0];
+          v += __shfl_xor_sync(kFull, v, 1);
+          v += __shfl_xor_sync(kFull, v, 2);
+          v += __shfl_xor_sync(kFull, v, 4);
+          if (c < past && l8 == 0)
+            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(first + 8u * (uint32_t)c), "l"(order_key(v)) : "memory");
+        } else {
+          // eight sums over eight lanes, each lane left with one row's: 7 shuffles for 24
+          double v[ROWS];
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) v[r] = s[u][r];
+#pragma unroll
+          for (int o = ROWS / 2; o > 0; o >>= 1) {
+            const bool up = (l8 & o) != 0;
+#pragma unroll
+            for (int r = 0; r < o; ++r) {
+              const double send = up ? v[r] : v[r + o], keep = up ? v[r + o] : v[r];
+              v[r] = keep + __shfl_xor_sync(kFull, send, o);
+            }
+          }
+          if (c < past) pk_keys[l8 * blocks + c] = order_key(v[0]);
+        }
       }
     }
-    s += __shfl_xor_sync(kFull, s, 1);
-    s += __shfl_xor_sync(kFull, s, 2);
-    s += __shfl_xor_sync(kFull, s, 4);
-    if (c < past && l8 == 0) pk_keys[c] = order_key(s);
   }
-  __syncthreads();
-  auto key = [&](int c) { return pk_keys[c]; };
-  unsigned long long prefix, mask;
-  int ties;
-  select_threshold<unsigned long long>(key, past, topk, sm, prefix, mask, ties);
-  select_emit<unsigned long long>(key, past, prefix, mask, ties, sm, [&](int rank, int c) { idx[rank] = c; });
+  if (ROWS == 1 && ranks > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank > 0) return;
+  } else {
+    __syncthreads();
+  }
+  if (ROWS == 1) {
+    if (i0 >= n) return;
+    int* idx = row_index(i0);
+    if (past <= topk) {
+      for (int e = tid; e < topk; e += kPickThreads) idx[e] = e < past ? e : -1;
+      return;
+    }
+    auto key = [&](int c) { return pk_keys[c]; };
+    unsigned long long prefix, mask;
+    int ties;
+    select_threshold<unsigned long long>(key, past, topk, sm, prefix, mask, ties);
+    select_emit<unsigned long long>(key, past, prefix, mask, ties, sm, [&](int rk, int c) { idx[rk] = c; });
+    return;
+  }
+  // a warp per row: the topk-th largest order key bit by bit from the top, then one ordered pass
+  static_assert(ROWS == 1 || ROWS == kPickThreads / 32, "a warp per row");
+  const int r = tid >> 5, lane = tid & 31, i = i0 + r;
+  if (i >= n) return;
+  int* idx = row_index(i);
+  const int mine = row_past(i);
+  if (mine <= topk) {
+    for (int e = lane; e < topk; e += 32) idx[e] = e < mine ? e : -1;
+    return;
+  }
+  const unsigned long long* kr = pk_keys + (size_t)(ROWS == 1 ? 0 : r) * blocks;
+  // The threshold is the largest T with at least topk keys >= T; the search ends early when exactly
+  // topk are.
+  unsigned long long T = 0;
+  for (int bit = 63; bit >= 0; --bit) {
+    const unsigned long long t = T | (1ull << bit);
+    int cnt = 0;
+    for (int c = lane; c < mine; c += 32) cnt += kr[c] >= t;
+    cnt = __reduce_add_sync(kFull, cnt);
+    if (cnt >= topk) T = t;
+    if (cnt == topk) break;
+  }
+  int above = 0;
+  for (int c = lane; c < mine; c += 32) above += kr[c] > T;
+  int ties = topk - __reduce_add_sync(kFull, above), out = 0;
+  for (int c0 = 0; c0 < mine; c0 += 32) {
+    const int c = c0 + lane;
+    const unsigned long long k = c < mine ? kr[c] : 0ull;
+    const unsigned tie = __ballot_sync(kFull, c < mine && k == T);
+    const bool take = c < mine && (k > T || (k == T && __popc(tie & ((1u << lane) - 1)) < ties));
+    const unsigned chosen = __ballot_sync(kFull, take);
+    if (take) idx[out + __popc(chosen & ((1u << lane) - 1))] = c;
+    out += __popc(chosen);
+    ties -= min(ties, __popc(tie));
+  }
 }
 
 cudaLaunchConfig_t kc_cfg(dim3 grid, dim3 block, size_t smem, cudaStream_t s, cudaLaunchAttribute* attr) {
@@ -342,12 +463,30 @@ cudaError_t launch_kv_block_keys(const float* kc, const int* pos, int batch, int
 cudaError_t launch_kv_pick(const float* q, const float* keys, const int* pos, int batch, int n, int hq, int hkv,
                            int max_t, int block, int topk, int* index, int device, cudaStream_t s) {
   const int blocks = (max_t + block - 1) / block;
+  const int64_t rows = (int64_t)batch * n * hkv;
+  cudaLaunchAttribute attr[2];
+  // eight tokens a CTA where that still fills the SMs and their order keys fit
+  if (n >= kPickRows && rows / kPickRows >= 74 && (size_t)blocks * 8 * kPickRows <= 128 * 1024) {
+    static int configured[128] = {0};
+    cudaError_t e = ensure_smem((const void*)kv_pick_kernel<kPickRows>, configured, device, 128 * 1024, false);
+    if (e != cudaSuccess) return e;
+    const int64_t lists = (int64_t)batch * hkv * ((n + kPickRows - 1) / kPickRows);
+    cudaLaunchConfig_t cfg = kc_cfg(dim3((unsigned)lists), dim3(kPickThreads), (size_t)blocks * 8 * kPickRows, s, attr);
+    return cudaLaunchKernelEx(&cfg, kv_pick_kernel<kPickRows>, q, keys, pos, n, hq, hkv, max_t, block, blocks, topk, index);
+  }
   static int configured[128] = {0};
-  cudaError_t e = ensure_smem((const void*)kv_pick_kernel, configured, device, (size_t)kKvMaxBlocks * 8, false);
+  cudaError_t e = ensure_smem((const void*)kv_pick_kernel<1>, configured, device, (size_t)kKvMaxBlocks * 8, false);
   if (e != cudaSuccess) return e;
-  cudaLaunchAttribute attr[1];
-  cudaLaunchConfig_t cfg = kc_cfg(dim3((unsigned)((int64_t)batch * n * hkv)), dim3(kPickThreads), (size_t)blocks * 8, s, attr);
-  return cudaLaunchKernelEx(&cfg, kv_pick_kernel, q, keys, pos, n, hq, hkv, max_t, block, blocks, topk, index);
+  // a cluster of CTAs per row while there are SMs for it; at least 64 blocks a CTA
+  unsigned ranks = 1;
+  while (ranks < 8 && rows * ranks * 2 <= 296 && blocks >= 128 * (int)ranks) ranks *= 2;
+  cudaLaunchConfig_t cfg = kc_cfg(dim3((unsigned)(rows * ranks)), dim3(kPickThreads), (size_t)blocks * 8, s, attr);
+  attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+  attr[cfg.numAttrs].val.clusterDim.x = ranks;
+  attr[cfg.numAttrs].val.clusterDim.y = 1;
+  attr[cfg.numAttrs].val.clusterDim.z = 1;
+  ++cfg.numAttrs;
+  return cudaLaunchKernelEx(&cfg, kv_pick_kernel<1>, q, keys, pos, n, hq, hkv, max_t, block, blocks, topk, index);
 }
 
 }  // namespace q8lin

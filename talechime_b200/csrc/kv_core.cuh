@@ -39,6 +39,7 @@ struct KvArgs {
   int least;              // chunks a CTA takes at least
   int rgs;                // row groups of a kv head (tree, causal) or of a token (blocks)
   int units;
+  int weight_reps;        // scores stored: groups of 128 keys a CTA of the merge adds the weights of
   int split;              // 1: kKvGrid CTAs share all chunks evenly; 0: whole units
   float c;                // log2(e) * f32(1/sqrt(128))
 };
