@@ -28,6 +28,8 @@ HEAD_DIM = 128
 
 
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device) -> None:
+    if t.dtype is dtype and t.device == device and t.is_contiguous():
+        return
     if t.dtype != dtype:
         raise Q8LinError(_lib.ERR_INVALID_ARGUMENT, f"{name} dtype {t.dtype} is not {dtype}")
     if not t.is_contiguous():
@@ -88,12 +90,16 @@ def _scratch(workspace: Optional[torch.Tensor], size: int, dev: torch.device) ->
 
 
 def _call(fn, dev: torch.device, *args) -> None:
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if torch.cuda.current_device() == dev.index:
-        check(fn(*args, stream))
+    # the raw handle of the current stream: torch.cuda.current_stream builds an object for it, a
+    # fifth of a small call's time
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, stream))
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status != _lib.OK:
+        check(status)
 
 
 def rope_attention_tree(qkv: torch.Tensor, parents: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor,

@@ -10,6 +10,11 @@ residual adds fused into the projections); the position and the current token li
 in device memory, so ``step()`` is capture-safe and one captured CUDA graph replays for
 every decode step (``q8lin_argmax`` writes the next token and advances the position).
 
+Beyond the reference's loop (talechime_b200/attention.py): ``verify_tree`` / ``accept_path`` /
+``step_tree`` run a tree of drafted tokens as one forward; the "tracked" mode accumulates
+every cached row's attention weight and ``evict`` keeps the heaviest rows; the "blocks" mode
+attends over the blocks of rows that score highest.
+
 Weights are GGUF Q8_0 block arrays (bytes / numpy / torch uint8) and f32 norm vectors;
 q|k|v and gate|up are stored as fused weights (rows q, then k, then v; gate, then up).
 """
@@ -22,7 +27,7 @@ from typing import Optional
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, attention
 from ._lib import check
 from .qmatmul import QMatMul, _stream_ptr
 from .tp_mlp import swiglu
@@ -40,6 +45,7 @@ class DecoderConfig:
     max_t: int = 640
     eps: float = 1e-5
     rope_theta: float = 10000.0
+    max_pos: int = 0  # rows of the RoPE tables beyond max_t: positions that evictions make room for
 
     @property
     def qkv_rows(self) -> int:
@@ -49,13 +55,13 @@ class DecoderConfig:
 def rope_tables(cfg: DecoderConfig, factors: Optional[np.ndarray] = None) -> tuple[np.ndarray, np.ndarray]:
     """cos/sin [max_t][head_dim/2] as transformer.rs:48-60 builds them: freq_i =
     theta^(-2i/d) in f64 rounded to f32, divided by the factors (f32), angle = pos * freq
-    (f32), then f32 cos/sin."""
+    (f32), then f32 cos/sin; max_pos rows where that is more."""
     half = cfg.head_dim // 2
     freq = np.array([cfg.rope_theta ** (-(2 * i) / cfg.head_dim) for i in range(half)], dtype=np.float64)
     f = freq.astype(np.float32)
     if factors is not None:
         f = (f / np.asarray(factors, dtype=np.float32)).astype(np.float32)
-    pos = np.arange(cfg.max_t, dtype=np.float32)[:, None]
+    pos = np.arange(max(cfg.max_t, cfg.max_pos), dtype=np.float32)[:, None]
     ang = (pos * f[None, :]).astype(np.float32)
     return np.cos(ang).astype(np.float32), np.sin(ang).astype(np.float32)
 
@@ -136,9 +142,14 @@ class Q8Decoder:
         return cls(cfg, weights, device=device, rope_factors=factors)
 
     def __init__(self, cfg: DecoderConfig, weights: dict, device: torch.device | int | str = 0,
-                 rope_factors: Optional[np.ndarray] = None, batch: int = 1):
+                 rope_factors: Optional[np.ndarray] = None, batch: int = 1, track_weights: bool = False,
+                 blocks: Optional[tuple[int, int]] = None):
         """`batch` sequences share the weights and the position; each has its own KV cache
-        (prefill() takes [batch, T] tokens); the decode step serves batch 1."""
+        (prefill() takes [batch, T] tokens); the decode step serves batch 1.
+
+        track_weights: hold an accumulated attention weight per cached row (kv_weight), filled by
+        the "tracked" modes and read by evict().  blocks = (rows of a block, blocks per token):
+        hold the blocks' mean keys for the "blocks" modes."""
         if batch < 1:
             raise ValueError("batch must be positive")
         self.batch = int(batch)
@@ -182,6 +193,16 @@ class Q8Decoder:
             kv_shape = (self.batch,) + kv_shape
         self.k_cache = [torch.zeros(kv_shape, device=dev) for _ in range(cfg.layers)]
         self.v_cache = [torch.zeros(kv_shape, device=dev) for _ in range(cfg.layers)]
+        self.kv_weight = [torch.zeros(kv_shape[:-1], device=dev) for _ in range(cfg.layers)] if track_weights else None
+        self.blocks = blocks
+        self.block_keys = None
+        if blocks is not None:
+            nb = -(-cfg.max_t // blocks[0])
+            self.block_keys = [torch.zeros((self.batch, cfg.kv_heads, nb, cfg.head_dim), device=dev)
+                               for _ in range(cfg.layers)]
+            self._keys_stale = False
+        self.evicted = 0  # rows evict() took out: RoPE positions run ahead of cache rows by this many
+        self._row0 = torch.zeros(self.batch, dtype=torch.int32, device=dev)
         f = lambda n: torch.zeros(n, device=dev)
         self.x, self.h = f(H), f(H)
         self.qkv, self.q = f(cfg.qkv_rows), f(cfg.heads * cfg.head_dim)
@@ -203,8 +224,18 @@ class Q8Decoder:
         """Empty the cache (position 0) and set the current token."""
         self.pos.zero_()
         self.token.fill_(int(token))
+        if self.evicted:
+            self.evicted = 0
+            self._drop_step_handle()
+        for w in self.kv_weight or ():
+            w.zero_()
 
-    MODES = ("persistent", "fused", "unfused")
+    def _rope(self) -> tuple[ctypes.c_void_p, ctypes.c_void_p]:
+        """The RoPE tables from the position of cache row 0 on."""
+        off = self.evicted * (self.cfg.head_dim // 2) * 4
+        return ctypes.c_void_p(self.cos.data_ptr() + off), ctypes.c_void_p(self.sin.data_ptr() + off)
+
+    MODES = ("persistent", "fused", "unfused", "tracked", "blocks")
 
     def step(self, mode: str = "fused") -> None:
         """One decode step for the token at self.token / position self.pos; afterwards
@@ -215,30 +246,53 @@ class Q8Decoder:
         "fused": one launch per operation with rms_norm and SwiGLU inside the following
         projection's activation quantization, the residual adds inside the o / down
         projections and RoPE + KV append inside the attention kernel (5 launches per
-        layer); "unfused": 11 launches per layer, one per reference operation."""
+        layer); "unfused": 11 launches per layer, one per reference operation; "tracked"
+        (track_weights): the fused step whose attention also adds every cached row's weight to
+        kv_weight; "blocks" (blocks=...): the fused step whose attention goes over the blocks
+        of rows that score highest."""
         if self.batch != 1:
             raise ValueError("the decode step serves batch 1; this decoder holds "
                              f"{self.batch} sequences (prefill only)")
+        if mode not in self.MODES:
+            raise ValueError(f"mode must be one of {self.MODES}")
+        self._check_mode(mode)
         if mode == "persistent":
             check(_lib.lib().q8lin_step_run(self._persistent(), ctypes.c_void_p(_stream_ptr(self.device))))
-        elif mode == "fused":
-            self._step_fused()
         elif mode == "unfused":
             self._step_unfused()
         else:
-            raise ValueError(f"mode must be one of {self.MODES}")
+            self._step_fused(mode)
+
+    def _check_mode(self, mode: str) -> None:
+        """The mode has what it needs; block keys are up to date for "blocks", and not behind any other."""
+        if mode == "tracked" and self.kv_weight is None:
+            raise ValueError("the tracked mode needs a decoder made with track_weights=True")
+        if mode == "blocks" and self.blocks is None:
+            raise ValueError("the blocks mode needs a decoder made with blocks=(rows of a block, blocks per token)")
+        if self.blocks is not None:
+            if mode != "blocks":
+                self._keys_stale = True
+            elif self._keys_stale:
+                self.refresh_block_keys()
+
+    def refresh_block_keys(self) -> None:
+        """Recompute the mean keys of all blocks from the caches (after steps of other modes)."""
+        for li in range(self.cfg.layers):
+            attention.block_keys(self.k_cache[li], self._row0, self.cfg.max_t, self.blocks[0], keys=self.block_keys[li])
+        self._keys_stale = False
 
     def _persistent(self) -> ctypes.c_void_p:
         """The decode step as a q8lin_step program (built once, then reused)."""
         if getattr(self, "_step_handle", None) is not None:
             return self._step_handle
         cfg, L, P = self.cfg, _lib.lib(), lambda t: t.data_ptr()
+        cos, sin = (t.value for t in self._rope())
         ops = [_lib.Op(kind=_lib.OP_EMBED, weight=self.embed.handle.value, y=P(self.x))]
         for li, w in enumerate(self.layers):
             ops.append(_lib.Op(kind=_lib.OP_GEMV, prologue=_lib.PROLOGUE_RMSNORM, weight=w["qkv"].handle.value,
                                x=P(self.x), y=P(self.qkv), norm_weight=P(w["attn_norm"]), eps=cfg.eps))
             ops.append(_lib.Op(kind=_lib.OP_ATTENTION, x=P(self.qkv), y=P(self.attn), k_cache=P(self.k_cache[li]),
-                               v_cache=P(self.v_cache[li]), cos_t=P(self.cos), sin_t=P(self.sin), hq=cfg.heads,
+                               v_cache=P(self.v_cache[li]), cos_t=cos, sin_t=sin, hq=cfg.heads,
                                hkv=cfg.kv_heads, head_dim=cfg.head_dim, max_t=cfg.max_t))
             ops.append(_lib.Op(kind=_lib.OP_GEMV, weight=w["o"].handle.value, x=P(self.attn), y=P(self.x),
                                residual=P(self.x)))
@@ -258,6 +312,13 @@ class Q8Decoder:
         self._step_handle = h
         return h
 
+    def _drop_step_handle(self) -> None:
+        h = getattr(self, "_step_handle", None)
+        if h is not None and h.value:
+            torch.cuda.synchronize(self.device)  # a queued step may still read it
+            check(_lib.lib().q8lin_step_destroy(h))
+        self._step_handle = None
+
     def __del__(self):
         h = getattr(self, "_step_handle", None)
         if h is not None and h.value:
@@ -267,17 +328,35 @@ class Q8Decoder:
                 pass
             self._step_handle = None
 
-    def _step_fused(self) -> None:
+    def _attend(self, mode: str, li: int, q: torch.Tensor, pos: torch.Tensor, out: torch.Tensor) -> None:
+        """Attention of q's rows (their keys appended) of layer `li` in the "tracked" or "blocks"
+        mode; q, out [batch, t, heads, head_dim], pos int32 [batch]."""
+        if mode == "tracked":
+            attention.attention_weights(q, self.k_cache[li], self.v_cache[li], pos, self.kv_weight[li], out=out)
+        else:
+            block, topk = self.blocks
+            attention.block_keys(self.k_cache[li], pos, q.shape[1], block, keys=self.block_keys[li])
+            attention.attention_blocks(q, self.k_cache[li], self.v_cache[li], self.block_keys[li], pos, block, topk,
+                                       out=out)
+
+    def _step_fused(self, mode: str = "fused") -> None:
         cfg, L, P = self.cfg, _lib.lib(), self._p
         s = ctypes.c_void_p(_stream_ptr(self.device))
+        cos, sin = self._rope()
+        row = (1, 1, cfg.heads, cfg.head_dim)
         check(L.q8lin_embed_rows(self.embed.handle, P(self.token), 1, P(self.x), s))
         for li, w in enumerate(self.layers):
             w["qkv"].forward_fused(self.x, self.qkv, QMatMul.PROLOGUE_RMSNORM, w["attn_norm"], cfg.eps)
-            # the step starts with the embedding launch after the previous step's argmax,
-            # so the position and the cached rows are ready before this launch's wait
-            check(L.q8lin_rope_attention_decode_ex(P(self.qkv), P(self.pos), P(self.cos), P(self.sin),
-                                                   P(self.k_cache[li]), P(self.v_cache[li]), cfg.heads, cfg.kv_heads,
-                                                   cfg.head_dim, cfg.max_t, P(self.attn), 1, s))
+            if mode == "fused":
+                # the step starts with the embedding launch after the previous step's argmax,
+                # so the position and the cached rows are ready before this launch's wait
+                check(L.q8lin_rope_attention_decode_ex(P(self.qkv), P(self.pos), cos, sin, P(self.k_cache[li]),
+                                                       P(self.v_cache[li]), cfg.heads, cfg.kv_heads, cfg.head_dim,
+                                                       cfg.max_t, P(self.attn), 1, s))
+            else:
+                check(L.q8lin_rope_kv(P(self.qkv), P(self.pos), cos, sin, P(self.k_cache[li]), P(self.v_cache[li]),
+                                      cfg.heads, cfg.kv_heads, cfg.head_dim, cfg.max_t, P(self.q), s))
+                self._attend(mode, li, self.q.view(row), self.pos, self.attn.view(row))
             w["o"].forward_fused(self.attn, self.x, residual=self.x)
             w["gate_up"].forward_fused(self.x, self.gu, QMatMul.PROLOGUE_RMSNORM, w["ffn_norm"], cfg.eps)
             w["down"].forward_fused(self.gu, self.x, QMatMul.PROLOGUE_SWIGLU, residual=self.x)
@@ -289,13 +368,13 @@ class Q8Decoder:
         cfg, L, P = self.cfg, _lib.lib(), self._p
         s = ctypes.c_void_p(_stream_ptr(self.device))
         H = cfg.hidden
+        cos, sin = self._rope()
         check(L.q8lin_embed_rows(self.embed.handle, P(self.token), 1, P(self.x), s))
         for li, w in enumerate(self.layers):
             check(L.q8lin_rmsnorm(P(self.x), P(w["attn_norm"]), 1, H, cfg.eps, P(self.h), s))
             w["qkv"].forward(self.h.view(1, H), out=self.qkv.view(1, -1))
-            check(L.q8lin_rope_kv(P(self.qkv), P(self.pos), P(self.cos), P(self.sin), P(self.k_cache[li]),
-                                  P(self.v_cache[li]), cfg.heads, cfg.kv_heads, cfg.head_dim, cfg.max_t,
-                                  P(self.q), s))
+            check(L.q8lin_rope_kv(P(self.qkv), P(self.pos), cos, sin, P(self.k_cache[li]), P(self.v_cache[li]),
+                                  cfg.heads, cfg.kv_heads, cfg.head_dim, cfg.max_t, P(self.q), s))
             check(L.q8lin_attention_decode(P(self.q), P(self.k_cache[li]), P(self.v_cache[li]), P(self.pos),
                                            cfg.heads, cfg.kv_heads, cfg.head_dim, cfg.max_t, P(self.attn_ws),
                                            self.attn_ws.numel(), P(self.attn), s))
@@ -310,7 +389,7 @@ class Q8Decoder:
         check(L.q8lin_argmax(P(self.logits), cfg.vocab, P(self.argmax_ws), self.argmax_ws.numel(), P(self.token),
                              P(self.pos), s))
 
-    def prefill(self, tokens) -> torch.Tensor:
+    def prefill(self, tokens, mode: str = "dense") -> torch.Tensor:
         """Run a prompt as ONE batched forward: `tokens` [T] (batch 1) or [batch, T] ids at
         positions pos .. pos + T - 1 of every sequence (crates/voxcpm/src/model.rs:492-495,
         transformer.rs:107-155 with offset = pos): the linears at M = batch * T, RoPE and
@@ -321,8 +400,11 @@ class Q8Decoder:
         holds the last row's logits (batch 1; self.prefill_logits [batch, vocab]) and,
         for batch 1, self.token the next token -- the state T decode steps over the same
         tokens leave.  Raises Q8LinError(ERR_SHAPE) past max_t, as the reference's
-        "Transformer context limit exceeded" (transformer.rs:110-113)."""
+        "Transformer context limit exceeded" (transformer.rs:110-113).  mode "tracked" or
+        "blocks": the attention of step()'s mode of that name."""
         cfg, L, P = self.cfg, _lib.lib(), self._p
+        if mode not in ("dense", "tracked", "blocks"):
+            raise ValueError("mode must be one of ('dense', 'tracked', 'blocks')")
         tok = torch.as_tensor(np.asarray(tokens.cpu() if isinstance(tokens, torch.Tensor) else tokens),
                               dtype=torch.int32)
         if tok.dim() == 1:
@@ -335,9 +417,10 @@ class Q8Decoder:
             raise _lib.Q8LinError(_lib.ERR_SHAPE, "prefill needs at least one token")
         if pos0 + T > cfg.max_t:
             raise _lib.Q8LinError(_lib.ERR_SHAPE, "Transformer context limit exceeded")
-        return self._prefill_launches(tok.reshape(-1).to(self.device), B, T, pos0)
+        self._check_mode(mode)
+        return self._prefill_launches(tok.reshape(-1).to(self.device), B, T, pos0, mode)
 
-    def _prefill_launches(self, tok_d: torch.Tensor, B: int, T: int, pos0: int) -> torch.Tensor:
+    def _prefill_launches(self, tok_d: torch.Tensor, B: int, T: int, pos0: int, mode: str = "dense") -> torch.Tensor:
         """The device work of ``prefill`` for `tok_d` (int32 [B * T] on the device) at a
         host-known position pos0 (checked by the caller): kernel launches on the current
         stream and tensor allocations only, no host synchronisation."""
@@ -348,15 +431,20 @@ class Q8Decoder:
         e = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)
         x, hn, qkv, q, att, t1 = e(M, H), e(M, H), e(M, cfg.qkv_rows), e(M, hd), e(M, hd), e(M, H)
         gu, hm = e(M, 2 * cfg.inter), e(M, cfg.inter)
+        cos, sin = self._rope()
+        pos_d = torch.full((B,), pos0, dtype=torch.int32, device=dev) if mode != "dense" else None
+        rows = (B, T, cfg.heads, cfg.head_dim)
         check(L.q8lin_embed_rows(self.embed.handle, P(tok_d), M, P(x), s))
         check(L.q8lin_rmsnorm(P(x), P(self.layers[0]["attn_norm"]), M, H, cfg.eps, P(hn), s))
         for li, w in enumerate(self.layers):
             w["qkv"].forward(hn, out=qkv)
-            check(L.q8lin_rope_kv_rows(P(qkv), B, T, pos0, P(self.cos), P(self.sin), P(self.k_cache[li]),
-                                       P(self.v_cache[li]), cfg.heads, cfg.kv_heads, cfg.head_dim, cfg.max_t,
-                                       P(q), s))
-            check(L.q8lin_attention_prefill(P(q), P(self.k_cache[li]), P(self.v_cache[li]), B, T, pos0, cfg.heads,
-                                            cfg.kv_heads, cfg.head_dim, cfg.max_t, P(att), s))
+            check(L.q8lin_rope_kv_rows(P(qkv), B, T, pos0, cos, sin, P(self.k_cache[li]), P(self.v_cache[li]),
+                                       cfg.heads, cfg.kv_heads, cfg.head_dim, cfg.max_t, P(q), s))
+            if mode == "dense":
+                check(L.q8lin_attention_prefill(P(q), P(self.k_cache[li]), P(self.v_cache[li]), B, T, pos0, cfg.heads,
+                                                cfg.kv_heads, cfg.head_dim, cfg.max_t, P(att), s))
+            else:
+                self._attend(mode, li, q.view(rows), pos_d, att.view(rows))
             w["o"].forward(att, out=t1)
             # residual add + the norm after it, one pass: x += o(att); hn = ffn_norm(x)
             check(L.q8lin_add_rmsnorm(P(x), P(t1), P(w["ffn_norm"]), M, H, cfg.eps, P(hn), s))
@@ -385,9 +473,132 @@ class Q8Decoder:
             self.token.copy_(nxt)
         return nxt
 
+    # ---- drafted tokens ------------------------------------------------------------------
+
+    def verify_tree(self, tokens, parents) -> torch.Tensor:
+        """One forward of a tree of tokens behind the cached rows (batch 1): `tokens` [n] ids (n <=
+        256), `parents` [n] each node's parent, a node before it, or -1 for the cached history.
+        Node i sits at RoPE position (cached rows + its depth) and sees the history and its
+        ancestors (q8lin_rope_attention_tree).  Returns the greedy next token of every node
+        (int32 [n] on the device); tree_logits [n, vocab] holds the logits.  The cached rows
+        pos .. pos + n - 1 hold the nodes until accept_path() or the next step; pos and token
+        stay.  Raises Q8LinError(ERR_SHAPE) past max_t."""
+        if self.batch != 1:
+            raise ValueError("verify_tree serves batch 1")
+        i32 = lambda v: torch.as_tensor(np.asarray(v.cpu() if isinstance(v, torch.Tensor) else v), dtype=torch.int32)
+        tok, par = i32(tokens), i32(parents)
+        if tok.dim() != 1 or par.shape != tok.shape or not 1 <= tok.numel() <= 256:
+            raise _lib.Q8LinError(_lib.ERR_SHAPE, f"tokens and parents must be [n] with 1 <= n <= 256; got "
+                                                  f"{tuple(tok.shape)} and {tuple(par.shape)}")
+        n = tok.numel()
+        if bool((par < -1).any()) or bool((par >= torch.arange(n, dtype=torch.int32)).any()):
+            raise _lib.Q8LinError(_lib.ERR_INVALID_ARGUMENT, "a node's parent is a node before it, or -1")
+        if int(self.pos.item()) + n > self.cfg.max_t:
+            raise _lib.Q8LinError(_lib.ERR_SHAPE, "Transformer context limit exceeded")
+        return self._tree_launches(tok.to(self.device), par.to(self.device).view(1, n))
+
+    def _tree_launches(self, tok_d: torch.Tensor, par_d: torch.Tensor) -> torch.Tensor:
+        """The device work of ``verify_tree``: launches and tensor allocations only."""
+        cfg, L, P = self.cfg, _lib.lib(), self._p
+        dev, H, n = self.device, cfg.hidden, tok_d.numel()
+        s = ctypes.c_void_p(_stream_ptr(dev))
+        e = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)
+        x, hn, qkv, t1 = e(n, H), e(n, H), e(n, cfg.qkv_rows), e(n, H)
+        att = e(1, n, cfg.heads, cfg.head_dim)
+        gu, hm = e(n, 2 * cfg.inter), e(n, cfg.inter)
+        cos, sin = self.cos[self.evicted:], self.sin[self.evicted:]
+        check(L.q8lin_embed_rows(self.embed.handle, P(tok_d), n, P(x), s))
+        check(L.q8lin_rmsnorm(P(x), P(self.layers[0]["attn_norm"]), n, H, cfg.eps, P(hn), s))
+        for li, w in enumerate(self.layers):
+            w["qkv"].forward(hn, out=qkv)
+            attention.rope_attention_tree(qkv.view(1, n, -1), par_d, self.pos, cos, sin, self.k_cache[li],
+                                          self.v_cache[li], out=att)
+            w["o"].forward(att.view(n, -1), out=t1)
+            check(L.q8lin_add_rmsnorm(P(x), P(t1), P(w["ffn_norm"]), n, H, cfg.eps, P(hn), s))
+            w["gate_up"].forward(hn, out=gu)
+            check(L.q8lin_swiglu(P(gu), n, cfg.inter, P(hm), s))
+            w["down"].forward(hm, out=t1)
+            norm = self.layers[li + 1]["attn_norm"] if li + 1 < len(self.layers) else self.out_norm
+            check(L.q8lin_add_rmsnorm(P(x), P(t1), P(norm), n, H, cfg.eps, P(hn), s))
+        self.tree_logits = e(n, cfg.vocab)
+        self.lm_head.forward(hn, out=self.tree_logits)
+        nxt = torch.empty(n, dtype=torch.int32, device=dev)
+        for i in range(n):
+            check(L.q8lin_argmax(ctypes.c_void_p(self.tree_logits.data_ptr() + i * cfg.vocab * 4), cfg.vocab,
+                                 P(self.argmax_ws), self.argmax_ws.numel(), ctypes.c_void_p(nxt.data_ptr() + 4 * i),
+                                 None, s))
+        return nxt
+
+    def accept_path(self, path, token: int) -> None:
+        """Keep the nodes `path` (a path of the last verify_tree from a root down, ascending) as the
+        next cached rows and set the current token; the other nodes are dropped."""
+        idx = [int(i) for i in path]
+        if any(b <= a for a, b in zip(idx, idx[1:])) or (idx and idx[0] < 0):
+            raise _lib.Q8LinError(_lib.ERR_INVALID_ARGUMENT, "a path's nodes are ascending")
+        if idx and idx[-1] != len(idx) - 1:  # the first nodes in a row are where they belong
+            d = torch.tensor([idx], dtype=torch.int32, device=self.device)
+            for li in range(self.cfg.layers):
+                attention.kv_move_rows(self.k_cache[li], self.v_cache[li], d, base=self.pos)
+        self.pos += len(idx)
+        self.token.fill_(int(token))
+        if self.blocks is not None:
+            self._keys_stale = True
+
+    def step_tree(self, tokens, parents) -> list[int]:
+        """A greedy decode step over drafted tokens: node 0 is the current token, the other nodes
+        drafts of what follows their parents.  Runs verify_tree, keeps the longest path from
+        node 0 whose drafts are what the model picks, and returns the new tokens: the accepted
+        drafts and the model's own pick after the last of them -- the tokens that as many plain
+        steps give."""
+        tok = [int(t) for t in (tokens.tolist() if isinstance(tokens, torch.Tensor) else tokens)]
+        par = [int(p) for p in (parents.tolist() if isinstance(parents, torch.Tensor) else parents)]
+        if not tok or par[:1] != [-1] or -1 in par[1:]:
+            raise _lib.Q8LinError(_lib.ERR_INVALID_ARGUMENT, "node 0, the current token, is the only root")
+        if tok[0] != int(self.token.item()):
+            raise _lib.Q8LinError(_lib.ERR_INVALID_ARGUMENT, f"node 0 is {tok[0]}, the current token {int(self.token.item())}")
+        nxt = self.verify_tree(tok, par).tolist()
+        path = [0]
+        while True:
+            child = next((i for i in range(path[-1] + 1, len(tok)) if par[i] == path[-1] and tok[i] == nxt[path[-1]]), None)
+            if child is None:
+                break
+            path.append(child)
+        self.accept_path(path, nxt[path[-1]])
+        return [tok[i] for i in path[1:]] + [nxt[path[-1]]]
+
+    # ---- eviction ------------------------------------------------------------------------
+
+    def evict(self, keep: int, sink: int = 0, recent: int = 0) -> int:
+        """Shrink every head's cache to min(pos, keep) rows: the first `sink`, the last `recent`
+        and, of the others, those with the most accumulated attention weight of the tracked
+        steps (q8lin_kv_evict).  Later tokens take the rows after them at the RoPE positions
+        they would have had, so the tables need cfg.max_pos >= max_t + the rows evicted in
+        all.  Returns the number of rows taken out.  A captured step holds the old position
+        offset: capture again."""
+        if self.kv_weight is None:
+            raise ValueError("evict needs a decoder made with track_weights=True")
+        pos = int(self.pos.item())
+        gone = max(0, pos - keep)
+        if self.evicted + gone + self.cfg.max_t > self.cos.shape[0]:
+            raise _lib.Q8LinError(_lib.ERR_SHAPE, f"the RoPE tables hold {self.cos.shape[0]} positions; evicting "
+                                                  f"{gone} rows needs {self.evicted + gone + self.cfg.max_t} (max_pos)")
+        length = self.pos.expand(self.batch).contiguous()
+        for li in range(self.cfg.layers):
+            attention.kv_evict(self.kv_weight[li], self.k_cache[li], self.v_cache[li], length, keep, sink=sink,
+                               recent=recent, weight_out=self.kv_weight[li])
+        if gone:
+            self.pos -= gone
+            self.evicted += gone
+            self._drop_step_handle()
+            if self.blocks is not None:
+                self._keys_stale = True
+        return gone
+
     def launches_per_step(self, mode: str = "fused") -> int:
         if mode == "persistent":
             return 1
+        if mode in ("tracked", "blocks"):  # the fused step's five, with attention in 3 or 5
+            return 1 + self.cfg.layers * (7 if mode == "tracked" else 9) + 2
         fused = mode == "fused"
         return 1 + self.cfg.layers * (5 if fused else 11) + (2 if fused else 3)
 
