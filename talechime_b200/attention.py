@@ -39,7 +39,7 @@ def _need(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device) 
 
 
 def _shape(t: torch.Tensor, name: str, *shape: int) -> None:
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise Q8LinError(_lib.ERR_SHAPE, f"{name} is {tuple(t.shape)}, expected {shape}")
 
 
@@ -161,7 +161,7 @@ def attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
 
 def _weight(w: torch.Tensor, name: str, batch: int, hkv: int, max_t: int, dev: torch.device) -> None:
     _need(w, name, torch.float32, dev)
-    if tuple(w.shape) != (batch, hkv, max_t) and not (batch == 1 and tuple(w.shape) == (hkv, max_t)):
+    if w.shape != (batch, hkv, max_t) and not (batch == 1 and w.shape == (hkv, max_t)):
         raise Q8LinError(_lib.ERR_SHAPE, f"{name} is {tuple(w.shape)}, expected {(batch, hkv, max_t)}")
 
 

@@ -566,16 +566,17 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         float4* turn = reinterpret_cast<float4*>(&sm.turn[half][warp & 3][0][0]);
         const int row0 = (warp & 3) * 32;
 #pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = row0 + 4 * i + (lane >> 3);
+          const float4* src = reinterpret_cast<const float4*>(a.q + kv_row_offset<MASK>(a, x, min(r, x.nrows - 1))) +
+                              half * 8 + (lane & 7);
+          mine4[i] = src[0];
+          mine4[8 + i] = src[16];
+        }
+#pragma unroll
         for (int part = 0; part < 2; ++part) {  // the two stretches of 32 dimensions
-          float4 v[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = row0 + 4 * i + (lane >> 3);
-            v[i] = reinterpret_cast<const float4*>(a.q + kv_row_offset<MASK>(a, x, min(r, x.nrows - 1)))
-                [part * 16 + half * 8 + (lane & 7)];
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) turn[(4 * i + (lane >> 3)) * 9 + (lane & 7)] = v[i];
+          for (int i = 0; i < 8; ++i) turn[(4 * i + (lane >> 3)) * 9 + (lane & 7)] = mine4[part * 8 + i];
           __syncwarp();
 #pragma unroll
           for (int i = 0; i < 8; ++i) mine4[part * 8 + i] = turn[lane * 9 + i];
