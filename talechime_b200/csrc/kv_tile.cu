@@ -108,10 +108,11 @@ __device__ __forceinline__ void bar_arrive(uint64_t* b) {
 __device__ __forceinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort) {
   const uint64_t t0 = global_ns();
   while (!*abort) {
-    if (mb_try(bar, parity)) return true;
-    if (global_ns() - t0 > s_kt_wait_ns) {
+    if (global_ns() - t0 >= s_kt_wait_ns) {  // a limit of 0 allows no waiting at all
       atomicOr(&g_kv_tile_fault, 32u);
       *abort = 1;
+    } else if (mb_try(bar, parity)) {
+      return true;
     }
   }
   return false;

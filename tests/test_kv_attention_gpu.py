@@ -678,3 +678,36 @@ def test_tensors_that_do_not_fit_are_refused(cuda_device):
         attention.attention_blocks(c["q"], c["k"], c["v"], c["keys"], c["pos"], 24, 1)
     with pytest.raises(Q8LinError):
         attention.kv_move_rows(c["k"], c["v"], _i32([[0]], dev))
+
+
+def test_a_wait_that_runs_out_reports_itself(cuda_device):
+    """With a wait limit of 0 the tensor-core kernels give up at their first wait that is not over
+    at once: fault bit 5, rows NaN or right, the context usable, and the next call with the
+    usual limit right again."""
+    import ctypes
+
+    dev, L = cuda_device, _lib.lib()
+    g = _gen(91, dev)
+    B, t, hq, hkv, max_t = 2, 40, 16, 2, 700
+    k, v = _caches(g, B, hkv, max_t, dev)
+    q = torch.randn((B, t, hq, D), generator=g, device=dev)
+    pos = [600, 300]
+    flags = ctypes.c_uint32(0)
+    _lib.check(L.q8lin_fault_status(0, ctypes.byref(flags), 1))
+    ref, wref = _weights_ref(q, k, v, pos, torch.zeros((B, hkv, max_t), device=dev))
+    old = L.q8lin_wait_limit_ns()
+    try:
+        assert L.q8lin_set_wait_limit_ns(0) == 0
+        out = attention.attention_weights(q, k, v, _i32(pos, dev), torch.zeros((B, hkv, max_t), device=dev))
+        torch.cuda.synchronize()
+    finally:
+        L.q8lin_set_wait_limit_ns(old)
+    _lib.check(L.q8lin_fault_status(0, ctypes.byref(flags), 1))
+    assert flags.value == 32
+    assert torch.isnan(out).any()
+    w = torch.zeros((B, hkv, max_t), device=dev)
+    out = attention.attention_weights(q, k, v, _i32(pos, dev), w)
+    _close(out, ref)
+    _close(w, wref, "weight")
+    _lib.check(L.q8lin_fault_status(0, ctypes.byref(flags), 1))
+    assert flags.value == 0
