@@ -48,17 +48,19 @@ __device__ __forceinline__ float4 lds_f4(uint32_t addr) {
   return v;
 }
 
-template <int NT>
+constexpr int kKvList = 512;  // chosen blocks of a row held in shared memory; longer lists are read where they are
+template <int NT, int W>
 struct KvSmem {
   // each warp's ring of half chunks; after a unit's last chunk its output part [row][132]
-  alignas(16) uint8_t ring[kKvWarps][kKvSlots][kKvHalf];
+  alignas(16) uint8_t ring[W][kKvSlots][kKvHalf];
   // the unit's query rows as MMA fragments: [hi, lo][16 dimensions][8 rows][lane]
   alignas(16) float4 q[2][8][NT][32];
-  alignas(16) float p[kKvWarps][NT][kKvChunk][8];  // a chunk's probabilities
-  float m[kKvWarps][8 * NT], l[kKvWarps][8 * NT];
-  float f[kKvWarps][8 * NT];
+  alignas(16) float p[W][NT][kKvChunk][8];  // a chunk's probabilities
+  float m[W][8 * NT], l[W][8 * NT];
+  float f[W][8 * NT];
   float M[8 * NT], L[8 * NT];
   KvFind find;
+  int list[kKvList];
 };
 
 // The rows are the N side of the products and the keys, then the dimensions, the M side, so
@@ -67,10 +69,16 @@ struct KvSmem {
 //
 // What bounds it: with up to 16 rows a kv head the cache's bytes, read once; the tf32 split of
 // every key and value (4 operations each) and the products run beside the copies.
-template <int MASK, bool SCORES, int NT>
-__global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArgs a) {
+//
+// W warps: 8 on an SM, or with 8 rows and whole units 4, twice on an SM, so that one CTA's start
+// and end run beside the other's keys.  (8 against 4 warps: 512 units of 300 keys 59.6 and 44.5 us,
+// of 1000 keys 110.5 and 98.0; 1024 units of 2000 keys 329 and 326; 512 tokens that attend over
+// chosen blocks 203 and 186.  16 rows do not fit twice.)
+template <int MASK, bool SCORES, int NT, int W>
+__global__ void __launch_bounds__(W * 32, W == 4 ? 2 : 1) kv_attention_kernel(const KvArgs a) {
+  constexpr int kThreads = W * 32;
   extern __shared__ __align__(16) uint8_t kv_smem[];
-  KvSmem<NT>& sm = *reinterpret_cast<KvSmem<NT>*>(kv_smem);
+  KvSmem<NT, W>& sm = *reinterpret_cast<KvSmem<NT, W>*>(kv_smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
   pdl_wait();
@@ -78,7 +86,7 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArg
 
   int u, off, left;
   if (a.split) {
-    left = kv_find<MASK, kKvThreads>(a, sm.find, blockIdx.x);
+    left = kv_find<MASK, kThreads>(a, sm.find, blockIdx.x);
     u = sm.find.unit;
     off = sm.find.off;
   } else {
@@ -94,13 +102,22 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArg
     const float* kb = a.k + ((size_t)x.b * a.hkv + x.hk) * (size_t)a.max_t * kKvD;
     const float* vb = a.v + ((size_t)x.b * a.hkv + x.hk) * (size_t)a.max_t * kKvD;
 
-    // this warp's chunks: off + warp, off + warp + 8, ...  Half h of its stream: the keys
+    const int* list = nullptr;
+    if (MASK == kMaskBlocks) {
+      list = a.index + (((size_t)x.b * a.n + x.i0) * a.hkv + x.hk) * a.topk;
+      if (x.picked <= kKvList) {
+        for (int e = tid; e < x.picked; e += kThreads) sm.list[e] = list[e];
+        __syncthreads();
+        list = sm.list;
+      }
+    }
+    // this warp's chunks: off + warp, off + warp + W, ...  Half h of its stream: the keys
     // (h even) or values of its chunk h / 2, copied into ring slot h % 3.
     const int c0 = off + warp;
-    const int halves = c0 < c1 ? 2 * ((c1 - c0 + kKvWarps - 1) / kKvWarps) : 0;
+    const int halves = c0 < c1 ? 2 * ((c1 - c0 + W - 1) / W) : 0;
     auto load = [&](int h, int slot) {
       if (h < halves) {
-        const int j0 = kv_chunk_key<MASK>(a, x, c0 + (h >> 1) * kKvWarps);
+        const int j0 = kv_chunk_key<MASK>(a, x, list, c0 + (h >> 1) * W);
         const bool val = h & 1;
         const float* src = (val ? vb : kb) + (size_t)j0 * kKvD + lane * 4;
         const uint32_t dst = ring + slot * kKvHalf;
@@ -128,7 +145,7 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArg
 #pragma unroll
     for (int h = 0; h < kKvSlots; ++h) load(h, h);
     // query rows -> fragments
-    for (int e = tid; e < 8 * NT * 32; e += kKvThreads) {
+    for (int e = tid; e < 8 * NT * 32; e += kThreads) {
       const int ln = e & 31, nt = (e >> 5) % NT, pair = (e >> 5) / NT;
       const int r = (ln >> 2) + 8 * nt;
       float4 qv = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -160,7 +177,7 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArg
 
     int slot = 0;
     for (int h = 0; h < halves; h += 2) {
-      const int j0 = kv_chunk_key<MASK>(a, x, c0 + (h >> 1) * kKvWarps);
+      const int j0 = kv_chunk_key<MASK>(a, x, list, c0 + (h >> 1) * W);
       cp_async_wait(2);
       __syncwarp();
       // Scores: a lane takes dimensions 16 pair + 4t + e of keys g and g + 8.  The tensor cores
@@ -367,9 +384,9 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArg
     if (tid < x.nrows) {
       float M = -INFINITY, L = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kKvWarps; ++w) M = fmaxf(M, sm.m[w][tid]);
+      for (int w = 0; w < W; ++w) M = fmaxf(M, sm.m[w][tid]);
 #pragma unroll
-      for (int w = 0; w < kKvWarps; ++w) {
+      for (int w = 0; w < W; ++w) {
         const float f = M == -INFINITY ? 0.0f : exp2f(sm.m[w][tid] - M);
         sm.f[w][tid] = f;
         if (f != 0.0f) L = fmaf(sm.l[w][tid], f, L);  // an empty part's sums stay out
@@ -384,11 +401,11 @@ __global__ void __launch_bounds__(kKvThreads, 1) kv_attention_kernel(const KvArg
         a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + tid] = M == -INFINITY ? INFINITY : M + log2f(L);
     }
     __syncthreads();
-    for (int e = tid; e < x.nrows * 32; e += kKvThreads) {
+    for (int e = tid; e < x.nrows * 32; e += kThreads) {
       const int r = e >> 5, d = (e & 31) * 4;
       float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kKvWarps; ++w) {
+      for (int w = 0; w < W; ++w) {
         const float f = sm.f[w][r];
         const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(&sm.ring[w][0][0]) +
                                                           r * (kKvD + 4) + d);
@@ -671,16 +688,16 @@ size_t core_place(KvArgs& a, const KvPlan& p, bool stat, uint8_t* ws) {
   return o;
 }
 
-template <int MASK, bool SCORES, int NT>
+template <int MASK, bool SCORES, int NT, int W>
 cudaError_t launch_core_nt(const KvArgs& a, int device, cudaStream_t s) {
   static int configured[128] = {0};
-  cudaError_t e =
-      ensure_smem((const void*)kv_attention_kernel<MASK, SCORES, NT>, configured, device, sizeof(KvSmem<NT>), false);
+  cudaError_t e = ensure_smem((const void*)kv_attention_kernel<MASK, SCORES, NT, W>, configured, device,
+                              sizeof(KvSmem<NT, W>), W == 4);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
   cudaLaunchConfig_t cfg =
-      kv_cfg(dim3((unsigned)(a.split ? kKvGrid : a.units)), dim3(kKvThreads), sizeof(KvSmem<NT>), s, attr);
-  return cudaLaunchKernelEx(&cfg, kv_attention_kernel<MASK, SCORES, NT>, a);
+      kv_cfg(dim3((unsigned)(a.split ? kKvGrid : a.units)), dim3(W * 32), sizeof(KvSmem<NT, W>), s, attr);
+  return cudaLaunchKernelEx(&cfg, kv_attention_kernel<MASK, SCORES, NT, W>, a);
 }
 template <int MASK, bool SCORES>
 cudaError_t launch_core(const KvArgs& a, float* weight, int device, cudaStream_t s) {
@@ -688,7 +705,9 @@ cudaError_t launch_core(const KvArgs& a, float* weight, int device, cudaStream_t
   if (!SCORES && MASK != kMaskBlocks && a.rows == kKvTileRows)
     return launch_kv_tile(a, MASK, device, s);
   else
-    e = a.rows == 8 ? launch_core_nt<MASK, SCORES, 1>(a, device, s) : launch_core_nt<MASK, SCORES, 2>(a, device, s);
+    e = a.rows != 8 ? launch_core_nt<MASK, SCORES, 2, kKvWarps>(a, device, s)
+        : a.split   ? launch_core_nt<MASK, SCORES, 1, kKvWarps>(a, device, s)
+                    : launch_core_nt<MASK, SCORES, 1, 4>(a, device, s);
   if (e != cudaSuccess || (!a.split && !SCORES)) return e;
   const unsigned ranges =
       SCORES ? (unsigned)((a.max_t + kKvWeightKeys * a.weight_reps - 1) / (kKvWeightKeys * a.weight_reps)) : 0u;

@@ -10,8 +10,7 @@ namespace q8lin {
 constexpr int kKvD = 128;       // head width
 constexpr int kKvMaxRows = 16;  // query rows of a unit: 8 or 16
 constexpr int kKvChunk = 16;    // keys of a chunk: one warp's step
-constexpr int kKvWarps = 8;
-constexpr int kKvThreads = kKvWarps * 32;
+constexpr int kKvWarps = 8;     // warps of a CTA that shares its SM with no other
 constexpr int kKvSlots = 3;     // half chunks (16 keys or 16 values) of a warp's ring
 constexpr int kKvHalf = kKvChunk * kKvD * 4;
 constexpr int kKvGrid = 148;    // CTAs that share the chunks of all units (one per SM)
@@ -86,16 +85,13 @@ __device__ __forceinline__ KvUnit kv_unit(const KvArgs& a, int u) {
   return x;
 }
 
-// First key of chunk c of the unit.
+// First key of chunk c of the unit; `list`: the unit's chosen blocks.
 template <int MASK>
-__device__ __forceinline__ int kv_chunk_key(const KvArgs& a, const KvUnit& x, int c) {
+__device__ __forceinline__ int kv_chunk_key(const KvArgs& a, const KvUnit& x, const int* list, int c) {
   if (MASK != kMaskBlocks) return c * kKvChunk;
   const int per = a.block / kKvChunk;
   const int nb = c / per;
-  if (nb < x.picked) {
-    const int blk = a.index[(((size_t)x.b * a.n + x.i0) * a.hkv + x.hk) * a.topk + nb];
-    return blk * a.block + (c - nb * per) * kKvChunk;
-  }
+  if (nb < x.picked) return list[nb] * a.block + (c - nb * per) * kKvChunk;
   return (x.keys - 1) / a.block * a.block + (c - x.picked * per) * kKvChunk;
 }
 
