@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 2 : 1) kv_attention_kernel(co
   pdl_wait();
   pdl_launch_dependents();  // the merge waits for this grid before it reads anything
 
-  int u, off, left;
+  int u, off, left;  // left: chunks to take
   if (a.split) {
     left = kv_find<MASK, kThreads>(a, sm.find, blockIdx.x);
     u = sm.find.unit;
@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 2 : 1) kv_attention_kernel(co
     off = 0;
     left = 0x7fffffff;
   }
+  const int quota = left;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(&sm.ring[warp][0][0]);
 
   while (u < a.units && left > 0) {
@@ -127,14 +128,10 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 2 : 1) kv_attention_kernel(co
           for (int r = 0; r < kKvChunk; ++r)
             cp_async16(dst + r * (kKvD * 4) + ((lane ^ (val ? (r & 3) << 1 : (r & 1) << 2)) << 4), src + r * kKvD);
         } else {
+          const uint32_t rows = kv_rows_there<MASK>(a, x, j0);
 #pragma unroll 4
           for (int r = 0; r < kKvChunk; ++r) {
-            const int j = j0 + r;
-            bool there = j < x.keys;
-            if (MASK == kMaskTree && j >= x.p) {
-              const int e = j - x.p;  // a row no node was written to must not reach the sums
-              there = there && e < a.n && ((a.anc[((size_t)x.b * a.n + e) * a.words + (e >> 5)] >> (e & 31)) & 1u);
-            }
+            const bool there = (rows >> r) & 1u;
             cp_async16_zfill(dst + r * (kKvD * 4) + ((lane ^ (val ? (r & 3) << 1 : (r & 1) << 2)) << 4),
                              there ? src + r * kKvD : kb, there);
           }
@@ -178,6 +175,14 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 2 : 1) kv_attention_kernel(co
     int slot = 0;
     for (int h = 0; h < halves; h += 2) {
       const int j0 = kv_chunk_key<MASK>(a, x, list, c0 + (h >> 1) * W);
+      const bool masked = j0 + kKvChunk > open;
+      uint32_t see[NT];  // the keys that rows 2t (lower half) and 2t + 1 see, while the copies arrive
+      if (masked) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          see[nt] = __byte_perm(kv_sees<MASK>(a, x, nt * 8 + 2 * t, j0), kv_sees<MASK>(a, x, nt * 8 + 2 * t + 1, j0),
+                                0x5410) >> g;
+      }
       cp_async_wait(2);
       __syncwarp();
       // Scores: a lane takes dimensions 16 pair + 4t + e of keys g and g + 8.  The tensor cores
@@ -221,7 +226,6 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 2 : 1) kv_attention_kernel(co
       load(h + 3, slot);  // the keys are in registers: their slot is free
       slot = slot == kKvSlots - 1 ? 0 : slot + 1;
 
-      const bool masked = j0 + kKvChunk > open;
       float fac[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -232,10 +236,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 2 : 1) kv_attention_kernel(co
           const float low =
               __fadd_rn(__fadd_rn(cross[nt][0][e], cross[nt][1][e]), __fadd_rn(cross[nt][2][e], cross[nt][3][e]));
           p[e] = __fmul_rn(__fadd_rn(big, low), a.c);
-          if (masked) {
-            const int j = j0 + g + (e >> 1) * 8;
-            if (j >= x.keys || !kv_sees<MASK>(a, x, nt * 8 + 2 * t + (e & 1), j)) p[e] = -INFINITY;
-          }
+          if (masked && !((see[nt] >> ((e & 1) * 16 + (e >> 1) * 8)) & 1u)) p[e] = -INFINITY;
         }
         if (SCORES) {
           float* sc = a.scores + ((size_t)x.b * a.hkv + x.hk) * x.nrows * (size_t)a.score_stride + j0 + g;
@@ -381,6 +382,8 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 2 : 1) kv_attention_kernel(co
     __syncthreads();
     const size_t slot_id = a.split ? (size_t)blockIdx.x + u : (size_t)u;
     const bool whole = off == 0 && c1 == x.chunks;
+    if (a.split && off == 0 && tid == 0)  // for the merge: the first CTA, and how many there are
+      a.begun[u] = make_int2(blockIdx.x, 1 + (x.chunks - c1 + quota - 1) / quota);
     if (tid < x.nrows) {
       float M = -INFINITY, L = 0.0f;
 #pragma unroll
@@ -441,7 +444,6 @@ constexpr int kKvMergeThreads = 128;
 constexpr int kKvWeightKeys = kKvMergeThreads;  // one key a thread at a time
 template <int MASK, bool SCORES>
 __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs a, float* __restrict__ weight) {
-  __shared__ int red[kKvMergeThreads / 32][2];
   __shared__ float fac[kKvGrid], lse[kKvMaxRows], rm[kKvMergeThreads / 32], rl[kKvMergeThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, u = blockIdx.x;
   pdl_launch_dependents();
@@ -462,28 +464,9 @@ __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs 
   size_t slot0 = u;
   int parts = 1;
   if (a.split) {
-    int before = 0, total = 0;
-    for (int i = tid; i < a.units; i += kKvMergeThreads) {
-      const int c = kv_unit<MASK>(a, i).chunks;
-      total += c;
-      if (i < u) before += c;
-    }
-    total = __reduce_add_sync(kFull, total);
-    before = __reduce_add_sync(kFull, before);
-    if (lane == 0) {
-      red[warp][0] = total;
-      red[warp][1] = before;
-    }
-    __syncthreads();
-    total = before = 0;
-    for (int w = 0; w < kKvMergeThreads / 32; ++w) {
-      total += red[w][0];
-      before += red[w][1];
-    }
-    const int quota = max((total + kKvGrid - 1) / kKvGrid, a.least);
-    const int c0 = before / quota;
-    slot0 = (size_t)c0 + u;
-    parts = (before + x.chunks - 1) / quota - c0 + 1;
+    const int2 d = a.begun[u];
+    slot0 = (size_t)d.x + u;
+    parts = d.y;
   }
   const float* stat = a.stat + slot0 * 2 * a.rows;
   if (merging) {
@@ -665,8 +648,12 @@ KvPlan kv_plan(int64_t lists, int64_t rows_per_list, bool tile) {
   p.slots = !p.split ? (size_t)p.units : p.rows == kKvTileRows ? (size_t)(2 * kKvGrid) : (size_t)(kKvGrid + p.units);
   return p;
 }
+size_t begun_bytes(const KvPlan& p) {
+  return (p.rows == kKvTileRows ? (size_t)kKvGrid : (size_t)p.units) * sizeof(int2);
+}
 size_t core_bytes(const KvPlan& p, bool stat) {
-  return (p.split ? up256(p.slots * p.rows * kKvD * 4) : 0) + (p.split || stat ? up256(p.slots * 2 * p.rows * 4) : 0);
+  return (p.split ? up256(p.slots * p.rows * kKvD * 4) + up256(begun_bytes(p)) : 0) +
+         (p.split || stat ? up256(p.slots * 2 * p.rows * 4) : 0);
 }
 // Sets the core's part of the workspace; returns the bytes it takes.
 size_t core_place(KvArgs& a, const KvPlan& p, bool stat, uint8_t* ws) {
@@ -674,6 +661,8 @@ size_t core_place(KvArgs& a, const KvPlan& p, bool stat, uint8_t* ws) {
   if (p.split) {
     a.acc = reinterpret_cast<float*>(ws);
     o += up256(p.slots * p.rows * kKvD * 4);
+    a.begun = reinterpret_cast<int2*>(ws + o);
+    o += up256(begun_bytes(p));
   }
   if (p.split || stat) {
     a.stat = reinterpret_cast<float*>(ws + o);

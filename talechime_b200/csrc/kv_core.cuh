@@ -30,6 +30,7 @@ struct KvArgs {
   float* acc;             // [slot][rows][128] unnormalised sums of a unit's part
   float* stat;            // [slot][2][rows] its maxima and sums
   float* scores;          // causal with weights, n * group <= 16: [batch][hkv][n * group][score_stride]
+  int2* begun;            // split: where a unit's parts are, for the merge
   float* lse;             // causal with weights, else: [batch][hkv][n * group] log2 of the row's sum
   int batch, n, hq, hkv, group, max_t;
   int words, topk, block, score_stride;
@@ -115,16 +116,34 @@ __device__ __forceinline__ bool kv_row_valid(const KvArgs& a, const KvUnit& x, i
   if (MASK == kMaskTree) return (a.anc[((size_t)x.b * a.n + i) * a.words + (i >> 5)] >> (i & 31)) & 1u;
   return true;
 }
+// Bit e: does row r see key j + e (e < 32).  Two independent loads at most: a loop over the words,
+// or a look per key, is a chain of L2 latencies in front of the unit's last chunk.
 template <int MASK>
-__device__ __forceinline__ bool kv_sees(const KvArgs& a, const KvUnit& x, int r, int j) {
+__device__ __forceinline__ uint32_t kv_sees(const KvArgs& a, const KvUnit& x, int r, int j) {
   const int i = kv_token<MASK>(a, x, min(r, x.nrows - 1));
   if (MASK == kMaskTree) {
-    const int e = j - x.p;
-    if (e < 0) return true;
-    if (e >= a.n) return false;
-    return (a.anc[((size_t)x.b * a.n + i) * a.words + (e >> 5)] >> (e & 31)) & 1u;
+    const int e0 = j - x.p;  // node number of key j
+    if (e0 <= -32) return ~0u;
+    const uint32_t* anc = a.anc + ((size_t)x.b * a.n + i) * a.words;
+    const int w = e0 >> 5;  // -1: keys before the tree, which all rows see
+    const uint32_t lo = w < 0 ? ~0u : w < a.words ? anc[w] : 0u;
+    const uint32_t hi = w + 1 < a.words ? anc[w + 1] : 0u;
+    return __funnelshift_r(lo, hi, e0 & 31);
   }
-  return j <= x.p + i;
+  const int lim = min(x.p + i + 1, x.keys) - j;
+  return lim >= 32 ? ~0u : lim <= 0 ? 0u : (1u << lim) - 1;
+}
+// Bit e: is there a cache row j + e (e < 32); a tree's row that no node was written to is none, and
+// must not reach the sums.  By whole warps, a lane per row.
+template <int MASK>
+__device__ __forceinline__ uint32_t kv_rows_there(const KvArgs& a, const KvUnit& x, int j) {
+  j += threadIdx.x & 31;
+  bool there = j < x.keys;
+  if (MASK == kMaskTree && there && j >= x.p) {
+    const int e = j - x.p;
+    there = e < a.n && ((a.anc[((size_t)x.b * a.n + e) * a.words + (e >> 5)] >> (e & 31)) & 1u);
+  }
+  return __ballot_sync(kFull, there);
 }
 
 struct KvFind {

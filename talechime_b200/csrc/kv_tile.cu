@@ -93,6 +93,7 @@ struct KtSmem {
   KtCursor cursor[8];                  // the softmax warps' (registers are short there)
   alignas(16) float turn[2][4][32][36];  // rows of four warps: coalesced memory <-> a thread per row
   KvFind find;
+  int quota;                           // split: tiles a CTA takes
   uint32_t tmem;
   int abort;
 };
@@ -262,14 +263,6 @@ __device__ __forceinline__ float4 ld_row(const float4* p) {
 }
 
 template <int MASK>
-__device__ __forceinline__ bool kt_row_there(const KvArgs& a, const KvUnit& x, int j) {
-  if (j >= x.keys) return false;
-  if (MASK != kMaskTree || j < x.p) return true;
-  const int e = j - x.p;
-  return e < a.n && ((a.anc[((size_t)x.b * a.n + e) * a.words + (e >> 5)] >> (e & 31)) & 1u);
-}
-
-template <int MASK>
 __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, uint64_t wait_ns) {
   extern __shared__ uint8_t kt_raw[];
   // aligned by an offset, not by a cast, so that the compiler keeps seeing shared memory
@@ -308,6 +301,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
     start.left = kv_find<MASK, kKtThreads>(a, sm.find, blockIdx.x);
     start.u = sm.find.unit;
     start.off = sm.find.off;
+    if (tid == 0) sm.quota = start.left;
   } else {
     start.left = 0x7fffffff;
     start.u = blockIdx.x;
@@ -352,9 +346,10 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
 #pragma unroll
             for (int i = 0; i < 8; ++i) nx[i] = ld_row(row + i * 32);
           } else {
+            const uint32_t there = kv_rows_there<MASK>(a, x, j0);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              nx[i] = kt_row_there<MASK>(a, x, j0 + i) ? ld_row(row + i * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+              nx[i] = (there >> i) & 1u ? ld_row(row + i * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
           }
         } else {
           const float4* row = kp + (size_t)j0 * (kKvD / 4);
@@ -365,9 +360,10 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
               nx[2 * i + 1] = ld_row(row + i * 64 + 16);
             }
           } else {
+            const uint32_t rows = kv_rows_there<MASK>(a, x, j0) >> ky;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const bool there = kt_row_there<MASK>(a, x, j0 + ky + 2 * i);
+              const bool there = (rows >> (2 * i)) & 1u;
               nx[2 * i] = there ? ld_row(row + i * 64) : make_float4(0.f, 0.f, 0.f, 0.f);
               nx[2 * i + 1] = there ? ld_row(row + i * 64 + 16) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
@@ -556,6 +552,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       }
     KtCursor& cur = sm.cursor[warp];
     cur = start;
+    if (a.split && tid == 0) a.begun[blockIdx.x] = make_int2(-1, 0);
     for (bool more = cur.seek<MASK>(a); more; more = cur.next<MASK>(a)) {
       const KvUnit& x = cur.x;
       // half of the query row: scaled hi / lo to TMEM, dimensions in the order of the K tiles (32
@@ -667,6 +664,8 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       for (; t < tend; ++t) {
         const int s = t & 1;
         const uint32_t sat = mine + kTmS + 64 * s + 32 * half;
+        uint32_t see = ~0u;
+        if (t >= tmask) see = kv_sees<MASK>(a, x, row, (cur.off + t - cur.t0) * kKvTileKeys + 32 * half);
         wait(&sm.sfull[s], (t >> 1) & 1);
         tc_after();
         float cc[4];  // the factors of the thread's four groups of 8 keys
@@ -684,21 +683,6 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
           tm_ld32(sat, r);
           tm_wait_ld();
           if (t >= tmask) {
-            uint32_t see;
-            const int j = (cur.off + t - cur.t0) * kKvTileKeys + 32 * half;
-            const int token = kv_token<MASK>(a, x, min(row, x.nrows - 1));
-            if (MASK == kMaskTree) {
-              const int e0 = j - x.p;  // node number of the first
-              see = e0 <= -32 ? ~0u : e0 < 0 ? (1u << -e0) - 1 : 0u;
-              const uint32_t* anc = a.anc + ((size_t)x.b * a.n + token) * a.words;
-              for (int w = max(0, e0 >> 5); w < a.words && w * 32 - e0 < 32; ++w) {
-                const int sh = w * 32 - e0;
-                see |= sh >= 0 ? anc[w] << sh : anc[w] >> -sh;
-              }
-            } else {
-              const int lim = min(x.p + token + 1, x.keys) - j;
-              see = lim >= 32 ? ~0u : lim <= 0 ? 0u : (1u << lim) - 1;
-            }
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (!((see >> e) & 1u)) r[e] = 0xff800000u;  // -inf, back in TMEM for the second pass
@@ -820,6 +804,8 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       if (row < x.nrows) {
         if (half == 0) {
           if (!whole) {
+            if (row == 0 && cur.off == 0)  // for the merge: CTAs of quota tiles go on with the unit
+              a.begun[blockIdx.x] = make_int2(cur.u, 1 + (x.chunks - cur.n + sm.quota - 1) / sm.quota);
             a.stat[slot * 2 * a.rows + row] = m;
             a.stat[(slot * 2 + 1) * a.rows + row] = ok ? l * kUnscale : nan;
           }
@@ -839,48 +825,82 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
 
 // After a split: the parts of the units that more than one CTA worked on, in the order of the CTAs, and
 // zeros for units without keys.  A CTA has at most two parts: the rest of a unit that began before it (slot
-// 2 cta) and the beginning of one that ends after it (slot 2 cta + 1).  Block (c, y) merges rows 8 y
-// .. + 8 of the unit that CTA c began and did not end.
-constexpr int kKtMergeRows = 8;
+// 2 cta) and the beginning of one that ends after it (slot 2 cta + 1).  Block (c, y) merges rows 32 y
+// .. + 32 of the unit that CTA c began and did not end, four rows a warp with their loads in flight
+// together.
+constexpr int kKtMergeWarps = 8, kKtMergeEach = 4, kKtMergeRows = kKtMergeWarps * kKtMergeEach;
 template <int MASK>
-__global__ void __launch_bounds__(kKtMergeRows * 32) kv_tile_merge_kernel(const KvArgs a) {
-  __shared__ KvFind find;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y * kKtMergeRows + warp;
+__global__ void __launch_bounds__(kKtMergeWarps * 32) kv_tile_merge_kernel(const KvArgs a) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r0 = blockIdx.y * kKtMergeRows + warp * kKtMergeEach;
   pdl_launch_dependents();
   pdl_wait();
   for (int u = blockIdx.x; u < a.units; u += kKvGrid) {
     const KvUnit x = kv_unit<MASK>(a, u);
-    if (x.chunks > 0 || r >= x.nrows) continue;
-    reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, r))[lane] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (a.lse && lane == 0) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + r] = INFINITY;
+    if (x.chunks > 0) continue;
+    for (int r = r0; r < min(r0 + kKtMergeEach, x.nrows); ++r) {
+      reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, r))[lane] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (a.lse && lane == 0) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + r] = INFINITY;
+    }
   }
-  const int quota = kv_find<MASK, kKtMergeRows * 32>(a, find, blockIdx.x + 1);
-  const int u = find.unit, off = find.off;
-  if (u >= a.units || off == 0 || off > quota) return;  // nothing of CTA c's goes on in the next
-  const KvUnit x = kv_unit<MASK>(a, u);
-  if (r >= x.nrows) return;
-  const int parts = 1 + (x.chunks - off + quota - 1) / quota;
+  const int2 d = a.begun[blockIdx.x];
+  if (d.x < 0) return;  // nothing of CTA c's goes on in the next
+  const KvUnit x = kv_unit<MASK>(a, d.x);
+  if (r0 >= x.nrows) return;
+  const int parts = d.y;
   auto slot = [&](int s) { return 2 * ((size_t)blockIdx.x + s) + (s == 0 ? 1 : 0); };
-  float M = -INFINITY, L = 0.0f;
-  for (int s = lane; s < parts; s += 32) M = fmaxf(M, a.stat[slot(s) * 2 * a.rows + r]);
+  int row[kKtMergeEach];
+  float M[kKtMergeEach], L[kKtMergeEach];
+  float4 A[kKtMergeEach];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, o));
-  float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (M != -INFINITY) {
-#pragma unroll 4
-    for (int s = 0; s < parts; ++s) {
-      const float f = exp2f(a.stat[slot(s) * 2 * a.rows + r] - M), l = a.stat[(slot(s) * 2 + 1) * a.rows + r];
-      const float4 v = reinterpret_cast<const float4*>(a.acc + (slot(s) * a.rows + r) * kKvD)[lane];
-      if (f != 0.0f) {  // an empty part's sums are 0, and stay out
-        L = fmaf(l, f, L);
-        A = make_float4(fmaf(v.x, f, A.x), fmaf(v.y, f, A.y), fmaf(v.z, f, A.z), fmaf(v.w, f, A.w));
+  for (int i = 0; i < kKtMergeEach; ++i) {
+    row[i] = min(r0 + i, x.nrows - 1);
+    M[i] = -INFINITY;
+    L[i] = 0.0f;
+    A[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  for (int s = lane; s < parts; s += 32)
+#pragma unroll
+    for (int i = 0; i < kKtMergeEach; ++i) M[i] = fmaxf(M[i], a.stat[slot(s) * 2 * a.rows + row[i]]);
+#pragma unroll
+  for (int i = 0; i < kKtMergeEach; ++i)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M[i] = fmaxf(M[i], __shfl_xor_sync(kFull, M[i], o));
+  for (int s0 = 0; s0 < parts; s0 += 32) {  // a lane per part for the factors, then a part at a time
+    float f[kKtMergeEach];
+    const int s1 = s0 + lane;
+#pragma unroll
+    for (int i = 0; i < kKtMergeEach; ++i) {
+      f[i] = 0.0f;
+      if (s1 < parts && M[i] != -INFINITY) {
+        f[i] = exp2f(a.stat[slot(s1) * 2 * a.rows + row[i]] - M[i]);
+        if (f[i] != 0.0f) L[i] = fmaf(a.stat[(slot(s1) * 2 + 1) * a.rows + row[i]], f[i], L[i]);
       }
     }
-    A = make_float4(__fdiv_rn(A.x, L), __fdiv_rn(A.y, L), __fdiv_rn(A.z, L), __fdiv_rn(A.w, L));
+    const int n = min(32, parts - s0);
+#pragma unroll 2
+    for (int s = 0; s < n; ++s) {
+      const float* acc = a.acc + slot(s0 + s) * a.rows * kKvD;
+#pragma unroll
+      for (int i = 0; i < kKtMergeEach; ++i) {
+        const float4 v = reinterpret_cast<const float4*>(acc + row[i] * kKvD)[lane];
+        const float fs = __shfl_sync(kFull, f[i], s);
+        if (fs != 0.0f)  // an empty part's sums stay out
+          A[i] = make_float4(fmaf(v.x, fs, A[i].x), fmaf(v.y, fs, A[i].y), fmaf(v.z, fs, A[i].z), fmaf(v.w, fs, A[i].w));
+      }
+    }
   }
-  reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, r))[lane] = A;
-  if (a.lse && lane == 0)
-    a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + r] = M == -INFINITY ? INFINITY : M + log2f(L);
+#pragma unroll
+  for (int i = 0; i < kKtMergeEach; ++i) {
+    const float sum = warp_sum(L[i]);
+    if (r0 + i >= x.nrows) break;
+    if (M[i] != -INFINITY)
+      A[i] = make_float4(__fdiv_rn(A[i].x, sum), __fdiv_rn(A[i].y, sum), __fdiv_rn(A[i].z, sum), __fdiv_rn(A[i].w, sum));
+    reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, row[i]))[lane] = A[i];
+    if (a.lse && lane == 0)
+      a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row[i]] =
+          M[i] == -INFINITY ? INFINITY : M[i] + log2f(sum);
+  }
 }
 
 // ---------------------------------------------------------------------------------
@@ -1171,7 +1191,7 @@ cudaError_t launch_tile(const KvArgs& a, int device, cudaStream_t s) {
   if (e != cudaSuccess || !a.split) return e;
   const int rows = a.units > a.batch * a.hkv ? kKvTileRows : a.n * a.group;  // of the largest unit
   cfg.gridDim = dim3(kKvGrid, (unsigned)((rows + kKtMergeRows - 1) / kKtMergeRows));
-  cfg.blockDim = dim3(kKtMergeRows * 32);
+  cfg.blockDim = dim3(kKtMergeWarps * 32);
   cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, kv_tile_merge_kernel<MASK>, a);
 }
