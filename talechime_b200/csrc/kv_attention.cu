@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 2 : 1) kv_attention_kernel(co
     off = 0;
     left = 0x7fffffff;
   }
-  const int quota = left;
+  const int quota = a.split ? sm.find.quota : left;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(&sm.ring[warp][0][0]);
 
   while (u < a.units && left > 0) {
@@ -176,8 +176,8 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 2 : 1) kv_attention_kernel(co
     for (int h = 0; h < halves; h += 2) {
       const int j0 = kv_chunk_key<MASK>(a, x, list, c0 + (h >> 1) * W);
       const bool masked = j0 + kKvChunk > open;
-      uint32_t see[NT];  // the keys that rows 2t (lower half) and 2t + 1 see, while the copies arrive
-      if (masked) {
+      uint32_t see[NT];  // tree: the keys that rows 2t (lower half) and 2t + 1 see, loaded beside the copies
+      if (MASK == kMaskTree && masked) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           see[nt] = __byte_perm(kv_sees<MASK>(a, x, nt * 8 + 2 * t, j0), kv_sees<MASK>(a, x, nt * 8 + 2 * t + 1, j0),
@@ -236,7 +236,12 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 2 : 1) kv_attention_kernel(co
           const float low =
               __fadd_rn(__fadd_rn(cross[nt][0][e], cross[nt][1][e]), __fadd_rn(cross[nt][2][e], cross[nt][3][e]));
           p[e] = __fmul_rn(__fadd_rn(big, low), a.c);
-          if (masked && !((see[nt] >> ((e & 1) * 16 + (e >> 1) * 8)) & 1u)) p[e] = -INFINITY;
+          if (masked) {
+            const int j = j0 + g + (e >> 1) * 8;
+            if (MASK == kMaskTree ? !((see[nt] >> ((e & 1) * 16 + (e >> 1) * 8)) & 1u)
+                                  : j >= min(x.keys, x.p + kv_token<MASK>(a, x, min(nt * 8 + 2 * t + (e & 1), x.nrows - 1)) + 1))
+              p[e] = -INFINITY;
+          }
         }
         if (SCORES) {
           float* sc = a.scores + ((size_t)x.b * a.hkv + x.hk) * x.nrows * (size_t)a.score_stride + j0 + g;
@@ -670,7 +675,9 @@ size_t core_place(KvArgs& a, const KvPlan& p, bool stat, uint8_t* ws) {
   }
   a.rows = p.rows;
   a.chunk = p.rows == kKvTileRows ? kKvTileKeys : kKvChunk;
-  a.least = p.rows == kKvTileRows ? 2 : kKvWarps;
+  a.each = p.units < kKvGrid ? (int)(kKvGrid / p.units) : 0;
+  a.least = kKvLeast;
+  a.pass = kKvPass;
   a.rgs = p.rgs;
   a.units = (int)p.units;
   a.split = p.split ? 1 : 0;

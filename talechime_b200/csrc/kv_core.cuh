@@ -16,6 +16,10 @@ constexpr int kKvHalf = kKvChunk * kKvD * 4;
 constexpr int kKvGrid = 148;    // CTAs that share the chunks of all units (one per SM)
 constexpr int kKvTileRows = 128;  // query rows of a unit of the tcgen05 kernel
 constexpr int kKvTileKeys = 64;   // keys of its tiles
+// Chunks a CTA takes at least, and chunks that take as long as starting on a unit: about 5 us
+// against 0.6 a chunk, and 9 us against 2.2 a tile.
+constexpr int kKvLeast = kKvWarps, kKvPass = kKvWarps;
+constexpr int kKvTileLeast = 2, kKvTilePass = 4;
 
 enum KvMask : int { kMaskCausal = 0, kMaskTree = 1, kMaskBlocks = 2 };
 
@@ -37,6 +41,8 @@ struct KvArgs {
   int rows;               // rows of a unit: 8, 16 or 128
   int chunk;              // keys of a chunk: 16, or 64 with units of 128 rows
   int least;              // chunks a CTA takes at least
+  int each;               // CTAs for every unit (0: not one for each)
+  int pass;               // chunks that take as long as starting on a unit
   int rgs;                // row groups of a kv head (tree, causal) or of a token (blocks)
   int units;
   int weight_reps;        // scores stored: groups of 128 keys a CTA of the merge adds the weights of
@@ -147,53 +153,91 @@ __device__ __forceinline__ uint32_t kv_rows_there(const KvArgs& a, const KvUnit&
 }
 
 struct KvFind {
-  int seg[32];  // chunk sums of the warps
-  int unit, off;
+  int sum[32], top[32], before[32];  // of the warps
+  int unit, off, left, quota;
 };
 
-// Where CTA `cta` of the shared split starts: fills unit / off and returns the chunk
-// count of one CTA (the whole work when it does not reach this CTA: unit = units).
+// The split of all units' chunks over the kKvGrid CTAs: fills what CTA `cta` starts with (unit =
+// units: nothing) and the chunks of a CTA's share, and returns those that CTA `cta` takes.
+// Evenly, a CTA takes quota chunks wherever they lie and so begins a second unit in most cases; or
+// every unit gets CTAs of its own, which then take up to `quota` chunks of it.  Starting on a
+// unit costs about a.pass chunks' time (query rows, first copies, joining the parts), so units
+// get their own CTAs where that adds at most a.pass chunks to the share.  (Trees of 64 nodes x 8 heads
+// behind 200 rows 32.6 us evenly, 27.5 so; 5 ragged trees of 33 nodes 45.2 and 38.4; 16 heads of 16 K
+// rows 70.2 and 62.1.  64 units of 122 tiles stay even: 53 tiles to a CTA, not 64.)
 template <int MASK, int THREADS>
 __device__ int kv_find(const KvArgs& a, KvFind& sm, int cta) {
-  const int tid = threadIdx.x;
-  const int per = (a.units + THREADS - 1) / THREADS;
-  const int u0 = min(a.units, tid * per), u1 = min(a.units, u0 + per);
-  int mine = 0;
-  for (int u = u0; u < u1; ++u) mine += kv_unit<MASK>(a, u).chunks;
-  int upto = mine;  // chunks of this thread's units and of those before them
+  constexpr int kPer = (2 * kKvGrid + THREADS - 1) / THREADS;  // more units are not split
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int c[kPer], sum = 0, top = 0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(kFull, upto, o);
-    if ((tid & 31) >= o) upto += v;
+  for (int i = 0; i < kPer; ++i) {
+    c[i] = tid * kPer + i < a.units ? kv_unit<MASK>(a, tid * kPer + i).chunks : 0;
+    sum += c[i];
+    top = max(top, c[i]);
   }
-  if ((tid & 31) == 31) sm.seg[tid >> 5] = upto;
+  sum = __reduce_add_sync(kFull, sum);
+  top = __reduce_max_sync(kFull, top);
+  if (lane == 0) {
+    sm.sum[warp] = sum;
+    sm.top[warp] = top;
+  }
   if (tid == 0) {
     sm.unit = a.units;
     sm.off = 0;
+    sm.left = 0;
   }
   __syncthreads();
-  int total = 0;
+  sum = top = 0;
 #pragma unroll
   for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < (tid >> 5)) upto += sm.seg[w];
-    total += sm.seg[w];
+    sum += sm.sum[w];
+    top = max(top, sm.top[w]);
   }
-  const int quota = max((total + kKvGrid - 1) / kKvGrid, a.least);
-  const int start = cta * quota;
-  if (upto - mine <= start && start < upto) {
-    int at = upto - mine;
-    for (int u = u0; u < u1; ++u) {
-      const int c = kv_unit<MASK>(a, u).chunks;
-      if (start < at + c) {
-        sm.unit = u;
-        sm.off = start - at;
-        break;
-      }
-      at += c;
+  int quota = max((sum + kKvGrid - 1) / kKvGrid, a.least);
+  bool own = false;
+  if (a.each > 0) {
+    // a share for which the units' CTAs are no more than there are
+    const int spare = kKvGrid - a.units;
+    const int q = max(min((top + a.each - 1) / a.each, (sum + spare - 1) / spare), a.least);
+    if (q <= quota + a.pass) {
+      own = true;
+      quota = q;
     }
   }
+  // before a unit: the CTAs that the ones in front of it get, or their chunks
+  int w[kPer], upto = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    w[i] = own ? (c[i] + quota - 1) / quota : c[i];
+    upto += w[i];
+  }
+  int at = -upto;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(kFull, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) sm.before[warp] = upto;
   __syncthreads();
-  return quota;
+#pragma unroll
+  for (int v = 0; v < THREADS / 32; ++v)
+    if (v < warp) upto += sm.before[v];
+  at += upto;
+  const int start = own ? cta : cta * quota;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (at <= start && start < at + w[i]) {
+      const int off = own ? (start - at) * quota : start - at;
+      sm.unit = tid * kPer + i;
+      sm.off = off;
+      sm.left = own ? min(quota, c[i] - off) : quota;
+    }
+    at += w[i];
+  }
+  if (tid == 0) sm.quota = quota;
+  __syncthreads();
+  return sm.left;
 }
 
 }  // namespace q8lin

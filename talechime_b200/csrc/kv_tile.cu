@@ -93,7 +93,6 @@ struct KtSmem {
   KtCursor cursor[8];                  // the softmax warps' (registers are short there)
   alignas(16) float turn[2][4][32][36];  // rows of four warps: coalesced memory <-> a thread per row
   KvFind find;
-  int quota;                           // split: tiles a CTA takes
   uint32_t tmem;
   int abort;
 };
@@ -262,6 +261,27 @@ __device__ __forceinline__ float4 ld_row(const float4* p) {
   return make_float4(__int_as_float(v.x), __int_as_float(v.y), __int_as_float(v.z), __int_as_float(v.w));
 }
 
+// kv_find as a call of its own, on the fields it needs: inlined, its values stay in the roles' way
+// (64-node trees 182 us instead of 165), and KvArgs by reference or value goes through memory.
+template <int MASK>
+__device__ __noinline__ int kt_find(KvFind& find, const int* pos, int n, int hkv, int group, int max_t, int rgs,
+                                    int units, int each) {
+  KvArgs a = {};
+  a.pos = pos;
+  a.n = n;
+  a.hkv = hkv;
+  a.group = group;
+  a.max_t = max_t;
+  a.rgs = rgs;
+  a.units = units;
+  a.each = each;
+  a.rows = kKvTileRows;
+  a.chunk = kKvTileKeys;
+  a.least = kKvTileLeast;
+  a.pass = kKvTilePass;
+  return kv_find<MASK, kKtThreads>(a, find, blockIdx.x);
+}
+
 template <int MASK>
 __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, uint64_t wait_ns) {
   extern __shared__ uint8_t kt_raw[];
@@ -298,10 +318,9 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
   pdl_launch_dependents();
   KtCursor start;
   if (a.split) {
-    start.left = kv_find<MASK, kKtThreads>(a, sm.find, blockIdx.x);
+    start.left = kt_find<MASK>(sm.find, a.pos, a.n, a.hkv, a.group, a.max_t, a.rgs, a.units, a.each);
     start.u = sm.find.unit;
     start.off = sm.find.off;
-    if (tid == 0) sm.quota = start.left;
   } else {
     start.left = 0x7fffffff;
     start.u = blockIdx.x;
@@ -664,8 +683,9 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       for (; t < tend; ++t) {
         const int s = t & 1;
         const uint32_t sat = mine + kTmS + 64 * s + 32 * half;
-        uint32_t see = ~0u;
-        if (t >= tmask) see = kv_sees<MASK>(a, x, row, (cur.off + t - cur.t0) * kKvTileKeys + 32 * half);
+        uint32_t see;
+        auto look = [&]() { see = kv_sees<MASK>(a, x, row, (cur.off + t - cur.t0) * kKvTileKeys + 32 * half); };
+        if (MASK == kMaskTree && t >= tmask) look();  // its loads beside the wait
         wait(&sm.sfull[s], (t >> 1) & 1);
         tc_after();
         float cc[4];  // the factors of the thread's four groups of 8 keys
@@ -683,6 +703,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
           tm_ld32(sat, r);
           tm_wait_ld();
           if (t >= tmask) {
+            if (MASK != kMaskTree) look();
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (!((see >> e) & 1u)) r[e] = 0xff800000u;  // -inf, back in TMEM for the second pass
@@ -805,7 +826,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         if (half == 0) {
           if (!whole) {
             if (row == 0 && cur.off == 0)  // for the merge: CTAs of quota tiles go on with the unit
-              a.begun[blockIdx.x] = make_int2(cur.u, 1 + (x.chunks - cur.n + sm.quota - 1) / sm.quota);
+              a.begun[blockIdx.x] = make_int2(cur.u, 1 + (x.chunks - cur.n + sm.find.quota - 1) / sm.find.quota);
             a.stat[slot * 2 * a.rows + row] = m;
             a.stat[(slot * 2 + 1) * a.rows + row] = ok ? l * kUnscale : nan;
           }
