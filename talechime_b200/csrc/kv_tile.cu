@@ -54,16 +54,16 @@ struct KtCursor {
   int n;             // tiles of the unit here
   int t0 = 0;        // tiles of the CTA before it
   KvUnit x;
-  template <int MASK>
-  __device__ static KvUnit in_order(const KvArgs& a, int k) {
+  // Unit k of the order without a split.
+  __device__ static int in_order(const KvArgs& a, int k) {
     const int lists = a.units / a.rgs;
-    return kv_unit<MASK>(a, k % lists * a.rgs + a.rgs - 1 - k / lists);
+    return k % lists * a.rgs + a.rgs - 1 - k / lists;
   }
   // Moves to the first unit from u on with work; false when there is none.
   template <int MASK>
   __device__ bool seek(const KvArgs& a) {
     while (u < a.units && left > 0) {
-      x = a.split ? kv_unit<MASK>(a, u) : in_order<MASK>(a, u);
+      x = kv_unit<MASK>(a, a.split ? u : in_order(a, u));
       n = min(x.chunks - off, left);
       if (n > 0) return true;
       off = 0;
@@ -71,13 +71,11 @@ struct KtCursor {
     }
     return false;
   }
-  template <int MASK>
-  __device__ bool next(const KvArgs& a) {
+  __device__ void pass(const KvArgs& a) {  // to the unit behind
     if (a.split) left -= n;
     t0 += n;
     off = 0;
     u += a.split ? 1 : kKvGrid;
-    return seek<MASK>(a);
   }
 };
 
@@ -136,19 +134,37 @@ __device__ __forceinline__ uint64_t desc_sw128(const void* base) {
 }
 // kind::f16, f16 operands, f32 sums, M = 128.
 __host__ __device__ constexpr uint32_t kt_idesc(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
-// D (+)= A (TMEM) B^T (shared memory); called by a converged warp, one lane issues.
+// D (+)= A (TMEM) B^T (shared memory); by one lane.
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p, e;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
-      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
       ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// The lane that issues a warp's MMAs and commits.
+__device__ __forceinline__ bool elected() {
+  uint32_t e;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(e));
+  return e != 0;
+}
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile(
-      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
-      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(su32(bar))
-      : "memory");
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(su32(bar)) : "memory");
+}
+// D = A B^T over 16 STEPS columns as lo.hi + hi.lo + hi.hi; HALF: bytes from B's first 64 columns to
+// the next.  The three run through one piece of code: the roles' loops fill the instruction caches.
+template <int STEPS, int HALF>
+__device__ __forceinline__ void mma_pairs(uint32_t d, uint32_t ah, uint32_t al, const void* bh, const void* bl,
+                                          uint32_t idesc) {
+  const uint64_t dh = desc_sw128(bh), dl = desc_sw128(bl);
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const uint32_t a = pass == 0 ? al : ah;
+    const uint64_t b = pass == 1 ? dl : dh;
+#pragma unroll
+    for (int kk = 0; kk < STEPS; ++kk)
+      mma_ts(d, a + 8 * kk, b + 2 * (kk & 3) + (kk >> 2) * (HALF >> 4), idesc, pass + kk > 0);
+  }
 }
 
 #define KT_R32(a) \
@@ -338,7 +354,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
     const int h = lane & 15, ky = lane >> 4;
     KtCursor cur = start;
     bool dead = false;
-    for (bool more = cur.seek<MASK>(a); more; more = cur.next<MASK>(a)) {
+    for (; cur.seek<MASK>(a); cur.pass(a)) {
       const KvUnit& x = cur.x;
       const size_t head = ((size_t)x.b * a.hkv + x.hk) * (size_t)a.max_t;
       // lane's pieces of a row: K dimensions 4 h .. and 64 + 4 h .. of row 2 i + lane / 16, V
@@ -354,7 +370,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         return c < n ? c : -1;
       };
       auto is_v = [](int item) { return item >= 16 && !((item >> 3) & 1); };
-      float4 nx[8];
+      float4 nx[8] = {};
       auto load = [&](int item) {
         const int c = tile_of(item);
         if (c < 0) return;
@@ -389,13 +405,13 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
           }
         }
       };
-      int item = warp - kKtConvertWarp;
-      load(item);
-      for (; item < items; item += kKtConverters) {
+      // the first round only loads
+      for (int item = warp - kKtConvertWarp - kKtConverters; item < items; item += kKtConverters) {
         float4 r[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) r[i] = nx[i];
         if (item + kKtConverters < items) load(item + kKtConverters);
+        if (item < 0) continue;
         const int c = tile_of(item), g = item & 7;
         if (c < 0) continue;
         const int t = cur.t0 + c;
@@ -405,7 +421,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         if (!is_v(item)) {
           const int s = t & 1;
           unsigned top = __reduce_max_sync(kFull, __float_as_uint(m));
-          if (top >= 0x7f800000u) {  // an infinite key: the scale of the others
+          if (__builtin_expect(top >= 0x7f800000u, 0)) {  // an infinite key: the scale of the others
             m = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -445,7 +461,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
           }
           unsigned top = __reduce_max_sync(kFull, z.x + z.y == 0.0f ? __float_as_uint(m) : 0x7f800000u);
           unsigned bad = 0;
-          if (top >= 0x7f800000u) {
+          if (__builtin_expect(top >= 0x7f800000u, 0)) {
             // 0 * inf must not reach the rows that do not see the key: its value row leaves the
             // product (0) and the rows that see it add it one by one
             m = 0.0f;
@@ -499,53 +515,48 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
     // ---------------- MMA issue ----------------
     constexpr uint32_t id_qk = kt_idesc(kKvTileKeys), id_pv = kt_idesc(kKvD);
     bool ok = true;
-    int t = 0, units = 0;
-    auto issue_pv = [&](int w) {  // O = P V of tile w, once every warp wrote its P and has the O before
-      const int s = w & 1, vs = w % 3;
-      ok = ok && bar_wait(&sm.vfull[vs], (w / 3) & 1, abort);
-      ok = ok && bar_wait(&sm.pfull[s], (w >> 1) & 1, abort);
-      if (w > 0) ok = ok && bar_wait(&sm.ofree, (w - 1) & 1, abort);
-      if (!ok) return;
-      tc_after();
-      const uint64_t vh = desc_sw128(sm.v[vs][0]), vl = desc_sw128(sm.v[vs][1]);
-      const uint32_t ph = tmem + kTmP + 64 * s, pl = ph + 32, d = tmem + kTmO;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) mma_ts(d, pl + 8 * kk, vh + 2 * kk, id_pv, kk > 0);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) mma_ts(d, ph + 8 * kk, vl + 2 * kk, id_pv, 1);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) mma_ts(d, ph + 8 * kk, vh + 2 * kk, id_pv, 1);
-      mma_commit(&sm.vfree[vs]);
-      mma_commit(&sm.ofull);
-    };
+    int units = 0;
     KtCursor cur = start;
-    for (bool more = cur.seek<MASK>(a); ok && more; more = cur.next<MASK>(a), ++units) {
+    for (; ok && cur.seek<MASK>(a); cur.pass(a), ++units) {
       ok = bar_wait(&sm.qfull, units & 1, abort);
-      for (int i = 0; ok && i < cur.n; ++i, ++t) {
-        // S = Q K^T; its buffer is free: P of tile t - 2 was waited for
-        const int s = t & 1;
-        ok = bar_wait(&sm.kfull[s], (t >> 1) & 1, abort);
-        if (!ok) break;
-        if (lane == 0) bar_arrive(&sm.sfull[s]);  // passes on what the converters wrote beside the tile
-        tc_after();
-        const uint64_t kh0 = desc_sw128(sm.k[s][0][0]), kh1 = desc_sw128(sm.k[s][0][1]);
-        const uint64_t kl0 = desc_sw128(sm.k[s][1][0]), kl1 = desc_sw128(sm.k[s][1][1]);
-        const uint32_t qh = tmem + kTmQ, ql = qh + 64, d = tmem + kTmS + 64 * s;
-        __syncwarp();
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) mma_ts(d, ql + 8 * kk, (kk < 4 ? kh0 : kh1) + 2 * (kk & 3), id_qk, kk > 0);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) mma_ts(d, qh + 8 * kk, (kk < 4 ? kl0 : kl1) + 2 * (kk & 3), id_qk, 1);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) mma_ts(d, qh + 8 * kk, (kk < 4 ? kh0 : kh1) + 2 * (kk & 3), id_qk, 1);
-        mma_commit(&sm.kfree[s]);
-        mma_commit(&sm.sfull[s]);
-        if (i > 0) issue_pv(t - 1);
+      // step i: S of tile i, then O of the tile before
+      for (int i = 0; ok && i <= cur.n; ++i) {
+        if (i < cur.n) {
+          // S = Q K^T; its buffer is free: P of tile t - 2 was waited for
+          const int t = cur.t0 + i, s = t & 1;
+          ok = bar_wait(&sm.kfull[s], (t >> 1) & 1, abort);
+          if (!ok) break;
+          if (lane == 0) bar_arrive(&sm.sfull[s]);  // passes on what the converters wrote beside the tile
+          tc_after();
+          __syncwarp();
+          if (elected()) {
+            mma_pairs<8, sizeof(sm.k[0][0][0])>(tmem + kTmS + 64 * s, tmem + kTmQ, tmem + kTmQ + 64, sm.k[s][0][0],
+                                                sm.k[s][1][0], id_qk);
+            mma_commit(&sm.kfree[s]);
+            mma_commit(&sm.sfull[s]);
+          }
+          __syncwarp();
+        }
+        if (i > 0) {
+          // O = P V, once every warp wrote its P and has the O before
+          const int w = cur.t0 + i - 1, s = w & 1, vs = w % 3;
+          ok = bar_wait(&sm.vfull[vs], (w / 3) & 1, abort) && bar_wait(&sm.pfull[s], (w >> 1) & 1, abort) &&
+               (w == 0 || bar_wait(&sm.ofree, (w - 1) & 1, abort));
+          if (!ok) break;
+          tc_after();
+          __syncwarp();
+          if (elected()) {
+            mma_pairs<4, 0>(tmem + kTmO, tmem + kTmP + 64 * s, tmem + kTmP + 64 * s + 32, sm.v[vs][0], sm.v[vs][1], id_pv);
+            mma_commit(&sm.vfree[vs]);
+            mma_commit(&sm.ofull);
+          }
+          __syncwarp();
+        }
       }
-      issue_pv(t - 1);
     }
     // nothing of this CTA's may be at work in shared memory or TMEM when it ends
-    mma_commit(&sm.done);
+    if (elected()) mma_commit(&sm.done);
+    __syncwarp();
     mb_wait_ns(su32(&sm.done), 0, kDrainLimitNs, nullptr);
   } else {
     // ---------------- softmax, output ----------------
@@ -563,16 +574,17 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
     auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory"); };
     if (!a.split)  // units without keys have no tiles
       for (int u = blockIdx.x; u < a.units; u += kKvGrid) {
-        const KvUnit x = KtCursor::in_order<MASK>(a, u);
+        const KvUnit x = kv_unit<MASK>(a, KtCursor::in_order(a, u));
         if (x.chunks > 0 || row >= x.nrows || half > 0) continue;
         float4* dst = reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, row));
+#pragma unroll 1
         for (int i = 0; i < kKvD / 4; ++i) dst[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (a.lse) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] = INFINITY;
       }
     KtCursor& cur = sm.cursor[warp];
     cur = start;
     if (a.split && tid == 0) a.begun[blockIdx.x] = make_int2(-1, 0);
-    for (bool more = cur.seek<MASK>(a); more; more = cur.next<MASK>(a)) {
+    for (; cur.seek<MASK>(a); cur.pass(a)) {
       const KvUnit& x = cur.x;
       // half of the query row: scaled hi / lo to TMEM, dimensions in the order of the K tiles (32
       // half .. + 32 and 64 + 32 half .. + 32).  A thread that reads its own row takes 32 memory
@@ -655,6 +667,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         if (const unsigned long long bad = *reinterpret_cast<const unsigned long long*>(&sm.vbad[w & 3][0])) {
           const float2* vb = reinterpret_cast<const float2*>(
               a.v + (((size_t)x.b * a.hkv + x.hk) * (size_t)a.max_t + (size_t)(cur.off + w - cur.t0) * kKvTileKeys) * kKvD);
+#pragma unroll 1
           for (int key = 0; key < kKvTileKeys; ++key) {
             if (!((bad >> key) & 1)) continue;
             const uint32_t hi = tm_ld1(mine + kTmP + 64 * (w & 1) + (key >> 1));
@@ -680,7 +693,9 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         __syncwarp();
         if (lane == 0) bar_arrive(&sm.ofree);
       };
-      for (; t < tend; ++t) {
+      for (;; ++t) {
+        float next = 1.0f;
+        if (t < tend) {
         const int s = t & 1;
         const uint32_t sat = mine + kTmS + 64 * s + 32 * half;
         uint32_t see;
@@ -688,17 +703,13 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         if (MASK == kMaskTree && t >= tmask) look();  // its loads beside the wait
         wait(&sm.sfull[s], (t >> 1) & 1);
         tc_after();
-        float cc[4];  // the factors of the thread's four groups of 8 keys
-        {
-          const float4 k4 = *reinterpret_cast<const float4*>(&sm.ksc[t & 3][4 * half]);
-          const float cq = a.c * qinv;
-          cc[0] = fmaxf(cq * k4.x, 1.17549435e-38f);  // a factor of 0 would make NaN of -inf
-          cc[1] = fmaxf(cq * k4.y, 1.17549435e-38f);
-          cc[2] = fmaxf(cq * k4.z, 1.17549435e-38f);
-          cc[3] = fmaxf(cq * k4.w, 1.17549435e-38f);
-        }
+        const float cq = a.c * qinv;
+        constexpr float kLeastFactor = 1.17549435e-38f;  // a factor of 0 would make NaN of -inf
         float top = -INFINITY;
         {
+          const float4 k4 = *reinterpret_cast<const float4*>(&sm.ksc[t & 3][4 * half]);
+          const float cc[4] = {fmaxf(cq * k4.x, kLeastFactor), fmaxf(cq * k4.y, kLeastFactor),
+                               fmaxf(cq * k4.z, kLeastFactor), fmaxf(cq * k4.w, kLeastFactor)};
           uint32_t r[32];
           tm_ld32(sat, r);
           tm_wait_ld();
@@ -722,24 +733,25 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         meet();
         const float n_m = fmaxf(m, fmaxf(top, sm.top[s][half ^ 1][row]));
         const float base = n_m == -INFINITY ? 0.0f : n_m;
-        const float next = ex2(m - base);
+        next = ex2(m - base);
         m = n_m;
         // the values' scales: the largest inverse is the tile's factor, each group's share of it
         // (1 but for groups of another magnitude) goes to its probabilities
         wait(&sm.vinfo[t & 3], (t >> 2) & 1);
-        const float4 va = *reinterpret_cast<const float4*>(&sm.vsc[t & 3][4 * half]);
         const float vi = __uint_as_float((254u << 23) - __float_as_uint(tile_factor(sm.vsc[t & 3])));  // 1 / a power of 2
-        const float share[4] = {va.x * vi, va.y * vi, va.z * vi, va.w * vi};
         const float b14 = kKtPScale - base;
         float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
+#pragma unroll 1
         for (int part = 0; part < 2; ++part) {
           uint32_t r[16], hi[8], lo[8];
           tm_ld16(sat + 16 * part, r);
+          const float2 k2 = *reinterpret_cast<const float2*>(&sm.ksc[t & 3][4 * half + 2 * part]);
+          const float2 v2 = *reinterpret_cast<const float2*>(&sm.vsc[t & 3][4 * half + 2 * part]);
+          const float c0 = fmaxf(cq * k2.x, kLeastFactor), c8 = fmaxf(cq * k2.y, kLeastFactor);
           tm_wait_ld();
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float c1 = cc[2 * part + (e >> 2)], sh = share[2 * part + (e >> 2)];
+            const float c1 = e < 4 ? c0 : c8, sh = e < 4 ? v2.x * vi : v2.y * vi;
             float2 p = fma2(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), make_float2(c1, c1),
                             make_float2(b14, b14));
             p.x = ex2(p.x);
@@ -753,6 +765,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         if (const unsigned long long bad_t = *reinterpret_cast<const unsigned long long*>(&sm.vbad[t & 3][0])) {
           // a key whose value row is left out keeps its probability as it is, for add_o
           tm_wait_st();
+#pragma unroll 1
           for (int e = 0; e < 32; ++e) {
             if (!((bad_t >> (32 * half + e)) & 1)) continue;
             const uint32_t at = mine + kTmP + 64 * s + 16 * half + (e >> 1);
@@ -773,10 +786,11 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         __syncwarp();
         if (lane == 0) bar_arrive(&sm.pfull[s]);
         l = fmaf(l, next, sum.x + sum.y);
+        }
         if (t > cur.t0) add_o(t - 1, corr);
+        if (t == tend) break;
         corr = next;
       }
-      add_o(t - 1, corr);
       // the row's sum over both halves (the maxima's place is free: the last tile's was read
       // before its P was given away, and t moves on)
       meet();
@@ -792,6 +806,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       constexpr float kUnscale = 1.0f / (1 << kKtPScale);  // P' = 2^14 p is in both sums
       float f = kUnscale;
       if (whole) f = m == -INFINITY ? 0.0f : __fdiv_rn(1.0f, l);
+      ok = ok && !*abort;  // another warp that went on without its data
       if (!ok) f = nan;
       {
         // 32 dimensions of the pair's 32 rows at a time, turned back and written by rows
@@ -1054,19 +1069,16 @@ kv_column_tile_kernel(const KvArgs a, float* weight, float* __restrict__ part, u
       if (ok && t >= 2) ok = bar_wait(&sm.sfree[s], ((t >> 1) - 1) & 1, abort);
       if (!ok) break;
       tc_after();
-      const uint64_t qh0 = desc_sw128(sm.q[s][0][0]), qh1 = desc_sw128(sm.q[s][0][1]);
-      const uint64_t ql0 = desc_sw128(sm.q[s][1][0]), ql1 = desc_sw128(sm.q[s][1][1]);
-      const uint32_t kh = tmem, kl = tmem + 64, d = tmem + 128 + 64 * s;
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk) mma_ts(d, kl + 8 * kk, (kk < 4 ? qh0 : qh1) + 2 * (kk & 3), id, kk > 0);
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk) mma_ts(d, kh + 8 * kk, (kk < 4 ? ql0 : ql1) + 2 * (kk & 3), id, 1);
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk) mma_ts(d, kh + 8 * kk, (kk < 4 ? qh0 : qh1) + 2 * (kk & 3), id, 1);
-      mma_commit(&sm.qfree[s]);
-      mma_commit(&sm.sfull[s]);
+      __syncwarp();
+      if (elected()) {
+        mma_pairs<8, sizeof(sm.q[0][0][0])>(tmem + 128 + 64 * s, tmem, tmem + 64, sm.q[s][0][0], sm.q[s][1][0], id);
+        mma_commit(&sm.qfree[s]);
+        mma_commit(&sm.sfull[s]);
+      }
+      __syncwarp();
     }
-    mma_commit(&sm.done);
+    if (elected()) mma_commit(&sm.done);
+    __syncwarp();
     mb_wait_ns(su32(&sm.done), 0, kDrainLimitNs, nullptr);
   } else if (warp < kKcConvertWarp) {
     // ---------------- a key per thread ----------------
@@ -1124,7 +1136,7 @@ kv_column_tile_kernel(const KvArgs a, float* weight, float* __restrict__ part, u
       tc_after();
       // rows from this one on see the whole key tile
       const bool masked = p + (first + t * splits) * kKcRows / a.group < j0 + kKcKeys - 1;
-#pragma unroll
+#pragma unroll 1
       for (int part = 0; part < 2; ++part) {
         uint32_t r[32];
         tm_ld32(mine + 128 + 64 * s + 32 * part, r);
@@ -1156,7 +1168,7 @@ kv_column_tile_kernel(const KvArgs a, float* weight, float* __restrict__ part, u
       if (lane == 0) bar_arrive(&sm.sfree[s]);  // after the last look at the tile's constants too
     }
     if (j < keys) {
-      const float w = ok ? sum.x + sum.y : __uint_as_float(0x7fffffffu);
+      const float w = ok && !*abort ? sum.x + sum.y : __uint_as_float(0x7fffffffu);
       if (part)
         part[((size_t)blockIdx.z * gridDim.y + bh) * a.max_t + j] = w;
       else

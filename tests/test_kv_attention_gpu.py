@@ -698,13 +698,16 @@ def test_a_wait_that_runs_out_reports_itself(cuda_device):
     old = L.q8lin_wait_limit_ns()
     try:
         assert L.q8lin_set_wait_limit_ns(0) == 0
-        out = attention.attention_weights(q, k, v, _i32(pos, dev), torch.zeros((B, hkv, max_t), device=dev))
+        w = torch.zeros((B, hkv, max_t), device=dev)
+        out = attention.attention_weights(q, k, v, _i32(pos, dev), w)
         torch.cuda.synchronize()
     finally:
         L.q8lin_set_wait_limit_ns(old)
     _lib.check(L.q8lin_fault_status(0, ctypes.byref(flags), 1))
     assert flags.value == 32
-    assert torch.isnan(out).any()
+    # which of the kernels had to wait is a matter of timing; what one gave up on is NaN
+    assert torch.isnan(out).any() or torch.isnan(w).any()
+    _close(torch.where(torch.isnan(out), ref.to(out.dtype), out), ref)
     w = torch.zeros((B, hkv, max_t), device=dev)
     out = attention.attention_weights(q, k, v, _i32(pos, dev), w)
     _close(out, ref)
