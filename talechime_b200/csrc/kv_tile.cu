@@ -1012,16 +1012,23 @@ kv_column_tile_kernel(const KvArgs a, float* weight, float* __restrict__ part, u
     const int there = keys - p <= 0 ? 0 : min(rows, (keys - p) * a.group);  // rows inside the cache
     float4 qr[8];
     auto load = [&](int rt) {
+      const int r = rt * kKcRows + cw * 8 + ky;
+      int tok = r / a.group, head = r - tok * a.group;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int r = rt * kKcRows + cw * 8 + ky + 2 * i;
         qr[2 * i] = qr[2 * i + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < there) {
-          const int tok = r / a.group;
-          const float4* row = qb + ((size_t)tok * a.hq + (r - tok * a.group)) * (kKvD / 4);
+        if (r + 2 * i < there) {
+          const float4* row = qb + ((size_t)tok * a.hq + head) * (kKvD / 4);
           qr[2 * i] = row[0];
           qr[2 * i + 1] = row[16];
         }
+        head += 2;  // the row after the next, with no division
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (head >= a.group) {
+            head -= a.group;
+            ++tok;
+          }
       }
     };
     bool dead = false;
@@ -1194,12 +1201,12 @@ kv_column_add_kernel(const float* __restrict__ part, const int* __restrict__ pos
   weight[(size_t)bh * max_t + j] += s;
 }
 
-// Row splits of the column sums: about 444 CTAs (three for each of two places on an SM) over the
+// Row splits of the column sums: about 592 CTAs (two for each of two places on an SM) over the
 // keys of the new rows alone, 8 row tiles a CTA at least (its start costs as much as some tiles).
 int column_splits(int batch, int n, int hkv, int group) {
   const int64_t tiles = ((int64_t)n * group + kKcRows - 1) / kKcRows;
   const int64_t places = (int64_t)batch * hkv * ((n + kKcKeys - 1) / kKcKeys);
-  const int64_t want = (444 + places - 1) / places;
+  const int64_t want = (592 + places - 1) / places;
   const int64_t most = tiles / 8 > 64 ? 64 : tiles / 8;
   return (int)(want < most ? want : most < 1 ? 1 : most);
 }
