@@ -297,7 +297,8 @@ int q8lin_attention_prefill(const float* q, const float* k_cache, const float* v
  * 128; scores times the f32 rounding of 1/sqrt(128), softmax statistics and sums in f32.
  * A row at or past max_t (or of a sequence with pos < 0) is no row: its output is 0, nothing
  * is written for it and nothing sees it.  Cache rows that no row of the call sees may hold
- * anything; visible keys and values are finite.  Workspaces need no initialisation, are
+ * anything; queries and visible keys and values are finite.  Outputs overlap no input (but
+ * weight_out may be weight).  Workspaces need no initialisation, are
  * 16-byte aligned, and serve one call at a time (a captured graph keeps its own).  All calls
  * are stream-ordered, allocate nothing, and run on the current device.
  */

@@ -641,7 +641,11 @@ struct KvPlan {
   bool split = false;
   size_t slots = 0;
 };
-// Rows a kv head from which the tcgen05 kernel (128 rows a unit) takes over.
+// Rows a kv head from which the tcgen05 kernel (128 rows a unit) takes over: from there on the
+// core reads the keys more than once (16 rows a unit).  Lengths are in device memory, so rows alone
+// decide: 24 rows a kv head behind 100 rows 17.4 us there and 15.1 here, behind 8 K rows 30.0 and 27.6;
+// 128 rows 19.0 and 16.0, 32.2 and 37.9; 512 rows 22.4 and 19.6, 38.2 and 102.6; four sequences of
+// 24 rows 17.2 and 15.3, 35.2 and 38.0, of 128 rows 19.0 and 16.5, 37.1 and 103.
 constexpr int64_t kKvTileMinRows = 17;
 KvPlan kv_plan(int64_t lists, int64_t rows_per_list, bool tile) {
   KvPlan p;
@@ -653,9 +657,7 @@ KvPlan kv_plan(int64_t lists, int64_t rows_per_list, bool tile) {
   p.slots = !p.split ? (size_t)p.units : p.rows == kKvTileRows ? (size_t)(2 * kKvGrid) : (size_t)(kKvGrid + p.units);
   return p;
 }
-size_t begun_bytes(const KvPlan& p) {
-  return (p.rows == kKvTileRows ? (size_t)kKvGrid : (size_t)p.units) * sizeof(int2);
-}
+size_t begun_bytes(const KvPlan& p) { return (size_t)p.units * sizeof(int2); }
 size_t core_bytes(const KvPlan& p, bool stat) {
   return (p.split ? up256(p.slots * p.rows * kKvD * 4) + up256(begun_bytes(p)) : 0) +
          (p.split || stat ? up256(p.slots * 2 * p.rows * 4) : 0);

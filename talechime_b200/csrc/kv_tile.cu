@@ -18,15 +18,20 @@
 //     the PV that follows a softmax, and K behind it would hold up the next QK;
 //   * 1 issues the MMAs, S = Q K^T and O = P V (Q and P in TMEM, S and P double-buffered), so that
 //     QK of a tile runs while the softmax of the one before is at work.  Issuing waits for the
-//     tensor cores' queue, 1600 cycles a tile: a warp with other work cannot do it beside;
+//     tensor cores' queue, most of the tile's MMA time: a warp with other work cannot do it beside;
 //   * 8 softmax: two threads a row, one for each half of the keys and then of the dimensions;
 //     scores from TMEM, running maximum and sum, P' = 2^14 p back to TMEM as hi / lo; then the
 //     O tile of the tile before is added to registers.
 // The tensor cores cut their f32 sums, so an O tile starts from 0 and joins the running sum with
 // rounding.  TMEM (512 columns): Q 128, S 2 x 64, P 2 x 64, O 128.
 //
-// What bounds it: per 128 rows x 64 keys 24 MMAs of N = 64 and 12 of N = 128, about 1600
-// cycles; conversion, softmax and O need about 1000 issue slots of each scheduler beside them.
+// What bounds it: per 128 rows x 64 keys 24 MMAs of N = 64 and 12 of N = 128, 1632 cycles, a third
+// of the 2.3 us that a tile takes (64 trees' units of 122 tiles, 53 tiles a CTA, 153 us with the
+// launches around it).  Issue slots are 57 % busy; the rest is the roles' chain through a tile (S,
+// maximum, P, O) and instruction fetch: the unrolled loops of three roles are more than the
+// instruction caches hold, so what shortens their code shortens the tile (one issue loop for the
+// three products, one site each for the converters' loads and for adding O: 163 -> 154 us; two
+// copies of the converter's loop in turn: 254).  A unit costs about 9 us beside its tiles.
 #include <cmath>
 
 #include "common.cuh"
@@ -583,7 +588,6 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       }
     KtCursor& cur = sm.cursor[warp];
     cur = start;
-    if (a.split && tid == 0) a.begun[blockIdx.x] = make_int2(-1, 0);
     for (; cur.seek<MASK>(a); cur.pass(a)) {
       const KvUnit& x = cur.x;
       // half of the query row: scaled hi / lo to TMEM, dimensions in the order of the K tiles (32
@@ -837,11 +841,11 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
           meet();
         }
       }
+      if (a.split && tid == 0 && cur.off == 0)  // for the merge: the first CTA, and how many there are
+        a.begun[cur.u] = make_int2(blockIdx.x, 1 + (x.chunks - cur.n + sm.find.quota - 1) / sm.find.quota);
       if (row < x.nrows) {
         if (half == 0) {
           if (!whole) {
-            if (row == 0 && cur.off == 0)  // for the merge: CTAs of quota tiles go on with the unit
-              a.begun[blockIdx.x] = make_int2(cur.u, 1 + (x.chunks - cur.n + sm.find.quota - 1) / sm.find.quota);
             a.stat[slot * 2 * a.rows + row] = m;
             a.stat[(slot * 2 + 1) * a.rows + row] = ok ? l * kUnscale : nan;
           }
@@ -861,35 +865,33 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
 
 // After a split: the parts of the units that more than one CTA worked on, in the order of the CTAs, and
 // zeros for units without keys.  A CTA has at most two parts: the rest of a unit that began before it (slot
-// 2 cta) and the beginning of one that ends after it (slot 2 cta + 1).  Block (c, y) merges rows 32 y
-// .. + 32 of the unit that CTA c began and did not end, four rows a warp with their loads in flight
-// together.
-constexpr int kKtMergeWarps = 8, kKtMergeEach = 4, kKtMergeRows = kKtMergeWarps * kKtMergeEach;
-template <int MASK>
+// 2 cta) and the beginning of one that ends after it (slot 2 cta + 1).  A warp takes EACH rows of
+// unit blockIdx.x and has eight parts' rows in flight.
+constexpr int kKtMergeWarps = 8;
+template <int MASK, int EACH>
 __global__ void __launch_bounds__(kKtMergeWarps * 32) kv_tile_merge_kernel(const KvArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r0 = blockIdx.y * kKtMergeRows + warp * kKtMergeEach;
+  const int r0 = (blockIdx.y * kKtMergeWarps + warp) * EACH;
   pdl_launch_dependents();
   pdl_wait();
-  for (int u = blockIdx.x; u < a.units; u += kKvGrid) {
-    const KvUnit x = kv_unit<MASK>(a, u);
-    if (x.chunks > 0) continue;
-    for (int r = r0; r < min(r0 + kKtMergeEach, x.nrows); ++r) {
+  const KvUnit x = kv_unit<MASK>(a, blockIdx.x);
+  if (r0 >= x.nrows) return;
+  if (x.chunks == 0) {  // no CTA came by
+    for (int r = r0; r < min(r0 + EACH, x.nrows); ++r) {
       reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, r))[lane] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (a.lse && lane == 0) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + r] = INFINITY;
     }
+    return;
   }
   const int2 d = a.begun[blockIdx.x];
-  if (d.x < 0) return;  // nothing of CTA c's goes on in the next
-  const KvUnit x = kv_unit<MASK>(a, d.x);
-  if (r0 >= x.nrows) return;
   const int parts = d.y;
-  auto slot = [&](int s) { return 2 * ((size_t)blockIdx.x + s) + (s == 0 ? 1 : 0); };
-  int row[kKtMergeEach];
-  float M[kKtMergeEach], L[kKtMergeEach];
-  float4 A[kKtMergeEach];
+  if (parts == 1) return;
+  auto slot = [&](int s) { return 2 * ((size_t)d.x + s) + (s == 0 ? 1 : 0); };
+  int row[EACH];
+  float M[EACH], L[EACH];
+  float4 A[EACH];
 #pragma unroll
-  for (int i = 0; i < kKtMergeEach; ++i) {
+  for (int i = 0; i < EACH; ++i) {
     row[i] = min(r0 + i, x.nrows - 1);
     M[i] = -INFINITY;
     L[i] = 0.0f;
@@ -897,16 +899,16 @@ __global__ void __launch_bounds__(kKtMergeWarps * 32) kv_tile_merge_kernel(const
   }
   for (int s = lane; s < parts; s += 32)
 #pragma unroll
-    for (int i = 0; i < kKtMergeEach; ++i) M[i] = fmaxf(M[i], a.stat[slot(s) * 2 * a.rows + row[i]]);
+    for (int i = 0; i < EACH; ++i) M[i] = fmaxf(M[i], a.stat[slot(s) * 2 * a.rows + row[i]]);
 #pragma unroll
-  for (int i = 0; i < kKtMergeEach; ++i)
+  for (int i = 0; i < EACH; ++i)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M[i] = fmaxf(M[i], __shfl_xor_sync(kFull, M[i], o));
   for (int s0 = 0; s0 < parts; s0 += 32) {  // a lane per part for the factors, then a part at a time
-    float f[kKtMergeEach];
+    float f[EACH];
     const int s1 = s0 + lane;
 #pragma unroll
-    for (int i = 0; i < kKtMergeEach; ++i) {
+    for (int i = 0; i < EACH; ++i) {
       f[i] = 0.0f;
       if (s1 < parts && M[i] != -INFINITY) {
         f[i] = exp2f(a.stat[slot(s1) * 2 * a.rows + row[i]] - M[i]);
@@ -914,20 +916,28 @@ __global__ void __launch_bounds__(kKtMergeWarps * 32) kv_tile_merge_kernel(const
       }
     }
     const int n = min(32, parts - s0);
-#pragma unroll 2
-    for (int s = 0; s < n; ++s) {
-      const float* acc = a.acc + slot(s0 + s) * a.rows * kKvD;
+    constexpr int kAhead = 8 / EACH;  // parts whose rows are loaded before one is used
+    for (int s = 0; s < n; s += kAhead) {
+      float4 v[kAhead][EACH];
 #pragma unroll
-      for (int i = 0; i < kKtMergeEach; ++i) {
-        const float4 v = reinterpret_cast<const float4*>(acc + row[i] * kKvD)[lane];
-        const float fs = __shfl_sync(kFull, f[i], s);
-        if (fs != 0.0f)  // an empty part's sums stay out
-          A[i] = make_float4(fmaf(v.x, fs, A[i].x), fmaf(v.y, fs, A[i].y), fmaf(v.z, fs, A[i].z), fmaf(v.w, fs, A[i].w));
-      }
+      for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+          if (s + j < n)
+            v[j][i] = ld_row(reinterpret_cast<const float4*>(a.acc + (slot(s0 + s + j) * a.rows + row[i]) * kKvD) + lane);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          const float fs = __shfl_sync(kFull, f[i], (s + j) & 31);
+          if (s + j < n && fs != 0.0f)  // an empty part's sums stay out
+            A[i] = make_float4(fmaf(v[j][i].x, fs, A[i].x), fmaf(v[j][i].y, fs, A[i].y), fmaf(v[j][i].z, fs, A[i].z),
+                               fmaf(v[j][i].w, fs, A[i].w));
+        }
     }
   }
 #pragma unroll
-  for (int i = 0; i < kKtMergeEach; ++i) {
+  for (int i = 0; i < EACH; ++i) {
     const float sum = warp_sum(L[i]);
     if (r0 + i >= x.nrows) break;
     if (M[i] != -INFINITY)
@@ -1229,11 +1239,16 @@ cudaError_t launch_tile(const KvArgs& a, int device, cudaStream_t s) {
   cfg.numAttrs = pdl_enabled() ? 1 : 0;
   e = cudaLaunchKernelEx(&cfg, kv_tile_kernel<MASK>, a, wait_limit_ns());
   if (e != cudaSuccess || !a.split) return e;
+  // Few units have few rows, of many parts each: a warp per row.  With many, the CTAs' starts count.
+  // (A tree over 2 units of 63 parts 68 us with four rows a warp, 33 with one; 30 units of 4 parts 39
+  // and 33; 64 units of 3 parts 152 and 155.)
   const int rows = a.units > a.batch * a.hkv ? kKvTileRows : a.n * a.group;  // of the largest unit
-  cfg.gridDim = dim3(kKvGrid, (unsigned)((rows + kKtMergeRows - 1) / kKtMergeRows));
+  const int each = a.units <= kKvGrid / 4 ? 1 : 4;
+  cfg.gridDim = dim3((unsigned)a.units, (unsigned)((rows + kKtMergeWarps * each - 1) / (kKtMergeWarps * each)));
   cfg.blockDim = dim3(kKtMergeWarps * 32);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, kv_tile_merge_kernel<MASK>, a);
+  return each == 1 ? cudaLaunchKernelEx(&cfg, kv_tile_merge_kernel<MASK, 1>, a)
+                   : cudaLaunchKernelEx(&cfg, kv_tile_merge_kernel<MASK, 4>, a);
 }
 
 }  // namespace
