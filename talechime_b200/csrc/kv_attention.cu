@@ -641,12 +641,15 @@ struct KvPlan {
   bool split = false;
   size_t slots = 0;
 };
-// Rows a kv head from which the tcgen05 kernel (128 rows a unit) takes over: from there on the
-// core reads the keys more than once (16 rows a unit).  Lengths are in device memory, so rows alone
-// decide: 24 rows a kv head behind 100 rows 17.4 us there and 15.1 here, behind 8 K rows 30.0 and 27.6;
-// 128 rows 19.0 and 16.0, 32.2 and 37.9; 512 rows 22.4 and 19.6, 38.2 and 102.6; four sequences of
-// 24 rows 17.2 and 15.3, 35.2 and 38.0, of 128 rows 19.0 and 16.5, 37.1 and 103.
+// Rows a kv head from which the tcgen05 kernel (128 rows a unit) takes over: from there on the core
+// reads the keys more than once (16 rows a unit).  Its units start faster, so it keeps what can be no
+// more than kKvCoreRows units x rows of the cache, about ten chunks a CTA.  (Trees, core and tcgen05
+// kernel: 24 rows a kv head behind 100 rows 15.1 and 17.4 us, behind 8 K rows (16 K x 2) 27.6 and 30.0;
+// 128 rows behind 500 (8 K) 18.6 and 20.9, behind 2 K (32 K) 23.1 and 22.8, behind 8 K 37.9 and 32.2;
+// 512 rows behind 100 (6.4 K) 19.6 and 22.4, behind 500 (32 K) 25.2 and 22.5, behind 8 K 102.6 and
+// 38.2; four sequences of 128 rows behind 500 (32 K) 23.1 and 21.5.)
 constexpr int64_t kKvTileMinRows = 17;
+constexpr int64_t kKvCoreRows = 10 * kKvGrid * kKvChunk;
 KvPlan kv_plan(int64_t lists, int64_t rows_per_list, bool tile) {
   KvPlan p;
   p.rows = tile && rows_per_list >= kKvTileMinRows ? kKvTileRows : rows_per_list <= 8 ? 8 : kKvMaxRows;
@@ -656,6 +659,10 @@ KvPlan kv_plan(int64_t lists, int64_t rows_per_list, bool tile) {
   p.split = p.units < 2 * kKvGrid;
   p.slots = !p.split ? (size_t)p.units : p.rows == kKvTileRows ? (size_t)(2 * kKvGrid) : (size_t)(kKvGrid + p.units);
   return p;
+}
+KvPlan tree_plan(int batch, int n, int hq, int hkv, int max_t) {
+  const int64_t lists = (int64_t)batch * hkv, rows = (int64_t)n * (hq / hkv);
+  return kv_plan(lists, rows, lists * ((rows + kKvMaxRows - 1) / kKvMaxRows) * max_t > kKvCoreRows);
 }
 size_t begun_bytes(const KvPlan& p) { return (size_t)p.units * sizeof(int2); }
 size_t core_bytes(const KvPlan& p, bool stat) {
@@ -739,8 +746,11 @@ int score_stride(int max_t) { return (max_t + kKvChunk - 1) / kKvChunk * kKvChun
 }  // namespace
 
 size_t attention_tree_workspace_bytes(int batch, int n, int hq, int hkv) {
-  const KvPlan p = kv_plan((int64_t)batch * hkv, (int64_t)n * (hq / hkv), true);
-  return up256((size_t)batch * n * hq * kKvD * 4) + up256((size_t)batch * n * tree_words(n) * 4) + core_bytes(p, false);
+  // max_t decides on the kernel: room for either
+  const int64_t lists = (int64_t)batch * hkv, rows = (int64_t)n * (hq / hkv);
+  const size_t core = core_bytes(kv_plan(lists, rows, false), false), tile = core_bytes(kv_plan(lists, rows, true), false);
+  return up256((size_t)batch * n * hq * kKvD * 4) + up256((size_t)batch * n * tree_words(n) * 4) +
+         (core > tile ? core : tile);
 }
 
 cudaError_t launch_rope_attention_tree(const float* qkv, const int* parents, const int* pos, const float* cos_t,
@@ -754,7 +764,7 @@ cudaError_t launch_rope_attention_tree(const float* qkv, const int* parents, con
   KvArgs a = kv_args(q, kc, vc, pos, batch, n, hq, hkv, max_t, out);
   a.anc = anc;
   a.words = tree_words(n);
-  core_place(a, kv_plan((int64_t)batch * hkv, (int64_t)n * a.group, true), false, w);
+  core_place(a, tree_plan(batch, n, hq, hkv, max_t), false, w);
   cudaLaunchAttribute attr[1];
   cudaLaunchConfig_t cfg = kv_cfg(dim3((unsigned)n, (unsigned)batch), dim3(kKvMaxTree), 0, s, attr);
   cudaError_t e = cudaLaunchKernelEx(&cfg, rope_tree_kernel, qkv, parents, pos, cos_t, sin_t, kc, vc, n, a.words, hq,

@@ -160,6 +160,17 @@ def test_tree_matches_its_definition(cuda_device, B, n, hq, hkv, pos, max_t, kin
     assert torch.equal(torch.nan_to_num(v, 7.0), torch.nan_to_num(vr, 7.0))
 
 
+ROOMY = 24000  # rows of a cache in which more than 16 rows a kv head take the tcgen05 kernel whatever their number
+
+
+@pytest.mark.parametrize("B,n,hq,hkv,pos,max_t,kind", [(*c[:5], ROOMY, c[6]) for c in TREES if c[1] * c[2] // c[3] > 16] + [
+    (1, 3, 16, 2, [40], ROOMY, "random"),
+    (2, 20, 8, 1, [ROOMY - 10, ROOMY - 20], ROOMY, "chain"),  # nodes past the cache; exactly full
+])
+def test_tree_in_a_roomy_cache(cuda_device, B, n, hq, hkv, pos, max_t, kind):
+    test_tree_matches_its_definition(cuda_device, B, n, hq, hkv, pos, max_t, kind)
+
+
 def test_tree_nodes_without_a_path_are_no_rows(cuda_device):
     """A parent that is the node itself, behind it or below -1, and everything under such a
     node: output 0, no cache row, seen by nobody; the other nodes as without them."""
@@ -180,10 +191,10 @@ def test_tree_nodes_without_a_path_are_no_rows(cuda_device):
 
 
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
-@pytest.mark.parametrize("n,hq,hkv", [(12, 4, 2), (40, 16, 2)])
-def test_tree_siblings_do_not_meet(cuda_device, bad, n, hq, hkv):
+@pytest.mark.parametrize("n,hq,hkv,max_t", [(12, 4, 2, 100), (40, 16, 2, 100), (40, 16, 2, ROOMY)])
+def test_tree_siblings_do_not_meet(cuda_device, bad, n, hq, hkv, max_t):
     """A node whose value row is not finite spoils itself and what is below it, nothing else."""
-    dev, max_t = cuda_device, 100
+    dev = cuda_device
     g = _gen(6, dev)
     k, v = _caches(g, 1, hkv, max_t, dev)
     qkv = torch.randn((1, n, (hq + 2 * hkv) * D), generator=g, device=dev)
@@ -343,11 +354,11 @@ def test_weights_values_of_very_different_sizes(cuda_device, t):
     assert float((w.double() - wref).norm() / wref.norm()) <= 10 * REL_L2
 
 
-@pytest.mark.parametrize("n,hq,hkv", [(12, 4, 2), (40, 16, 2)])
-def test_tree_finite_part_of_a_value_row_counts(cuda_device, n, hq, hkv):
+@pytest.mark.parametrize("n,hq,hkv,max_t", [(12, 4, 2, 200), (40, 16, 2, 200), (40, 16, 2, ROOMY)])
+def test_tree_finite_part_of_a_value_row_counts(cuda_device, n, hq, hkv, max_t):
     """A history value with one infinite dimension spoils that dimension of the rows that see it
     and counts as it is in the others."""
-    dev, max_t, p0 = cuda_device, 200, 100
+    dev, p0 = cuda_device, 100
     g = _gen(14, dev)
     k, v = _caches(g, 1, hkv, max_t, dev)
     v[0, :, 97, 9] = math.inf  # in the last tile, before the tree
