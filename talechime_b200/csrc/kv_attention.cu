@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 2 : 1) kv_attention_kernel(co
           if (masked) {
             const int j = j0 + g + (e >> 1) * 8;
             if (MASK == kMaskTree ? !((see[nt] >> ((e & 1) * 16 + (e >> 1) * 8)) & 1u)
-                                  : j >= min(x.keys, x.p + kv_token<MASK>(a, x, min(nt * 8 + 2 * t + (e & 1), x.nrows - 1)) + 1))
+                                  : j >= x.keys || j > x.p + kv_token<MASK>(a, x, min(nt * 8 + 2 * t + (e & 1), x.nrows - 1)))
               p[e] = -INFINITY;
           }
         }

@@ -162,9 +162,10 @@ struct KvFind {
 // Evenly, a CTA takes quota chunks wherever they lie and so begins a second unit in most cases; or
 // every unit gets CTAs of its own, which then take up to `quota` chunks of it.  Starting on a
 // unit costs about a.pass chunks' time (query rows, first copies, joining the parts), so units
-// get their own CTAs where that adds at most a.pass chunks to the share.  (Trees of 64 nodes x 8 heads
-// behind 200 rows 32.6 us evenly, 27.5 so; 5 ragged trees of 33 nodes 45.2 and 38.4; 16 heads of 16 K
-// rows 70.2 and 62.1.  64 units of 122 tiles stay even: 53 tiles to a CTA, not 64.)
+// get their own CTAs where that adds at most a.pass chunks to the share.  (Evenly and so: trees of 64
+// nodes x 8 heads behind 200 rows 27.8 and 21.7 us, 5 ragged trees of 33 nodes 36.5 and 33.0, 16 heads
+// of 16 K rows 70.0 and 61.9, one block-sparse token 21.8 and 17.9.  64 units of 122 tiles stay
+// even, 53 tiles to a CTA and not 64: 154 us against 169.)
 template <int MASK, int THREADS>
 __device__ int kv_find(const KvArgs& a, KvFind& sm, int cta) {
   constexpr int kPer = (2 * kKvGrid + THREADS - 1) / THREADS;  // more units are not split

@@ -249,7 +249,8 @@ class Q8Decoder:
         layer); "unfused": 11 launches per layer, one per reference operation; "tracked"
         (track_weights): the fused step whose attention also adds every cached row's weight to
         kv_weight; "blocks" (blocks=...): the fused step whose attention goes over the blocks
-        of rows that score highest."""
+        of rows that score highest (a replayed graph of another mode goes unnoticed: call
+        refresh_block_keys() before the next "blocks" step)."""
         if self.batch != 1:
             raise ValueError("the decode step serves batch 1; this decoder holds "
                              f"{self.batch} sequences (prefill only)")
@@ -482,7 +483,7 @@ class Q8Decoder:
         ancestors (q8lin_rope_attention_tree).  Returns the greedy next token of every node
         (int32 [n] on the device); tree_logits [n, vocab] holds the logits.  The cached rows
         pos .. pos + n - 1 hold the nodes until accept_path() or the next step; pos and token
-        stay.  Raises Q8LinError(ERR_SHAPE) past max_t."""
+        stay.  A tree adds nothing to kv_weight.  Raises Q8LinError(ERR_SHAPE) past max_t."""
         if self.batch != 1:
             raise ValueError("verify_tree serves batch 1")
         i32 = lambda v: torch.as_tensor(np.asarray(v.cpu() if isinstance(v, torch.Tensor) else v), dtype=torch.int32)

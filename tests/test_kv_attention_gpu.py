@@ -137,6 +137,8 @@ TREES = [
     (1, 256, 8, 8, [10], 300, "star"),            # all siblings
     (8, 64, 16, 2, [900, 800, 1, 0, 64, 63, 65, 900], 1000, "random"),  # many units
     (4, 20, 8, 8, [90, 85, 100, -1], 100, "random"),  # nodes past the cache; no sequence
+    (20, 16, 16, 2, [50, 0, -1, 54, 60, 69, 70, 3, 16, 15] * 2, 70, "random"),  # 320 units of 16 rows in a small cache
+    (20, 2, 16, 16, [50, 0, -1, 54, 60, 69, 70, 3, 16, 15] * 2, 70, "random"),  # 320 units of 8
 ]
 
 
