@@ -956,7 +956,8 @@ __global__ void __launch_bounds__(kKtMergeWarps * 32) kv_tile_merge_kernel(const
 // stays in one register.  grid (key tiles, batch * hkv, splits): split z takes row tiles z, z +
 // splits, ... and leaves its sums in part[z]; kv_column_add_kernel adds them in split order.
 // Two CTAs per SM: 4 warps exponentials, 8 converters, 1 MMA; 24 MMAs of N = 64 a tile, about
-// 820 cycles, beside 512 cycles of exponentials.
+// 820 cycles, beside 512 cycles of exponentials; what it waits for is the converters' chain of load,
+// scale, split and hand-over.  4 x 1024 tokens, 16 heads on 2: 69 us, tensor pipe 26 % busy.
 constexpr int kKcThreads = 416, kKcConvertWarp = 4, kKcMmaWarp = 12;
 constexpr uint32_t kKcTmemCols = 256;
 constexpr int kKcKeys = 128, kKcRows = 64;
@@ -1213,6 +1214,7 @@ kv_column_add_kernel(const float* __restrict__ part, const int* __restrict__ pos
 
 // Row splits of the column sums: about 592 CTAs (two for each of two places on an SM) over the
 // keys of the new rows alone, 8 row tiles a CTA at least (its start costs as much as some tiles).
+// (4 x 1024 tokens with 256, 444 and 592 CTAs: 198, 191 and 187 us for the whole call.)
 int column_splits(int batch, int n, int hkv, int group) {
   const int64_t tiles = ((int64_t)n * group + kKcRows - 1) / kKcRows;
   const int64_t places = (int64_t)batch * hkv * ((n + kKcKeys - 1) / kKcKeys);
