@@ -586,9 +586,23 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         for (int i = 0; i < kKvD / 4; ++i) dst[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (a.lse) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] = INFINITY;
       }
+    // The warp's cursor is one object of its 32 lanes: one of them moves it on, between the others' last
+    // look at the unit behind and their first at the next.
     KtCursor& cur = sm.cursor[warp];
-    cur = start;
-    for (; cur.seek<MASK>(a); cur.pass(a)) {
+    auto forward = [&](bool begin) {
+      int more = 0;
+      __syncwarp();
+      if (lane == 0) {
+        if (begin)
+          cur = start;
+        else
+          cur.pass(a);
+        more = cur.seek<MASK>(a);
+      }
+      __syncwarp();
+      return __shfl_sync(kFull, more, 0) != 0;
+    };
+    for (bool begin = true; forward(begin); begin = false) {
       const KvUnit& x = cur.x;
       // half of the query row: scaled hi / lo to TMEM, dimensions in the order of the K tiles (32
       // half .. + 32 and 64 + 32 half .. + 32).  A thread that reads its own row takes 32 memory
