@@ -408,8 +408,6 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 2 : 1) kv_attention_kernel(co
         a.stat[slot_id * 2 * a.rows + tid] = M;
         a.stat[slot_id * 2 * a.rows + a.rows + tid] = L;
       }
-      if (a.lse && whole)
-        a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + tid] = M == -INFINITY ? INFINITY : M + log2f(L);
     }
     __syncthreads();
     for (int e = tid; e < x.nrows * 32; e += kThreads) {
@@ -461,10 +459,7 @@ __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs 
   const int row = blockIdx.y;
   if (merging && (row >= x.nrows || !a.split)) return;
   if (x.chunks == 0) {  // no CTA came by
-    if (merging) {
-      a.out[kv_row_offset<MASK>(a, x, row) + tid] = 0.0f;
-      if (a.lse && tid == 0) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] = INFINITY;
-    }
+    if (merging) a.out[kv_row_offset<MASK>(a, x, row) + tid] = 0.0f;
     return;
   }
   const int key0 = ((int)blockIdx.y - a.rows) * kKvWeightKeys * a.weight_reps;
@@ -504,8 +499,6 @@ __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs 
       A = f != 0.0f ? fmaf(v, f, A) : A;
     }
     a.out[kv_row_offset<MASK>(a, x, row) + tid] = M == -INFINITY ? 0.0f : __fdiv_rn(A, L);
-    if (a.lse && tid == 0)
-      a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] = M == -INFINITY ? INFINITY : M + log2f(L);
     return;
   }
   if (SCORES) {
@@ -707,15 +700,13 @@ cudaError_t launch_core_nt(const KvArgs& a, int device, cudaStream_t s) {
       kv_cfg(dim3((unsigned)(a.split ? kKvGrid : a.units)), dim3(W * 32), sizeof(KvSmem<NT, W>), s, attr);
   return cudaLaunchKernelEx(&cfg, kv_attention_kernel<MASK, SCORES, NT, W>, a);
 }
-template <int MASK, bool SCORES>
+// Units of 8 or 16 rows; causal rows come here with their scores stored.
+template <int MASK>
 cudaError_t launch_core(const KvArgs& a, float* weight, int device, cudaStream_t s) {
-  cudaError_t e;
-  if (!SCORES && MASK != kMaskBlocks && a.rows == kKvTileRows)
-    return launch_kv_tile(a, MASK, device, s);
-  else
-    e = a.rows != 8 ? launch_core_nt<MASK, SCORES, 2, kKvWarps>(a, device, s)
-        : a.split   ? launch_core_nt<MASK, SCORES, 1, kKvWarps>(a, device, s)
-                    : launch_core_nt<MASK, SCORES, 1, 4>(a, device, s);
+  constexpr bool SCORES = MASK == kMaskCausal;
+  cudaError_t e = a.rows != 8 ? launch_core_nt<MASK, SCORES, 2, kKvWarps>(a, device, s)
+                  : a.split   ? launch_core_nt<MASK, SCORES, 1, kKvWarps>(a, device, s)
+                              : launch_core_nt<MASK, SCORES, 1, 4>(a, device, s);
   if (e != cudaSuccess || (!a.split && !SCORES)) return e;
   const unsigned ranges =
       SCORES ? (unsigned)((a.max_t + kKvWeightKeys * a.weight_reps - 1) / (kKvWeightKeys * a.weight_reps)) : 0u;
@@ -773,7 +764,7 @@ cudaError_t launch_rope_attention_tree(const float* qkv, const int* parents, con
   cudaError_t e = cudaLaunchKernelEx(&cfg, rope_tree_kernel, qkv, parents, pos, cos_t, sin_t, kc, vc, n, a.words, hq,
                                      hkv, max_t, q, anc);
   if (e != cudaSuccess) return e;
-  return launch_core<kMaskTree, false>(a, nullptr, device, s);
+  return a.rows == kKvTileRows ? launch_kv_tile(a, kMaskTree, device, s) : launch_core<kMaskTree>(a, nullptr, device, s);
 }
 
 size_t attention_weights_workspace_bytes(int batch, int n, int hq, int hkv, int max_t) {
@@ -798,10 +789,10 @@ cudaError_t launch_attention_weights(const float* q, const float* kc, const floa
     // about eight CTAs an SM: each starts with a look at all units
     const int64_t groups = (int64_t)a.units * ((max_t + kKvWeightKeys - 1) / kKvWeightKeys);
     a.weight_reps = (int)(groups / 1184 < 1 ? 1 : groups / 1184 > 16 ? 16 : groups / 1184);
-    return launch_core<kMaskCausal, true>(a, weight, device, s);
+    return launch_core<kMaskCausal>(a, weight, device, s);
   }
   a.lse = reinterpret_cast<float*>(w);
-  cudaError_t e = launch_core<kMaskCausal, false>(a, weight, device, s);
+  cudaError_t e = launch_kv_tile(a, kMaskCausal, device, s);
   if (e != cudaSuccess) return e;
   w += up256((size_t)batch * hq * n * 4);
   return launch_kv_column_tile(a, weight, reinterpret_cast<float*>(w), device, s);
@@ -819,7 +810,7 @@ cudaError_t launch_attention_blocks(const float* q, const float* kc, const float
   a.block = block;
   a.topk = topk;
   core_place(a, kv_plan((int64_t)batch * n * hkv, a.group, false), false, static_cast<uint8_t*>(ws));
-  return launch_core<kMaskBlocks, false>(a, nullptr, device, s);
+  return launch_core<kMaskBlocks>(a, nullptr, device, s);
 }
 
 }  // namespace q8lin

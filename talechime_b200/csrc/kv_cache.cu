@@ -388,7 +388,7 @@ kv_pick_kernel(const float* __restrict__ q, const float* __restrict__ keys, cons
     for (int e = lane; e < topk; e += 32) idx[e] = e < mine ? e : -1;
     return;
   }
-  const unsigned long long* kr = pk_keys + (size_t)(ROWS == 1 ? 0 : r) * blocks;
+  const unsigned long long* kr = pk_keys + (size_t)r * blocks;
   // The threshold is the largest T with at least topk keys >= T; the search ends early when exactly
   // topk are.
   unsigned long long T = 0;
