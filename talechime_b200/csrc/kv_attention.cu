@@ -278,14 +278,15 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 2 : 1) kv_attention_kernel(co
       cp_async_wait(2);
       __syncwarp();  // the values have landed, the probabilities are written
       const uint32_t vst = ring + slot * kKvHalf;
-      // a value row that is not finite must not reach the rows that do not see it (0 * inf):
-      // such a chunk, only where a mask is at work, takes the exact loop below
+      // a value row that is not finite, or whose hi part is not (it rounds up), must not reach the
+      // rows that do not see it (0 * inf): such a chunk, only where a mask is at work, takes the
+      // exact loop below
       bool odd = false;
+      constexpr float kHiFinite = 0x1.ffep127f;  // from here on hi is infinite
       if (masked) {
         for (int r = 0; r < kKvChunk; ++r) {
           const float4 w = lds_f4(vst + r * (kKvD * 4) + lane * 16);
-          odd |= !(fabsf(w.x) <= 3.402823466e38f && fabsf(w.y) <= 3.402823466e38f && fabsf(w.z) <= 3.402823466e38f &&
-                   fabsf(w.w) <= 3.402823466e38f);
+          odd |= !(fabsf(w.x) < kHiFinite && fabsf(w.y) < kHiFinite && fabsf(w.z) < kHiFinite && fabsf(w.w) < kHiFinite);
         }
         odd = __any_sync(kFull, odd);
       }

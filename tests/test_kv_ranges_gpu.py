@@ -1,0 +1,73 @@
+"""Sizes of queries, keys and values in the attention kernels over the KV caches: what a row does not
+see may be of any size and does not move its result.  Bounds: those of tests/test_kv_attention_gpu.py."""
+import pytest
+import torch
+
+from talechime_b200 import attention
+from test_kv_attention_gpu import D, _caches, _close, _gen, _i32, _paths, _tables, _tree_ref, _weights_ref
+
+pytestmark = pytest.mark.gpu
+
+MAX = torch.finfo(torch.float32).max
+SIZES = [2.0 ** 16, 2.0 ** 24, 2.0 ** 36, 1e30, MAX]
+FORMS = [(12, 4, 2, 100), (40, 16, 2, 100)]
+
+
+def _grow(x, size):
+    """x at that size; the type's largest number in the signs of x."""
+    return torch.sign(x) * MAX if size == MAX else x * size
+
+
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("n,hq,hkv,max_t", FORMS)
+def test_tree_rows_beside_unseen_rows_of_any_size(cuda_device, n, hq, hkv, max_t, size):
+    """A draft whose key, value, or both are far larger than its siblings': rows that do not see it
+    give what they give without it."""
+    dev, p0 = cuda_device, 50
+    parents = [-1, 0, 0, 1, 1, 2, 2] + [1 + (i % 2) for i in range(7, n)]
+    free = [i for i, path in enumerate(_paths(parents, p0, max_t)) if 2 not in path]
+    cos, sin = _tables(max_t, dev)
+    for what in ("key", "value", "both"):
+        g = _gen(101, dev)
+        k, v = _caches(g, 1, hkv, max_t, dev)
+        qkv = torch.randn((1, n, (hq + 2 * hkv) * D), generator=g, device=dev)
+        ref, _, _ = _tree_ref(qkv, _i32([parents], dev), [p0], cos, sin, k, v, hq)
+        rows = qkv.view(1, n, -1, D)[0, 2]
+        if what != "value":
+            rows[hq:hq + hkv] = _grow(rows[hq:hq + hkv], size)
+        if what != "key":
+            rows[hq + hkv:] = _grow(rows[hq + hkv:], size)
+        out = attention.rope_attention_tree(qkv, _i32([parents], dev), _i32([p0], dev), cos, sin, k, v)
+        _close(out[0, free], ref[0, free], what)
+
+
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("t,hq,hkv,p0", [(3, 4, 2, 20), (3, 16, 4, 0)])
+def test_prompt_rows_before_larger_rows(cuda_device, t, hq, hkv, p0, size):
+    """Rows in front of far larger ones, the first of a prompt among them: two later rows whose keys and
+    values are that much larger leave the outputs before them as they are."""
+    dev, max_t = cuda_device, 100
+    g = _gen(102, dev)
+    k, v = _caches(g, 1, hkv, max_t, dev)
+    q = torch.randn((1, t, hq, D), generator=g, device=dev)
+    zero = lambda: torch.zeros((1, hkv, max_t), device=dev)
+    ref, _ = _weights_ref(q, k, v, [p0], zero())
+    for row in {t - 1, max(1, t // 3)}:
+        k[0, :, p0 + row] = _grow(k[0, :, p0 + row], size)
+        v[0, :, p0 + row] = _grow(v[0, :, p0 + row], size)
+    out = attention.attention_weights(q, k, v, _i32([p0], dev), zero())
+    first = max(1, t // 3)
+    _close(out[:, :first], ref[:, :first])
+    if p0 == 0:
+        _close(out[0, 0].view(hkv, -1, D), v[0, :, :1].double().expand(hkv, hq // hkv, D))
+
+
+def _graded(dev, t, hq, hkv, L, drop, seed):
+    """Queries and keys whose scores are -drop[j] and a little, values e^drop[j] times unit normal."""
+    g = _gen(seed, dev)
+    k, v = _caches(g, 1, hkv, L, dev)
+    q = 0.1 * torch.randn((1, t, hq, D), generator=g, device=dev)
+    q[..., 0] = math.sqrt(D)
+    k *= 0.1
+    k[..., 0] = -drop
+    return q, k, v * torch.exp(drop)[:, None]
