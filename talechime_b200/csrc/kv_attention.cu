@@ -445,13 +445,14 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 2 : 1) kv_attention_kernel(co
 }
 
 // Merge of the parts of every unit, and the weights of the keys where the scores were stored:
-// weight[j] += sum over the rows of 2^(s_j - log2 sum).  grid (units, rows + key ranges): CTA
-// (u, r) merges row r, CTA (u, rows + k) adds the weights of range k.
+// weight[j] += sum over the rows of 2^(s_j - maximum) / sum.  (Not 2^(s_j - log2 of all): a maximum of
+// 2^20 leaves the logarithm of the sum four bits.)  grid (units, rows + key ranges): CTA (u, r)
+// merges row r, CTA (u, rows + k) adds the weights of range k.
 constexpr int kKvMergeThreads = 128;
 constexpr int kKvWeightKeys = kKvMergeThreads;  // one key a thread at a time
 template <int MASK, bool SCORES>
 __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs a, float* __restrict__ weight) {
-  __shared__ float fac[kKvGrid], lse[kKvMaxRows], rm[kKvMergeThreads / 32], rl[kKvMergeThreads / 32];
+  __shared__ float fac[kKvGrid], top[kKvMaxRows], inv[kKvMaxRows], rm[kKvMergeThreads / 32], rl[kKvMergeThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, u = blockIdx.x;
   pdl_launch_dependents();
   pdl_wait();
@@ -524,7 +525,10 @@ __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs 
         if (f != 0.0f) L = fmaf(stat[(s * 2 + 1) * a.rows + r], f, L);
       }
       L = warp_sum(L);
-      if (lane == 0) lse[r] = M == -INFINITY ? INFINITY : M + log2f(L);
+      if (lane == 0) {
+        top[r] = M;
+        inv[r] = M == -INFINITY ? 0.0f : __fdiv_rn(1.0f, L);
+      }
     }
     __syncthreads();
     for (int rep = 0; rep < a.weight_reps; ++rep) {
@@ -534,7 +538,7 @@ __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs 
       float w = 0.0f;
 #pragma unroll
       for (int r = 0; r < kKvMaxRows; ++r)
-        if (r < x.nrows && lse[r] != INFINITY) w += exp2f(sc[r] - lse[r]);
+        if (r < x.nrows && inv[r] != 0.0f) w = fmaf(exp2f(sc[r] - top[r]), inv[r], w);
       weight[bh * a.max_t + key] = old + w;
     }
   }

@@ -71,3 +71,22 @@ def _graded(dev, t, hq, hkv, L, drop, seed):
     k *= 0.1
     k[..., 0] = -drop
     return q, k, v * torch.exp(drop)[:, None]
+
+
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 10, 2.0 ** 20, 2.0 ** 24, 2.0 ** 40])
+@pytest.mark.parametrize("t,hq,hkv,L", [(1, 16, 2, 100), (2, 16, 2, 100), (1, 16, 16, 3000)])
+def test_equal_keys_share_the_weight_at_any_score(cuda_device, t, hq, hkv, L, size):
+    """Keys that are all alike have scores that are all alike, however large: each row spreads its unit evenly
+    and its output is the mean of the values, to the bound that scores of ordinary size have."""
+    dev = cuda_device
+    g = _gen(108, dev)
+    k, v = _caches(g, 1, hkv, L, dev)
+    k[:] = k[:, :, :1].clone()
+    q = torch.randn((1, t, hq, D), generator=g, device=dev) * size
+    w = torch.zeros((1, hkv, L), device=dev)
+    out = attention.attention_weights(q, k, v, _i32([L - t], dev), w)
+    seen = (torch.arange(L, device=dev) <= L - t + torch.arange(t, device=dev)[:, None]).double()
+    p = seen / seen.sum(-1, keepdim=True)
+    ref = torch.einsum("tl,bhld->bthd", p, v.double()).repeat_interleave(hq // hkv, 2)
+    _close(out, ref)
+    _close(w, (p.sum(0) * (hq // hkv)).expand(1, hkv, L), "weight")
