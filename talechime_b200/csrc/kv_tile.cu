@@ -2,26 +2,29 @@
 // 64 keys, for kv heads with many rows (wide trees, prompt chunks).
 //
 // Products: f32 operands as pairs of f16 numbers under a power-of-two scale, three
-// tcgen05.mma kind::f16 per product.  x s = hi + lo with a power of two s for each query row and
-// each group of 8 keys or values, which brings the largest |x s| of them into [2^10, 2^14); hi =
-// x s rounded to f16, lo = x s - hi (exact) rounded to f16; a.b = lo.hi + hi.lo + hi.hi.  An
-// element is off by at most 2^-23 of itself or 2^-35 of its group's largest, and the dropped
-// lo.lo is at most 2^-22 of a product.  So f32's exponent range fits.
-// The keys' scales leave with the scores' factor.  The values' scales differ inside a sum: the
-// probabilities of a group are lowered by its scale over the tile's smallest, which leaves one
-// factor for the tile.
+// tcgen05.mma kind::f16 per product.  x s = hi + lo with a power of two s for each row (query, key or
+// value), which brings the row's largest |x s| into [2^2, 2^14); hi = x s rounded to f16, lo = x s - hi
+// (exact) rounded to f16; a.b = lo.hi + hi.lo + hi.hi.  An element is off by at most 2^-23 of itself or
+// 2^-27 of its row's largest, and the dropped lo.lo is at most 2^-22 of a product.  A row's scale
+// depends on other rows only where these are near it in size (row_scales), so a row that a
+// query does not see may hold anything.
+// The keys' scales leave with the scores.  The values' scales differ inside a sum: with 1 / s_j = w_j,
+//   sum_j p_j v_j = 2^(d - 14) sum_j (2^(14 - d) p_j w_j) (v_j s_j),   d = ceil(log2 max_j p_j w_j)
+// over the keys that the row sees, running as the maximum of the scores does.  So a probability is
+// rounded (22 bits) against the largest share that a key the row sees has in its output, and neither
+// unseen values nor heavy keys with small ones take bits from it.
 //
 // One CTA per SM, 16 warps of 128 registers:
 //   * 7 convert, in turn, groups of 8 keys or values: cache rows to registers one group ahead, then
 //     scaled hi / lo to swizzled shared memory, K as [64 keys][128 dims] in two stages, V transposed
-//     as [128 dims][64 keys] in three.  K runs two tiles ahead of V: a V stage is free only after
-//     the PV that follows a softmax, and K behind it would hold up the next QK;
+//     as [128 dims][64 keys] in three.  K and V of a tile behind each other: the softmax needs
+//     the scales of both (K two tiles ahead of V: 64 trees' units 191 us for 189);
 //   * 1 issues the MMAs, S = Q K^T and O = P V (Q and P in TMEM, S and P double-buffered), so that
 //     QK of a tile runs while the softmax of the one before is at work.  Issuing waits for the
 //     tensor cores' queue, most of the tile's MMA time: a warp with other work cannot do it beside;
 //   * 8 softmax: two threads a row, one for each half of the keys and then of the dimensions;
-//     scores from TMEM, running maximum and sum, P' = 2^14 p back to TMEM as hi / lo; then the
-//     O tile of the tile before is added to registers.
+//     scores from TMEM, running maximum, share and sum, P' = 2^(14 - d) p w back to TMEM as hi / lo;
+//     then the O tile of the tile before is added to registers.
 // The tensor cores cut their f32 sums, so an O tile starts from 0 and joins the running sum with
 // rounding.  TMEM (512 columns): Q 128, S 2 x 64, P 2 x 64, O 128.
 //
@@ -46,7 +49,10 @@ constexpr int kKtThreads = 512;
 constexpr int kKtConvertWarp = 8, kKtConverters = 7, kKtMmaWarp = 15;
 constexpr uint32_t kKtTmemCols = 512;
 constexpr uint32_t kTmQ = 0, kTmS = 128, kTmP = 256, kTmO = 384;
-constexpr int kKtPScale = 14;     // P' = 2^14 p
+constexpr int kKtPScale = 14;     // P' = 2^(14 - d) p w
+// A value row's 1 / s is at least this: p' = 2^(14 - d) p fits f32.  (It is reached by rows whose largest
+// value is below 2^-102: they lose bits, under 2^-137 of size each.)
+constexpr int kKtLeastShare = -112;
 
 __device__ unsigned int g_kv_tile_fault;
 __shared__ uint64_t s_kt_wait_ns;
@@ -87,9 +93,10 @@ struct KtCursor {
 struct KtSmem {
   alignas(1024) uint8_t k[2][2][2][kKvTileKeys * 128];  // [stage][hi, lo][64 dims][key][128 B]
   alignas(1024) uint8_t v[3][2][kKvD * 128];            // [stage][hi, lo][dim][64 keys]
-  alignas(16) float ksc[4][8], vsc[4][8];               // inverse scales of the groups of tiles t % 4
+  alignas(16) float ksc[4][kKvTileKeys], vsc[4][kKvTileKeys];  // inverse scales of the rows of tiles t % 4
+  alignas(16) float vlog[4][kKvTileKeys];               // log2 of vsc
   alignas(8) uint8_t vbad[4][8];                        // keys of the tile whose value row is not finite
-  float top[2][2][kKvTileRows];                         // the rows' maxima over either half of a tile
+  alignas(8) float2 top[2][2][kKvTileRows];             // the rows' maxima over either half of a tile
   alignas(8) uint64_t kfull[2], kfree[2], vfull[3], vfree[3];
   uint64_t vinfo[4];
   uint64_t sfull[2], pfull[2], qfull, ofull, ofree, done;
@@ -186,14 +193,12 @@ __device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t (&r)[32]) {
       : "memory");
 #undef KT_OUT
 }
-__device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t (&r)[32]) {
-#define KT_IN(i) "r"(r[i])
+__device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::KT_R32(KT_IN),
-      "r"(addr)
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
       : "memory");
-#undef KT_IN
 }
 __device__ __forceinline__ void tm_ld16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
@@ -212,9 +217,6 @@ __device__ __forceinline__ uint32_t tm_ld1(uint32_t addr) {
   uint32_t r;
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(addr) : "memory");
   return r;
-}
-__device__ __forceinline__ void tm_st1(uint32_t addr, uint32_t r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%1], {%0};" ::"r"(r), "r"(addr) : "memory");
 }
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -238,6 +240,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
   return d;
 }
+__device__ __forceinline__ float2 times(float2 a, float b) { return mul2(a, make_float2(b, b)); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -260,20 +263,53 @@ __device__ __forceinline__ void split_f16(float2 x, uint32_t& hi, uint32_t& lo) 
   const float2 l = fma2(unpack_f16(hi), make_float2(-1.0f, -1.0f), x);
   lo = pack_f16(l.x, l.y);
 }
-// The largest of a tile's inverse scales.
-__device__ __forceinline__ float tile_factor(const float* inv) {
-  const float4 a = *reinterpret_cast<const float4*>(inv), b = *reinterpret_cast<const float4*>(inv + 4);
-  return fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w)));
-}
-// Largest magnitude (bits of a float) -> the scale that brings it into [2^10, 2^14) and its
-// inverse.  Exponents in steps of 4: neighbouring groups mostly agree.
-__device__ __forceinline__ void scale_of(unsigned top, float& scale, float& inverse) {
-  const int e = min(251, 267 - (int)(top >> 23 | 3u));
+// Largest magnitude (bits of a float) -> the scale that brings it into [2^10, 2^14), at most 2^(most -
+// 127), and its inverse.
+__device__ __forceinline__ void scale_of(unsigned top, float& scale, float& inverse, int most = 251) {
+  const int e = min(most, 267 - (int)(min(top, 0x7f7fffffu) >> 23 | 3u));
   scale = __uint_as_float((unsigned)e << 23);
   inverse = __uint_as_float((unsigned)(254 - e) << 23);
 }
 __device__ __forceinline__ float mag(float m, float x) { return fmaxf(m, fabsf(x)); }
+__device__ __forceinline__ float mag4(float m, const float4& v) { return mag(mag(mag(mag(m, v.x), v.y), v.z), v.w); }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// The scale of 8 rows: that of the largest where each row has an element within 2^-8 of it; otherwise (an
+// outlier, a row that is not there) every row is brought to its own scale here and `scale` is 1.  r:
+// whole rows, 4 dimensions a lane (ROWS 8), or row 2 i + lane / 16 in r[2 i], r[2 i + 1] (ROWS 4);
+// m: the lane's largest magnitudes of each.  Returns the inverse of row lane % 8's whole scale.
+template <int ROWS>
+__device__ __forceinline__ float row_scales(float4 (&r)[8], const float (&m)[ROWS], float& scale, bool one_each = false,
+                                            int most = 251) {
+  const int lane = threadIdx.x & 31, up = ROWS == 4 ? lane >> 4 : 0;
+  float all = m[0], inverse;
+#pragma unroll
+  for (int i = 1; i < ROWS; ++i) all = fmaxf(all, m[i]);
+  const unsigned top = __reduce_max_sync(kFull, __float_as_uint(all));
+  const unsigned near = top > (8u << 23) ? top - (8u << 23) : 0u;
+  unsigned has = 0;
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) has |= (__float_as_uint(m[i]) >= near ? 1u : 0u) << (ROWS == 4 ? 2 * i : i);
+  has = __reduce_or_sync(kFull, has << up);
+  scale_of(top, scale, inverse, most);
+  if (__builtin_expect(one_each || has != 255u || top >= 0x7f800000u, one_each)) {
+    unsigned mine = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = ROWS == 8 ? m[e % ROWS] : (e & 1) == up ? m[e / 2 % ROWS] : 0.0f;
+      const unsigned t = __reduce_max_sync(kFull, __float_as_uint(x));
+      if ((lane & 7) == e) mine = t;
+    }
+    scale_of(mine, scale, inverse, most);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float s = __shfl_sync(kFull, scale, ROWS == 8 ? i : (i & ~1) + up);
+      r[i] = make_float4(r[i].x * s, r[i].y * s, r[i].z * s, r[i].w * s);
+    }
+    scale = 1.0f;
+  }
+  return inverse;
+}
 
 // Cache rows pass the SM once: past L1, whose small rest beside 200 KB of shared memory holds
 // the tree's masks and what registers cannot (a reload from L2 is 600 cycles of a warp's time).
@@ -354,8 +390,8 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
 
   if (warp >= kKtConvertWarp && warp < kKtMmaWarp) {
     // ---------------- converters ----------------
-    // The unit's groups in order: K of tile 0, K of tile 1, then V of tile i and K of tile i + 2 in
-    // turn, 8 groups each; warp w takes groups w, w + 7, ..., with no barrier between warps.
+    // The unit's groups in order: K and V of a tile in turn, 8 groups each; warp w takes groups w, w +
+    // 7, ..., with no barrier between warps.
     const int h = lane & 15, ky = lane >> 4;
     KtCursor cur = start;
     bool dead = false;
@@ -366,20 +402,13 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       // dimensions 4 lane .. of row i
       const float4* kp = reinterpret_cast<const float4*>(a.k + (head + ky) * kKvD) + h;
       const float4* vp = reinterpret_cast<const float4*>(a.v + head * kKvD) + lane;
-      const int c0 = cur.off, n = cur.n, items = (2 * n + 1) * 8;
+      const int c0 = cur.off, n = cur.n, items = 16 * n;
       const int plain = MASK == kMaskTree ? x.p : x.keys;  // rows below need no look
-      // item -> tile of the unit, or -1 where there is none
-      auto tile_of = [&](int item) {
-        const int s = item >> 3;
-        const int c = s == 0 ? 0 : s & 1 ? (s + 1) >> 1 : (s - 2) >> 1;
-        return c < n ? c : -1;
-      };
-      auto is_v = [](int item) { return item >= 16 && !((item >> 3) & 1); };
+      auto tile_of = [](int item) { return item >> 4; };
+      auto is_v = [](int item) { return (item & 8) != 0; };
       float4 nx[8] = {};
       auto load = [&](int item) {
-        const int c = tile_of(item);
-        if (c < 0) return;
-        const int j0 = (c0 + c) * kKvTileKeys + (item & 7) * 8;
+        const int j0 = (c0 + tile_of(item)) * kKvTileKeys + (item & 7) * 8;
         if (is_v(item)) {
           const float4* row = vp + (size_t)j0 * (kKvD / 4);
           if (j0 + 8 <= plain) {
@@ -417,77 +446,61 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         for (int i = 0; i < 8; ++i) r[i] = nx[i];
         if (item + kKtConverters < items) load(item + kKtConverters);
         if (item < 0) continue;
-        const int c = tile_of(item), g = item & 7;
-        if (c < 0) continue;
-        const int t = cur.t0 + c;
-        float m = 0.0f, scale, inverse;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = mag(mag(mag(mag(m, r[i].x), r[i].y), r[i].z), r[i].w);
+        const int t = cur.t0 + tile_of(item), g = item & 7;
         if (!is_v(item)) {
           const int s = t & 1;
-          unsigned top = __reduce_max_sync(kFull, __float_as_uint(m));
-          if (__builtin_expect(top >= 0x7f800000u, 0)) {  // an infinite key: the scale of the others
-            m = 0.0f;
+          float m[4], scale;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              m = finite(r[i].x) ? mag(m, r[i].x) : m;
-              m = finite(r[i].y) ? mag(m, r[i].y) : m;
-              m = finite(r[i].z) ? mag(m, r[i].z) : m;
-              m = finite(r[i].w) ? mag(m, r[i].w) : m;
-            }
-            top = __reduce_max_sync(kFull, __float_as_uint(m));
-          }
-          scale_of(top, scale, inverse);
+          for (int i = 0; i < 4; ++i) m[i] = mag4(mag4(0.0f, r[2 * i]), r[2 * i + 1]);
+          const float inverse = row_scales<4>(r, m, scale);
           if (t >= 2 && !dead) dead = !bar_wait(&sm.kfree[s], ((t >> 1) - 1) & 1, abort);
-          const float2 sc = make_float2(scale, scale);
           uint8_t* dst = &sm.k[s][0][h >> 3][(g * 8 + ky) * 128];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint4 hi, lo;
-            split_f16(mul2(lo2(r[2 * i]), sc), hi.x, lo.x);
-            split_f16(mul2(hi2(r[2 * i]), sc), hi.y, lo.y);
-            split_f16(mul2(lo2(r[2 * i + 1]), sc), hi.z, lo.z);
-            split_f16(mul2(hi2(r[2 * i + 1]), sc), hi.w, lo.w);
+            split_f16(times(lo2(r[2 * i]), scale), hi.x, lo.x);
+            split_f16(times(hi2(r[2 * i]), scale), hi.y, lo.y);
+            split_f16(times(lo2(r[2 * i + 1]), scale), hi.z, lo.z);
+            split_f16(times(hi2(r[2 * i + 1]), scale), hi.w, lo.w);
             const int at = i * 256 + (((h & 7) ^ (2 * i + ky)) << 4);
             *reinterpret_cast<uint4*>(dst + at) = hi;
             *reinterpret_cast<uint4*>(dst + sizeof(sm.k[0][0]) + at) = lo;
           }
-          if (lane == 0) sm.ksc[t & 3][g] = inverse;
+          if (lane < 8) sm.ksc[t & 3][g * 8 + lane] = inverse;
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) bar_arrive(&sm.kfull[s]);
         } else {
           const int s = t % 3;
           float2 z = make_float2(0.f, 0.f);  // NaN unless all are finite
+          float m[8], scale;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             z = fma2(lo2(r[i]), make_float2(0.f, 0.f), z);
             z = fma2(hi2(r[i]), make_float2(0.f, 0.f), z);
+            m[i] = mag4(0.0f, r[i]);
           }
-          unsigned top = __reduce_max_sync(kFull, z.x + z.y == 0.0f ? __float_as_uint(m) : 0x7f800000u);
           unsigned bad = 0;
-          if (__builtin_expect(top >= 0x7f800000u, 0)) {
+          if (__builtin_expect(__any_sync(kFull, !(z.x + z.y == 0.0f)), 0)) {
             // 0 * inf must not reach the rows that do not see the key: its value row leaves the
             // product (0) and the rows that see it add it one by one
-            m = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              if (__any_sync(kFull, !(finite(r[i].x) && finite(r[i].y) && finite(r[i].z) && finite(r[i].w)))) {
+              const bool x = finite(r[i].x), y = finite(r[i].y), zz = finite(r[i].z), w = finite(r[i].w);
+              m[i] = mag4(0.0f, make_float4(x ? r[i].x : 0.f, y ? r[i].y : 0.f, zz ? r[i].z : 0.f, w ? r[i].w : 0.f));
+              if (__any_sync(kFull, !(x && y && zz && w))) {
                 r[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                 bad |= 1u << i;
               }
-              m = mag(mag(mag(mag(m, r[i].x), r[i].y), r[i].z), r[i].w);
             }
-            top = __reduce_max_sync(kFull, __float_as_uint(m));
           }
-          scale_of(top, scale, inverse);
+          const float inverse = row_scales<8>(r, m, scale, false, 127 - kKtLeastShare);
           if (t >= 3 && !dead) dead = !bar_wait(&sm.vfree[s], (t / 3 - 1) & 1, abort);
-          const float2 sc = make_float2(scale, scale);
           // dimension 4 lane + e sits in row 32 e + lane, the group's 8 keys in one piece of it
           uint8_t* dst = &sm.v[s][0][lane * 128 + ((g ^ (lane & 7)) << 4)];
           auto put = [&](int e, float2 w0, float2 w1, float2 w2, float2 w3, float2 w4, float2 w5, float2 w6, float2 w7) {
-            const float2 w[8] = {mul2(w0, sc), mul2(w1, sc), mul2(w2, sc), mul2(w3, sc),
-                                 mul2(w4, sc), mul2(w5, sc), mul2(w6, sc), mul2(w7, sc)};
+            const float2 w[8] = {times(w0, scale), times(w1, scale), times(w2, scale), times(w3, scale),
+                                 times(w4, scale), times(w5, scale), times(w6, scale), times(w7, scale)};
             uint32_t h0[4], h1[4], l0[4], l1[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -503,10 +516,11 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
           };
           put(0, lo2(r[0]), lo2(r[1]), lo2(r[2]), lo2(r[3]), lo2(r[4]), lo2(r[5]), lo2(r[6]), lo2(r[7]));
           put(2, hi2(r[0]), hi2(r[1]), hi2(r[2]), hi2(r[3]), hi2(r[4]), hi2(r[5]), hi2(r[6]), hi2(r[7]));
-          if (lane == 0) {
-            sm.vsc[t & 3][g] = inverse;
-            sm.vbad[t & 3][g] = (uint8_t)bad;
+          if (lane < 8) {
+            sm.vsc[t & 3][g * 8 + lane] = inverse;
+            sm.vlog[t & 3][g * 8 + lane] = (float)((int)(__float_as_uint(inverse) >> 23) - 127);
           }
+          if (lane == 0) sm.vbad[t & 3][g] = (uint8_t)bad;
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
@@ -632,12 +646,12 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         float m = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) m = mag(mag(mag(mag(m, mine4[i].x), mine4[i].y), mine4[i].z), mine4[i].w);
-        sm.top[0][half][row] = m;
+        sm.top[0][half][row].x = m;
         meet();
-        m = fmaxf(m, sm.top[0][half ^ 1][row]);
+        m = fmaxf(m, sm.top[0][half ^ 1][row].x);
         meet();
         float scale;
-        scale_of(min(__float_as_uint(m), 0x7f7fffffu), scale, qinv);
+        scale_of(__float_as_uint(m), scale, qinv);
         const float2 sc = make_float2(scale, scale);
 #pragma unroll
         for (int part = 0; part < 4; ++part) {
@@ -661,16 +675,18 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       float2 o[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) o[i] = make_float2(0.f, 0.f);
-      float m = -INFINITY, l = 0.0f, corr = 0.0f;
+      // o stands for sum p v 2^(14 - share) against the maximum m, l for sum p
+      float m = -INFINITY, share = kKtLeastShare, l = 0.0f, corr = 0.0f;
+      constexpr float kLeastFactor = 1.17549435e-38f;  // a factor of 0 would make NaN of -inf
+      const float cq = fmaxf(a.c * qinv, kLeastFactor);
       // tiles from this one on hold a key that some row of the unit does not see
       const int tend = cur.t0 + cur.n, tmask = cur.t0 - cur.off + (MASK == kMaskTree ? x.p : x.p + x.i0 + 1) / kKvTileKeys;
-      // o = o * f + the O tile of tile w, whose P stood against the maximum of then
+      // o = o * f + the O tile of tile w, whose P stood against the maximum and the share of then
       // (the tile's scales are still in place: their next writer waits for the PV after this)
       auto add_o = [&](int w, float f) {
         wait(&sm.ofull, w & 1);
         tc_after();
-        const float fv = tile_factor(sm.vsc[w & 3]);
-        const float2 f2 = make_float2(f, f), v2 = make_float2(fv, fv);
+        const float2 f2 = make_float2(f, f);
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
           uint32_t r[32];
@@ -679,8 +695,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             o[part * 16 + i] =
-                fma2(o[part * 16 + i], f2,
-                     mul2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), v2));
+                fma2(o[part * 16 + i], f2, make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])));
         }
         if (const unsigned long long bad = *reinterpret_cast<const unsigned long long*>(&sm.vbad[w & 3][0])) {
           const float2* vb = reinterpret_cast<const float2*>(
@@ -692,8 +707,9 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
             const uint32_t lo = tm_ld1(mine + kTmP + 64 * (w & 1) + 32 + (key >> 1));
             tm_wait_ld();
             const int sh = (key & 1) * 16;
-            const float p = __half2float(__ushort_as_half((unsigned short)(hi >> sh))) +
-                            __half2float(__ushort_as_half((unsigned short)(lo >> sh)));
+            float p = __half2float(__ushort_as_half((unsigned short)(hi >> sh))) +
+                      __half2float(__ushort_as_half((unsigned short)(lo >> sh)));
+            p *= __uint_as_float((254u << 23) - __float_as_uint(sm.vsc[w & 3][key]));  // over a power of 2
             if (p != 0.0f) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
@@ -721,89 +737,90 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         if (MASK == kMaskTree && t >= tmask) look();  // its loads beside the wait
         wait(&sm.sfull[s], (t >> 1) & 1);
         tc_after();
-        const float cq = a.c * qinv;
-        constexpr float kLeastFactor = 1.17549435e-38f;  // a factor of 0 would make NaN of -inf
-        float top = -INFINITY;
-        {
-          const float4 k4 = *reinterpret_cast<const float4*>(&sm.ksc[t & 3][4 * half]);
-          const float cc[4] = {fmaxf(cq * k4.x, kLeastFactor), fmaxf(cq * k4.y, kLeastFactor),
-                               fmaxf(cq * k4.z, kLeastFactor), fmaxf(cq * k4.w, kLeastFactor)};
-          uint32_t r[32];
-          tm_ld32(sat, r);
+        wait(&sm.vinfo[t & 3], (t >> 2) & 1);
+        float top = -INFINITY, heavy = -INFINITY;  // of the scores x, and of x - top + log2 w
+        if (t >= tmask && MASK != kMaskTree) look();
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {
+          uint32_t r[16];
+          float2 x[8];
+          tm_ld16(sat + 16 * part, r);
           tm_wait_ld();
           if (t >= tmask) {
-            if (MASK != kMaskTree) look();
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((see >> e) & 1u)) r[e] = 0xff800000u;  // -inf, back in TMEM for the second pass
-            tm_st32(sat, r);
-            tm_wait_st();
+            for (int e = 0; e < 16; ++e)
+              if (!((see >> (16 * part + e)) & 1u)) r[e] = 0xff800000u;  // -inf
           }
+          // a key's scale, then the query's: one power of two of both may be 0.  Scores are rounded here, so
+          // that the largest is the maximum itself at any size.
 #pragma unroll
-          for (int gi = 0; gi < 4; ++gi) {
-            float y = __uint_as_float(r[8 * gi]);
+          for (int e = 0; e < 4; ++e) {
+            const float4 k4 = *reinterpret_cast<const float4*>(&sm.ksc[t & 3][32 * half + 16 * part + 4 * e]);
+            x[2 * e] = times(mul2(make_float2(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1])), lo2(k4)), cq);
+            x[2 * e + 1] =
+                times(mul2(make_float2(__uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3])), hi2(k4)), cq);
+          }
+          float up = top;
 #pragma unroll
-            for (int e = 1; e < 8; ++e) y = fmaxf(y, __uint_as_float(r[8 * gi + e]));
-            top = fmaxf(top, y * cc[gi]);
+          for (int e = 0; e < 8; ++e) {
+            up = fmaxf(fmaxf(up, x[e].x), x[e].y);
+            r[2 * e] = __float_as_uint(x[e].x);
+            r[2 * e + 1] = __float_as_uint(x[e].y);
+          }
+          tm_st16(sat + 16 * part, r);  // for the second pass
+          const float h = up == -INFINITY ? 0.0f : -up;
+          heavy += top + h;
+          top = up;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float4 w4 = *reinterpret_cast<const float4*>(&sm.vlog[t & 3][32 * half + 16 * part + 4 * e]);
+            const float2 y = add2(add2(x[2 * e], make_float2(h, h)), lo2(w4));
+            const float2 z = add2(add2(x[2 * e + 1], make_float2(h, h)), hi2(w4));
+            heavy = fmaxf(fmaxf(heavy, y.x), y.y);
+            heavy = fmaxf(fmaxf(heavy, z.x), z.y);
           }
         }
-        sm.top[s][half][row] = top;
+        tm_wait_st();
+        sm.top[s][half][row] = make_float2(top, heavy);
         meet();
-        const float n_m = fmaxf(m, fmaxf(top, sm.top[s][half ^ 1][row]));
-        const float base = n_m == -INFINITY ? 0.0f : n_m;
-        next = ex2(m - base);
+        // maximum and share in whole powers of two: what stands against them is rescaled without rounding
+        const float2 other = sm.top[s][half ^ 1][row];
+        const float n_m = fmaxf(m, ceilf(fmaxf(top, other.x)));
+        const float base = n_m == -INFINITY ? 0.0f : n_m, fall = m - base;
+        const float n_share = fmaxf(fmaxf(share + fall, (float)kKtLeastShare),
+                                    ceilf(fmaxf(heavy + (top - base), other.y + (other.x - base))));
+        next = ex2(share + fall - n_share);
+        l *= ex2(fall);
         m = n_m;
-        // the values' scales: the largest inverse is the tile's factor, each group's share of it
-        // (1 but for groups of another magnitude) goes to its probabilities
-        wait(&sm.vinfo[t & 3], (t >> 2) & 1);
-        const float vi = __uint_as_float((254u << 23) - __float_as_uint(tile_factor(sm.vsc[t & 3])));  // 1 / a power of 2
-        const float b14 = kKtPScale - base;
+        share = n_share;
+        const float2 b2 = make_float2(-base, -base);
+        const float lift = ex2(kKtPScale - share);
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll 1
         for (int part = 0; part < 2; ++part) {
           uint32_t r[16], hi[8], lo[8];
           tm_ld16(sat + 16 * part, r);
-          const float2 k2 = *reinterpret_cast<const float2*>(&sm.ksc[t & 3][4 * half + 2 * part]);
-          const float2 v2 = *reinterpret_cast<const float2*>(&sm.vsc[t & 3][4 * half + 2 * part]);
-          const float c0 = fmaxf(cq * k2.x, kLeastFactor), c8 = fmaxf(cq * k2.y, kLeastFactor);
           tm_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float c1 = e < 4 ? c0 : c8, sh = e < 4 ? v2.x * vi : v2.y * vi;
-            float2 p = fma2(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), make_float2(c1, c1),
-                            make_float2(b14, b14));
-            p.x = ex2(p.x);
-            p.y = ex2(p.y);
-            sum = add2(sum, p);
-            split_f16(mul2(p, make_float2(sh, sh)), hi[e], lo[e]);
+          for (int e = 0; e < 8; e += 2) {
+            const float4 w4 = *reinterpret_cast<const float4*>(&sm.vsc[t & 3][32 * half + 16 * part + 2 * e]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float2 p = add2(make_float2(__uint_as_float(r[2 * (e + i)]), __uint_as_float(r[2 * (e + i) + 1])), b2);
+              p.x = ex2(p.x);
+              p.y = ex2(p.y);
+              sum = add2(sum, p);
+              split_f16(times(mul2(p, i ? hi2(w4) : lo2(w4)), lift), hi[e + i], lo[e + i]);
+            }
           }
           tm_st8(mine + kTmP + 64 * s + 16 * half + 8 * part, hi);
           tm_st8(mine + kTmP + 64 * s + 32 + 16 * half + 8 * part, lo);
-        }
-        if (const unsigned long long bad_t = *reinterpret_cast<const unsigned long long*>(&sm.vbad[t & 3][0])) {
-          // a key whose value row is left out keeps its probability as it is, for add_o
-          tm_wait_st();
-#pragma unroll 1
-          for (int e = 0; e < 32; ++e) {
-            if (!((bad_t >> (32 * half + e)) & 1)) continue;
-            const uint32_t at = mine + kTmP + 64 * s + 16 * half + (e >> 1);
-            const uint32_t sv = tm_ld1(sat + e), ph = tm_ld1(at), pl = tm_ld1(at + 32);
-            tm_wait_ld();
-            const float p = ex2(fmaf(__uint_as_float(sv), fmaxf(a.c * qinv * sm.ksc[t & 3][4 * half + (e >> 3)],
-                                                                1.17549435e-38f), b14));
-            uint32_t hi, lo;
-            split_f16(make_float2(p, p), hi, lo);
-            const uint32_t mask = e & 1 ? 0xffff0000u : 0xffffu;
-            tm_st1(at, (ph & ~mask) | (hi & mask));
-            tm_st1(at + 32, (pl & ~mask) | (lo & mask));
-            tm_wait_st();
-          }
         }
         tm_wait_st();
         tc_before();
         __syncwarp();
         if (lane == 0) bar_arrive(&sm.pfull[s]);
-        l = fmaf(l, next, sum.x + sum.y);
+        l += sum.x + sum.y;
         }
         if (t > cur.t0) add_o(t - 1, corr);
         if (t == tend) break;
@@ -812,18 +829,17 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       // the row's sum over both halves (the maxima's place is free: the last tile's was read
       // before its P was given away, and t moves on)
       meet();
-      sm.top[0][half][row] = l;
+      sm.top[0][half][row].x = l;
       meet();
-      l = sm.top[0][0][row] + sm.top[0][1][row];
+      l = sm.top[0][0][row].x + sm.top[0][1][row].x;
       meet();
       // the row: whole, or this CTA's part of it
       const bool whole = cur.off == 0 && cur.n == x.chunks;
       const size_t slot = 2 * (size_t)blockIdx.x + (cur.off > 0 ? 0 : 1);
       const float nan = __uint_as_float(0x7fffffffu);
       if (!kv_row_valid<MASK>(a, x, row)) m = -INFINITY;
-      constexpr float kUnscale = 1.0f / (1 << kKtPScale);  // P' = 2^14 p is in both sums
-      float f = kUnscale;
-      if (whole) f = m == -INFINITY ? 0.0f : __fdiv_rn(1.0f, l);
+      float f = ex2(share - kKtPScale);
+      if (whole) f = m == -INFINITY ? 0.0f : __fdiv_rn(f, l);
       ok = ok && !*abort;  // another warp that went on without its data
       if (!ok) f = nan;
       {
@@ -861,11 +877,11 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         if (half == 0) {
           if (!whole) {
             a.stat[slot * 2 * a.rows + row] = m;
-            a.stat[(slot * 2 + 1) * a.rows + row] = ok ? l * kUnscale : nan;
+            a.stat[(slot * 2 + 1) * a.rows + row] = ok ? l : nan;
           }
           if (a.lse && whole)
             a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] =
-                m == -INFINITY ? INFINITY : m + log2f(l) - kKtPScale;
+                m == -INFINITY ? INFINITY : m + log2f(l);
         }
       }
     }
@@ -1063,7 +1079,7 @@ kv_column_tile_kernel(const KvArgs a, float* weight, float* __restrict__ part, u
       float m = 0.0f, scale, inverse;
 #pragma unroll
       for (int i = 0; i < 8; ++i) m = mag(mag(mag(mag(m, qr[i].x), qr[i].y), qr[i].z), qr[i].w);
-      scale_of(min(__reduce_max_sync(kFull, __float_as_uint(m)), 0x7f7fffffu), scale, inverse);
+      scale_of(__reduce_max_sync(kFull, __float_as_uint(m)), scale, inverse);
       if (t >= 2 && !dead) dead = !bar_wait(&sm.qfree[s], ((t >> 1) - 1) & 1, abort);
       const float2 sc = make_float2(scale, scale);
       uint8_t* dst = &sm.q[s][0][h >> 3][(cw * 8 + ky) * 128];
@@ -1129,7 +1145,7 @@ kv_column_tile_kernel(const KvArgs a, float* weight, float* __restrict__ part, u
         if (i == lane) m = top;
       }
       float scale;
-      scale_of(min(m, 0x7f7fffffu), scale, kinv);
+      scale_of(m, scale, kinv);
       const float2 sc = make_float2(scale, scale);
       float4* turn = reinterpret_cast<float4*>(&sm.turn[warp][0]);
 #pragma unroll

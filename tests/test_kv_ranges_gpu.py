@@ -1,16 +1,25 @@
 """Sizes of queries, keys and values in the attention kernels over the KV caches: what a row does not
-see may be of any size and does not move its result.  Bounds: those of tests/test_kv_attention_gpu.py."""
+see may be of any size, what it sees may differ in size from key to key, and neither moves its result
+beyond the error of its own scores.
+
+Bounds.  Scores of ordinary size are held to the bound of tests/test_kv_attention_gpu.py.  Where scores
+reach S in size, a score is a rounded product of two rounded operands, three halves of an f32 step (2^-24
+of S each) and as much again for the pairs that the operands are split into (below 2^-22 of S): under
+1.5 * 2^-21 * S, which is the relative error of its probability and, over rows of 128 dimensions
+that all move together, at most that of the output: 1.5 * 2^-21 * S + 1e-5."""
+import math
+
 import pytest
 import torch
 
 from talechime_b200 import attention
-from test_kv_attention_gpu import D, _caches, _close, _gen, _i32, _paths, _tables, _tree_ref, _weights_ref
+from test_kv_attention_gpu import (D, REL_L2, ROOMY, _caches, _close, _gen, _i32, _paths, _tables, _tree_ref, _weights_ref)
 
 pytestmark = pytest.mark.gpu
 
 MAX = torch.finfo(torch.float32).max
 SIZES = [2.0 ** 16, 2.0 ** 24, 2.0 ** 36, 1e30, MAX]
-FORMS = [(12, 4, 2, 100), (40, 16, 2, 100)]
+FORMS = [(12, 4, 2, 100), (40, 16, 2, 100), (40, 16, 2, ROOMY)]  # 16-row kernel, twice; tensor-core kernel
 
 
 def _grow(x, size):
@@ -42,7 +51,7 @@ def test_tree_rows_beside_unseen_rows_of_any_size(cuda_device, n, hq, hkv, max_t
 
 
 @pytest.mark.parametrize("size", SIZES)
-@pytest.mark.parametrize("t,hq,hkv,p0", [(3, 4, 2, 20), (3, 16, 4, 0)])
+@pytest.mark.parametrize("t,hq,hkv,p0", [(3, 4, 2, 20), (3, 16, 4, 0), (40, 4, 2, 20), (70, 16, 2, 0)])
 def test_prompt_rows_before_larger_rows(cuda_device, t, hq, hkv, p0, size):
     """Rows in front of far larger ones, the first of a prompt among them: two later rows whose keys and
     values are that much larger leave the outputs before them as they are."""
@@ -90,3 +99,76 @@ def test_equal_keys_share_the_weight_at_any_score(cuda_device, t, hq, hkv, L, si
     ref = torch.einsum("tl,bhld->bthd", p, v.double()).repeat_interleave(hq // hkv, 2)
     _close(out, ref)
     _close(w, (p.sum(0) * (hq // hkv)).expand(1, hkv, L), "weight")
+
+
+@pytest.mark.parametrize("t", [1, 40])
+@pytest.mark.parametrize("kind", ["alternating", "by_tile", "by_range"])
+def test_small_weights_of_large_values(cuda_device, t, kind):
+    """Keys of low score with values as much larger: their share of the output is that of the others,
+    beside each other in the cache, in tiles of their own, and over the whole of a long cache."""
+    dev, hq, hkv, L = cuda_device, 16, 2, 700
+    j = torch.arange(L, device=dev)
+    S = 20.0  # values 2^29 times larger
+    drop = {"alternating": (j % 2) * S, "by_tile": (j // 64 % 2) * S, "by_range": (j < 350) * S}[kind].float()
+    q, k, v = _graded(dev, t, hq, hkv, L, drop, 103)
+    w = torch.zeros((1, hkv, L), device=dev)
+    ref, wref = _weights_ref(q, k, v, [L - t], w)
+    out = attention.attention_weights(q, k, v, _i32([L - t], dev), w)
+    bound = 1.5 * 2.0 ** -21 * S + REL_L2
+    for i in range(t):
+        assert float((out[0, i].double() - ref[0, i]).norm() / ref[0, i].norm()) <= bound, i
+    assert float((w.double() - wref).norm() / wref.norm()) <= bound
+
+
+@pytest.mark.parametrize("t", [1, 40])
+@pytest.mark.parametrize("small", [0.0, 1e-12, 1e-30])
+def test_heavy_keys_with_small_values(cuda_device, t, small):
+    """Keys that take all but 2^-43 of the weight, with values that are zero or next to it: the output is
+    the other keys' and has its accuracy."""
+    dev, hq, hkv, L = cuda_device, 16, 2, 300
+    S = 30.0
+    drop = torch.full((L,), S, device=dev)
+    heavy = [0, 1, 70, 77]
+    drop[heavy] = 0.0
+    q, k, v = _graded(dev, t, hq, hkv, L, drop, 104)
+    v = v / math.exp(S)
+    v[:, :, heavy] *= small * math.exp(S)
+    w = torch.zeros((1, hkv, L), device=dev)
+    ref, _ = _weights_ref(q, k, v, [L - t], w)
+    out = attention.attention_weights(q, k, v, _i32([L - t], dev), w)
+    for i in range(t):
+        assert float((out[0, i].double() - ref[0, i]).norm() / ref[0, i].norm()) <= 1.5 * 2.0 ** -21 * S + REL_L2, i
+
+
+@pytest.mark.parametrize("qs,ks,vs", [(1e-18, 1e18, 1e30), (1e12, 1e-12, 1e-30), (1e-12, 1e12, 1e-25), (1.0, 1.0, 1e36)])
+@pytest.mark.parametrize("t,L", [(1, 70), (40, 70), (40, 1500)])
+def test_large_and_small_numbers_in_prompts(cuda_device, t, L, qs, ks, vs):
+    """Queries, keys and values of very different sizes whose scores are ordinary, in a cache that one CTA
+    takes whole and in one that several share."""
+    dev, hq, hkv = cuda_device, 16, 2
+    g = _gen(105, dev)
+    k, v = _caches(g, 1, hkv, L, dev)
+    q = torch.randn((1, t, hq, D), generator=g, device=dev)
+    q, k, v = q * qs, k * ks, v * vs
+    w = torch.zeros((1, hkv, L), device=dev)
+    ref, wref = _weights_ref(q, k, v, [L - t], w)
+    out = attention.attention_weights(q, k, v, _i32([L - t], dev), w)
+    assert float((out.double() - ref).norm() / ref.norm()) <= REL_L2
+    _close(w, wref, "weight")
+
+
+def test_tree_of_one_path_among_many_sizes(cuda_device):
+    """Nodes that grow by 2^10 from child to child: a node sees only smaller ones and itself, and its
+    output is its own size's."""
+    dev, n, hq, hkv, max_t, p0 = cuda_device, 12, 32, 2, ROOMY, 64
+    g = _gen(107, dev)
+    k, v = _caches(g, 1, hkv, max_t, dev)
+    qkv = torch.randn((1, n, (hq + 2 * hkv) * D), generator=g, device=dev)
+    size = torch.exp2(10.0 * torch.arange(n, device=dev))
+    qkv.view(1, n, -1, D)[..., hq + hkv:, :] *= size[:, None, None]
+    cos, sin = _tables(max_t, dev)
+    parents = _i32([list(range(-1, n - 1))], dev)
+    ref, _, _ = _tree_ref(qkv, parents, [p0], cos, sin, k, v, hq)
+    out = attention.rope_attention_tree(qkv, parents, _i32([p0], dev), cos, sin, k, v)
+    for i in range(n):
+        _close(out[0, i], ref[0, i], str(i))
