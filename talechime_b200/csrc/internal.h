@@ -190,7 +190,7 @@ cudaError_t launch_attention_blocks(const float* q, const float* kc, const float
 // The tcgen05 form of the core for units of 128 rows (kv_tile.cu); mask: KvMask, not blocks.
 struct KvArgs;
 cudaError_t launch_kv_tile(const KvArgs& a, int mask, int device, cudaStream_t s);
-// Column sums of the softmax from the rows' log2 sums (a.lse); `part`: its scratch.
+// Column sums of the softmax from the rows' maxima and sums (a.norm, a.qscale); `part`: its scratch.
 size_t kv_column_tile_bytes(int batch, int n, int hq, int hkv, int max_t);
 cudaError_t launch_kv_column_tile(const KvArgs& a, float* weight, float* part, int device, cudaStream_t s);
 cudaError_t read_kv_tile_fault(unsigned int* flags, bool clear);  // bit 5

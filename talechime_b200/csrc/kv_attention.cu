@@ -777,7 +777,7 @@ size_t attention_weights_workspace_bytes(int batch, int n, int hq, int hkv, int 
   const KvPlan p = kv_plan((int64_t)batch * hkv, (int64_t)n * group, true);
   const bool stored = weights_stored(n, group);
   return core_bytes(p, stored) + (stored ? up256((size_t)batch * hq * n * score_stride(max_t) * 4)
-                                         : up256((size_t)batch * hq * n * 4) +
+                                         : up256((size_t)batch * hq * n * 8) + up256((size_t)batch * hq * n * 4) +
                                                up256(kv_column_tile_bytes(batch, n, hq, hkv, max_t)));
 }
 
@@ -796,10 +796,12 @@ cudaError_t launch_attention_weights(const float* q, const float* kc, const floa
     a.weight_reps = (int)(groups / 1184 < 1 ? 1 : groups / 1184 > 16 ? 16 : groups / 1184);
     return launch_core<kMaskCausal>(a, weight, device, s);
   }
-  a.lse = reinterpret_cast<float*>(w);
+  a.norm = reinterpret_cast<float2*>(w);
+  w += up256((size_t)batch * hq * n * 8);
+  a.qscale = reinterpret_cast<float*>(w);
+  w += up256((size_t)batch * hq * n * 4);
   cudaError_t e = launch_kv_tile(a, kMaskCausal, device, s);
   if (e != cudaSuccess) return e;
-  w += up256((size_t)batch * hq * n * 4);
   return launch_kv_column_tile(a, weight, reinterpret_cast<float*>(w), device, s);
 }
 

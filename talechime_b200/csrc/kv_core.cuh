@@ -35,7 +35,8 @@ struct KvArgs {
   float* stat;            // [slot][2][rows] its maxima and sums
   float* scores;          // causal with weights, n * group <= 16: [batch][hkv][n * group][score_stride]
   int2* begun;            // split: where a unit's parts are, for the merge
-  float* lse;             // causal with weights, else: [batch][hkv][n * group] log2 of the row's sum
+  float2* norm;           // causal with weights, else: [batch][hkv][n * group] the row's maximum and 1 / sum
+  float* qscale;          // and the power of two that its query went into the products under
   int batch, n, hq, hkv, group, max_t;
   int words, topk, block, score_stride;
   int rows;               // rows of a unit: 8, 16 or 128

@@ -163,16 +163,17 @@ __device__ __forceinline__ bool elected() {
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(su32(bar)) : "memory");
 }
-// D = A B^T over 16 STEPS columns as lo.hi + hi.lo + hi.hi; HALF: bytes from B's first 64 columns to
-// the next.  The three run through one piece of code: the roles' loops fill the instruction caches.
-template <int STEPS, int HALF>
+// D = A B^T over 16 STEPS columns as lo.hi + hi.lo + hi.hi, SWAP: as hi.lo + lo.hi + hi.hi, which for A and
+// B exchanged is the same sum in the same order.  HALF: bytes from B's first 64 columns to the next.
+// The three run through one piece of code: the roles' loops fill the instruction caches.
+template <int STEPS, int HALF, bool SWAP = false>
 __device__ __forceinline__ void mma_pairs(uint32_t d, uint32_t ah, uint32_t al, const void* bh, const void* bl,
                                           uint32_t idesc) {
   const uint64_t dh = desc_sw128(bh), dl = desc_sw128(bl);
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
-    const uint32_t a = pass == 0 ? al : ah;
-    const uint64_t b = pass == 1 ? dl : dh;
+    const uint32_t a = pass == (SWAP ? 1 : 0) ? al : ah;
+    const uint64_t b = pass == (SWAP ? 0 : 1) ? dl : dh;
 #pragma unroll
     for (int kk = 0; kk < STEPS; ++kk)
       mma_ts(d, a + 8 * kk, b + 2 * (kk & 3) + (kk >> 2) * (HALF >> 4), idesc, pass + kk > 0);
@@ -274,25 +275,26 @@ __device__ __forceinline__ float mag(float m, float x) { return fmaxf(m, fabsf(x
 __device__ __forceinline__ float mag4(float m, const float4& v) { return mag(mag(mag(mag(m, v.x), v.y), v.z), v.w); }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
+// 2^-8 of a largest magnitude (bits of a float); 0 where that is no normal number.
+__device__ __forceinline__ unsigned near_of(unsigned top) { return top > (8u << 23) ? top - (8u << 23) : 0u; }
 // The scale of 8 rows: that of the largest where each row has an element within 2^-8 of it; otherwise (an
 // outlier, a row that is not there) every row is brought to its own scale here and `scale` is 1.  r:
 // whole rows, 4 dimensions a lane (ROWS 8), or row 2 i + lane / 16 in r[2 i], r[2 i + 1] (ROWS 4);
 // m: the lane's largest magnitudes of each.  Returns the inverse of row lane % 8's whole scale.
 template <int ROWS>
-__device__ __forceinline__ float row_scales(float4 (&r)[8], const float (&m)[ROWS], float& scale, bool one_each = false,
-                                            int most = 251) {
+__device__ __forceinline__ float row_scales(float4 (&r)[8], const float (&m)[ROWS], float& scale, int most = 251) {
   const int lane = threadIdx.x & 31, up = ROWS == 4 ? lane >> 4 : 0;
   float all = m[0], inverse;
 #pragma unroll
   for (int i = 1; i < ROWS; ++i) all = fmaxf(all, m[i]);
   const unsigned top = __reduce_max_sync(kFull, __float_as_uint(all));
-  const unsigned near = top > (8u << 23) ? top - (8u << 23) : 0u;
+  const unsigned near = near_of(top);
   unsigned has = 0;
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) has |= (__float_as_uint(m[i]) >= near ? 1u : 0u) << (ROWS == 4 ? 2 * i : i);
   has = __reduce_or_sync(kFull, has << up);
   scale_of(top, scale, inverse, most);
-  if (__builtin_expect(one_each || has != 255u || top >= 0x7f800000u, one_each)) {
+  if (__builtin_expect(has != 255u || top >= 0x7f800000u, 0)) {
     unsigned mine = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -337,6 +339,15 @@ __device__ __noinline__ int kt_find(KvFind& find, const int* pos, int n, int hkv
   a.least = kKvTileLeast;
   a.pass = kKvTilePass;
   return kv_find<MASK, kKtThreads>(a, find, blockIdx.x);
+}
+
+constexpr float kLeastFactor = 1.17549435e-38f;  // a factor of 0 would make NaN of -inf
+// A row's maximum and the inverse of its sum; a row that sees nothing gives no key a weight.
+__device__ __forceinline__ float2 row_norm(float m, float l) {
+  return m == -INFINITY ? make_float2(INFINITY, 0.0f) : make_float2(m, __fdiv_rn(1.0f, l));
+}
+__device__ __forceinline__ size_t kv_row_number(const KvArgs& a, const KvUnit& x, int row) {
+  return ((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row;
 }
 
 template <int MASK>
@@ -403,7 +414,13 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       const float4* kp = reinterpret_cast<const float4*>(a.k + (head + ky) * kKvD) + h;
       const float4* vp = reinterpret_cast<const float4*>(a.v + head * kKvD) + lane;
       const int c0 = cur.off, n = cur.n, items = 16 * n;
-      const int plain = MASK == kMaskTree ? x.p : x.keys;  // rows below need no look
+      // Rows below `plain` need no look.  Causal units read all the rows that were appended, also those behind
+      // their own last: a key's scale depends on the group it is in, and all units have to agree on it.
+      const int plain = MASK == kMaskTree ? x.p : min(x.p + a.n, a.max_t);
+      auto rows_there = [&](int j0) {
+        if (MASK == kMaskTree) return kv_rows_there<MASK>(a, x, j0);
+        return __ballot_sync(kFull, j0 + lane < plain);
+      };
       auto tile_of = [](int item) { return item >> 4; };
       auto is_v = [](int item) { return (item & 8) != 0; };
       float4 nx[8] = {};
@@ -415,7 +432,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
 #pragma unroll
             for (int i = 0; i < 8; ++i) nx[i] = ld_row(row + i * 32);
           } else {
-            const uint32_t there = kv_rows_there<MASK>(a, x, j0);
+            const uint32_t there = rows_there(j0);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
               nx[i] = (there >> i) & 1u ? ld_row(row + i * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -429,7 +446,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
               nx[2 * i + 1] = ld_row(row + i * 64 + 16);
             }
           } else {
-            const uint32_t rows = kv_rows_there<MASK>(a, x, j0) >> ky;
+            const uint32_t rows = rows_there(j0) >> ky;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const bool there = (rows >> (2 * i)) & 1u;
@@ -494,7 +511,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
               }
             }
           }
-          const float inverse = row_scales<8>(r, m, scale, false, 127 - kKtLeastShare);
+          const float inverse = row_scales<8>(r, m, scale, 127 - kKtLeastShare);
           if (t >= 3 && !dead) dead = !bar_wait(&sm.vfree[s], (t / 3 - 1) & 1, abort);
           // dimension 4 lane + e sits in row 32 e + lane, the group's 8 keys in one piece of it
           uint8_t* dst = &sm.v[s][0][lane * 128 + ((g ^ (lane & 7)) << 4)];
@@ -598,7 +615,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         float4* dst = reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, row));
 #pragma unroll 1
         for (int i = 0; i < kKvD / 4; ++i) dst[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (a.lse) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] = INFINITY;
+        if (a.norm) a.norm[kv_row_number(a, x, row)] = make_float2(INFINITY, 0.0f);
       }
     // The warp's cursor is one object of its 32 lanes: one of them moves it on, between the others' last
     // look at the unit behind and their first at the next.
@@ -652,6 +669,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         meet();
         float scale;
         scale_of(__float_as_uint(m), scale, qinv);
+        if (a.norm && cur.off == 0 && half == 0 && row < x.nrows) a.qscale[kv_row_number(a, x, row)] = scale;
         const float2 sc = make_float2(scale, scale);
 #pragma unroll
         for (int part = 0; part < 4; ++part) {
@@ -677,7 +695,6 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       for (int i = 0; i < 32; ++i) o[i] = make_float2(0.f, 0.f);
       // o stands for sum p v 2^(14 - share) against the maximum m, l for sum p
       float m = -INFINITY, share = kKtLeastShare, l = 0.0f, corr = 0.0f;
-      constexpr float kLeastFactor = 1.17549435e-38f;  // a factor of 0 would make NaN of -inf
       const float cq = fmaxf(a.c * qinv, kLeastFactor);
       // tiles from this one on hold a key that some row of the unit does not see
       const int tend = cur.t0 + cur.n, tmask = cur.t0 - cur.off + (MASK == kMaskTree ? x.p : x.p + x.i0 + 1) / kKvTileKeys;
@@ -879,9 +896,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
             a.stat[slot * 2 * a.rows + row] = m;
             a.stat[(slot * 2 + 1) * a.rows + row] = ok ? l : nan;
           }
-          if (a.lse && whole)
-            a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row] =
-                m == -INFINITY ? INFINITY : m + log2f(l);
+          if (a.norm && whole) a.norm[kv_row_number(a, x, row)] = row_norm(m, l);
         }
       }
     }
@@ -909,7 +924,7 @@ __global__ void __launch_bounds__(kKtMergeWarps * 32) kv_tile_merge_kernel(const
   if (x.chunks == 0) {  // no CTA came by
     for (int r = r0; r < min(r0 + EACH, x.nrows); ++r) {
       reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, r))[lane] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (a.lse && lane == 0) a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + r] = INFINITY;
+      if (a.norm && lane == 0) a.norm[kv_row_number(a, x, r)] = make_float2(INFINITY, 0.0f);
     }
     return;
   }
@@ -973,15 +988,16 @@ __global__ void __launch_bounds__(kKtMergeWarps * 32) kv_tile_merge_kernel(const
     if (M[i] != -INFINITY)
       A[i] = make_float4(__fdiv_rn(A[i].x, sum), __fdiv_rn(A[i].y, sum), __fdiv_rn(A[i].z, sum), __fdiv_rn(A[i].w, sum));
     reinterpret_cast<float4*>(a.out + kv_row_offset<MASK>(a, x, row[i]))[lane] = A[i];
-    if (a.lse && lane == 0)
-      a.lse[((size_t)x.b * a.hkv + x.hk) * a.n * a.group + x.r0 + row[i]] =
-          M[i] == -INFINITY ? INFINITY : M[i] + log2f(sum);
+    if (a.norm && lane == 0) a.norm[kv_row_number(a, x, row[i])] = row_norm(M[i], sum);
   }
 }
 
 // ---------------------------------------------------------------------------------
 // Column sums of the softmax of causal rows: weight[j] += sum over the rows that see key j of
-// 2^(s_rj - z_r), z_r the rows' log2 sums, from every score once more.  Keys are the M side
+// 2^(s_rj - m_r) / l_r, m_r and l_r the rows' maxima and sums, from every score once more.  The scores
+// are the tile kernel's bit for bit: the same scale for every row and key, the same products in the same
+// order, the same roundings.  (Any others, however exact, would give a row of large scores more or less
+// than one unit in all: at scores of 2^24 a rounding is a factor of two.)  Keys are the M side
 // (128 a CTA, hi / lo in TMEM, a thread owns a key), tiles of 64 rows the N side, so a key's sum
 // stays in one register.  grid (key tiles, batch * hkv, splits): split z takes row tiles z, z +
 // splits, ... and leaves its sums in part[z]; kv_column_add_kernel adds them in split order.
@@ -994,8 +1010,8 @@ constexpr int kKcKeys = 128, kKcRows = 64;
 
 struct KcSmem {
   alignas(1024) uint8_t q[2][2][2][kKcRows * 128];  // [stage][hi, lo][64 dims][row][128 B]
-  alignas(16) float qsc[4][8];                      // inverse scales of the groups of 8 rows
-  alignas(16) float lse[4][kKcRows];
+  alignas(16) float factor[4][kKcRows];             // from a product under the row's scale to its score
+  alignas(16) float top[4][kKcRows], inv[4][kKcRows];  // the rows' -maxima and 1 / sums
   alignas(16) int last[4][kKcRows];                 // the last key a row sees
   alignas(16) float turn[4][32 * 20];               // rows of a warp's keys: memory <-> a thread per key
   alignas(8) uint64_t qfull[2], qfree[2], info[4], sfull[2], sfree[2], kfull, done;
@@ -1052,7 +1068,13 @@ kv_column_tile_kernel(const KvArgs a, float* weight, float* __restrict__ part, u
     const float4* qb = reinterpret_cast<const float4*>(a.q + ((size_t)b * a.n * a.hq + hk * a.group) * kKvD) + h;
     const int there = keys - p <= 0 ? 0 : min(rows, (keys - p) * a.group);  // rows inside the cache
     float4 qr[8];
+    const unsigned row0 = blockIdx.y * (unsigned)rows;  // all rows together are fewer than 2^31
+    float constant;  // of row lane % 8: maximum (lanes below 8), 1 / sum (16), scale (24)
     auto load = [&](int rt) {
+      const int rl = rt * kKcRows + cw * 8 + (lane & 7);
+      constant = lane < 8 ? INFINITY : lane < 16 ? 0.0f : 1.0f;
+      if (rl < there)
+        constant = lane < 16 ? reinterpret_cast<const float*>(a.norm)[2 * (row0 + rl) + (lane >> 3)] : a.qscale[row0 + rl];
       const int r = rt * kKcRows + cw * 8 + ky;
       int tok = r / a.group, head = r - tok * a.group;
 #pragma unroll
@@ -1076,29 +1098,28 @@ kv_column_tile_kernel(const KvArgs a, float* weight, float* __restrict__ part, u
     if (n > 0) load(first);
     for (int t = 0; t < n; ++t) {
       const int s = t & 1, rt = first + t * splits;
-      float m = 0.0f, scale, inverse;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m = mag(mag(mag(mag(m, qr[i].x), qr[i].y), qr[i].z), qr[i].w);
-      scale_of(__reduce_max_sync(kFull, __float_as_uint(m)), scale, inverse);
       if (t >= 2 && !dead) dead = !bar_wait(&sm.qfree[s], ((t >> 1) - 1) & 1, abort);
-      const float2 sc = make_float2(scale, scale);
       uint8_t* dst = &sm.q[s][0][h >> 3][(cw * 8 + ky) * 128];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        const float scale = __shfl_sync(kFull, constant, 16 + 2 * i + ky);
         uint4 hi, lo;
-        split_f16(mul2(lo2(qr[2 * i]), sc), hi.x, lo.x);
-        split_f16(mul2(hi2(qr[2 * i]), sc), hi.y, lo.y);
-        split_f16(mul2(lo2(qr[2 * i + 1]), sc), hi.z, lo.z);
-        split_f16(mul2(hi2(qr[2 * i + 1]), sc), hi.w, lo.w);
+        split_f16(times(lo2(qr[2 * i]), scale), hi.x, lo.x);
+        split_f16(times(hi2(qr[2 * i]), scale), hi.y, lo.y);
+        split_f16(times(lo2(qr[2 * i + 1]), scale), hi.z, lo.z);
+        split_f16(times(hi2(qr[2 * i + 1]), scale), hi.w, lo.w);
         const int at = i * 256 + (((h & 7) ^ (2 * i + ky)) << 4);
         *reinterpret_cast<uint4*>(dst + at) = hi;
         *reinterpret_cast<uint4*>(dst + sizeof(sm.q[0][0]) + at) = lo;
       }
-      if (lane == 0) sm.qsc[t & 3][cw] = inverse;
+      const int at = cw * 8 + (lane & 7);
       if (lane < 8) {
-        const int r = rt * kKcRows + cw * 8 + lane;
-        sm.lse[t & 3][cw * 8 + lane] = r < there ? a.lse[bh * rows + r] : INFINITY;
-        sm.last[t & 3][cw * 8 + lane] = p + r / a.group;
+        sm.top[t & 3][at] = -constant;
+        sm.last[t & 3][at] = p + (rt * kKcRows + at) / a.group;
+      } else if (lane < 16) {
+        sm.inv[t & 3][at] = constant;
+      } else if (lane < 24) {
+        sm.factor[t & 3][at] = fmaxf(a.c * __uint_as_float((254u << 23) - __float_as_uint(constant)), kLeastFactor);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -1119,7 +1140,7 @@ kv_column_tile_kernel(const KvArgs a, float* weight, float* __restrict__ part, u
       tc_after();
       __syncwarp();
       if (elected()) {
-        mma_pairs<8, sizeof(sm.q[0][0][0])>(tmem + 128 + 64 * s, tmem, tmem + 64, sm.q[s][0][0], sm.q[s][1][0], id);
+        mma_pairs<8, sizeof(sm.q[0][0][0]), true>(tmem + 128 + 64 * s, tmem, tmem + 64, sm.q[s][0][0], sm.q[s][1][0], id);
         mma_commit(&sm.qfree[s]);
         mma_commit(&sm.sfull[s]);
       }
@@ -1144,8 +1165,14 @@ kv_column_tile_kernel(const KvArgs a, float* weight, float* __restrict__ part, u
         const unsigned top = __reduce_max_sync(kFull, __float_as_uint(mag(mag(mag(mag(0.0f, v.x), v.y), v.z), v.w)));
         if (i == lane) m = top;
       }
+      // the scale that row_scales gives the key
+      if (j >= keys) m = 0;
+      unsigned top = m;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(kFull, top, o));
+      const bool even = (__ballot_sync(kFull, m >= near_of(top)) >> (lane & 24) & 255u) == 255u && top < 0x7f800000u;
       float scale;
-      scale_of(m, scale, kinv);
+      scale_of(even ? top : m, scale, kinv);
       const float2 sc = make_float2(scale, scale);
       float4* turn = reinterpret_cast<float4*>(&sm.turn[warp][0]);
 #pragma unroll
@@ -1175,7 +1202,6 @@ kv_column_tile_kernel(const KvArgs a, float* weight, float* __restrict__ part, u
       if (lane == 0) bar_arrive(&sm.kfull);
     }
     bool ok = true;
-    const float ck = a.c * kinv;
     float2 sum = make_float2(0.f, 0.f);
     for (int t = 0; ok && t < n; ++t) {
       const int s = t & 1;
@@ -1189,16 +1215,17 @@ kv_column_tile_kernel(const KvArgs a, float* weight, float* __restrict__ part, u
         uint32_t r[32];
         tm_ld32(mine + 128 + 64 * s + 32 * part, r);
         tm_wait_ld();
-        const float4 q4 = *reinterpret_cast<const float4*>(&sm.qsc[t & 3][4 * part]);
-        const float cc[4] = {ck * q4.x, ck * q4.y, ck * q4.z, ck * q4.w};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float4 z = *reinterpret_cast<const float4*>(&sm.lse[t & 3][32 * part + 4 * e]);
-          const float c1 = cc[e >> 1];
-          float2 x = fma2(make_float2(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1])), make_float2(c1, c1),
-                          make_float2(-z.x, -z.y));
-          float2 y = fma2(make_float2(__uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3])), make_float2(c1, c1),
-                          make_float2(-z.z, -z.w));
+          const float4 c4 = *reinterpret_cast<const float4*>(&sm.factor[t & 3][32 * part + 4 * e]);
+          const float4 m4 = *reinterpret_cast<const float4*>(&sm.top[t & 3][32 * part + 4 * e]);
+          const float4 v4 = *reinterpret_cast<const float4*>(&sm.inv[t & 3][32 * part + 4 * e]);
+          // the product is rounded to the score, as in the tile kernel; the key's scale, a power of two, passes
+          // through the sum exactly
+          float2 x = mul2(make_float2(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1])), lo2(c4));
+          float2 y = mul2(make_float2(__uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3])), hi2(c4));
+          x = fma2(x, make_float2(kinv, kinv), lo2(m4));
+          y = fma2(y, make_float2(kinv, kinv), hi2(m4));
           x = make_float2(ex2(x.x), ex2(x.y));
           y = make_float2(ex2(y.x), ex2(y.y));
           if (masked) {
@@ -1208,7 +1235,8 @@ kv_column_tile_kernel(const KvArgs a, float* weight, float* __restrict__ part, u
             y.x = j <= la.z ? y.x : 0.0f;
             y.y = j <= la.w ? y.y : 0.0f;
           }
-          sum = add2(sum, add2(x, y));
+          sum = fma2(x, lo2(v4), sum);
+          sum = fma2(y, hi2(v4), sum);
         }
       }
       tc_before();

@@ -83,7 +83,7 @@ def _graded(dev, t, hq, hkv, L, drop, seed):
 
 
 @pytest.mark.parametrize("size", [1.0, 2.0 ** 10, 2.0 ** 20, 2.0 ** 24, 2.0 ** 40])
-@pytest.mark.parametrize("t,hq,hkv,L", [(1, 16, 2, 100), (2, 16, 2, 100), (1, 16, 16, 3000)])
+@pytest.mark.parametrize("t,hq,hkv,L", [(1, 16, 2, 100), (2, 16, 2, 100), (1, 16, 16, 3000), (40, 16, 2, 100), (70, 16, 2, 1500)])
 def test_equal_keys_share_the_weight_at_any_score(cuda_device, t, hq, hkv, L, size):
     """Keys that are all alike have scores that are all alike, however large: each row spreads its unit evenly
     and its output is the mean of the values, to the bound that scores of ordinary size have."""
@@ -155,6 +155,54 @@ def test_large_and_small_numbers_in_prompts(cuda_device, t, L, qs, ks, vs):
     out = attention.attention_weights(q, k, v, _i32([L - t], dev), w)
     assert float((out.double() - ref).norm() / ref.norm()) <= REL_L2
     _close(w, wref, "weight")
+
+
+@pytest.mark.parametrize("size", [2.0 ** -12, 2.0 ** -24, 2.0 ** -36])
+@pytest.mark.parametrize("t,L", [(64, 200), (130, 1500)])
+def test_weights_of_query_rows_of_different_sizes(cuda_device, t, L, size):
+    """Every third query that much smaller than its neighbours, over keys that give it ordinary scores and the
+    others, but for a few, one key each: every row adds one unit, on the keys of its own softmax.
+
+    A score of size S is off by 1.5 * 2^-21 * S at most (above), and so is the weight of a row whose
+    weight is not all on one key; the rows whose is (to 1e-6 of it) are off by less than 1e-6 of that."""
+    dev, hq, hkv = cuda_device, 16, 2
+    g = _gen(106, dev)
+    k, v = _caches(g, 1, hkv, L, dev)
+    q = torch.randn((1, t, hq, D), generator=g, device=dev)
+    q[:, ::3] *= size
+    k /= size
+    w = torch.zeros((1, hkv, L), device=dev)
+    ref, wref = _weights_ref(q, k, v, [L - t], w)
+    top, off = 0.0, 0
+    for h in range(hq):
+        s = (q[0, :, h].double() @ k[0, h // (hq // hkv)].double().T) / math.sqrt(D)
+        s = s.masked_fill(torch.arange(L, device=dev) > L - t + torch.arange(t, device=dev)[:, None], -math.inf)
+        large = [i for i in range(t) if i % 3]
+        one = torch.softmax(s, -1).amax(-1)[large] > 1 - 1e-6
+        top = max(top, float(s[large].masked_fill(s[large] == -math.inf, 0.0).abs().max()))
+        off += int((~one).sum())
+    out = attention.attention_weights(q, k, v, _i32([L - t], dev), w)
+    _close(out[:, ::3], ref[:, ::3])
+    bound = REL_L2 + (off * 1.5 * 2.0 ** -21 * top + t * hq * 1e-6) / float(wref.norm())
+    assert float((w.double() - wref).norm() / wref.norm()) <= bound
+    torch.testing.assert_close(w.sum(-1), torch.full((1, hkv), float(t * hq // hkv), device=dev), rtol=1e-5, atol=0)
+
+
+@pytest.mark.parametrize("t,hq,hkv,p0", [(3, 16, 2, 61), (77, 16, 2, 61), (130, 12, 4, 0), (130, 16, 2, 1003)])
+def test_every_row_adds_one_unit_of_weight(cuda_device, t, hq, hkv, p0):
+    """Keys whose sizes differ by up to 2^30 within any group, queries whose scores reach 2^30: the weights of
+    each row add up to 1 all the same (f32 sums of at most t * hq / hkv units: 1e-5)."""
+    dev, max_t = cuda_device, p0 + t + 20
+    g = _gen(109, dev)
+    k, v = _caches(g, 1, hkv, max_t, dev, fill=[p0 + t])
+    k *= torch.exp2(torch.randint(-30, 1, (1, hkv, max_t, 1), generator=g, device=dev).float())
+    q = torch.randn((1, t, hq, D), generator=g, device=dev)
+    q *= torch.exp2(torch.randint(0, 31, (1, t, hq, 1), generator=g, device=dev).float())
+    w = torch.zeros((1, hkv, max_t), device=dev)
+    out = attention.attention_weights(q, k, v, _i32([p0], dev), w)
+    assert torch.isfinite(out).all() and torch.count_nonzero(w[..., p0 + t:]) == 0
+    torch.testing.assert_close(w.double().sum(-1), torch.full((1, hkv), float(t * hq // hkv), device=dev).double(), rtol=1e-5,
+                               atol=0)
 
 
 def test_tree_of_one_path_among_many_sizes(cuda_device):
