@@ -122,6 +122,19 @@ def weights_from_gguf(g, cfg: DecoderConfig, prefix: str = "") -> tuple[dict, Op
             "layers": layers}, factors
 
 
+def longest_path(tokens, parents, picks) -> list[int]:
+    """The longest path from node 0 of a tree of drafted tokens whose drafts are the picks of their
+    parents (the one that ends at the lowest node, of several).  Siblings may hold the same token."""
+    depth = [0] + [-1] * (len(tokens) - 1)  # -1: not on such a path
+    for i in range(1, len(tokens)):
+        if depth[parents[i]] >= 0 and tokens[i] == picks[parents[i]]:
+            depth[i] = depth[parents[i]] + 1
+    path = [depth.index(max(depth))]
+    while path[-1] != 0:
+        path.append(parents[path[-1]])
+    return path[::-1]
+
+
 class Q8Decoder:
     """Weights, KV cache and step buffers of one decoder on one GPU."""
 
@@ -558,12 +571,7 @@ class Q8Decoder:
         if tok[0] != int(self.token.item()):
             raise _lib.Q8LinError(_lib.ERR_INVALID_ARGUMENT, f"node 0 is {tok[0]}, the current token {int(self.token.item())}")
         nxt = self.verify_tree(tok, par).tolist()
-        path = [0]
-        while True:
-            child = next((i for i in range(path[-1] + 1, len(tok)) if par[i] == path[-1] and tok[i] == nxt[path[-1]]), None)
-            if child is None:
-                break
-            path.append(child)
+        path = longest_path(tok, par, nxt)
         self.accept_path(path, nxt[path[-1]])
         return [tok[i] for i in path[1:]] + [nxt[path[-1]]]
 
