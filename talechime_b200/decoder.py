@@ -215,6 +215,7 @@ class Q8Decoder:
                                for _ in range(cfg.layers)]
             self._keys_stale = False
         self.evicted = 0  # rows evict() took out: RoPE positions run ahead of cache rows by this many
+        self._tree: Optional[tuple[list[int], int]] = None  # the last tree's parents and its history's rows, to accept from
         self._row0 = torch.zeros(self.batch, dtype=torch.int32, device=dev)
         f = lambda n: torch.zeros(n, device=dev)
         self.x, self.h = f(H), f(H)
@@ -237,6 +238,7 @@ class Q8Decoder:
         """Empty the cache (position 0) and set the current token."""
         self.pos.zero_()
         self.token.fill_(int(token))
+        self._tree = None
         if self.evicted:
             self.evicted = 0
             self._drop_step_handle()
@@ -432,6 +434,7 @@ class Q8Decoder:
         if pos0 + T > cfg.max_t:
             raise _lib.Q8LinError(_lib.ERR_SHAPE, "Transformer context limit exceeded")
         self._check_mode(mode)
+        self._tree = None
         return self._prefill_launches(tok.reshape(-1).to(self.device), B, T, pos0, mode)
 
     def _prefill_launches(self, tok_d: torch.Tensor, B: int, T: int, pos0: int, mode: str = "dense") -> torch.Tensor:
@@ -507,9 +510,12 @@ class Q8Decoder:
         n = tok.numel()
         if bool((par < -1).any()) or bool((par >= torch.arange(n, dtype=torch.int32)).any()):
             raise _lib.Q8LinError(_lib.ERR_INVALID_ARGUMENT, "a node's parent is a node before it, or -1")
-        if int(self.pos.item()) + n > self.cfg.max_t:
+        pos = int(self.pos.item())
+        if pos + n > self.cfg.max_t:
             raise _lib.Q8LinError(_lib.ERR_SHAPE, "Transformer context limit exceeded")
-        return self._tree_launches(tok.to(self.device), par.to(self.device).view(1, n))
+        nxt = self._tree_launches(tok.to(self.device), par.to(self.device).view(1, n))
+        self._tree = par.tolist(), pos
+        return nxt
 
     def _tree_launches(self, tok_d: torch.Tensor, par_d: torch.Tensor) -> torch.Tensor:
         """The device work of ``verify_tree``: launches and tensor allocations only."""
@@ -544,17 +550,24 @@ class Q8Decoder:
         return nxt
 
     def accept_path(self, path, token: int) -> None:
-        """Keep the nodes `path` (a path of the last verify_tree from a root down, ascending) as the
-        next cached rows and set the current token; the other nodes are dropped."""
+        """Keep the nodes `path` (from a root of the last verify_tree down, each node the parent of the
+        next) as the next cached rows and set the current token; the other nodes are dropped, and
+        the tree cannot be accepted from again.  Refuses where the history has changed since
+        (a step, a prompt, an eviction, a reset)."""
         idx = [int(i) for i in path]
-        if any(b <= a for a, b in zip(idx, idx[1:])) or (idx and idx[0] < 0):
-            raise _lib.Q8LinError(_lib.ERR_INVALID_ARGUMENT, "a path's nodes are ascending")
+        if idx:
+            parents, pos = self._tree if self._tree is not None else ([], -1)
+            if pos != int(self.pos.item()):
+                raise _lib.Q8LinError(_lib.ERR_INVALID_ARGUMENT, "no tree was verified behind the cached rows as they are")
+            if not all(0 <= i < len(parents) and parents[i] == p for p, i in zip([-1] + idx, idx)):
+                raise _lib.Q8LinError(_lib.ERR_INVALID_ARGUMENT, f"{idx} is no path of the last tree from a root down")
         if idx and idx[-1] != len(idx) - 1:  # the first nodes in a row are where they belong
             d = torch.tensor([idx], dtype=torch.int32, device=self.device)
             for li in range(self.cfg.layers):
                 attention.kv_move_rows(self.k_cache[li], self.v_cache[li], d, base=self.pos)
         self.pos += len(idx)
         self.token.fill_(int(token))
+        self._tree = None
         if self.blocks is not None:
             self._keys_stale = True
 
@@ -598,6 +611,7 @@ class Q8Decoder:
         if gone:
             self.pos -= gone
             self.evicted += gone
+            self._tree = None
             self._drop_step_handle()
             if self.blocks is not None:
                 self._keys_stale = True
