@@ -72,17 +72,17 @@ VOXCPM_BASELM_EXPECT = {"embedding_length": 2048, "block_count": 28, "feed_forwa
                         "attention.key_length": 128, "attention.value_length": 128}
 
 
-def config_from_gguf(g, max_t: int = 640, arch: Optional[str] = None) -> DecoderConfig:
+def config_from_gguf(g, max_t: int = 640, arch: Optional[str] = None, max_pos: int = 0) -> DecoderConfig:
     """DecoderConfig from a GGUF file's `{arch}.*` metadata (general.architecture when
     `arch` is None); eps and RoPE theta are the reference's constants
-    (transformer.rs:49-51,104)."""
+    (transformer.rs:49-51,104).  max_t, max_pos: as DecoderConfig."""
     arch = arch or g.value("general.architecture")
     u = lambda name: g.to_u32(f"{arch}.{name}")
     heads = u("attention.head_count")
     hidden = u("embedding_length")
     return DecoderConfig(hidden=hidden, layers=u("block_count"), heads=heads,
                          kv_heads=u("attention.head_count_kv"), head_dim=u("attention.key_length"),
-                         inter=u("feed_forward_length"), vocab=u("vocab_size"), max_t=max_t)
+                         inter=u("feed_forward_length"), vocab=u("vocab_size"), max_t=max_t, max_pos=max_pos)
 
 
 def weights_from_gguf(g, cfg: DecoderConfig, prefix: str = "") -> tuple[dict, Optional[np.ndarray]]:
@@ -140,19 +140,22 @@ class Q8Decoder:
 
     @classmethod
     def from_gguf(cls, path: str, device: torch.device | int | str = 0, max_t: int = 640,
-                  expect: Optional[dict] = None, arch: Optional[str] = None) -> "Q8Decoder":
+                  expect: Optional[dict] = None, arch: Optional[str] = None, max_pos: int = 0, batch: int = 1,
+                  track_weights: bool = False, blocks: Optional[tuple[int, int]] = None) -> "Q8Decoder":
         """Load a decoder from a GGUF file (Model::load_files_with_cancel's BaseLM half,
         crates/voxcpm/src/model.rs:118-145).  `expect` maps `{arch}.`-relative metadata
-        keys to required u32 values (VOXCPM_BASELM_EXPECT for the production file)."""
+        keys to required u32 values (VOXCPM_BASELM_EXPECT for the production file).  max_pos:
+        rows of the RoPE tables, for evict(); batch, track_weights, blocks: as Q8Decoder."""
         from .gguf import GGUFFile
 
         with GGUFFile(path) as g:
             arch = arch or g.value("general.architecture")
             for name, val in (expect or {}).items():
                 g.expect_u32(f"{arch}.{name}", val)
-            cfg = config_from_gguf(g, max_t=max_t, arch=arch)
+            cfg = config_from_gguf(g, max_t=max_t, arch=arch, max_pos=max_pos)
             weights, factors = weights_from_gguf(g, cfg)
-        return cls(cfg, weights, device=device, rope_factors=factors)
+        return cls(cfg, weights, device=device, rope_factors=factors, batch=batch, track_weights=track_weights,
+                   blocks=blocks)
 
     def __init__(self, cfg: DecoderConfig, weights: dict, device: torch.device | int | str = 0,
                  rope_factors: Optional[np.ndarray] = None, batch: int = 1, track_weights: bool = False,
