@@ -267,8 +267,9 @@ class Q8Decoder:
         layer); "unfused": 11 launches per layer, one per reference operation; "tracked"
         (track_weights): the fused step whose attention also adds every cached row's weight to
         kv_weight; "blocks" (blocks=...): the fused step whose attention goes over the blocks
-        of rows that score highest (a replayed graph of another mode goes unnoticed: call
-        refresh_block_keys() before the next "blocks" step)."""
+        of rows that score highest (which keys are out of date is known from step() calls:
+        call refresh_block_keys() after replays of another mode's graph, and before replays of
+        a "blocks" graph that follow steps of another mode)."""
         if self.batch != 1:
             raise ValueError("the decode step serves batch 1; this decoder holds "
                              f"{self.batch} sequences (prefill only)")
@@ -293,6 +294,8 @@ class Q8Decoder:
                 self._keys_stale = True
             elif self._keys_stale:
                 self.refresh_block_keys()
+                # a capture records the refresh (each replay begins with one) and runs none
+                self._keys_stale = torch.cuda.is_current_stream_capturing()
 
     def refresh_block_keys(self) -> None:
         """Recompute the mean keys of all blocks from the caches (after steps of other modes)."""
