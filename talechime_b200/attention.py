@@ -43,6 +43,13 @@ def _shape(t: torch.Tensor, name: str, *shape: int) -> None:
         raise Q8LinError(_lib.ERR_SHAPE, f"{name} is {tuple(t.shape)}, expected {shape}")
 
 
+def _int32(**sizes: int) -> None:
+    """The numbers that the C entry points take as they are fit (ctypes would cut them)."""
+    for name, n in sizes.items():
+        if not -2 ** 31 <= n < 2 ** 31:
+            raise Q8LinError(_lib.ERR_SHAPE, f"{name} {n} does not fit 32 bits")
+
+
 def _caches(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor]) -> tuple[int, int, int, torch.device]:
     """(batch, kv heads, max_t, device) of a pair of caches."""
     dev = k_cache.device
@@ -174,6 +181,7 @@ def kv_evict(weight: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     NaN: lowest).  Rows behind the kept ones stay as they were.  ``weight_out`` (may be
     ``weight``) gets the kept rows' weights and 0 behind them.  Returns the kept rows' former
     places, int32 [batch, kv_heads, keep], -1 behind the last (q8lin_kv_evict)."""
+    _int32(keep=keep, sink=sink, recent=recent)
     batch, hkv, max_t, dev = _caches(k_cache, v_cache)
     _weight(weight, "weight", batch, hkv, max_t, dev)
     _need(length, "length", torch.int32, dev)
@@ -217,6 +225,7 @@ def block_keys(k_cache: torch.Tensor, pos: torch.Tensor, t: int, block: int,
     """Write the mean key of every block of ``block`` rows that rows pos .. pos + t - 1 complete
     into ``keys`` [batch, kv_heads, ceil(max_t / block), 128]; other blocks stay as they were (0
     in a new tensor).  Returns keys (q8lin_kv_block_keys)."""
+    _int32(t=t, block=block)
     batch, hkv, max_t, dev = _caches(k_cache, None)
     _need(pos, "pos", torch.int32, dev)
     _shape(pos, "pos", batch)
@@ -243,6 +252,7 @@ def attention_blocks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     equal scores: the lower block; NaN: lowest).  Returns out [batch, t, heads, 128] and the
     chosen blocks, int32 [batch, t, kv_heads, topk], ascending, -1 behind the last
     (q8lin_attention_blocks)."""
+    _int32(block=block, topk=topk)
     batch, hkv, max_t, dev = _caches(k_cache, v_cache)
     t, hq = _queries(q, batch, hkv, dev)
     _need(pos, "pos", torch.int32, dev)
