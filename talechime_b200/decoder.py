@@ -169,6 +169,12 @@ class Q8Decoder:
         if batch < 1:
             raise ValueError("batch must be positive")
         self.batch = int(batch)
+        if blocks is not None:
+            rows, topk = blocks
+            # what q8lin_attention_blocks takes, said before the first step of a "blocks" mode
+            if rows not in (16, 32, 64, 128) or not 1 <= topk <= 16384 or -(-cfg.max_t // rows) > 16384:
+                raise _lib.Q8LinError(_lib.ERR_SHAPE, f"blocks {tuple(blocks)}: blocks have 16, 32, 64 or 128 rows, a token 1 "
+                                                      "to 16384 of them, a cache at most 16384")
         if cfg.head_dim != 128:
             raise _lib.Q8LinError(_lib.ERR_SHAPE, "the decode attention kernel takes head_dim 128")
         self.cfg = cfg

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from talechime_b200 import Q8LinError, _lib, attention
+from talechime_b200.decoder import DecoderConfig, Q8Decoder
 
 K = torch.zeros((1, 2, 64, 128))
 POS = torch.zeros(1, dtype=torch.int32)
@@ -26,3 +27,10 @@ def test_numbers_beyond_32_bits_are_refused(big):
                lambda: attention.kv_evict(W, K, K, POS, 8, recent=big)):
         assert _status(fn) == _lib.ERR_SHAPE
     assert _status(lambda: attention.block_keys(K, POS, 4, 16)) == _lib.ERR_DEVICE  # the CPU is what is left to refuse
+
+
+@pytest.mark.parametrize("blocks,max_t", [((0, 4), 640), ((-16, 4), 640), ((24, 4), 640), ((256, 4), 640), ((64, 0), 640),
+                                          ((64, 16385), 640), ((16, 4), 16 * 16384 + 1)])
+def test_decoder_refuses_block_sizes_before_it_is_made(blocks, max_t):
+    cfg = DecoderConfig(hidden=256, layers=1, heads=4, kv_heads=2, inter=512, vocab=100, max_t=max_t)
+    assert _status(lambda: Q8Decoder(cfg, {}, blocks=blocks)) == _lib.ERR_SHAPE
