@@ -858,7 +858,10 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
       float f = ex2(share - kKtPScale);
       if (whole) f = m == -INFINITY ? 0.0f : __fdiv_rn(f, l);
       ok = ok && !*abort;  // another warp that went on without its data
-      if (!ok) f = nan;
+      if (!ok) {  // NaN however the parts are joined: an infinite maximum leaves no other part a share
+        f = l = nan;
+        m = INFINITY;
+      }
       {
         // 32 dimensions of the pair's 32 rows at a time, turned back and written by rows
         float* turn = &sm.turn[0][warp & 3][0][0];
@@ -894,7 +897,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv_tile_kernel(const KvArgs a, 
         if (half == 0) {
           if (!whole) {
             a.stat[slot * 2 * a.rows + row] = m;
-            a.stat[(slot * 2 + 1) * a.rows + row] = ok ? l : nan;
+            a.stat[(slot * 2 + 1) * a.rows + row] = l;
           }
           if (a.norm && whole) a.norm[kv_row_number(a, x, row)] = row_norm(m, l);
         }
