@@ -157,6 +157,29 @@ def test_large_and_small_numbers_in_prompts(cuda_device, t, L, qs, ks, vs):
     _close(w, wref, "weight")
 
 
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 20, 2.0 ** 40])
+@pytest.mark.parametrize("n,hq,hkv,max_t", FORMS + [(2, 16, 2, 100)])
+def test_tree_nodes_of_equal_keys_take_the_mean_at_any_score(cuda_device, n, hq, hkv, max_t, size):
+    """A tree without rotation (cos 1, sin 0) whose keys are those of the history, all alike: a node's output is
+    the mean of the values it sees, however large the scores."""
+    dev, p0 = cuda_device, 50
+    g = _gen(111, dev)
+    k, v = _caches(g, 1, hkv, max_t, dev)
+    k[:] = k[:, :, :1].clone()
+    qkv = torch.randn((1, n, (hq + 2 * hkv) * D), generator=g, device=dev)
+    rows = qkv.view(n, hq + 2 * hkv, D)
+    rows[:, :hq] *= size
+    rows[:, hq:hq + hkv] = k[0, :, 0]
+    one, zero = torch.ones((max_t, 64), device=dev), torch.zeros((max_t, 64), device=dev)
+    parents = [(i - 1) // 2 if i else -1 for i in range(n)]
+    ref = []
+    for i, path in enumerate(_paths(parents, p0, max_t)):
+        seen = torch.cat([v[0, :, :p0], rows[path, hq + hkv:].transpose(0, 1)], 1).double()
+        ref.append(seen.mean(1).repeat_interleave(hq // hkv, 0))
+    out = attention.rope_attention_tree(qkv, _i32([parents], dev), _i32([p0], dev), one, zero, k, v)
+    _close(out[0], torch.stack(ref))
+
+
 @pytest.mark.parametrize("size", [2.0 ** -12, 2.0 ** -24, 2.0 ** -36])
 @pytest.mark.parametrize("t,L", [(64, 200), (130, 1500)])
 def test_weights_of_query_rows_of_different_sizes(cuda_device, t, L, size):
