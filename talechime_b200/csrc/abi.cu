@@ -394,10 +394,14 @@ int q8lin_forward(const q8lin_weight* w, const float* x, float* y, int64_t m, q8
 
 size_t q8lin_workspace_bytes(int64_t max_m, int64_t max_k) {
   if (max_m <= 0 || max_k <= 0 || max_k % kQK || max_m > (int64_t)1 << 24 || max_k > (int64_t)1 << 24) return 0;
-  // the int8 tensor-core path up to M = 32, the f16 path above it: each grows with M and K
-  const size_t b = workspace_bytes(max_m < kSkinnyMaxM ? max_m : kSkinnyMaxM, max_k);
-  const size_t t = workspace_bytes(max_m, max_k);
-  return t > b ? t : b;
+  // The f16 path above M = 32 grows with M; up to there the kernels take turns (from M = 12 mma.sync
+  // needs less than the int8 tensor-core path below it), so every M counts.  All grow with K.
+  size_t b = workspace_bytes(max_m, max_k);
+  for (int64_t m = 1; m <= max_m && m <= kSkinnyMaxM; ++m) {
+    const size_t t = workspace_bytes(m, max_k);
+    b = t > b ? t : b;
+  }
+  return b;
 }
 
 int q8lin_workspace_create(int device, int64_t max_m, int64_t max_k, q8lin_workspace** out) {

@@ -82,3 +82,19 @@ def test_accept_path_of_a_graph_that_moved_on(cuda_device, model):
     with pytest.raises(Q8LinError):
         dec.accept_path([0], 3)
     del graph
+
+
+def test_trees_of_any_size_behind_one_another(cuda_device):
+    """Wide feed-forward layers (6144, the production width): a tree after a larger one, where another kernel
+    serves the linears and needs more scratch, gives what it gives on its own."""
+    cfg = _cfg(layers=1, inter=6144)
+    w = synthetic_weights(cfg, seed=6)
+    dec = Q8Decoder(cfg, w, device=cuda_device)
+    dec.prefill(PROMPT)
+    for n in (16, 8, 11, 2, 12, 9, 5, 33, 16, 8):
+        tok, par = [(7 * i + n) % cfg.vocab for i in range(n)], [(i - 1) // 2 if i else -1 for i in range(n)]
+        dec.verify_tree(tok, par)
+        alone = Q8Decoder(cfg, w, device=cuda_device)
+        alone.prefill(PROMPT)
+        alone.verify_tree(tok, par)
+        assert torch.equal(dec.tree_logits, alone.tree_logits), n
