@@ -447,12 +447,14 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 2 : 1) kv_attention_kernel(co
 // Merge of the parts of every unit, and the weights of the keys where the scores were stored:
 // weight[j] += sum over the rows of 2^(s_j - maximum) / sum.  (Not 2^(s_j - log2 of all): a maximum of
 // 2^20 leaves the logarithm of the sum four bits.)  grid (units, rows + key ranges): CTA (u, r)
-// merges row r, CTA (u, rows + k) adds the weights of range k.
+// merges row r, CTA (u, rows + k) adds the weights of range k.  Five CTAs on an SM: with four (8 registers
+// more) the weights of 8 tokens x 16 heads over 8 K keys take 28 us, with five 22.
 constexpr int kKvMergeThreads = 128;
 constexpr int kKvWeightKeys = kKvMergeThreads;  // one key a thread at a time
 template <int MASK, bool SCORES>
-__global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs a, float* __restrict__ weight) {
-  __shared__ float fac[kKvGrid], top[kKvMaxRows], inv[kKvMaxRows], rm[kKvMergeThreads / 32], rl[kKvMergeThreads / 32];
+__global__ void __launch_bounds__(kKvMergeThreads, 5) kv_merge_kernel(const KvArgs a, float* __restrict__ weight) {
+  __shared__ float fac[kKvGrid], rm[kKvMergeThreads / 32], rl[kKvMergeThreads / 32];
+  __shared__ float2 norm[kKvMaxRows];  // the rows' maxima and 1 / sums
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, u = blockIdx.x;
   pdl_launch_dependents();
   pdl_wait();
@@ -525,10 +527,7 @@ __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs 
         if (f != 0.0f) L = fmaf(stat[(s * 2 + 1) * a.rows + r], f, L);
       }
       L = warp_sum(L);
-      if (lane == 0) {
-        top[r] = M;
-        inv[r] = M == -INFINITY ? 0.0f : __fdiv_rn(1.0f, L);
-      }
+      if (lane == 0) norm[r] = make_float2(M, M == -INFINITY ? 0.0f : __fdiv_rn(1.0f, L));
     }
     __syncthreads();
     for (int rep = 0; rep < a.weight_reps; ++rep) {
@@ -538,7 +537,10 @@ __global__ void __launch_bounds__(kKvMergeThreads) kv_merge_kernel(const KvArgs 
       float w = 0.0f;
 #pragma unroll
       for (int r = 0; r < kKvMaxRows; ++r)
-        if (r < x.nrows && inv[r] != 0.0f) w = fmaf(exp2f(sc[r] - top[r]), inv[r], w);
+        if (r < x.nrows) {
+          const float2 n = norm[r];
+          if (n.y != 0.0f) w = fmaf(exp2f(sc[r] - n.x), n.y, w);
+        }
       weight[bh * a.max_t + key] = old + w;
     }
   }
@@ -645,10 +647,10 @@ struct KvPlan {
 // Rows a kv head from which the tcgen05 kernel (128 rows a unit) takes over: from there on the core
 // reads the keys more than once (16 rows a unit).  Its units start faster, so it keeps what can be no
 // more than kKvCoreRows units x rows of the cache, about ten chunks a CTA.  (Trees, core and tcgen05
-// kernel: 24 rows a kv head behind 100 rows 15.1 and 17.4 us, behind 8 K rows (16 K x 2) 27.6 and 30.0;
-// 128 rows behind 500 (8 K) 18.6 and 20.9, behind 2 K (32 K) 23.1 and 22.8, behind 8 K 37.9 and 32.2;
-// 512 rows behind 100 (6.4 K) 19.6 and 22.4, behind 500 (32 K) 25.2 and 22.5, behind 8 K 102.6 and
-// 38.2; four sequences of 128 rows behind 500 (32 K) 23.1 and 21.5.)
+// kernel: 24 rows a kv head behind 100 rows 15.4 and 17.3 us, behind 8 K rows (16 K x 2) 29.1 and 30.4;
+// 128 rows behind 500 (8 K) 19.4 and 20.6, behind 2 K (32 K) 23.9 and 22.8, behind 8 K 38.9 and 32.9;
+// 512 rows behind 100 (6.4 K) 20.1 and 22.4, behind 500 (32 K) 25.9 and 22.5, behind 8 K 103.1 and
+// 37.8; four sequences of 128 rows behind 500 (32 K) 24.2 and 21.8.)
 constexpr int64_t kKvTileMinRows = 17;
 constexpr int64_t kKvCoreRows = 10 * kKvGrid * kKvChunk;
 KvPlan kv_plan(int64_t lists, int64_t rows_per_list, bool tile) {
