@@ -11,6 +11,9 @@ sequence had before the call.
 * ``block_keys`` / ``attention_blocks`` -- attention over the blocks of keys that a score
   against the blocks' mean keys selects.
 
+What a row does not see may hold anything; queries and visible keys and values are finite (their
+sizes: include/q8lin.h).  Outputs overlap no input.
+
 All arithmetic runs in libq8lin.so on the current stream of the tensors' device; this module
 checks arguments, allocates outputs and scratch (from torch's caching allocator, so a captured
 graph keeps its own) and passes pointers.

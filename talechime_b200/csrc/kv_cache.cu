@@ -448,7 +448,7 @@ cudaError_t launch_kv_move(float* kc, float* vc, const int* index, const int* ba
                            int max_t, int count, cudaStream_t s) {
   // slices of 128 bytes, or of 32 (a DRAM sector) where the heads alone leave SMs idle (the whole
   // eviction of 64 heads, 8001 to 4096 rows: 114 us in slices of 128, 133 in slices of 32; of 2 heads,
-  // 640 to 320: 10.3 and 9.1)
+  // 640 to 320, replayed from a graph: 10.3 and 9.1)
   const int lanes = batch * hkv * 2 * 4 >= 296 ? 8 : 2;
   cudaLaunchAttribute attr[1];
   cudaLaunchConfig_t cfg =
@@ -484,7 +484,8 @@ cudaError_t launch_kv_pick(const float* q, const float* keys, const int* pos, in
   cudaError_t e = ensure_smem((const void*)kv_pick_kernel<1>, configured, device, (size_t)kKvMaxBlocks * 8, false);
   if (e != cudaSuccess) return e;
   // a cluster of CTAs per row while there are SMs for it; at least 64 blocks a CTA (one token over 500
-  // blocks, with its attention: 17.5 us, one CTA a row 24.9; 8 x 16 rows over 250: 47.8 and 50.7)
+  // blocks, with its attention, replayed from a graph: 17.5 us, one CTA a row 24.9; 8 x 16 rows over 250: 47.8
+  // and 50.7)
   unsigned ranks = 1;
   while (ranks < 8 && rows * ranks * 2 <= 296 && blocks >= 128 * (int)ranks) ranks *= 2;
   cudaLaunchConfig_t cfg = kc_cfg(dim3((unsigned)(rows * ranks)), dim3(kPickThreads), (size_t)blocks * 8, s, attr);

@@ -164,9 +164,9 @@ struct KvFind {
 // every unit gets CTAs of its own, which then take up to `quota` chunks of it.  Starting on a
 // unit costs about a.pass chunks' time (query rows, first copies, joining the parts), so units
 // get their own CTAs where that adds at most a.pass chunks to the share.  (Evenly and so: trees of 64
-// nodes x 8 heads behind 200 rows 27.8 and 21.7 us, 5 ragged trees of 33 nodes 36.5 and 33.0, 16 heads
-// of 16 K rows 70.0 and 61.9, one block-sparse token 21.8 and 17.9.  64 units of 122 tiles stay
-// even, 53 tiles to a CTA and not 64: 154 us against 169.)
+// nodes x 8 heads behind 200 rows 26.4 and 21.5 us, 5 ragged trees of 33 nodes 37.6 and 33.4, 16 heads
+// of 16 K rows 71.4 and 63.8, one block-sparse token 21.6 and 17.9.  64 units of 122 tiles stay
+// even, 53 tiles to a CTA and not 64: 157 us against 173.)
 template <int MASK, int THREADS>
 __device__ int kv_find(const KvArgs& a, KvFind& sm, int cta) {
   constexpr int kPer = (2 * kKvGrid + THREADS - 1) / THREADS;  // more units are not split

@@ -29,12 +29,13 @@
 // rounding.  TMEM (512 columns): Q 128, S 2 x 64, P 2 x 64, O 128.
 //
 // What bounds it: per 128 rows x 64 keys 24 MMAs of N = 64 and 12 of N = 128, 1632 cycles, a third
-// of the 2.3 us that a tile takes (64 trees' units of 122 tiles, 53 tiles a CTA, 153 us with the
-// launches around it).  Issue slots are 57 % busy; the rest is the roles' chain through a tile (S,
-// maximum, P, O) and instruction fetch: the unrolled loops of three roles are more than the
-// instruction caches hold, so what shortens their code shortens the tile (one issue loop for the
-// three products, one site each for the converters' loads and for adding O: 163 -> 154 us; two
-// copies of the converter's loop in turn: 254).  A unit costs about 9 us beside its tiles.
+// of a tile's time (64 trees' units of 122 tiles, 53 tiles a CTA: 157 us with the launches around it
+// where two inputs alternate in a graph, 180 where three do, by the clock that power leaves).  Issue
+// slots are 57 % busy; the rest is the roles' chain through a tile (S, maximum, P, O) and instruction
+// fetch: the unrolled loops of three roles are more than the instruction caches hold, so what
+// shortens their code shortens the tile (one issue loop for the three products, one site each for the
+// converters' loads and for adding O: 163 -> 154 us; the softmax's first pass 16 keys at a time: 196
+// -> 193; two copies of the converter's loop in turn: 254).  A unit costs about 9 us beside its tiles.
 #include <cmath>
 
 #include "common.cuh"
@@ -1006,7 +1007,7 @@ __global__ void __launch_bounds__(kKtMergeWarps * 32) kv_tile_merge_kernel(const
 // splits, ... and leaves its sums in part[z]; kv_column_add_kernel adds them in split order.
 // Two CTAs per SM: 4 warps exponentials, 8 converters, 1 MMA; 24 MMAs of N = 64 a tile, about
 // 820 cycles, beside 512 cycles of exponentials; what it waits for is the converters' chain of load,
-// scale, split and hand-over.  4 x 1024 tokens, 16 heads on 2: 69 us, tensor pipe 26 % busy.
+// scale, split and hand-over.  4 x 1024 tokens, 16 heads on 2: 74 us, tensor pipe 24 % busy.
 constexpr int kKcThreads = 416, kKcConvertWarp = 4, kKcMmaWarp = 12;
 constexpr uint32_t kKcTmemCols = 256;
 constexpr int kKcKeys = 128, kKcRows = 64;
@@ -1275,7 +1276,7 @@ kv_column_add_kernel(const float* __restrict__ part, const int* __restrict__ pos
 
 // Row splits of the column sums: about 592 CTAs (two for each of two places on an SM) over the
 // keys of the new rows alone, 8 row tiles a CTA at least (its start costs as much as some tiles).
-// (4 x 1024 tokens with 256, 444 and 592 CTAs: 198, 191 and 187 us for the whole call.)
+// (4 x 1024 tokens with 256, 444 and 592 CTAs: 198, 193 and 190 us for the whole call.)
 int column_splits(int batch, int n, int hkv, int group) {
   const int64_t tiles = ((int64_t)n * group + kKcRows - 1) / kKcRows;
   const int64_t places = (int64_t)batch * hkv * ((n + kKcKeys - 1) / kKcKeys);
@@ -1303,8 +1304,8 @@ cudaError_t launch_tile(const KvArgs& a, int device, cudaStream_t s) {
   e = cudaLaunchKernelEx(&cfg, kv_tile_kernel<MASK>, a, wait_limit_ns());
   if (e != cudaSuccess || !a.split) return e;
   // Few units have few rows, of many parts each: a warp per row.  With many, the CTAs' starts count.
-  // (A tree over 2 units of 63 parts 68 us with four rows a warp, 33 with one; 30 units of 4 parts 39
-  // and 33; 64 units of 3 parts 152 and 155.)
+  // (A tree over 2 units of 63 parts 68 us with four rows a warp, 33 with one; 30 units of 4 parts 37
+  // and 33; 64 units of 3 parts 157 and 159.)
   const int rows = a.units > a.batch * a.hkv ? kKvTileRows : a.n * a.group;  // of the largest unit
   const int each = a.units <= kKvGrid / 4 ? 1 : 4;
   cfg.gridDim = dim3((unsigned)a.units, (unsigned)((rows + kKtMergeWarps * each - 1) / (kKtMergeWarps * each)));
