@@ -298,8 +298,8 @@ int q8lin_attention_prefill(const float* q, const float* k_cache, const float* v
  * A row at or past max_t (or of a sequence with pos < 0) is no row: its output is 0, nothing
  * is written for it and nothing sees it.  What a row does not see, be it a cache row behind
  * the call's or a sibling's, may hold anything and does not reach the row's result.  Queries and
- * visible keys and values are finite, queries and keys below 2^90 in size, values such that
- * their weighted sums stay in f32's range; scores may have any size.  f32 accuracy: 2e-7 to 5e-7
+ * visible keys and values are finite, queries and keys below 2^90 in size, values below 3.4e38 and
+ * such that their weighted sums stay in f32's range; scores may have any size.  f32 accuracy: 2e-7 to 5e-7
  * of ordinary outputs; operands pass the tensor cores as two parts that keep 2^-22 of an element,
  * with more than 16 rows a kv head 2^-23 of it or 2^-27 of its row's largest, whichever is more.
  * Outputs overlap no input (but weight_out may be weight).  Workspaces need no initialisation,
